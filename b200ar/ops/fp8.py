@@ -1,0 +1,172 @@
+"""Linear layers with 8-bit weights and activations (``csrc/fp8``).
+
+e4m3 values with an fp32 scale for each block of 128 along K: one scale for
+each row and block of the activations, one for each 128 x 128 block of a
+weight. A block's scale is ``amax / 448`` (1 for a block of zeros), a value's
+code ``x / scale`` rounded to the nearest e4m3 number, both quotients in fp32.
+
+* ``quantize_fp8_weight(w)``       once, when weights are loaded
+* ``linear_fp8(x, w_q, w_scale)``  ``x @ w.T`` for bf16 or fp16 activations
+* ``quantize_fp8(x)``              the activations' codes and scales, for inputs
+                                   that several layers share
+
+CPU tensors run the fp32 reference math; CUDA tensors always run the kernels.
+A row that holds a NaN or an infinity gives NaN or infinite outputs. These ops
+have no backward pass.
+"""
+
+from __future__ import annotations
+
+from typing import Optional, Tuple
+
+import torch
+
+from .._native import _C
+from .gemm import error_word
+
+BLOCK = 128
+E4M3_MAX = 448.0
+_FLOATS = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _blocks(n: int) -> int:
+    return -(-n // BLOCK)
+
+
+def _rows_2d(x: torch.Tensor) -> torch.Tensor:
+    """[rows, K] with contiguous rows on 16-byte boundaries (copied if x has none)."""
+    x2 = x.reshape(-1, x.shape[-1])
+    step = 16 // x2.element_size()
+    if (x2.shape[1] > 1 and x2.stride(1) != 1) or x2.stride(0) % step or x2.data_ptr() % 16:
+        x2 = x2.clone(memory_format=torch.contiguous_format)
+    return x2
+
+
+def _check_input(t: torch.Tensor, name: str) -> None:
+    if t.dim() < 1 or t.dtype not in _FLOATS:
+        raise TypeError(f"{name} must be bfloat16, float16 or float32")
+    if t.shape[-1] < 1 or t.shape[-1] % 16:
+        raise ValueError(f"K must be a positive multiple of 16, got {t.shape[-1]}")
+
+
+def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``x`` [..., K] -> (codes float8_e4m3fn [..., K], scales fp32 [..., ceil(K / 128)]).
+
+    The scales are a view of storage that keeps the rows of a block together,
+    which is what ``linear_fp8`` reads."""
+    _check_input(x, "x")
+    x2 = _rows_2d(x)
+    m, k = x2.shape
+    codes = torch.empty(m, k, dtype=torch.float8_e4m3fn, device=x.device)
+    scale = torch.empty(_blocks(k), m, dtype=torch.float32, device=x.device)
+    if x.device.type == "cpu":
+        ref_codes, ref_scale = ref_quantize_fp8(x2)
+        codes.copy_(ref_codes)
+        scale.copy_(ref_scale.t())
+    else:
+        _C.quantize_fp8(x2, codes, scale)
+    return codes.view(x.shape), scale.t().unflatten(0, x.shape[:-1]) if x.dim() > 1 else scale.t()[0]
+
+
+def quantize_fp8_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``w`` [N, K] -> (codes float8_e4m3fn [N, K], scales fp32 [ceil(N / 128), ceil(K / 128)])."""
+    if w.dim() != 2:
+        raise ValueError("w must be [N, K]")
+    _check_input(w, "w")
+    n, k = w.shape
+    if w.device.type == "cpu":
+        return ref_quantize_fp8_weight(w)
+    error_word(w.device)  # exists before a graph that uses it is captured
+    codes = torch.empty(n, k, dtype=torch.float8_e4m3fn, device=w.device)
+    scale = torch.empty(_blocks(n), _blocks(k), dtype=torch.float32, device=w.device)
+    _C.quantize_fp8_weight(_rows_2d(w), codes, scale)
+    return codes, scale
+
+
+def linear_fp8(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
+               x_scale: Optional[torch.Tensor] = None, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``x @ w.T`` with the weight as ``quantize_fp8_weight`` gives it.
+
+    ``x`` [..., K] bf16 or fp16 is quantized here and gives an output of its
+    type; with ``x_scale`` it is the codes of ``quantize_fp8`` and the output
+    is of ``dtype`` (bf16 or fp16). K must be a multiple of 16 and N of 8.
+    Products are exact, sums fp32, and each block of 128 along K is scaled
+    before it is added."""
+    if w_q.dim() != 2 or w_q.dtype != torch.float8_e4m3fn or not w_q.is_contiguous():
+        raise TypeError("w_q must be contiguous float8_e4m3fn [N, K]")
+    n, k = w_q.shape
+    if k < 1 or k % 16 or n < 1 or n % 8:
+        raise ValueError(f"K must be a multiple of 16 and N of 8, got N {n}, K {k}")
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError(f"x must be [..., {k}]")
+    if w_scale.dtype != torch.float32 or tuple(w_scale.shape) != (_blocks(n), _blocks(k)) or \
+            not w_scale.is_contiguous():
+        raise ValueError(f"w_scale must be contiguous fp32 [{_blocks(n)}, {_blocks(k)}]")
+    if w_q.device != x.device or w_scale.device != x.device:
+        raise ValueError(f"the weight must be on {x.device}")
+    if x_scale is None:
+        if x.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError("x must be bfloat16 or float16, or codes with their x_scale")
+        dtype = x.dtype
+        codes, scale = quantize_fp8(x)
+    else:
+        if x.dtype != torch.float8_e4m3fn:
+            raise TypeError("with x_scale, x must be float8_e4m3fn")
+        if dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError("dtype must be bfloat16 or float16")
+        if tuple(x_scale.shape) != (*x.shape[:-1], _blocks(k)) or x_scale.dtype != torch.float32 or \
+                x_scale.device != x.device:
+            raise ValueError(f"x_scale must be fp32 [..., {_blocks(k)}] on {x.device}")
+        codes, scale = x, x_scale
+    codes = codes.reshape(-1, k).contiguous()
+    if codes.data_ptr() % 16:
+        codes = codes.clone()
+    m = codes.shape[0]
+    scale = scale.reshape(m, _blocks(k)).t()
+    if (m > 1 and scale.stride(1) != 1) or scale.stride(0) < m:
+        scale = scale.contiguous()
+    shape = (*x.shape[:-1], n)
+    if out is None:
+        out = torch.empty(shape, dtype=dtype, device=x.device)
+    elif tuple(out.shape) != shape or out.dtype != dtype or out.device != x.device:
+        raise ValueError(f"out must be {dtype} {list(shape)} on {x.device}")
+    out2 = out.view(m, n)
+    if x.device.type == "cpu":
+        out2.copy_(ref_linear_fp8(codes, scale.t(), w_q, w_scale).to(dtype))
+        return out
+    _C.linear_fp8(codes, scale, w_q, w_scale, out2, error_word(x.device))
+    return out
+
+
+# ------------------------------------------------------------------ references
+def ref_quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp32 reference of ``quantize_fp8`` for [rows, K]."""
+    m, k = x.shape
+    full = torch.zeros(m, _blocks(k) * BLOCK, device=x.device)
+    full[:, :k] = x.float()
+    full = full.view(m, -1, BLOCK)
+    amax = full.abs().amax(-1)
+    scale = torch.where(amax == 0, torch.ones_like(amax), amax / torch.full_like(amax, E4M3_MAX))
+    codes = (full / scale[..., None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
+    return codes.view(m, -1)[:, :k].contiguous(), scale
+
+
+def ref_quantize_fp8_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp32 reference of ``quantize_fp8_weight``."""
+    n, k = w.shape
+    nb, kb = _blocks(n), _blocks(k)
+    full = torch.zeros(nb * BLOCK, kb * BLOCK, device=w.device)
+    full[:n, :k] = w.float()
+    full = full.view(nb, BLOCK, kb, BLOCK)
+    amax = full.abs().amax(dim=(1, 3))
+    scale = torch.where(amax == 0, torch.ones_like(amax), amax / torch.full_like(amax, E4M3_MAX))
+    codes = (full / scale[:, None, :, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
+    return codes.view(nb * BLOCK, kb * BLOCK)[:n, :k].contiguous(), scale
+
+
+def ref_linear_fp8(x_q, x_scale, w_q, w_scale) -> torch.Tensor:
+    """fp32 reference of the product of codes and scales, [M, N]."""
+    n, k = w_q.shape
+    a = x_q.float() * x_scale.repeat_interleave(BLOCK, 1)[:, :k]
+    b = w_q.float() * w_scale.repeat_interleave(BLOCK, 0)[:n].repeat_interleave(BLOCK, 1)[:, :k]
+    return a @ b.t()

@@ -25,14 +25,22 @@ def error_word(device) -> torch.Tensor:
     return _ERR[idx]
 
 
+# What the codes of the error word above the bounded waits' say.
+_ERROR_TEXT = {3: "a token's position is outside the rotary table or before its sequence",
+               4: "a position that a row needs has no page in the pool"}
+
+
 def check_errors(device=None) -> None:
-    """Raises if a GEMM reported an expired wait (synchronises the device)."""
+    """Raises if a kernel reported an expired wait, or a paged op a position
+    or page that it had to skip (synchronises the device)."""
     for idx, t in _ERR.items():
         if device is not None and idx != (torch.device(device).index or 0):
             continue
         v = int(t.item())
         if v:
             t.zero_()
+            if v in _ERROR_TEXT:
+                raise RuntimeError(f"paged KV cache on cuda:{idx}: {_ERROR_TEXT[v]} (error {v}); it was skipped")
             raise RuntimeError(f"tcgen05 GEMM on cuda:{idx} reported error {v} (a bounded wait expired)")
 
 

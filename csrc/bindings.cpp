@@ -366,4 +366,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("register_graph_buffers", &compat_register_graph_buffers, "register graph buffers");
 
   register_ops(m);
+  register_serving_ops(m);
 }

@@ -1,0 +1,185 @@
+// Quantization to e4m3 with one scale for each block of 128.
+//
+//   scale = amax / 448 (1 for a block of zeros),  q = e4m3(x / scale)
+//
+// Both quotients are the correctly rounded fp32 ones, so the codes are those
+// of the formula and not an approximation of it. The maximum is taken over the
+// bit patterns of |x|, in which NaN is above infinity: a block that holds a
+// NaN gets the scale NaN, one that holds an infinity the scale infinity, and
+// either reaches the outputs of its row.
+//
+// Memory bounds both kernels: 3 bytes a value move, and a division costs about
+// ten instructions of the forty that the SM issues in the time of those bytes.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+
+#include "../common/check.h"
+#include "../common/pdl.h"
+#include "../common/trace.h"
+#include "fp8.h"
+
+namespace b200ar {
+namespace fp8 {
+
+namespace {
+
+constexpr float kMax = 448.f;
+constexpr int kThreads = 256;
+
+// Eight consecutive values as fp32.
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, float* v);
+template <>
+__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float* v) {
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __bfloat1622float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+template <>
+__device__ __forceinline__ void load8<__half>(const __half* p, float* v) {
+  const uint4 w = *reinterpret_cast<const uint4*>(p);
+  const __half2* h = reinterpret_cast<const __half2*>(&w);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(h[i]);
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+template <>
+__device__ __forceinline__ void load8<float>(const float* p, float* v) {
+  *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
+  *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
+}
+
+__device__ __forceinline__ unsigned abs_max8(const float* v) {
+  unsigned m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+  return m;
+}
+__device__ __forceinline__ float scale_of(unsigned amax_bits) {
+  return amax_bits == 0u ? 1.f : __fdiv_rn(__uint_as_float(amax_bits), kMax);
+}
+__device__ __forceinline__ uint2 encode8(const float* v, float scale) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    w[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[2 * i], scale), __fdiv_rn(v[2 * i + 1], scale)),
+                                    __NV_SATFINITE, __NV_E4M3);
+  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+}
+
+// Sixteen lanes share a block of 128 values; grid (row, 16 blocks of the row).
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    quantize_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, float* __restrict__ scale,
+                    int64_t lds, int64_t M, int K) {
+  const int64_t m = blockIdx.x;
+  const int lane = threadIdx.x & 15;
+  const int b = blockIdx.y * (kThreads / 16) + (threadIdx.x >> 4);
+  const int k = b * kBlock + lane * 8;
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  pdl_wait();
+  pdl_trigger();
+  if (k < K) load8<T>(x + m * ldx + k, v);
+  unsigned amax = abs_max8(v);
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  const float s = scale_of(amax);
+  if (k >= K) return;
+  *reinterpret_cast<uint2*>(q + m * K + k) = encode8(v, s);
+  if (lane == 0) scale[b * lds + m] = s;
+}
+
+// One CTA for each 128 x 128 block: 16 lanes on a row, 8 rows a thread.
+template <typename T>
+__global__ void __launch_bounds__(kThreads)
+    quantize_weight_kernel(const T* __restrict__ w, int64_t ldw, uint8_t* __restrict__ q, float* __restrict__ scale,
+                           int64_t N, int K) {
+  __shared__ unsigned part[kThreads / 32];
+  const int lane = threadIdx.x & 15, r0 = threadIdx.x >> 4;
+  const int k = blockIdx.x * kBlock + lane * 8;
+  const int64_t n0 = static_cast<int64_t>(blockIdx.y) * kBlock;
+  float v[8][8];
+  unsigned amax = 0;
+  pdl_wait();
+  pdl_trigger();
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t n = n0 + r0 + 16 * i;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+    if (n < N && k < K) load8<T>(w + n * ldw + k, v[i]);
+    amax = max(amax, abs_max8(v[i]));
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kThreads / 32; ++i) amax = max(amax, part[i]);
+  const float s = scale_of(amax);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int64_t n = n0 + r0 + 16 * i;
+    if (n < N && k < K) *reinterpret_cast<uint2*>(q + n * K + k) = encode8(v[i], s);
+  }
+  if (threadIdx.x == 0) scale[blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x] = s;
+}
+
+template <typename T>
+void launch_rows(const void* x, int64_t ldx, uint8_t* q, float* scale, int64_t lds, int64_t M, int64_t K,
+                 cudaStream_t s) {
+  const int64_t blocks = (K + kBlock - 1) / kBlock;
+  const dim3 grid(static_cast<unsigned>(M), static_cast<unsigned>((blocks + kThreads / 16 - 1) / (kThreads / 16)));
+  launch_pdl(quantize_kernel<T>, grid, dim3(kThreads), 0, s, 1, static_cast<const T*>(x), ldx, q, scale, lds, M,
+             static_cast<int>(K));
+}
+template <typename T>
+void launch_weight(const void* w, int64_t ldw, uint8_t* q, float* scale, int64_t N, int64_t K, cudaStream_t s) {
+  const dim3 grid(static_cast<unsigned>((K + kBlock - 1) / kBlock), static_cast<unsigned>((N + kBlock - 1) / kBlock));
+  launch_pdl(quantize_weight_kernel<T>, grid, dim3(kThreads), 0, s, 1, static_cast<const T*>(w), ldw, q, scale, N,
+             static_cast<int>(K));
+}
+
+void check_shape(int64_t rows, int64_t K) {
+  B200AR_CHECK(rows >= 0 && rows < (1ll << 31) && K > 0 && K < (1ll << 30), "bad shape for quantization");
+  B200AR_CHECK(K % 16 == 0, "K must be a multiple of 16");
+}
+
+}  // namespace
+
+void quantize(const void* x, int64_t ldx, uint8_t* q, float* scale, int64_t lds, int64_t M, int64_t K, Type type,
+              cudaStream_t s) {
+  const TraceRange trace("b200ar::quantize_fp8");
+  check_shape(M, K);
+  if (M == 0) return;
+  switch (type) {
+    case Type::kBf16: return launch_rows<__nv_bfloat16>(x, ldx, q, scale, lds, M, K, s);
+    case Type::kFp16: return launch_rows<__half>(x, ldx, q, scale, lds, M, K, s);
+    case Type::kFp32: return launch_rows<float>(x, ldx, q, scale, lds, M, K, s);
+  }
+}
+
+void quantize_weight(const void* w, int64_t ldw, uint8_t* q, float* scale, int64_t N, int64_t K, Type type,
+                     cudaStream_t s) {
+  const TraceRange trace("b200ar::quantize_fp8_weight");
+  check_shape(N, K);
+  B200AR_CHECK(N <= 65535ll * kBlock, "weights of at most 65535 * 128 rows");
+  if (N == 0) return;
+  switch (type) {
+    case Type::kBf16: return launch_weight<__nv_bfloat16>(w, ldw, q, scale, N, K, s);
+    case Type::kFp16: return launch_weight<__half>(w, ldw, q, scale, N, K, s);
+    case Type::kFp32: return launch_weight<float>(w, ldw, q, scale, N, K, s);
+  }
+}
+
+}  // namespace fp8
+}  // namespace b200ar
