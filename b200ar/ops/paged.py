@@ -14,9 +14,10 @@ keeps heads before tokens. Position p of sequence s lives in slot
 
 Lengths, offsets and page tables stay on the device: nothing is read back, so
 both calls can be captured into a CUDA graph and replayed with other lengths.
-What only the device sees is checked there. A page that is missing or outside
-the pool, or a position outside the rotary table, is skipped and reported by
-``b200ar.ops.gemm.check_errors``.
+What only the device sees is checked there: a page that is missing or outside
+the pool, or a position outside the rotary table, is not accessed and reported
+by ``b200ar.ops.gemm.check_errors``. The rotary step skips such a token; the
+rows of attention that need such a page have no defined result.
 
 CPU tensors run the fp32 reference math; CUDA tensors always run the kernels.
 These ops have no backward pass.
@@ -172,6 +173,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     rows, hq, d = q.shape
     _check_pools(k_pages, v_pages, q, d)
     hkv = k_pages.shape[2]
+    if k_pages.shape[1] % 8:
+        raise ValueError(f"the page size must be a multiple of 8, got {k_pages.shape[1]}")
     if hkv < 1 or hq < 1 or hq % hkv:
         raise ValueError("query heads must be a multiple of the KV heads")
     _check_batch(batch, rows, q.device)

@@ -7,6 +7,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <optional>
 
 #include "../fp8/fp8.h"
@@ -54,6 +55,7 @@ Pool pool_of(const at::Tensor& t, const at::Tensor& like, const at::Tensor& firs
                   t.stride(0) >= 0 && t.stride(1) >= 0 && t.stride(2) >= 0 &&
                   reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
               name, " must have contiguous heads that start on 16-byte boundaries");
+  for (int i = 0; i < 3; ++i) TORCH_CHECK(t.size(i) == 1 || t.stride(i) > 0, name, " must not be expanded");
   return Pool{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
 }
 
@@ -189,6 +191,7 @@ void register_serving_ops(py::module& m) {
         TORCH_CHECK(k_pages.dim() == 4, "k_pages must be [pages, page_size, kv_heads, d]");
         const int64_t hq = q.size(1), d = q.size(2), hkv = k_pages.size(2);
         TORCH_CHECK(hkv >= 1 && hq >= hkv && hq % hkv == 0, "query heads must be a multiple of the KV heads");
+        TORCH_CHECK(k_pages.size(1) % 8 == 0, "the page size must be a multiple of 8");
         TORCH_CHECK(window >= 0 && window <= kInt && (causal || window == 0),
                     "window must be 0 (all) or a number of positions, with causal attention");
         b200ar::paged::AttnArgs a{};
@@ -207,11 +210,17 @@ void register_serving_ops(py::module& m) {
         a.hkv = static_cast<int>(hkv);
         a.num_pages = static_cast<int>(k_pages.size(0));
         a.page_size = static_cast<int>(k_pages.size(1));
-        a.window = static_cast<int>(window);
+        const int64_t capacity = std::min<int64_t>(table.size(1) * k_pages.size(1), 1 << 30);
+        a.capacity = static_cast<int>(capacity);
+        a.window = window >= capacity ? 0 : static_cast<int>(window);  // a window over every position hides nothing
         a.causal = causal;
         a.scale = static_cast<float>(scale);
         const at::cuda::OptionalCUDAGuard guard(device_of(q));
-        b200ar::paged::paged_attention(a, static_cast<int>(d), type, stream_of());
+        // From the caching allocator on this stream: concurrent calls, eager or captured, never share it.
+        const at::Tensor workspace =
+            at::empty({b200ar::paged::paged_attention_workspace(q.size(0), a.hq, a.hkv, static_cast<int>(d))},
+                      q.options().dtype(at::kFloat));
+        b200ar::paged::paged_attention(a, static_cast<int>(d), type, workspace.data_ptr<float>(), stream_of());
       },
       "attention of new tokens over a paged KV cache", py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
       py::arg("page_table"), py::arg("kv_len"), py::arg("q_start"), py::arg("out"), py::arg("err"), py::arg("scale"),

@@ -1,36 +1,78 @@
-// Attention of new tokens over a paged KV cache.
+// Attention of new tokens over a paged KV cache, on the 5th-generation tensor cores.
 //
-//   o[i] = sum_p softmax_p(scale q[i] . k[p]) v[p]  over the positions p that row i sees
+//   o[i] = sum_p w[i, p] v[p] / sum_p w[i, p],   w[i, p] = exp(scale q[i] . k[p])
 //
-// The simplest form: one warp for each (row, query head) walks the positions
-// with a running maximum and sum.
+// over the positions p that row i sees. The G query heads of a KV head share
+// keys and values, so the rows of a product are (token, head) pairs: a block
+// is 256 of them (schedule.cuh), and for each tile of 128 tokens
+//
+//   S [128 rows x 128 tokens] = Q K^T   (tcgen05.mma, Q and K in shared memory)
+//   O [128 rows x d]         += P V     (tcgen05.mma, P in tensor memory)
+//
+// with P = exp2(scale log2(e) S - m) rounded to the type of V, m a running
+// bound on the row's maximum and the sum of P kept in fp32.
+//
+//   warps 0-3, 4-7  softmax: group t owns S_t, P_t (in the columns of S_t) and
+//                   O_t in tensor memory; a thread owns one row
+//   warp 8          TMA producer: a lane loads one run of tokens of one page
+//   warp 9          TMEM allocation and MMA issue (one thread)
+//
+// Steps alternate between the two groups, so that one's products run during
+// the other's softmax. What the groups work on depends on the block's rows:
+//   over 128   group t has rows 128 t .. 128 t + 127; both use every tile
+//   33 to 128  both have the same rows; group t takes the tiles t, t + 2, ...
+//   up to 32   as before, and the 32 rows are held four times: warp w of a
+//              group takes the tokens 32 w .. 32 w + 31 of a tile. The products
+//              cost the same, the softmax of a tile a quarter
+// and the states of a row (its maximum, sum and O) are joined at the end.
+//
+// S(k + 2) is issued after P V(k), in the order of which the tensor core
+// works, so a group that sees S(k + 2) knows that O holds step k: it may
+// rescale O then. It does so only when the row's maximum has grown by 2^8 or
+// more over the bound m in use (2^6 for fp16, whose P has a factor 2^8 to keep
+// small weights out of the subnormals): P stays in the type's range, and
+// numerator and denominator have the same factor.
+//
+// Pages are read by TMA boxes of the largest power of two of tokens (8 to
+// 128) that divides the page size. Runs that no row sees are not looked up:
+// their boxes lie outside the pool and read as zeros. The tokens behind a
+// sequence in its last page, and those before the window in its first, hold
+// anything; they are masked in S and zeroed in V, where a zero weight does not
+// hide a NaN. A position that some rows of a
+// tile see and others do not may also hold an infinity or NaN: the rows that
+// come out as NaN are computed again one by one (attention_row), which touches
+// only what they see.
+//
+// Every wait is bounded: on expiry the error word is set and all roles run
+// down without waiting.
+#include <cuda.h>
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
+
 #include "../common/check.h"
 #include "../common/pdl.h"
 #include "../common/trace.h"
-#include "batch.cuh"
+#include "../gemm/tcgen05.cuh"
+#include "schedule.cuh"
 
 namespace b200ar {
 namespace paged {
 
 namespace {
 
+constexpr float kLog2e = 1.4426950408889634f;
+
+// ------------------------------------------------------------------ one row
+// One row by one warp, position by position. Every position that the row does
+// not see is left unread.
 template <typename T, int D>
-__global__ void __launch_bounds__(128) attention_simple_kernel(const AttnArgs a) {
+__device__ __noinline__ void attention_row(const AttnArgs& a, int s, int row, int pos, int len, int h, int kh) {
   constexpr int kPairs = D / 64;  // pairs of elements that a lane holds
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + warp;
-  pdl_wait();
-  pdl_trigger();
-  if (item >= static_cast<int64_t>(a.rows) * a.hq) return;
-  const int row = static_cast<int>(item / a.hq), h = static_cast<int>(item % a.hq);
-  const int s = sequence_of_row(a.batch, row);
-  if (s < 0) return;
-  const int first = q_begin(a.batch, s), n = q_begin(a.batch, s + 1) - first;
-  const int len = __ldg(a.batch.kv_len + s);
-  const int pos = len - n + (row - first);
+  const int lane = threadIdx.x & 31;
   const int end = a.causal ? pos + 1 : len;
   const int begin = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  const int kh = h / (a.hq / a.hkv);
   float2 q[kPairs], o[kPairs];
   const T* qp = static_cast<const T*>(a.q) + row * a.q_tok + h * a.q_head;
 #pragma unroll
@@ -41,10 +83,7 @@ __global__ void __launch_bounds__(128) attention_simple_kernel(const AttnArgs a)
   float m = -INFINITY, l = 0.f;
   for (int p = begin; p < end; ++p) {
     const int page = page_of(a.batch, s, p / a.page_size, a.num_pages);
-    if (page < 0) {
-      if (lane == 0) atomicExch(a.err, kErrPage);
-      continue;
-    }
+    if (page < 0) continue;  // reported by the producer
     const int slot = p % a.page_size;
     const T* kp = static_cast<const T*>(a.k.base) + page * a.k.page + slot * a.k.tok + kh * a.k.head;
     const T* vp = static_cast<const T*>(a.v.base) + page * a.v.page + slot * a.v.tok + kh * a.v.head;
@@ -56,10 +95,10 @@ __global__ void __launch_bounds__(128) attention_simple_kernel(const AttnArgs a)
     }
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-    const float x = dot * a.scale * 1.4426950408889634f;
+    const float x = dot * a.scale * kLog2e;
     const float mn = fmaxf(m, x);
     const float f = m == -INFINITY ? 0.f : exp2f(m - mn);
-    const float e = exp2f(x - mn);
+    const float e = mn == -INFINITY ? 0.f : exp2f(x - mn);
     m = mn;
     l = l * f + e;
 #pragma unroll
@@ -69,29 +108,783 @@ __global__ void __launch_bounds__(128) attention_simple_kernel(const AttnArgs a)
       o[i].y = o[i].y * f + e * v.y;
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   T* op = static_cast<T*>(a.out) + row * a.o_tok + h * a.o_head;
 #pragma unroll
   for (int i = 0; i < kPairs; ++i)
     *reinterpret_cast<uint32_t*>(op + i * 64 + lane * 2) = pack2<T>(o[i].x * inv, o[i].y * inv);
 }
 
+// ------------------------------------------------------------------ workspace
+// CTA c leaves at most two parts of blocks that others work on too: its first
+// and its last item (slots 2 c and 2 c + 1).
+struct PartDesc {
+  int s, h, b, rows;
+  int t0, t1, tiles, used;
+};
+
+struct Workspace {
+  PartDesc* desc;  // [2 CTAs]
+  float* ml;       // [2 CTAs][row_cap][2]: bound on the maximum (log2 units), sum
+  float* acc;      // [2 CTAs][row_cap][d]
+  int row_cap;
+};
+
+// ------------------------------------------------------------------ shared memory
+template <int D>
+struct Cfg {
+  static constexpr int kHalves = D / 64;                    // 128-byte wide halves of a row
+  static constexpr uint32_t kHalfBytes = 128 * 128;         // 128 rows x 128 bytes
+  static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;
+  static constexpr int kSlots = D == 128 ? 5 : 8;           // ring of K and V tiles
+  static constexpr uint32_t kQ = 0;                         // two tiles of queries
+  static constexpr uint32_t kRing = 2 * kTileBytes;
+  static constexpr uint32_t kMisc = kRing + kSlots * kTileBytes;
+  static constexpr size_t kSmem = 1024 + kMisc + 768;
+};
+
+constexpr int kThreads = 384;
+constexpr uint32_t kTmemCols = 512;
+constexpr uint32_t kColO = 256;  // S_0, S_1 at columns 0 and 128, O_0, O_1 at 256 and 384
+
+struct Barriers {
+  uint64_t full[8], empty[8];  // ring slots
+  uint64_t qready[2];          // queries of group t written
+  uint64_t sfull[2];           // S_t computed (and the O_t of the step before)
+  uint64_t pready[2];          // P_t written, O_t rescaled
+  uint64_t ofull[2];           // last P V of group t in a block done
+  uint64_t drained;
+};
+struct Misc {
+  Barriers bar;
+  int64_t red[33];
+  Part part;
+  uint32_t tmem;
+  int err;
+  unsigned bad;  // rows of a 32-row block that came out as NaN
+};
+static_assert(sizeof(Misc) <= 768, "miscellaneous shared memory");
+
+// exp2 of the arguments that a softmax makes: 0 below the normal numbers.
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+
+template <typename T>
+struct Weights;
+template <>
+struct Weights<__nv_bfloat16> {
+  static constexpr float kBias = 0.f, kSlack = 8.f;
+  static constexpr uint32_t kFormat = 1;
+};
+template <>
+struct Weights<__half> {
+  static constexpr float kBias = 8.f, kSlack = 6.f;
+  static constexpr uint32_t kFormat = 0;
+};
+// Instruction descriptor: D fp32, A and B of type T, shape 128 x n; B MN-major if `bt`.
+template <typename T>
+constexpr uint32_t idesc(int n, bool bt) {
+  return (1u << 4) | (Weights<T>::kFormat << 7) | (Weights<T>::kFormat << 10) | (bt ? 1u << 16 : 0u) |
+         (static_cast<uint32_t>(n >> 3) << 17) | (128u >> 4 << 24);
+}
+
+// Steps of an item: step k belongs to group k & 1.
+struct Steps {
+  bool wide;  // over 128 rows: both groups use every tile
+  int nt;     // tiles
+  __device__ __forceinline__ Steps(const Item& it) : wide(it.rows > 128), nt(it.t1 - it.t0) {}
+  __device__ __forceinline__ int count() const { return wide ? 2 * nt : nt; }
+  __device__ __forceinline__ int tile(int k) const { return wide ? k >> 1 : k; }
+  // Place of tile j's K and V in the ring's order of loads: the order of first use.
+  __device__ __forceinline__ int k_at(int j) const { return wide ? 2 * j : (j == 0 ? 0 : 2 * j - 1); }
+  __device__ __forceinline__ int v_at(int j) const { return wide ? 2 * j + 1 : (j + 1 < nt ? 2 * j + 2 : 2 * nt - 1); }
+  // The inverse: the i-th load is K (even result) or V (odd) of tile result / 2.
+  __device__ __forceinline__ int load(int i) const {
+    if (wide || i == 0) return i;
+    if (i == 2 * nt - 1) return 2 * (nt - 1) + 1;
+    return i & 1 ? i + 1 : i - 1;
+  }
+};
+
 template <typename T, int D>
-void launch(const AttnArgs& a, cudaStream_t s) {
-  const int64_t items = static_cast<int64_t>(a.rows) * a.hq;
-  launch_pdl(attention_simple_kernel<T, D>, dim3(static_cast<unsigned>((items + 3) / 4)), dim3(128), 0, s, 1, a);
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                     const __grid_constant__ AttnArgs a, const Workspace ws, int group, int box, float q_sign, float scale_log2) {
+  using C = Cfg<D>;
+  constexpr int kSlots = C::kSlots;
+  extern __shared__ __align__(1024) uint8_t attention_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(attention_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + C::kRing;
+  Misc& misc = *reinterpret_cast<Misc*>(smem + C::kMisc);
+  Barriers& bar = misc.bar;
+  volatile int* s_err = &misc.err;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  PartDesc* desc = ws.desc + 2 * blockIdx.x;  // thread 0 writes them
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kSlots; ++i) {
+      sm100::mbar_init(&bar.full[i], 1);
+      sm100::mbar_init(&bar.empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      sm100::mbar_init(&bar.qready[i], 4);
+      sm100::mbar_init(&bar.sfull[i], 1);
+      sm100::mbar_init(&bar.pready[i], 4);
+      sm100::mbar_init(&bar.ofull[i], 1);
+    }
+    sm100::mbar_init(&bar.drained, 1);
+    misc.err = 0;
+    misc.bad = 0;
+    sm100::fence_barrier_init();
+    sm100::prefetch_tmap(&tk);
+    sm100::prefetch_tmap(&tv);
+  }
+  if (warp == 9) {
+    sm100::tmem_alloc(&misc.tmem, kTmemCols);
+    sm100::tmem_relinquish();
+  }
+  pdl_wait();  // lengths, offsets, pages, queries and the cache may come from the kernel before
+  pdl_trigger();
+  if (threadIdx.x == 0) desc[0].used = desc[1].used = 0;
+  find_part<kThreads>(a, group, misc.red, &misc.part);
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = misc.tmem;
+  // A wait that does nothing once any role of the CTA has given up.
+  auto wait = [&](uint64_t* b, uint32_t parity) {
+    if (*s_err) return;
+    if (!sm100::mbar_wait(b, parity)) *s_err = 1;
+  };
+  Walk walk;
+  walk.start(a, group, misc.part);
+  Item it;
+
+  if (warp == 8) {
+    // ------------------------------------------------------------ TMA producer
+    const int boxes = kTile / box;           // page runs of a tile
+    unsigned count = 0;                      // loads issued so far
+    while (walk.next(a, group, it)) {
+      if (__any_sync(0xffffffffu, *s_err)) break;
+      const Steps st(it);
+      if (it.over && lane == 0) atomicExch(a.err, kErrPage);
+      for (int i = 0; i < 2 * st.nt; ++i, ++count) {
+        const int load = st.load(i);
+        const int c0 = (it.tile0 + it.t0 + (load >> 1)) * kTile;
+        // Page and slot of this lane's run (lane % boxes), looked up before the slot is free.
+        const int run = lane % boxes, pos = c0 + run * box;
+        int page = a.num_pages, slot = 0;  // outside the pool: zeros
+        if (pos + box > it.begin && pos < it.end) {
+          page = page_of(a.batch, it.s, pos / a.page_size, a.num_pages);
+          slot = pos % a.page_size;
+          if (page < 0) {
+            atomicExch(a.err, kErrPage);
+            page = a.num_pages;
+          }
+        }
+        const int sl = count % kSlots;
+        wait(&bar.empty[sl], ((count / kSlots) & 1u) ^ 1u);
+        if (__any_sync(0xffffffffu, *s_err)) break;
+        if (lane == 0) sm100::mbar_arrive_expect_tx(&bar.full[sl], C::kTileBytes);
+        __syncwarp();
+        uint8_t* dst = ring + sl * C::kTileBytes + run * box * 128;
+        for (int j = lane; j < boxes * C::kHalves; j += 32)  // 32 lanes are a multiple of the runs
+          sm100::tma_load_4d(dst + (j / boxes) * C::kHalfBytes, load & 1 ? &tv : &tk, &bar.full[sl],
+                             (j / boxes) * 64, it.h, slot, page);
+        __syncwarp();
+      }
+    }
+    // Never leave while a copy into this CTA's shared memory is in flight.
+    if (lane == 0)
+      for (unsigned i = count > kSlots ? count - kSlots : 0; i < count; ++i)
+        sm100::mbar_wait(&bar.full[i % kSlots], (i / kSlots) & 1u);
+  } else if (warp == 9) {
+    // ------------------------------------------------------------ MMA issue
+    if (sm100::elect_one()) {
+      unsigned base = 0;                   // loads of the items before
+      unsigned nq[2] = {0, 0}, np[2] = {0, 0};
+      auto slot_of = [&](int i) { return (base + i) % kSlots; };
+      auto phase_of = [&](int i) { return ((base + i) / kSlots) & 1u; };
+      while (walk.next(a, group, it) && !*s_err) {
+        const Steps st(it);
+        const int steps = st.count();
+        wait(&bar.qready[0], nq[0]++ & 1u);
+        if (st.wide) wait(&bar.qready[1], nq[1]++ & 1u);
+        auto scores = [&](int k) {
+          const int t = k & 1, at = st.k_at(st.tile(k));
+          wait(&bar.full[slot_of(at)], phase_of(at));
+          sm100::tc_fence_after();
+          const uint8_t* qt = smem + C::kQ + (st.wide ? t : 0) * C::kTileBytes;
+          const uint8_t* kt = ring + slot_of(at) * C::kTileBytes;
+#pragma unroll
+          for (int i = 0; i < D / 16; ++i) {
+            const uint64_t da = sm100::smem_desc_sw128(qt + (i >> 2) * C::kHalfBytes) + 2 * (i & 3);
+            const uint64_t db = sm100::smem_desc_sw128(kt + (i >> 2) * C::kHalfBytes) + 2 * (i & 3);
+            sm100::mma_bf16(tmem + t * 128, da, db, idesc<T>(128, false), i > 0 ? 1u : 0u);
+          }
+          sm100::mma_commit(&bar.sfull[t]);
+          if (!st.wide || t == 1) sm100::mma_commit(&bar.empty[slot_of(at)]);
+        };
+        scores(0);
+        if (steps > 1) scores(1);
+        for (int k = 0; k < steps && !*s_err; ++k) {
+          const int t = k & 1, at = st.v_at(st.tile(k));
+          wait(&bar.full[slot_of(at)], phase_of(at));
+          wait(&bar.pready[t], np[t]++ & 1u);
+          sm100::tc_fence_after();
+          const uint8_t* vt = ring + slot_of(at) * C::kTileBytes;
+#pragma unroll
+          for (int i = 0; i < kTile / 16; ++i)  // 16 tokens: 2048 bytes further in V, 8 columns in P
+            sm100::mma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + i * 8,
+                              sm100::smem_desc_mn_sw128(vt + i * 2048, C::kHalfBytes, 1024), idesc<T>(D, true),
+                              (k > 1 || i > 0) ? 1u : 0u);
+          if (!st.wide || t == 1) sm100::mma_commit(&bar.empty[slot_of(at)]);
+          if (k + 2 < steps)
+            scores(k + 2);
+          else
+            sm100::mma_commit(&bar.ofull[t]);
+        }
+        base += 2 * st.nt;
+      }
+      // Tensor memory is freed only after every product is done.
+      sm100::mma_commit(&bar.drained);
+      if (!sm100::mbar_wait(&bar.drained, 0)) *s_err = 1;
+    }
+    __syncwarp();
+  } else if (warp < 8) {
+    // ------------------------------------------------------------ softmax
+    const int t = warp >> 2, w4 = warp & 3;
+    const int row = w4 * 32 + lane;  // row of the group's tile
+    const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
+    const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + kColO + t * 128;
+    unsigned ns = 0, no = 0, base = 0;  // steps, blocks ends and loads so far
+    bool have = walk.next(a, group, it);
+    bool q_loaded = false;
+
+    // Writes the queries of an item into this group's tile (or, with at most
+    // 128 rows, group 0 into its own).
+    auto load_q = [&](const Item& i) {
+      const bool wide = i.rows > 128;
+      if (!wide && t == 1) return;
+      const int r = wide ? t * 128 + row : (i.rows <= 32 ? lane : row);
+      uint8_t* dst = smem + C::kQ + t * C::kTileBytes + row * 128;
+      const bool valid = r < i.rows;
+      const int tok = (i.row0 + r) / group, g = (i.row0 + r) % group;
+      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (i.q0 + tok) * a.q_tok +
+                                                        (i.h * group + g) * a.q_head);
+#pragma unroll
+      for (int c = 0; c < D / 8; ++c) {
+        uint4 v = valid ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+        if (q_sign != 1.f) {  // a negative or zero scale moves into the queries
+          uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float2 f = to_float2<T>(u[e]);
+            u[e] = pack2<T>(f.x * q_sign, f.y * q_sign);
+          }
+        }
+        *reinterpret_cast<uint4*>(dst + (c >> 3) * C::kHalfBytes + (((c & 7) ^ (row & 7)) << 4)) = v;
+      }
+      sm100::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&bar.qready[t]);
+    };
+
+    while (have) {
+      const Steps st(it);
+      const int steps = st.count();
+      const bool wide = st.wide, quad = it.rows <= 32;
+      if (!q_loaded) load_q(it);
+      q_loaded = false;
+      // This thread's row of the block and what it sees.
+      const int r = wide ? t * 128 + row : (quad ? lane : row);
+      const bool valid = r < it.rows;
+      const int rr = it.row0 + min(r, it.rows - 1);
+      const int pos = it.len - it.n + rr / group;
+      const int hi = valid ? (a.causal ? pos + 1 : it.len) : 0;
+      const int lo = a.window > 0 ? pos - a.window + 1 : 0;
+      // What every valid row of the warp sees.
+      const bool idle = __all_sync(0xffffffffu, !valid);
+      const int hi_all = __reduce_min_sync(0xffffffffu, valid ? hi : 0x7fffffff);
+      const int lo_all = __reduce_max_sync(0xffffffffu, valid ? lo : -0x7fffffff);
+
+      float m = -INFINITY, l = 0.f;  // bound on the maximum, in units of S; sum of P
+      int mine = 0;                  // steps of this group
+      for (int k = t; k < steps; k += 2, ++mine) {
+        const int j = st.tile(k);
+        const int c0 = (it.tile0 + it.t0 + j) * kTile;
+        wait(&bar.sfull[t], ns++ & 1u);
+        sm100::tc_fence_after();
+        if (!idle) {
+          // Columns of this thread: all, or the warp's quarter.
+          auto softmax = [&](auto cols_tag, auto masked_tag) {
+            constexpr int kCols = decltype(cols_tag)::value;
+            constexpr bool kMasked = decltype(masked_tag)::value;
+            const int first = kCols == 128 ? 0 : w4 * 32;
+            uint32_t x[kCols];
+#pragma unroll
+            for (int c = 0; c < kCols; c += 32) sm100::tmem_ld_32x32b_x32(tS + first + c, x + c);
+            sm100::tmem_ld_wait();
+            if constexpr (kMasked) {
+              const int from = lo - c0 - first, to = hi - c0 - first;
+#pragma unroll
+              for (int c = 0; c < kCols; ++c)
+                if (c < from || c >= to) x[c] = 0xff800000u;  // -inf
+            }
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int c = 0; c < kCols; c += 4)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) mx[e] = fmaxf(mx[e], __uint_as_float(x[c + e]));
+            const float top = fmaxf(m, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+            // -inf minus -inf is NaN, which is not above the slack: such a row keeps its bound.
+            if (__any_sync(0xffffffffu, (top - m) * scale_log2 > Weights<T>::kSlack)) {
+              const float f = m == -INFINITY ? 0.f : fast_exp2((m - top) * scale_log2);
+              m = top;
+              l *= f;
+              if (mine > 0) {
+#pragma unroll
+                for (int c = 0; c < D; c += 32) {
+                  uint32_t o[32];
+                  sm100::tmem_ld_32x32b_x32(tO + c, o);
+                  sm100::tmem_ld_wait();
+#pragma unroll
+                  for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+                  sm100::tmem_st_32x32b_x32(tO + c, o);
+                }
+                sm100::tmem_st_wait();
+              }
+            }
+            const float shift = m == -INFINITY ? 0.f : Weights<T>::kBias - m * scale_log2;
+            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c = 0; c < kCols; c += 32) {
+              uint32_t p[16];
+#pragma unroll
+              for (int e = 0; e < 32; e += 2) {
+                const float p0 = fast_exp2(fmaf(__uint_as_float(x[c + e]), scale_log2, shift));
+                const float p1 = fast_exp2(fmaf(__uint_as_float(x[c + e + 1]), scale_log2, shift));
+                sum[e & 2] += p0;
+                sum[(e & 2) + 1] += p1;
+                p[e / 2] = pack2<T>(p0, p1);
+              }
+              sm100::tmem_st_32x32b_x16(tS + (first + c) / 2, p);
+            }
+            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            if constexpr (kCols < 128) {
+              // The other quarters' tokens have no weight in this warp's rows.
+              const uint32_t zero[16] = {};
+#pragma unroll
+              for (int q = 1; q < 4; ++q) sm100::tmem_st_32x32b_x16(tS + ((w4 + q) & 3) * 16, zero);
+            }
+            sm100::tmem_st_wait();
+          };
+          using Yes = std::integral_constant<bool, true>;
+          using No = std::integral_constant<bool, false>;
+          if (quad) {
+            softmax(std::integral_constant<int, 32>{}, Yes{});
+          } else if (c0 >= lo_all && c0 + kTile <= hi_all) {
+            softmax(std::integral_constant<int, 128>{}, No{});
+          } else {
+            softmax(std::integral_constant<int, 128>{}, Yes{});
+          }
+        }
+        // Tokens behind the sequence and before every row's window may hold anything: zeros in V, since
+        // zero times NaN is NaN.
+        if (c0 + kTile > it.len || c0 < it.begin) {
+          const unsigned at = base + st.v_at(j);
+          wait(&bar.full[at % kSlots], (at / kSlots) & 1u);
+          if (c0 + row >= it.len || c0 + row < it.begin) {
+            uint8_t* vt = ring + (at % kSlots) * C::kTileBytes + row * 128;
+#pragma unroll
+            for (int c = 0; c < 8 * C::kHalves; ++c)
+              *reinterpret_cast<uint4*>(vt + (c >> 3) * C::kHalfBytes + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          sm100::fence_proxy_async_smem();
+        }
+        sm100::tc_fence_before();
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&bar.pready[t]);
+      }
+      base += 2 * st.nt;
+
+      // ---------------------------------------------------------- end of the block's part
+      Item next = it;
+      const bool more = walk.next(a, group, next);
+      if (more && wide) {  // this group's last S is done: its queries are free
+        load_q(next);
+        q_loaded = true;
+      }
+      if (mine > 0) {
+        wait(&bar.ofull[t], no++ & 1u);
+        sm100::tc_fence_after();
+      }
+      const bool whole = it.whole();
+      // The first item of a CTA may continue a block, the last may leave one; one that does both is the first.
+      const int which = it.t0 > 0 ? 0 : 1, slot = 2 * blockIdx.x + which;
+      float* acc = ws.acc + static_cast<int64_t>(slot) * ws.row_cap * D;
+      float* ml = ws.ml + static_cast<int64_t>(slot) * ws.row_cap * 2;
+      if (!whole && threadIdx.x == 0) desc[which] = PartDesc{it.s, it.h, it.b, it.rows, it.t0, it.t1, it.tiles, 1};
+      auto out_of = [&](int r2) {
+        const int x = it.row0 + r2;
+        return static_cast<T*>(a.out) + (it.q0 + x / group) * a.o_tok + (it.h * group + x % group) * a.o_head;
+      };
+      auto again = [&](int r2) {  // row r2 of the block by this warp
+        const int x = it.row0 + r2;
+        attention_row<T, D>(a, it.s, it.q0 + x / group, it.len - it.n + x / group, it.len, it.h * group + x % group,
+                            it.h);
+      };
+      // Stores 32 columns of a row: rounded with the factor inv, or as fp32 to the workspace.
+      auto store32 = [&](int r2, int c, const float* o, float inv, float& odd) {
+        if (whole) {
+          uint4* dst = reinterpret_cast<uint4*>(out_of(r2) + c);
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              y[i] = inv == 0.f ? 0.f : o[e + i] * inv;
+              odd += y[i] * 0.f;  // NaN if any is not finite
+            }
+            dst[e / 8] = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]),
+                                    pack2<T>(y[6], y[7]));
+          }
+        } else {
+          float4* dst = reinterpret_cast<float4*>(acc + static_cast<int64_t>(r2) * D + c);
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) dst[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        }
+      };
+      const float m2 = m == -INFINITY ? -INFINITY : m * scale_log2;
+
+      if (wide) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        float odd = 0.f;
+        if (!idle) {
+#pragma unroll 1
+          for (int c = 0; c < D; c += 32) {
+            uint32_t o[32];
+            sm100::tmem_ld_32x32b_x32(tO + c, o);
+            sm100::tmem_ld_wait();
+            if (valid) store32(r, c, reinterpret_cast<const float*>(o), inv, odd);
+          }
+          if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(m2, l);
+          unsigned redo = __ballot_sync(0xffffffffu, whole && valid && odd != 0.f);
+          for (; redo; redo &= redo - 1) again(t * 128 + w4 * 32 + __ffs(redo) - 1);
+        }
+      } else {
+        // Join the states of each row through shared memory that the queries held.
+        float2* sml = reinterpret_cast<float2*>(smem + C::kQ);
+        float* buf = reinterpret_cast<float*>(smem + C::kQ + C::kTileBytes);
+        constexpr int kBuf = C::kTileBytes / 4;
+        group_sync();  // every S of the block is done in both groups
+        sml[t * 128 + row] = make_float2(m2, l);
+        group_sync();
+        const int states = quad ? 8 : 2;
+        float mj = -INFINITY, lj = 0.f;
+        for (int i = 0; i < states; ++i) mj = fmaxf(mj, sml[quad ? i * 32 + lane : i * 128 + row].x);
+        auto factor = [&](float mm) { return mm == -INFINITY ? 0.f : fast_exp2(mm - mj); };
+        for (int i = 0; i < states; ++i) {
+          const float2 v = sml[quad ? i * 32 + lane : i * 128 + row];
+          lj += v.y * factor(v.x);
+        }
+        const float f = factor(m2);
+        if (!quad) {
+          const float inv = lj == 0.f ? 0.f : 1.f / lj;
+          float odd = 0.f;
+          // Group 1 hands over half of its columns at a time; its float4 c sits at place c ^ (row & 7).
+          constexpr int kPass = kBuf / 128;
+          const bool two = steps > 1;  // group 1 had a tile
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += kPass) {
+            if (c0) group_sync();
+            if (t == 1 && two && !idle) {
+#pragma unroll 1
+              for (int c = 0; c < kPass; c += 32) {
+                uint32_t o[32];
+                sm100::tmem_ld_32x32b_x32(tO + c0 + c, o);
+                sm100::tmem_ld_wait();
+                float4* dst = reinterpret_cast<float4*>(buf + row * kPass);
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                  dst[(c / 4 + e) ^ (row & 7)] =
+                      make_float4(__uint_as_float(o[4 * e]) * f, __uint_as_float(o[4 * e + 1]) * f,
+                                  __uint_as_float(o[4 * e + 2]) * f, __uint_as_float(o[4 * e + 3]) * f);
+              }
+            }
+            group_sync();
+            if (t == 0 && !idle) {
+#pragma unroll 1
+              for (int c = 0; c < kPass; c += 32) {
+                uint32_t o[32];
+                sm100::tmem_ld_32x32b_x32(tO + c0 + c, o);
+                sm100::tmem_ld_wait();
+                float y[32];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                  float4 other = make_float4(0.f, 0.f, 0.f, 0.f);
+                  if (two) other = reinterpret_cast<const float4*>(buf + row * kPass)[(c / 4 + e) ^ (row & 7)];
+                  y[4 * e] = __uint_as_float(o[4 * e]) * f + other.x;
+                  y[4 * e + 1] = __uint_as_float(o[4 * e + 1]) * f + other.y;
+                  y[4 * e + 2] = __uint_as_float(o[4 * e + 2]) * f + other.z;
+                  y[4 * e + 3] = __uint_as_float(o[4 * e + 3]) * f + other.w;
+                }
+                if (valid) store32(r, c0 + c, y, inv, odd);
+              }
+            }
+          }
+          if (t == 0 && !idle) {
+            if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
+            unsigned redo = __ballot_sync(0xffffffffu, whole && valid && odd != 0.f);
+            for (; redo; redo &= redo - 1) again(w4 * 32 + __ffs(redo) - 1);
+          }
+        } else {
+          // Eight states a row. A pass takes as many columns as fit: state-row i * rows + r, float4 c at
+          // place c ^ (r & 7); then a thread adds the states of four columns of a row.
+          int pass = D;
+          while (8 * it.rows * pass > kBuf) pass /= 2;  // 32 rows: D / 4 columns
+          const int state = t * 4 + w4;
+#pragma unroll 1
+          for (int c0 = 0; c0 < D; c0 += pass) {
+            if (c0) group_sync();
+#pragma unroll 1
+            for (int c = 0; c < pass; c += 16) {
+              uint32_t o[16];
+              sm100::tmem_ld_32x32b_x16(tO + c0 + c, o);
+              sm100::tmem_ld_wait();
+              if (valid) {
+                float4* dst = reinterpret_cast<float4*>(buf + (state * it.rows + r) * pass);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const float4 v = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
+                                               __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
+                  // A state that saw nothing holds no numbers yet, or zeros times whatever V holds.
+                  dst[(c / 4 + e) ^ (r & 3)] = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
+                                                        : make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
+                }
+              }
+            }
+            group_sync();
+            for (int i = threadIdx.x; i < it.rows * (pass / 4); i += 256) {
+              const int r2 = i / (pass / 4), c = i % (pass / 4);
+              float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+              float mr = -INFINITY, lr = 0.f;
+              for (int q = 0; q < 8; ++q) mr = fmaxf(mr, sml[q * 32 + r2].x);
+#pragma unroll
+              for (int q = 0; q < 8; ++q) {
+                const float4 v = reinterpret_cast<const float4*>(buf + (q * it.rows + r2) * pass)[c ^ (r2 & 3)];
+                y.x += v.x;
+                y.y += v.y;
+                y.z += v.z;
+                y.w += v.w;
+                const float2 s = sml[q * 32 + r2];
+                lr += s.x == -INFINITY ? 0.f : s.y * fast_exp2(s.x - mr);
+              }
+              if (whole) {
+                const float inv = lr == 0.f ? 0.f : 1.f / lr;
+                if (inv == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
+                y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+                if ((y.x + y.y + y.z + y.w) * 0.f != 0.f) atomicOr(&misc.bad, 1u << r2);
+                *reinterpret_cast<uint2*>(out_of(r2) + c0 + 4 * c) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+              } else {
+                *reinterpret_cast<float4*>(acc + static_cast<int64_t>(r2) * D + c0 + 4 * c) = y;
+                if (c0 == 0 && c == 0) *reinterpret_cast<float2*>(ml + r2 * 2) = make_float2(mr, lr);
+              }
+            }
+          }
+          group_sync();
+          const unsigned bad = *reinterpret_cast<volatile unsigned*>(&misc.bad);
+          if (bad) {
+            for (int r2 = warp; r2 < it.rows; r2 += 8)
+              if (bad >> r2 & 1u) again(r2);
+            group_sync();
+            if (threadIdx.x == 0) misc.bad = 0;
+          }
+        }
+        group_sync();  // the queries' memory is free again
+      }
+      sm100::tc_fence_before();
+      it = next;
+      have = more;
+    }
+  }
+
+  sm100::tc_fence_before();
+  __syncthreads();
+  if (warp == 9) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, kTmemCols);
+  }
+  if (threadIdx.x == 0 && *s_err) atomicExch(a.err, kErrTimeout);
+}
+
+// ------------------------------------------------------------------ merge
+// Joins the parts of the blocks that a cut fell into. Grid (CTAs of the
+// attention kernel, row groups); the CTA whose part starts such a block owns it.
+// Parts are added in the order of the tiles, so results do not depend on timing.
+constexpr int kMergeThreads = 256;
+constexpr int kMergeGroups = 8;
+constexpr int kMaxParts = 1024;
+
+template <typename T, int D>
+__global__ void __launch_bounds__(kMergeThreads)
+    merge_kernel(const __grid_constant__ AttnArgs a, const Workspace ws, int group, int ctas) {
+  __shared__ int part[kMaxParts];
+  __shared__ int parts;
+  pdl_wait();
+  pdl_trigger();
+  const PartDesc first = ws.desc[2 * blockIdx.x + 1];
+  if (!first.used || first.t1 == first.tiles) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (warp == 0) {
+    // Continuations follow in the order of the CTAs; one that reaches the last tile is the last.
+    int n = 1;
+    if (lane == 0) part[0] = 2 * blockIdx.x + 1;
+    for (int c0 = blockIdx.x + 1; c0 < ctas; c0 += 32) {
+      const int c = c0 + lane;
+      PartDesc d{};
+      if (c < ctas) d = ws.desc[2 * c];
+      const bool on = d.used && d.s == first.s && d.h == first.h && d.b == first.b;
+      const unsigned who = __ballot_sync(0xffffffffu, on);
+      if (on) part[n + __popc(who & ((1u << lane) - 1u))] = 2 * c;
+      n += __popc(who);
+      if (__any_sync(0xffffffffu, on && d.t1 == d.tiles)) break;
+    }
+    if (lane == 0) parts = n;
+  }
+  __syncthreads();
+  const int n = parts;
+  const int q0 = q_begin(a.batch, first.s), cnt = q_begin(a.batch, first.s + 1) - q0;
+  const int len = __ldg(a.batch.kv_len + first.s);
+  for (int r = blockIdx.y * (kMergeThreads / 32) + warp; r < first.rows; r += kMergeGroups * (kMergeThreads / 32)) {
+    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < n; ++i) m = fmaxf(m, __ldcg(ws.ml + (static_cast<int64_t>(part[i]) * ws.row_cap + r) * 2));
+    float o[D / 32] = {};
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const int64_t at = static_cast<int64_t>(part[i]) * ws.row_cap + r;
+      const float2 v = __ldcg(reinterpret_cast<const float2*>(ws.ml + at * 2));
+      const float f = v.x == -INFINITY ? 0.f : fast_exp2(v.x - m);
+      l += v.y * f;
+      if constexpr (D == 128) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(ws.acc + at * D) + lane);
+        if (f != 0.f) o[0] += x.x * f, o[1] += x.y * f, o[2] += x.z * f, o[3] += x.w * f;
+      } else {
+        const float2 x = __ldcg(reinterpret_cast<const float2*>(ws.acc + at * D) + lane);
+        if (f != 0.f) o[0] += x.x * f, o[1] += x.y * f;
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    float odd = 0.f;
+#pragma unroll
+    for (int e = 0; e < D / 32; ++e) {
+      o[e] = inv == 0.f ? 0.f : o[e] * inv;
+      odd += o[e] * 0.f;
+    }
+    const int x = first.b * kBlock + r, tok = x / group, h = first.h * group + x % group;
+    if (__any_sync(0xffffffffu, odd != 0.f)) {
+      attention_row<T, D>(a, first.s, q0 + tok, len - cnt + tok, len, h, first.h);
+      continue;
+    }
+    T* dst = static_cast<T*>(a.out) + (q0 + tok) * a.o_tok + h * a.o_head;
+    if constexpr (D == 128)
+      *reinterpret_cast<uint2*>(dst + lane * 4) = make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
+    else
+      *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack2<T>(o[0], o[1]);
+  }
+}
+
+// ------------------------------------------------------------------ host side
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode() {
+  static EncodeFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    B200AR_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q));
+    if (q != cudaDriverEntryPointSuccess || !ptr) throw std::runtime_error("cuTensorMapEncodeTiled unavailable");
+    return reinterpret_cast<EncodeFn>(ptr);
+  }();
+  return fn;
+}
+
+// 4-D map over a pool [pages, page_size, kv_heads, d] with its strides; box of
+// 64 dims x 1 head x `box` tokens x 1 page, 128-byte swizzle.
+CUtensorMap pool_map(const Pool& p, int d, int hkv, int page_size, int num_pages, int box, Half type) {
+  CUtensorMap m;
+  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(hkv),
+                              static_cast<cuuint64_t>(page_size), static_cast<cuuint64_t>(num_pages)};
+  // The stride of a dimension of one is never used; any valid one serves.
+  const auto bytes = [](int64_t n, int64_t stride) { return static_cast<cuuint64_t>(n == 1 ? 16 : stride * 2); };
+  const cuuint64_t strides[3] = {bytes(hkv, p.head), bytes(page_size, p.tok), bytes(num_pages, p.page)};
+  const cuuint32_t boxes[4] = {64, 1, static_cast<cuuint32_t>(box), 1};
+  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const CUresult r = encode()(
+      &m, type == Half::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, p.base, dims,
+      strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+      CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled (paged cache) failed: " + std::to_string(r));
+  return m;
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  B200AR_CUDA(cudaGetDevice(&dev));
+  B200AR_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+  return std::min(n, kMaxParts);
+}
+
+int row_cap(int64_t rows, int group) { return static_cast<int>(std::min<int64_t>(kBlock, rows * group)); }
+
+template <typename T, int D>
+void launch(const AttnArgs& a, Half type, float* workspace, cudaStream_t s) {
+  const int group = a.hq / a.hkv, ctas = sm_count();
+  int box = kTile;
+  while (a.page_size % box) box /= 2;
+  const CUtensorMap tk = pool_map(a.k, D, a.hkv, a.page_size, a.num_pages, box, type);
+  const CUtensorMap tv = pool_map(a.v, D, a.hkv, a.page_size, a.num_pages, box, type);
+  Workspace ws{};
+  ws.row_cap = row_cap(a.rows, group);
+  ws.desc = reinterpret_cast<PartDesc*>(workspace);
+  ws.ml = workspace + 2ll * ctas * (sizeof(PartDesc) / 4);
+  ws.acc = ws.ml + 2ll * ctas * ws.row_cap * 2;
+  auto kern = attention_kernel<T, D>;
+  static PerDeviceOnce attr;
+  attr([&] {
+    B200AR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     static_cast<int>(Cfg<D>::kSmem)));
+  });
+  const float sign = a.scale > 0.f ? 1.f : (a.scale < 0.f ? -1.f : 0.f);
+  const float scale_log2 = (sign == 0.f ? 1.f : a.scale * sign) * kLog2e;
+  launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), Cfg<D>::kSmem, s, 1, tk, tv, a, ws, group, box,
+             sign, scale_log2);
+  launch_pdl(merge_kernel<T, D>, dim3(static_cast<unsigned>(ctas), kMergeGroups), dim3(kMergeThreads), 0, s, 1, a, ws,
+             group, ctas);
 }
 
 }  // namespace
 
-void paged_attention(const AttnArgs& a, int d, Half type, cudaStream_t s) {
+int64_t paged_attention_workspace(int64_t rows, int hq, int hkv, int d) {
+  const int64_t ctas = sm_count(), cap = row_cap(rows, hq / hkv);
+  return 2 * ctas * (static_cast<int64_t>(sizeof(PartDesc)) / 4 + cap * (2 + d));
+}
+
+void paged_attention(const AttnArgs& a, int d, Half type, float* workspace, cudaStream_t s) {
   const TraceRange trace("b200ar::paged_attention");
   B200AR_CHECK(d == 64 || d == 128, "paged_attention is built for heads of 64 and 128");
+  B200AR_CHECK(a.page_size % 8 == 0, "the page size must be a multiple of 8");
+  B200AR_CHECK(static_cast<int64_t>(a.rows) * (a.hq / a.hkv) < (1ll << 31), "too many rows");
   if (a.rows == 0 || a.batch.seqs == 0) return;
   if (type == Half::kBf16)
-    d == 64 ? launch<__nv_bfloat16, 64>(a, s) : launch<__nv_bfloat16, 128>(a, s);
+    d == 64 ? launch<__nv_bfloat16, 64>(a, type, workspace, s) : launch<__nv_bfloat16, 128>(a, type, workspace, s);
   else
-    d == 64 ? launch<__half, 64>(a, s) : launch<__half, 128>(a, s);
+    d == 64 ? launch<__half, 64>(a, type, workspace, s) : launch<__half, 128>(a, type, workspace, s);
 }
 
 }  // namespace paged

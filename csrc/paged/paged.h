@@ -61,11 +61,15 @@ struct AttnArgs {
   Batch batch;
   int* err;
   int rows, hq, hkv, num_pages, page_size;
-  int window;  // positions that a row sees, its own included; 0: all
+  int capacity;  // positions of a row of the page table
+  int window;    // positions that a row sees, its own included; 0: all
   bool causal;
   float scale;
 };
-void paged_attention(const AttnArgs& a, int d, Half type, cudaStream_t s);
+// Floats of workspace for a call: partial results of the blocks that the
+// schedule cuts, and their descriptions. Not kept from call to call.
+int64_t paged_attention_workspace(int64_t rows, int hq, int hkv, int d);
+void paged_attention(const AttnArgs& a, int d, Half type, float* workspace, cudaStream_t s);
 
 }  // namespace paged
 }  // namespace b200ar

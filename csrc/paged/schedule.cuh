@@ -1,0 +1,207 @@
+// How the tiles of a paged attention call are given to CTAs, on the device.
+//
+// The new tokens of a sequence and the G query heads of a KV head are G n rows
+// that share keys and values (row r: token r / G, head r % G). A block is 256
+// such rows of one sequence and KV head; its work is the run of 128-token
+// tiles that some row sees. All blocks' tiles, in the order sequence, head,
+// block, tile, form one line, cut into equal parts, one for each CTA; a block
+// that a cut falls into is computed in parts and merged (merge_kernel).
+//
+// The line is measured in a weight that has a closed form and is near the
+// tiles' number: a block's tokens times G plus a constant for its start and
+// end. With causal rows it grows by the same step from block to block up to
+// the window's limit, so the position of any block is a short sum, and a CTA
+// finds its part from one scan over the sequences. Any weight gives a correct
+// cut: only the balance depends on it.
+#pragma once
+
+#include "batch.cuh"
+
+namespace b200ar {
+namespace paged {
+
+constexpr int kTile = 128;   // tokens of a K or V tile
+constexpr int kBlock = 256;  // rows of a block
+
+struct SeqWork {
+  int n, len, q0, blocks;
+  int64_t a, cap, head;  // weight of block 0, limit of a weight, weight of all blocks of one head
+  int step;              // growth from block to block
+
+  __device__ __forceinline__ void load(const AttnArgs& p, int group, int s) {
+    q0 = q_begin(p.batch, s);
+    n = max(q_begin(p.batch, s + 1) - q0, 0);
+    len = __ldg(p.batch.kv_len + s);
+    blocks = static_cast<int>((static_cast<int64_t>(n) * group + kBlock - 1) / kBlock);
+    const int64_t g = group, fixed = kTile * g;
+    if (p.causal) {
+      a = g * max(len - n, 0) + kBlock + fixed;
+      step = kBlock;
+      cap = p.window > 0 ? g * p.window + kBlock + 2 * fixed : (1ll << 60);
+    } else {
+      a = g * max(len, 0) + fixed;
+      step = 0;
+      cap = 1ll << 60;
+    }
+    head = before(blocks);
+  }
+  __device__ __forceinline__ int64_t weight(int b) const {
+    return min(a + static_cast<int64_t>(step) * b, cap);
+  }
+  // Weight of the blocks before b.
+  __device__ __forceinline__ int64_t before(int b) const {
+    int64_t ramp = a >= cap ? 0 : b;
+    if (step > 0 && a < cap) ramp = min(ramp, (cap - a + step - 1) / step);
+    return a * ramp + step * (ramp * (ramp - 1) / 2) + (b - ramp) * (step > 0 || a >= cap ? cap : 0);
+  }
+};
+
+// A CTA's part of the line: from offset off0 of sequence s0 to offset off1 of s1.
+struct Part {
+  int64_t off0, off1;
+  int s0, s1;
+  int active;
+};
+
+// A part of a block: tiles [t0, t1) of its `tiles`, the first of which starts
+// at token 128 tile0.
+struct Item {
+  int s, h, b;
+  int n, len, q0;
+  int row0, rows;  // rows of the block among the sequence's G n
+  int pos0;        // position of the block's first row
+  int begin, end;  // positions that some row sees
+  int tile0, tiles, t0, t1;
+  bool over;       // some row sees positions behind the page table
+
+  __device__ __forceinline__ bool whole() const { return t1 - t0 == tiles; }
+};
+
+// Walks a CTA's items. Every role of the kernel walks them by itself.
+struct Walk {
+  Part part;
+  SeqWork w;
+  int s, h, b;
+  int64_t at;  // offset of block b of head h in its sequence
+
+  __device__ __forceinline__ void start(const AttnArgs& p, int group, const Part& pt) {
+    part = pt;
+    s = pt.s0;
+    if (!pt.active) return;
+    w.load(p, group, s);
+    h = static_cast<int>(pt.off0 / w.head);
+    const int64_t rest = pt.off0 - h * w.head;
+    int lo = 0, hi = w.blocks - 1;  // the last block with before(b) <= rest
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if (w.before(mid) <= rest)
+        lo = mid;
+      else
+        hi = mid - 1;
+    }
+    b = lo;
+    at = h * w.head + w.before(b);
+  }
+
+  __device__ __forceinline__ bool next(const AttnArgs& p, int group, Item& it) {
+    if (!part.active) return false;
+    for (;;) {
+      if (b >= w.blocks) {
+        b = 0;
+        if (w.blocks == 0 || ++h >= p.hkv) {
+          if (++s > part.s1) return false;
+          h = 0;
+          at = 0;
+          w.load(p, group, s);
+          if (w.blocks == 0) continue;
+        }
+      }
+      if (s > part.s1 || (s == part.s1 && at >= part.off1)) return false;
+      const int64_t weight = w.weight(b);
+      it.s = s;
+      it.h = h;
+      it.b = b;
+      it.n = w.n;
+      it.len = w.len;
+      it.q0 = w.q0;
+      it.row0 = b * kBlock;
+      it.rows = min(kBlock, w.n * group - it.row0);
+      const int i0 = it.row0 / group, i1 = (it.row0 + it.rows - 1) / group;
+      it.pos0 = w.len - w.n + i0;
+      const int last = w.len - w.n + i1;
+      it.begin = p.window > 0 ? max(0, it.pos0 - p.window + 1) : 0;
+      it.end = max(0, p.causal ? last + 1 : w.len);
+      it.over = it.end > p.capacity;
+      it.end = min(it.end, p.capacity);
+      it.tile0 = it.begin / kTile;
+      it.tiles = it.end > it.begin ? (it.end + kTile - 1) / kTile - it.tile0 : 1;
+      const int64_t x0 = s == part.s0 ? max(part.off0 - at, static_cast<int64_t>(0)) : 0;
+      const int64_t x1 = s == part.s1 ? min(part.off1 - at, weight) : weight;
+      it.t0 = static_cast<int>(x0 * it.tiles / weight);
+      it.t1 = static_cast<int>(x1 * it.tiles / weight);
+      at += weight;
+      ++b;
+      if (it.t0 < it.t1) return true;
+    }
+  }
+};
+
+// Finds the calling CTA's part. Called by all `kThreads` threads; `red` is
+// shared scratch of 33 int64. One CTA gets at least about one tile.
+template <int kThreads>
+__device__ __forceinline__ void find_part(const AttnArgs& p, int group, int64_t* red, Part* part) {
+  constexpr int kWarps = kThreads / 32;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int per = (p.batch.seqs + kThreads - 1) / kThreads;
+  const int lo = min(static_cast<int>(threadIdx.x) * per, p.batch.seqs), hi = min(lo + per, p.batch.seqs);
+  int64_t mine = 0;
+  SeqWork w;
+  for (int s = lo; s < hi; ++s) {
+    w.load(p, group, s);
+    mine += w.head * p.hkv;
+  }
+  int64_t inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  if (threadIdx.x == 0) part->active = 0;
+  if (lane == 31) red[warp] = inc;
+  __syncthreads();
+  int64_t base = 0, total = 0;
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    if (i < warp) base += red[i];
+    total += red[i];
+  }
+  // Every part holds the weight of one tile at least (its tokens and its block's constant).
+  const int64_t least = static_cast<int64_t>(kTile) * group;
+  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), max((total + least - 1) / least, static_cast<int64_t>(1)));
+  const int64_t c = blockIdx.x;
+  if (c < ctas && total > 0) {
+    // total is below 2^60 / 2^10: the products stay inside 64 bits for any batch that fits memory.
+    const int64_t x0 = total / ctas * c + total % ctas * c / ctas;
+    const int64_t x1 = total / ctas * (c + 1) + total % ctas * (c + 1) / ctas;
+    int64_t off = base + inc - mine;  // the line's position of sequence lo
+    if (mine > 0 && x1 > off && x0 < off + mine)
+      for (int s = lo; s < hi; ++s) {
+        w.load(p, group, s);
+        const int64_t size = w.head * p.hkv;
+        if (size > 0 && x0 >= off && x0 < off + size) {
+          part->s0 = s;
+          part->off0 = x0 - off;
+          part->active = 1;
+        }
+        if (size > 0 && x1 > off && x1 <= off + size) {
+          part->s1 = s;
+          part->off1 = x1 - off;
+        }
+        off += size;
+      }
+  }
+  __syncthreads();
+}
+
+}  // namespace paged
+}  // namespace b200ar

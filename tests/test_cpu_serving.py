@@ -141,7 +141,8 @@ def test_rope_refusals():
     bad = [dict(hq=5), dict(hkv=0), dict(qkv=a["qkv"][0]), dict(v_pages=a["v_pages"][1:]), dict(q_gamma=g),
            dict(q_gamma=g, k_gamma=g.float()), dict(q_gamma=g, k_gamma=g[:32]),
            dict(rot=RotaryTable(128, 8, 1e4, "cpu")), dict(q_out=own[:2]), dict(q_out=own.float()),
-           dict(q_out=a["qkv"][:, 64:320].view(3, 4, 64)), dict(q_out=torch.zeros(1, 4, 64).bfloat16().expand(3, 4, 64)),
+           dict(q_out=a["qkv"][:, 64:320].view(3, 4, 64)),
+           dict(q_out=torch.zeros(1, 4, 64).bfloat16().expand(3, 4, 64)),
            dict(batch=PagedBatch(a["batch"].page_table, a["batch"].kv_len)),
            dict(k_pages=a["k_pages"][:1].expand(5, 16, 2, 64), v_pages=a["v_pages"][:1].expand(5, 16, 2, 64))]
     for kw in bad:
@@ -168,7 +169,8 @@ def test_attention_refusals():
                dict(window=-1), dict(window=4, causal=False), dict(scale=float("nan")),
                dict(out=torch.zeros(3, 255).bfloat16()), dict(out=torch.zeros(3, 256)),
                dict(out=a["q"].view(3, 256)), dict(out=torch.zeros(1, 256).bfloat16().expand(3, 256)),
-               dict(batch=PagedBatch(a["batch"].page_table, a["batch"].kv_len))):
+               dict(batch=PagedBatch(a["batch"].page_table, a["batch"].kv_len)),
+               dict(k_pages=a["k_pages"][:, :12], v_pages=a["v_pages"][:, :12])):
         with pytest.raises(ValueError):
             call(**kw)
     with pytest.raises(TypeError):
@@ -181,7 +183,8 @@ def test_linear_fp8_refusals():
     x, w = torch.zeros(3, 32).bfloat16(), torch.zeros(16, 32).bfloat16()
     w_q, w_s = quantize_fp8_weight(w)
     x_q, x_s = quantize_fp8(x)
-    for f in (lambda: quantize_fp8(x[:, :20]), lambda: quantize_fp8_weight(w[0]), lambda: linear_fp8(x[:, :16], w_q, w_s),
+    for f in (lambda: quantize_fp8(x[:, :20]), lambda: quantize_fp8_weight(w[0]),
+              lambda: linear_fp8(x[:, :16], w_q, w_s),
               lambda: linear_fp8(x, w_q[:12], w_s), lambda: linear_fp8(x, w_q, w_s[:, :0]),
               lambda: linear_fp8(x, w_q, w_s.double()), lambda: linear_fp8(x, w_q, w_s, out=torch.zeros(3, 16)),
               lambda: linear_fp8(x, w_q, w_s, out=torch.zeros(3, 8).bfloat16()),

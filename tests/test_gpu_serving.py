@@ -175,8 +175,10 @@ def test_attention_graph_with_other_lengths(decode):
     from b200ar.ops.paged import PagedBatch, paged_attention
 
     hq, hkv, d, page, rows = 8, 2, 128, 16, 12
-    cases = [([1] * 12, [40 + 9 * i for i in range(12)]), ([1] * 12, [700 - 50 * i for i in range(12)])] if decode else \
-        [([3, 1, 0, 8], [30, 600, 9, 8]), ([1, 1, 1, 1], [1, 2, 3, 900]), ([9, 0, 1, 1], [700, 5, 1, 64])]
+    if decode:
+        cases = [([1] * 12, [40 + 9 * i for i in range(12)]), ([1] * 12, [700 - 50 * i for i in range(12)])]
+    else:
+        cases = [([3, 1, 0, 8], [30, 600, 9, 8]), ([1, 1, 1, 1], [1, 2, 3, 900]), ([9, 0, 1, 1], [700, 5, 1, 64])]
     seqs = len(cases[0][0])
     table = torch.full((seqs, 60), -1, dtype=torch.int32, device="cuda")
     lens = torch.zeros(seqs, dtype=torch.int32, device="cuda")
@@ -484,7 +486,8 @@ def test_linear_fp8_strides_and_views():
 
     w_q, w_s = quantize_fp8_weight(randn((264, 256), BF, "cuda", 2))
     base = randn((2, 50, 512), BF, "cuda", 1)
-    for x in (base[..., :256], base[..., 8:264], base[..., 3:259], base[:, ::2, :256], base[0, :, :256].t().contiguous().t()):
+    for x in (base[..., :256], base[..., 8:264], base[..., 3:259], base[:, ::2, :256],
+              base[0, :, :256].t().contiguous().t()):
         plain = x.contiguous().view(-1, 256)
         want = linear_fp8(plain, w_q, w_s)
         assert torch.equal(linear_fp8(x, w_q, w_s).view(-1, 264), want)
