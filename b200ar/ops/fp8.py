@@ -108,7 +108,6 @@ def linear_fp8(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor, out: O
         if x.dtype not in (torch.bfloat16, torch.float16):
             raise TypeError("x must be bfloat16 or float16, or codes with their x_scale")
         dtype = x.dtype
-        codes, scale = quantize_fp8(x)
     else:
         if x.dtype != torch.float8_e4m3fn:
             raise TypeError("with x_scale, x must be float8_e4m3fn")
@@ -117,24 +116,26 @@ def linear_fp8(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor, out: O
         if tuple(x_scale.shape) != (*x.shape[:-1], _blocks(k)) or x_scale.dtype != torch.float32 or \
                 x_scale.device != x.device:
             raise ValueError(f"x_scale must be fp32 [..., {_blocks(k)}] on {x.device}")
-        codes, scale = x, x_scale
-    codes = codes.reshape(-1, k).contiguous()
-    if codes.data_ptr() % 16:
-        codes = codes.clone()
-    m = codes.shape[0]
-    scale = scale.reshape(m, _blocks(k)).t()
-    if (m > 1 and scale.stride(1) != 1) or scale.stride(0) < m:
-        scale = scale.contiguous()
     shape = (*x.shape[:-1], n)
     if out is None:
         out = torch.empty(shape, dtype=dtype, device=x.device)
     elif tuple(out.shape) != shape or out.dtype != dtype or out.device != x.device:
         raise ValueError(f"out must be {dtype} {list(shape)} on {x.device}")
-    out2 = out.view(m, n)
+    out2 = out.view(-1, n)
+    if x_scale is None:
+        x2, scale = _rows_2d(x), None
+    else:
+        x2 = x.reshape(-1, k).contiguous()
+        if x2.data_ptr() % 16:
+            x2 = x2.clone()
+        scale = x_scale.reshape(-1, _blocks(k)).t()
+        if (x2.shape[0] > 1 and scale.stride(1) != 1) or scale.stride(0) < x2.shape[0]:
+            scale = scale.contiguous()
     if x.device.type == "cpu":
-        out2.copy_(ref_linear_fp8(codes, scale.t(), w_q, w_scale).to(dtype))
+        codes, scale = ref_quantize_fp8(x2) if scale is None else (x2, scale.t())
+        out2.copy_(ref_linear_fp8(codes, scale, w_q, w_scale).to(dtype))
         return out
-    _C.linear_fp8(codes, scale, w_q, w_scale, out2, error_word(x.device))
+    _C.linear_fp8(x2, scale, w_q, w_scale, out2, error_word(x.device))
     return out
 
 

@@ -19,8 +19,9 @@ enum class Type { kBf16 = 0, kFp16 = 1, kFp32 = 2 };
 
 // x [M, K] (row stride ldx elements) to q [M, K] (contiguous) and scale
 // [blocks, M]: the scales of a block for all rows are contiguous, row stride lds.
+// `zero` (or null): `zeros` words that are set to zero on the way.
 void quantize(const void* x, int64_t ldx, uint8_t* q, float* scale, int64_t lds, int64_t M, int64_t K, Type type,
-              cudaStream_t s);
+              unsigned* zero, int64_t zeros, cudaStream_t s);
 
 // w [N, K] (row stride ldw) to q [N, K] and scale [ceil(N / 128), ceil(K / 128)].
 void quantize_weight(const void* w, int64_t ldw, uint8_t* q, float* scale, int64_t N, int64_t K, Type type,
@@ -35,7 +36,15 @@ struct LinearArgs {
   int64_t lds, ldo;
   int64_t M, N, K;
   int* err;
+  float* workspace;    // linear_scratch().floats
+  unsigned* counters;  // linear_scratch().counters words, zero
+  bool early;          // the kernel before is quantize() of x: the weights need no wait
 };
+// What a product needs besides its tensors; not kept from call to call.
+struct Scratch {
+  int64_t floats, counters;
+};
+Scratch linear_scratch(const LinearArgs& a);
 // out = sum over blocks b of sx[b, m] sw[n / 128, b] (x[m, b] . w[n, b])
 void linear(const LinearArgs& a, Type out, cudaStream_t s);
 

@@ -1,16 +1,37 @@
-// Matrix product of e4m3 operands with block scales:
+// Matrix product of e4m3 operands with block scales on the 5th-generation tensor cores:
 //
 //   out[m, n] = sum_b sx[b, m] sw[n / 128, b] sum_{k in block b} x[m, k] w[n, k]
 //
-// The simplest form: 64 x 64 output tiles, operands widened to fp32 in shared
-// memory, sums in fp32.
+// A block of 128 values of K is one 128-byte row of a swizzled tile and four
+// tcgen05.mma (kind::f8f6f4, K = 32). Scales differ from block to block, so the
+// tensor core sums one block at a time into tensor memory; four or eight warps
+// take it from there, scale it and add it in fp32 registers while the next
+// block is multiplied. Two kernels:
+//
+// rows_kernel (few rows of x). The weights' 128 rows are the product's M, the
+//   rows of x (16 to 128) its N, so a product moves each weight once whatever
+//   the number of rows. The K blocks are split over the CTAs of a cluster,
+//   which add their sums through distributed shared memory: no workspace.
+// pair_kernel (many rows). CTA pairs (cta_group::2) compute 256 x 256 tiles. All
+//   tiles' K blocks form one line that is cut into equal parts for the pairs,
+//   so no pair idles in a last partial wave. A tile that a cut falls into is
+//   finished by the pair that arrives last, which adds the parts in the order
+//   of K.
+//
+// Every wait is bounded: on expiry the error word is set and all roles run
+// down without waiting.
+#include <cuda.h>
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
+
+#include <algorithm>
+#include <stdexcept>
+#include <string>
 
 #include "../common/check.h"
 #include "../common/pdl.h"
 #include "../common/trace.h"
+#include "../gemm/tcgen05.cuh"
 #include "fp8.h"
 
 namespace b200ar {
@@ -18,61 +39,644 @@ namespace fp8 {
 
 namespace {
 
-__device__ __forceinline__ float decode(uint8_t c) {
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
-}
-__device__ __forceinline__ void put(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
-__device__ __forceinline__ void put(__half* p, float v) { *p = __float2half_rn(v); }
+constexpr int kErrTimeout = 1;
 
 template <typename T>
-__global__ void __launch_bounds__(256) linear_simple_kernel(const LinearArgs a) {
-  __shared__ float sx[16][65], sw[16][65];
-  const int64_t m0 = static_cast<int64_t>(blockIdx.x) * 64, n0 = static_cast<int64_t>(blockIdx.y) * 64;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  const int64_t kblocks = (a.K + kBlock - 1) / kBlock;
-  float acc[4][4] = {};
+__device__ __forceinline__ uint32_t pack2(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// D fp32, A and B e4m3, both K-major.
+__host__ __device__ constexpr uint32_t idesc_e4m3(int m, int n) {
+  return (1u << 4) | (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+__device__ __forceinline__ void mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_e4m3_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+struct Args {
+  const float* sx;  // [kblocks, M], row stride lds
+  const float* sw;  // [ceil(N / 128), kblocks]
+  void* out;        // [M, N], row stride ldo
+  int64_t lds, ldo;
+  int M, N, kblocks;
+  int* err;
+};
+
+// ------------------------------------------------------------------ few rows
+template <int MP>  // rows of x in a tile
+struct RowsCfg {
+  static constexpr int kThreads = 192;
+  static constexpr uint32_t kW = 128 * 128, kX = MP * 128, kStage = kW + kX;
+  // Two CTAs fit an SM, or one at 128 rows, whose sums need the space once the ring is done.
+  static constexpr int kStages = (100 * 1024) / kStage;
+  static constexpr int kBufs = MP == 128 ? 2 : 4;  // accumulators in tensor memory
+  static constexpr uint32_t kCols = kBufs * MP;    // a power of two from 64 to 256
+  static constexpr int kScales = 4;                // ring of K blocks' scales
+  static constexpr size_t kSmem = 1024 + kStages * kStage + kScales * MP * 4 + 256;
+  static_assert(MP * 128 * 4 <= kStages * kStage, "the sums of a CTA reuse the ring");
+};
+
+// Grid: clusters of `splits` CTAs along x; cluster (x / splits) has 128 rows of W, y 128 or fewer rows of x.
+template <typename T, int MP>
+__global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
+    rows_kernel(const __grid_constant__ CUtensorMap tw, const __grid_constant__ CUtensorMap tx, const Args a,
+                int splits, int early) {
+  using C = RowsCfg<MP>;
+  extern __shared__ __align__(1024) uint8_t rows_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rows_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t* sW = smem;
+  uint8_t* sX = smem + C::kStages * C::kW;
+  float* scales = reinterpret_cast<float*>(smem + C::kStages * C::kStage);  // [kScales][MP]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + C::kScales * MP);
+  uint64_t* empty = full + C::kStages;
+  uint64_t* tfull = empty + C::kStages;
+  uint64_t* tempty = tfull + C::kBufs;
+  uint64_t* drained = tempty + C::kBufs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* s_err = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  static_assert((2 * C::kStages + 2 * C::kBufs + 2) * 8 <= 256, "barriers");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int block = blockIdx.x / splits, rank = blockIdx.x % splits;
+  const int m0 = blockIdx.y * MP;
+  const int kb0 = a.kblocks * rank / splits, kb1 = a.kblocks * (rank + 1) / splits, nkb = kb1 - kb0;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < C::kStages; ++i) {
+      sm100::mbar_init(&full[i], 1);
+      sm100::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < C::kBufs; ++i) {
+      sm100::mbar_init(&tfull[i], 1);
+      sm100::mbar_init(&tempty[i], 4);
+    }
+    sm100::mbar_init(drained, 1);
+    *s_err = 0;
+    sm100::fence_barrier_init();
+    sm100::prefetch_tmap(&tw);
+    sm100::prefetch_tmap(&tx);
+  }
+  if (warp == 1) {
+    sm100::tmem_alloc(tmem_slot, C::kCols);
+    sm100::tmem_relinquish();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto wait = [&](uint64_t* b, uint32_t parity) {
+    if (*s_err) return;
+    if (!sm100::mbar_wait(b, parity)) *s_err = 1;
+  };
+
+  float acc[MP];
+#pragma unroll
+  for (int i = 0; i < MP; ++i) acc[i] = 0.f;
+
+  if (warp == 0) {
+    if (sm100::elect_one()) {
+      // With `early` the kernel before is the quantization of x, which started after everything before it was
+      // done: the weights are there, and the first ring of them is requested while x is still being written.
+      const int pre = early ? min(nkb, C::kStages) : 0;
+      for (int i = 0; i < pre; ++i) {
+        sm100::mbar_arrive_expect_tx(&full[i], C::kStage);
+        sm100::tma_load_2d(sW + i * C::kW, &tw, &full[i], (kb0 + i) * kBlock, block * 128);
+      }
+      pdl_wait();
+      for (int i = 0; i < pre; ++i) sm100::tma_load_2d(sX + i * C::kX, &tx, &full[i], (kb0 + i) * kBlock, m0);
+      int issued = pre;
+      for (; issued < nkb; ++issued) {
+        const int st = issued % C::kStages;
+        wait(&empty[st], ((issued / C::kStages) & 1) ^ 1);
+        if (*s_err) break;
+        sm100::mbar_arrive_expect_tx(&full[st], C::kStage);
+        sm100::tma_load_2d(sW + st * C::kW, &tw, &full[st], (kb0 + issued) * kBlock, block * 128);
+        sm100::tma_load_2d(sX + st * C::kX, &tx, &full[st], (kb0 + issued) * kBlock, m0);
+      }
+      // Never leave while a copy into this CTA's shared memory is in flight.
+      for (int i = max(0, issued - C::kStages); i < issued; ++i)
+        sm100::mbar_wait(&full[i % C::kStages], (i / C::kStages) & 1);
+    }
+    __syncwarp();
+    pdl_wait();
+  } else if (warp == 1) {
+    if (sm100::elect_one()) {
+      for (int i = 0; i < nkb && !*s_err; ++i) {
+        const int st = i % C::kStages, bf = i % C::kBufs;
+        wait(&tempty[bf], ((i / C::kBufs) & 1) ^ 1);
+        wait(&full[st], (i / C::kStages) & 1);
+        if (*s_err) break;
+        sm100::tc_fence_after();
+        const uint64_t dw = sm100::smem_desc_sw128(sW + st * C::kW);
+        const uint64_t dx = sm100::smem_desc_sw128(sX + st * C::kX);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_e4m3(tmem + bf * MP, dw + 2 * k, dx + 2 * k, idesc_e4m3(128, MP), k > 0 ? 1u : 0u);
+        sm100::mma_commit(&empty[st]);
+        sm100::mma_commit(&tfull[bf]);
+      }
+      sm100::mma_commit(drained);
+      if (!sm100::mbar_wait(drained, 0)) *s_err = 1;
+    }
+    __syncwarp();
+    pdl_wait();
+  } else {
+    // Thread = row of W. The scales of a K block, sx sw, are the same for all rows: 128 threads load them two
+    // blocks ahead and share them.
+    pdl_wait();
+    const int q4 = warp & 3, id = q4 * 32 + lane;
+    const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
+    const bool mine = id < MP && m0 + id < a.M;
+    const float* sx = a.sx + m0 + id;
+    const float* sw = a.sw + static_cast<int64_t>(block) * a.kblocks;
+    auto scale = [&](int i) {  // of the i-th K block
+      const int kb = kb0 + i;
+      return mine && i < nkb ? __ldg(sx + kb * a.lds) * __ldg(sw + kb) : 0.f;
+    };
+    float s2 = scale(2), s3 = scale(3);
+    if (id < MP) {
+      scales[id] = scale(0);
+      scales[MP + id] = scale(1);
+    }
+    for (int i = 0; i < nkb; ++i) {
+      const int bf = i % C::kBufs;
+      if (id < MP) scales[((i + 2) % C::kScales) * MP + id] = s2;
+      s2 = s3;
+      s3 = scale(i + 4);
+      // Orders the writes of block i + 2 against its reads, and all reads of block i - 2 (whose place the
+      // next step reuses) before them.
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      wait(&tfull[bf], (i / C::kBufs) & 1);
+      sm100::tc_fence_after();
+      const float4* sc = reinterpret_cast<const float4*>(scales + (i % C::kScales) * MP);
+      constexpr int kStep = MP < 32 ? MP : 32;
+#pragma unroll
+      for (int c = 0; c < MP; c += kStep) {
+        uint32_t r[kStep];
+        if constexpr (kStep == 16)
+          sm100::tmem_ld_32x32b_x16(tmem + lanes + bf * MP + c, r);
+        else
+          sm100::tmem_ld_32x32b_x32(tmem + lanes + bf * MP + c, r);
+        sm100::tmem_ld_wait();
+#pragma unroll
+        for (int e = 0; e < kStep; e += 4) {
+          const float4 s = sc[(c + e) / 4];
+          acc[c + e] = fmaf(__uint_as_float(r[e]), s.x, acc[c + e]);
+          acc[c + e + 1] = fmaf(__uint_as_float(r[e + 1]), s.y, acc[c + e + 1]);
+          acc[c + e + 2] = fmaf(__uint_as_float(r[e + 2]), s.z, acc[c + e + 2]);
+          acc[c + e + 3] = fmaf(__uint_as_float(r[e + 3]), s.w, acc[c + e + 3]);
+        }
+      }
+      sm100::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&tempty[bf]);
+    }
+  }
+  pdl_trigger();
+  sm100::tc_fence_before();
+  __syncthreads();  // copies and products are done: the ring is free
+  if (warp == 1) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc(tmem, C::kCols);
+  }
+  // Sums of the cluster: [row of x][row of W] in each CTA, added in the order of K.
+  float* sums = reinterpret_cast<float*>(smem);
+  if (warp >= 2) {
+    const int id = (warp & 3) * 32 + lane;
+#pragma unroll
+    for (int i = 0; i < MP; ++i)
+      if (m0 + i < a.M) sums[i * 128 + id] = acc[i];
+  }
+  if (splits > 1)
+    sm100::cluster_sync();
+  else
+    __syncthreads();
+  const int rows = min(MP, a.M - m0);
+  const uint32_t base = sm100::smem_u32(sums);
+  // Four columns of a row a thread; this CTA has every splits-th group of them.
+  for (int i = rank * C::kThreads + threadIdx.x; i < rows * 32; i += splits * C::kThreads) {
+    const int r = i >> 5, c = (i & 31) * 4, n = block * 128 + c;
+    if (n >= a.N) continue;
+    float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int p = 0; p < splits; ++p) {
+      const uint32_t addr = splits > 1 ? sm100::mapa_shared(base, p) + (r * 128 + c) * 4 : 0;
+      float4 v;
+      if (splits > 1)
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+                     : "r"(addr)
+                     : "memory");
+      else
+        v = *reinterpret_cast<const float4*>(sums + r * 128 + c);
+      y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
+    }
+    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + (m0 + r) * a.ldo + n) =
+        make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+  }
+  if (splits > 1) sm100::cluster_sync();  // no CTA leaves while another reads its sums
+  if (threadIdx.x == 0 && *s_err) atomicExch(a.err, kErrTimeout);
+}
+
+// ------------------------------------------------------------------ many rows
+namespace pair {
+
+constexpr int BM = 256, BN = 256;
+constexpr int kStages = 6;
+constexpr int kThreads = 384;  // three warpgroups of 168 registers a thread: 56 and twice 224 after the split
+constexpr uint32_t kA = 128 * 128, kB = 128 * 128, kStage = kA + kB;  // a CTA's halves
+constexpr size_t kSmem = 1024 + kStages * kStage + 256;
+constexpr uint32_t kCols = 512;
+constexpr int64_t kPartFloats = 128 * 256;  // a CTA's sums of a tile
+
+struct Line {
+  int tiles_m, tiles;
+  int64_t units;  // tiles * kblocks
+  int pairs;
+  float* parts;    // [pairs][2][2 CTAs][kPartFloats]
+  unsigned* done;  // [tiles][2], zero
+  __device__ __forceinline__ int64_t start(int p) const { return units * p / pairs; }
+  // The pair whose part holds a unit.
+  __device__ __forceinline__ int owner(int64_t u) const { return static_cast<int>((pairs * (u + 1) - 1) / units); }
+  __device__ __forceinline__ float* part(int p, int which, int rank) const {
+    return parts + (static_cast<int64_t>(p * 2 + which) * 2 + rank) * kPartFloats;
+  }
+};
+
+__device__ __forceinline__ uint64_t pack64(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack64(uint64_t v, float& lo, float& hi) {
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+  lo = __uint_as_float(a);
+  hi = __uint_as_float(b);
+}
+// Two fp32 sums in one instruction.
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kThreads, 1)
+    pair_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Args a,
+                const Line line) {
+  extern __shared__ __align__(1024) uint8_t pair_smem[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pair_smem) + 1023) & ~uintptr_t(1023));
+  uint8_t* sA = smem;
+  uint8_t* sB = smem + kStages * kA;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStage);
+  uint64_t* empty = full + kStages;
+  uint64_t* tfull = empty + kStages;  // [2]
+  uint64_t* tempty = tfull + 2;       // [2] (the leader's: 8 warps of each CTA)
+  uint64_t* drained = tempty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
+  volatile int* s_err = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* s_last = const_cast<int*>(s_err) + 1;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = sm100::cluster_ctarank();
+  const bool leader = rank == 0;
+  const int p = blockIdx.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      sm100::mbar_init(&full[i], 1);
+      sm100::mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      sm100::mbar_init(&tfull[i], 1);
+      sm100::mbar_init(&tempty[i], 16);
+    }
+    sm100::mbar_init(drained, 1);
+    *s_err = 0;
+    sm100::fence_barrier_init();
+    sm100::prefetch_tmap(&tx);
+    sm100::prefetch_tmap(&tw);
+  }
+  if (warp == 9) {
+    sm100::tmem_alloc_pair(tmem_slot, kCols);
+    sm100::tmem_relinquish_pair();
+  }
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::cluster_sync();  // both CTAs' barriers exist before any signal between them
+  sm100::tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  auto wait = [&](uint64_t* b, uint32_t parity) {
+    if (*s_err) return;
+    if (!sm100::mbar_wait_cluster(b, parity)) *s_err = 1;
+  };
   pdl_wait();
   pdl_trigger();
-  for (int64_t b = 0; b < kblocks; ++b) {
-    float part[4][4] = {};
-    for (int64_t k0 = b * kBlock; k0 < min((b + 1) * kBlock, a.K); k0 += 16) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < 64 * 16; i += 256) {
-        const int r = i >> 4, c = i & 15;
-        sx[c][r] = m0 + r < a.M ? decode(a.x[(m0 + r) * a.K + k0 + c]) : 0.f;
-        sw[c][r] = n0 + r < a.N ? decode(a.w[(n0 + r) * a.K + k0 + c]) : 0.f;
+  const int64_t u0 = line.start(p), u1 = line.start(p + 1);
+
+  if (warp >= 8) {
+    sm100::reg_give<56>();
+    if (warp == 8 && sm100::elect_one()) {
+      // -------------------------------------------------------- TMA producer
+      unsigned n = 0;
+      for (int64_t u = u0; u < u1; ++u, ++n) {
+        const int tile = static_cast<int>(u / a.kblocks), kb = static_cast<int>(u - int64_t(tile) * a.kblocks);
+        const int tm = tile % line.tiles_m, tn = tile / line.tiles_m, st = n % kStages;
+        wait(&empty[st], ((n / kStages) & 1u) ^ 1u);
+        if (*s_err) break;
+        const uint32_t fbar = sm100::mapa_shared(sm100::smem_u32(&full[st]), 0);
+        if (leader) sm100::mbar_arrive_expect_tx(&full[st], 2 * kStage);  // both CTAs' bytes
+        sm100::tma_load_2d_pair(sA + st * kA, &tx, fbar, kb * kBlock, tm * BM + static_cast<int>(rank) * 128);
+        sm100::tma_load_2d_pair(sB + st * kB, &tw, fbar, kb * kBlock, tn * BN + static_cast<int>(rank) * 128);
       }
-      __syncthreads();
-      for (int c = 0; c < 16; ++c)
-        for (int i = 0; i < 4; ++i)
-          for (int j = 0; j < 4; ++j) part[i][j] += sx[c][ty + 16 * i] * sw[c][tx + 16 * j];
+      if (leader)
+        for (unsigned i = n > kStages ? n - kStages : 0; i < n; ++i)
+          sm100::mbar_wait_cluster(&full[i % kStages], (i / kStages) & 1u);
     }
-    for (int i = 0; i < 4; ++i)
-      for (int j = 0; j < 4; ++j) {
-        const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-        if (m < a.M && n < a.N) acc[i][j] += part[i][j] * a.sx[b * a.lds + m] * a.sw[(n / kBlock) * kblocks + b];
+    if (warp == 9 && leader && sm100::elect_one()) {
+      // -------------------------------------------------------- MMA issue (leader)
+      unsigned n = 0;
+      for (int64_t u = u0; u < u1 && !*s_err; ++u, ++n) {
+        const int st = n % kStages, bf = n & 1;
+        wait(&tempty[bf], ((n >> 1) & 1u) ^ 1u);
+        wait(&full[st], (n / kStages) & 1u);
+        if (*s_err) break;
+        sm100::tc_fence_after();
+        const uint64_t da = sm100::smem_desc_sw128(sA + st * kA);
+        const uint64_t db = sm100::smem_desc_sw128(sB + st * kB);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          mma_e4m3_pair(tmem + bf * BN, da + 2 * k, db + 2 * k, idesc_e4m3(BM, BN), k > 0 ? 1u : 0u);
+        for (uint32_t r = 0; r < 2; ++r) sm100::mma_commit_pair(sm100::mapa_shared(sm100::smem_u32(&empty[st]), r));
+        for (uint32_t r = 0; r < 2; ++r) sm100::mma_commit_pair(sm100::mapa_shared(sm100::smem_u32(&tfull[bf]), r));
       }
+      sm100::mma_commit_pair(sm100::mapa_shared(sm100::smem_u32(drained), 0));
+      if (!sm100::mbar_wait_cluster(drained, 0)) *s_err = 1;
+    }
+  } else {
+    // ---------------------------------------------------------- scale, add, store: 8 warps
+    sm100::reg_take<224>();
+    const int g = warp >> 2, row = (warp & 3) * 32 + lane;  // 128 columns of the tile, row of the CTA
+    const uint32_t td = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * 128;
+    const uint32_t free_bar[2] = {sm100::mapa_shared(sm100::smem_u32(&tempty[0]), 0),
+                                  sm100::mapa_shared(sm100::smem_u32(&tempty[1]), 0)};
+    unsigned n = 0;
+    for (int64_t u = u0; u < u1;) {
+      const int tile = static_cast<int>(u / a.kblocks), k0 = static_cast<int>(u - int64_t(tile) * a.kblocks);
+      const int k1 = static_cast<int>(min(static_cast<int64_t>(a.kblocks), k0 + u1 - u));
+      const int tm = tile % line.tiles_m, tn = tile / line.tiles_m;
+      const int m = tm * BM + static_cast<int>(rank) * 128 + row, n0 = tn * BN + g * 128;
+      const float* sx = a.sx + min(m, a.M - 1);
+      const float* sw = a.sw + static_cast<int64_t>(min(n0, a.N - 1) / kBlock) * a.kblocks;
+      auto scale = [&](int kb) { return kb < k1 ? __ldg(sx + kb * a.lds) * __ldg(sw + kb) : 0.f; };
+      float s0 = scale(k0), s1 = scale(k0 + 1);
+      uint64_t acc[64];
+#pragma unroll
+      for (int i = 0; i < 64; ++i) acc[i] = 0;
+      for (int kb = k0; kb < k1; ++kb, ++n) {
+        const int bf = n & 1;
+        const uint64_t s = pack64(__float_as_uint(s0), __float_as_uint(s0));
+        s0 = s1;
+        s1 = scale(kb + 2);
+        wait(&tfull[bf], (n >> 1) & 1u);
+        sm100::tc_fence_after();
+#pragma unroll
+        for (int c = 0; c < 128; c += 64) {
+          uint32_t r[64];
+          sm100::tmem_ld_32x32b_x32(td + bf * BN + c, r);
+          sm100::tmem_ld_32x32b_x32(td + bf * BN + c + 32, r + 32);
+          sm100::tmem_ld_wait();
+          if (c == 64) {  // the accumulator is read: the next block but one may overwrite it
+            sm100::tc_fence_before();
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive_cluster(free_bar[bf]);
+          }
+#pragma unroll
+          for (int e = 0; e < 64; e += 2) acc[(c + e) / 2] = fma2(pack64(r[e], r[e + 1]), s, acc[(c + e) / 2]);
+        }
+      }
+      u += k1 - k0;
+
+      bool store = true;
+      int first = p, last = p;
+      if (k1 - k0 < a.kblocks) {
+        // A cut tile: whoever arrives last has all parts. Each CTA of the pair has its own rows.
+        first = line.owner(int64_t(tile) * a.kblocks);
+        last = line.owner(int64_t(tile + 1) * a.kblocks - 1);
+        unsigned* done = line.done + tile * 2 + rank;
+        if (threadIdx.x == 0) *s_last = atomicAdd(done, 0u) == static_cast<unsigned>(last - first);
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        if (!*reinterpret_cast<volatile int*>(s_last)) {
+          float4* dst = reinterpret_cast<float4*>(line.part(p, k0 > 0 ? 0 : 1, rank)) + g * 32 * 128 + row;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            float4 v;
+            unpack64(acc[2 * i], v.x, v.y);
+            unpack64(acc[2 * i + 1], v.z, v.w);
+            __stcg(dst + i * 128, v);
+          }
+          __threadfence();
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+          if (threadIdx.x == 0) *s_last = atomicAdd(done, 1u) == static_cast<unsigned>(last - first);
+          asm volatile("bar.sync 1, 256;" ::: "memory");
+        }
+        store = *reinterpret_cast<volatile int*>(s_last) != 0;
+        __threadfence();
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // s_last may be written again
+      }
+      if (!store) continue;
+      T* out = static_cast<T*>(a.out) + static_cast<int64_t>(m) * a.ldo + n0;
+#pragma unroll
+      for (int c = 0; c < 128; c += 8) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) unpack64(acc[c / 2 + e], y[2 * e], y[2 * e + 1]);
+        if (first < last) {
+          float own[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) own[e] = y[e], y[e] = 0.f;
+          for (int q = first; q <= last; ++q) {
+            if (q == p) {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) y[e] += own[e];
+            } else {
+              const float4* src =
+                  reinterpret_cast<const float4*>(line.part(q, q > first ? 0 : 1, rank)) + g * 32 * 128 + row;
+              const float4 v0 = __ldcg(src + (c / 4) * 128), v1 = __ldcg(src + (c / 4 + 1) * 128);
+              y[0] += v0.x, y[1] += v0.y, y[2] += v0.z, y[3] += v0.w;
+              y[4] += v1.x, y[5] += v1.y, y[6] += v1.z, y[7] += v1.w;
+            }
+          }
+        }
+        if (m < a.M && n0 + c < a.N)  // N is a multiple of 8
+          *reinterpret_cast<uint4*>(out + c) =
+              make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+      }
+    }
   }
-  for (int i = 0; i < 4; ++i)
-    for (int j = 0; j < 4; ++j) {
-      const int64_t m = m0 + ty + 16 * i, n = n0 + tx + 16 * j;
-      if (m < a.M && n < a.N) put(static_cast<T*>(a.out) + m * a.ldo + n, acc[i][j]);
-    }
+
+  sm100::tc_fence_before();
+  __syncthreads();
+  sm100::cluster_sync();  // neither CTA leaves while the pair's products or signals may touch it
+  if (warp == 9) {
+    sm100::tc_fence_after();
+    sm100::tmem_dealloc_pair(tmem, kCols);
+  }
+  if (threadIdx.x == 0 && *s_err) atomicExch(a.err, kErrTimeout);
+}
+
+}  // namespace pair
+
+// ------------------------------------------------------------------ host side
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                              const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                              CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+EncodeFn encode() {
+  static EncodeFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    B200AR_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &q));
+    if (q != cudaDriverEntryPointSuccess || !ptr) throw std::runtime_error("cuTensorMapEncodeTiled unavailable");
+    return reinterpret_cast<EncodeFn>(ptr);
+  }();
+  return fn;
+}
+
+// Codes [rows, K], box of box_rows x 128.
+CUtensorMap codes_map(const void* base, int64_t rows, int64_t K, int box_rows) {
+  CUtensorMap m;
+  const cuuint64_t dims[2] = {static_cast<cuuint64_t>(K), static_cast<cuuint64_t>(rows)};
+  const cuuint64_t strides[1] = {static_cast<cuuint64_t>(K)};
+  const cuuint32_t box[2] = {kBlock, static_cast<cuuint32_t>(box_rows)};
+  const cuuint32_t estr[2] = {1, 1};
+  const CUresult r = encode()(&m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled (e4m3) failed: " + std::to_string(r));
+  return m;
+}
+
+int sm_count() {
+  int dev = 0, n = 0;
+  B200AR_CUDA(cudaGetDevice(&dev));
+  B200AR_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
+  return n;
+}
+
+template <typename T, int MP>
+void launch_rows(const LinearArgs& l, const Args& a, int splits, cudaStream_t s) {
+  using C = RowsCfg<MP>;
+  const CUtensorMap tw = codes_map(l.w, l.N, l.K, 128), tx = codes_map(l.x, l.M, l.K, MP);
+  auto kern = rows_kernel<T, MP>;
+  static PerDeviceOnce attr;
+  attr([&] {
+    B200AR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem)));
+  });
+  const dim3 grid(static_cast<unsigned>((l.N + 127) / 128 * splits), static_cast<unsigned>((l.M + MP - 1) / MP));
+  launch_pdl(kern, grid, dim3(C::kThreads), C::kSmem, s, splits, tw, tx, a, splits, l.early ? 1 : 0);
+}
+
+int pairs_of(const LinearArgs& l) {
+  const int64_t tiles = (l.M + pair::BM - 1) / pair::BM * ((l.N + pair::BN - 1) / pair::BN);
+  const int64_t units = tiles * ((l.K + kBlock - 1) / kBlock);
+  return static_cast<int>(std::min<int64_t>(sm_count() / 2, units));
+}
+
+template <typename T>
+void launch_pair(const LinearArgs& l, const Args& a, cudaStream_t s) {
+  const CUtensorMap tx = codes_map(l.x, l.M, l.K, 128), tw = codes_map(l.w, l.N, l.K, 128);
+  pair::Line line{};
+  line.tiles_m = static_cast<int>((l.M + pair::BM - 1) / pair::BM);
+  line.tiles = line.tiles_m * static_cast<int>((l.N + pair::BN - 1) / pair::BN);
+  line.units = static_cast<int64_t>(line.tiles) * a.kblocks;
+  line.pairs = pairs_of(l);
+  line.parts = l.workspace;
+  line.done = l.counters;
+  auto kern = pair::pair_kernel<T>;
+  static PerDeviceOnce attr;
+  attr([&] {
+    B200AR_CUDA(
+        cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(pair::kSmem)));
+  });
+  launch_pdl(kern, dim3(static_cast<unsigned>(2 * line.pairs)), dim3(pair::kThreads), pair::kSmem, s, 2, tx, tw, a,
+             line);
+}
+
+// Rows up to which rows_kernel is taken.
+bool few_rows(const LinearArgs& l) { return l.M <= 512; }
+
+template <typename T>
+void dispatch(const LinearArgs& l, const Args& a, cudaStream_t s) {
+  if (!few_rows(l)) return launch_pair<T>(l, a, s);
+  const int mp = l.M <= 16 ? 16 : l.M <= 32 ? 32 : l.M <= 64 ? 64 : 128;
+  // Cluster size: the most CTAs that two to an SM hold, with two K blocks each at least.
+  const int64_t ctas = (l.N + 127) / 128 * ((l.M + mp - 1) / mp);
+  int splits = 1;
+  while (splits < 8 && ctas * splits * 2 <= 2 * sm_count() && a.kblocks >= splits * 4) splits *= 2;
+  switch (mp) {
+    case 16: return launch_rows<T, 16>(l, a, splits, s);
+    case 32: return launch_rows<T, 32>(l, a, splits, s);
+    case 64: return launch_rows<T, 64>(l, a, splits, s);
+    default: return launch_rows<T, 128>(l, a, splits, s);
+  }
+}
+
+void check(const LinearArgs& l) {
+  B200AR_CHECK(l.M >= 0 && l.M < (1ll << 30) && l.N > 0 && l.N < (1ll << 21) && l.K > 0 && l.K < (1ll << 30),
+               "bad shape for linear_fp8");
+  B200AR_CHECK(l.K % 16 == 0 && l.N % 8 == 0, "K must be a multiple of 16 and N of 8");
 }
 
 }  // namespace
 
-void linear(const LinearArgs& a, Type out, cudaStream_t s) {
+Scratch linear_scratch(const LinearArgs& l) {
+  check(l);
+  if (l.M == 0 || few_rows(l)) return {0, 0};
+  const int64_t tiles = (l.M + pair::BM - 1) / pair::BM * ((l.N + pair::BN - 1) / pair::BN);
+  return {pairs_of(l) * 4 * pair::kPartFloats, 2 * tiles};
+}
+
+void linear(const LinearArgs& l, Type out, cudaStream_t s) {
   const TraceRange trace("b200ar::linear_fp8");
-  B200AR_CHECK(a.M >= 0 && a.M < (1ll << 30) && a.N > 0 && a.N < (1ll << 21) && a.K > 0 && a.K < (1ll << 30),
-               "bad shape for linear_fp8");
-  B200AR_CHECK(a.K % 16 == 0 && a.N % 8 == 0, "K must be a multiple of 16 and N of 8");
-  if (a.M == 0) return;
-  const dim3 grid(static_cast<unsigned>((a.M + 63) / 64), static_cast<unsigned>((a.N + 63) / 64));
+  check(l);
+  if (l.M == 0) return;
+  Args a{};
+  a.sx = l.sx;
+  a.sw = l.sw;
+  a.out = l.out;
+  a.lds = l.lds;
+  a.ldo = l.ldo;
+  a.M = static_cast<int>(l.M);
+  a.N = static_cast<int>(l.N);
+  a.kblocks = static_cast<int>((l.K + kBlock - 1) / kBlock);
+  a.err = l.err;
   if (out == Type::kBf16)
-    launch_pdl(linear_simple_kernel<__nv_bfloat16>, grid, dim3(256), 0, s, 1, a);
+    dispatch<__nv_bfloat16>(l, a, s);
   else
-    launch_pdl(linear_simple_kernel<__half>, grid, dim3(256), 0, s, 1, a);
+    dispatch<__half>(l, a, s);
 }
 
 }  // namespace fp8

@@ -80,7 +80,7 @@ __device__ __forceinline__ uint2 encode8(const float* v, float scale) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads)
     quantize_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, float* __restrict__ scale,
-                    int64_t lds, int64_t M, int K) {
+                    int64_t lds, int64_t M, int K, unsigned* __restrict__ zero, int64_t zeros) {
   const int64_t m = blockIdx.x;
   const int lane = threadIdx.x & 15;
   const int b = blockIdx.y * (kThreads / 16) + (threadIdx.x >> 4);
@@ -88,6 +88,9 @@ __global__ void __launch_bounds__(kThreads)
   float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   pdl_wait();
   pdl_trigger();
+  for (int64_t i = (m * gridDim.y + blockIdx.y) * kThreads + threadIdx.x; i < zeros;
+       i += static_cast<int64_t>(gridDim.x) * gridDim.y * kThreads)
+    zero[i] = 0u;
   if (k < K) load8<T>(x + m * ldx + k, v);
   unsigned amax = abs_max8(v);
 #pragma unroll
@@ -136,11 +139,11 @@ __global__ void __launch_bounds__(kThreads)
 
 template <typename T>
 void launch_rows(const void* x, int64_t ldx, uint8_t* q, float* scale, int64_t lds, int64_t M, int64_t K,
-                 cudaStream_t s) {
+                 unsigned* zero, int64_t zeros, cudaStream_t s) {
   const int64_t blocks = (K + kBlock - 1) / kBlock;
   const dim3 grid(static_cast<unsigned>(M), static_cast<unsigned>((blocks + kThreads / 16 - 1) / (kThreads / 16)));
   launch_pdl(quantize_kernel<T>, grid, dim3(kThreads), 0, s, 1, static_cast<const T*>(x), ldx, q, scale, lds, M,
-             static_cast<int>(K));
+             static_cast<int>(K), zero, zeros);
 }
 template <typename T>
 void launch_weight(const void* w, int64_t ldw, uint8_t* q, float* scale, int64_t N, int64_t K, cudaStream_t s) {
@@ -157,14 +160,14 @@ void check_shape(int64_t rows, int64_t K) {
 }  // namespace
 
 void quantize(const void* x, int64_t ldx, uint8_t* q, float* scale, int64_t lds, int64_t M, int64_t K, Type type,
-              cudaStream_t s) {
+              unsigned* zero, int64_t zeros, cudaStream_t s) {
   const TraceRange trace("b200ar::quantize_fp8");
   check_shape(M, K);
   if (M == 0) return;
   switch (type) {
-    case Type::kBf16: return launch_rows<__nv_bfloat16>(x, ldx, q, scale, lds, M, K, s);
-    case Type::kFp16: return launch_rows<__half>(x, ldx, q, scale, lds, M, K, s);
-    case Type::kFp32: return launch_rows<float>(x, ldx, q, scale, lds, M, K, s);
+    case Type::kBf16: return launch_rows<__nv_bfloat16>(x, ldx, q, scale, lds, M, K, zero, zeros, s);
+    case Type::kFp16: return launch_rows<__half>(x, ldx, q, scale, lds, M, K, zero, zeros, s);
+    case Type::kFp32: return launch_rows<float>(x, ldx, q, scale, lds, M, K, zero, zeros, s);
   }
 }
 

@@ -280,6 +280,17 @@ SM100_DEV void mma_commit_pair(uint32_t bar_cluster_addr) {
                : "memory");
 }
 
+// Register budget of a warpgroup (all its warps). The groups' budgets together
+// stay within the registers that the block was launched with.
+template <int N>
+SM100_DEV void reg_take() {
+  asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+SM100_DEV void reg_give() {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
 SM100_DEV bool elect_one() {
   uint32_t pred = 0;
   asm volatile(

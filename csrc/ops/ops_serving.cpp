@@ -239,7 +239,8 @@ void register_serving_ops(py::module& m) {
                     "scale must be fp32 [ceil(K / 128), M]");
         const at::cuda::OptionalCUDAGuard guard(device_of(x));
         b200ar::fp8::quantize(x.data_ptr(), x.stride(0), static_cast<uint8_t*>(q.data_ptr()),
-                              scale.data_ptr<float>(), scale.stride(0), M, K, fp8_type(x, true, "x"), stream_of());
+                              scale.data_ptr<float>(), scale.stride(0), M, K, fp8_type(x, true, "x"), nullptr, 0,
+                              stream_of());
       },
       "e4m3 values and a scale for each row and block of 128", py::arg("x"), py::arg("q"), py::arg("scale"));
   m.def(
@@ -261,39 +262,62 @@ void register_serving_ops(py::module& m) {
       "e4m3 values and a scale for each 128 x 128 block", py::arg("w"), py::arg("q"), py::arg("scale"));
   m.def(
       "linear_fp8",
-      [](const at::Tensor& x, const at::Tensor& x_scale, const at::Tensor& w, const at::Tensor& w_scale,
-         at::Tensor& out, at::Tensor& err) {
-        check_codes(x, "x");
+      [](const at::Tensor& x, const std::optional<at::Tensor>& x_scale, const at::Tensor& w,
+         const at::Tensor& w_scale, at::Tensor& out, at::Tensor& err) {
         check_codes(w, "w_q");
+        TORCH_CHECK(x.dim() == 2, "x must be [M, K]");
+        const int64_t M = x.size(0), K = x.size(1), N = w.size(0), blocks = (K + 127) / 128;
         check_device(w, x, "w_q");
         check_device(out, x, "out");
-        check_device(x_scale, x, "x_scale");
         check_device(w_scale, x, "w_scale");
-        const int64_t M = x.size(0), K = x.size(1), N = w.size(0), blocks = (K + 127) / 128;
         TORCH_CHECK(w.size(1) == K, "x and w_q must have the same K");
-        TORCH_CHECK(x_scale.scalar_type() == at::kFloat && x_scale.dim() == 2 && x_scale.size(0) == blocks &&
-                        x_scale.size(1) == M && (M <= 1 || x_scale.stride(1) == 1) && x_scale.stride(0) >= M,
-                    "x_scale must be fp32 [ceil(K / 128), M]");
         TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.is_contiguous() && w_scale.dim() == 2 &&
                         w_scale.size(0) == (N + 127) / 128 && w_scale.size(1) == blocks,
                     "w_scale must be fp32 [ceil(N / 128), ceil(K / 128)]");
         check_rows_2d(out, "out");
         TORCH_CHECK(out.size(0) == M && out.size(1) == N, "out must be [M, N]");
+        const b200ar::fp8::Type type = fp8_type(out, false, "out");
+        const at::cuda::OptionalCUDAGuard guard(device_of(x));
+        const cudaStream_t s = stream_of();
         b200ar::fp8::LinearArgs a{};
-        a.x = static_cast<const uint8_t*>(x.data_ptr());
-        a.sx = x_scale.data_ptr<float>();
         a.w = static_cast<const uint8_t*>(w.data_ptr());
         a.sw = w_scale.data_ptr<float>();
         a.out = out.data_ptr();
-        a.lds = x_scale.stride(0);
         a.ldo = out.stride(0);
         a.M = M;
         a.N = N;
         a.K = K;
         a.err = err_of(err, x);
-        const at::cuda::OptionalCUDAGuard guard(device_of(x));
-        b200ar::fp8::linear(a, fp8_type(out, false, "out"), stream_of());
+        // Scratch from the caching allocator on this stream: concurrent calls, eager or captured, never share it.
+        const b200ar::fp8::Scratch need = b200ar::fp8::linear_scratch(a);
+        const auto bytes = x.options().dtype(at::kByte);
+        const at::Tensor scratch = at::empty({need.floats * 4 + need.counters * 4}, bytes);
+        a.workspace = static_cast<float*>(scratch.data_ptr());
+        a.counters = reinterpret_cast<unsigned*>(a.workspace + need.floats);
+        at::Tensor codes, scales;
+        if (x_scale.has_value()) {
+          check_codes(x, "x");
+          check_device(*x_scale, x, "x_scale");
+          TORCH_CHECK(x_scale->scalar_type() == at::kFloat && x_scale->dim() == 2 && x_scale->size(0) == blocks &&
+                          x_scale->size(1) == M && (M <= 1 || x_scale->stride(1) == 1) && x_scale->stride(0) >= M,
+                      "x_scale must be fp32 [ceil(K / 128), M]");
+          a.x = static_cast<const uint8_t*>(x.data_ptr());
+          a.sx = x_scale->data_ptr<float>();
+          a.lds = x_scale->stride(0);
+          if (M > 0 && need.counters) C10_CUDA_CHECK(cudaMemsetAsync(a.counters, 0, need.counters * 4, s));
+        } else {
+          check_rows_2d(x, "x");
+          codes = at::empty({M, K}, bytes);
+          scales = at::empty({blocks, M}, x.options().dtype(at::kFloat));
+          a.x = codes.data_ptr<uint8_t>();
+          a.sx = scales.data_ptr<float>();
+          a.lds = M;
+          a.early = true;
+          b200ar::fp8::quantize(x.data_ptr(), x.stride(0), codes.data_ptr<uint8_t>(), scales.data_ptr<float>(), M, M,
+                                K, fp8_type(x, false, "x"), a.counters, need.counters, s);
+        }
+        b200ar::fp8::linear(a, type, s);
       },
-      "product of e4m3 operands with block scales", py::arg("x"), py::arg("x_scale"), py::arg("w"),
-      py::arg("w_scale"), py::arg("out"), py::arg("err"));
+      "product of e4m3 operands with block scales; x is quantized unless it comes with its scales", py::arg("x"),
+      py::arg("x_scale"), py::arg("w"), py::arg("w_scale"), py::arg("out"), py::arg("err"));
 }

@@ -248,9 +248,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     sm100::tmem_relinquish();
   }
   pdl_wait();  // lengths, offsets, pages, queries and the cache may come from the kernel before
-  pdl_trigger();
   if (threadIdx.x == 0) desc[0].used = desc[1].used = 0;
   find_part<kThreads>(a, group, misc.red, &misc.part);
+  pdl_trigger();  // after a barrier: this CTA holds its tensor memory
   sm100::tc_fence_before();
   __syncthreads();
   sm100::tc_fence_after();
@@ -260,103 +260,110 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (*s_err) return;
     if (!sm100::mbar_wait(b, parity)) *s_err = 1;
   };
-  Walk walk;
-  walk.start(a, group, misc.part);
-  Item it;
-
-  if (warp == 8) {
-    // ------------------------------------------------------------ TMA producer
-    const int boxes = kTile / box;           // page runs of a tile
-    unsigned count = 0;                      // loads issued so far
-    while (walk.next(a, group, it)) {
-      if (__any_sync(0xffffffffu, *s_err)) break;
-      const Steps st(it);
-      if (it.over && lane == 0) atomicExch(a.err, kErrPage);
-      for (int i = 0; i < 2 * st.nt; ++i, ++count) {
-        const int load = st.load(i);
-        const int c0 = (it.tile0 + it.t0 + (load >> 1)) * kTile;
-        // Page and slot of this lane's run (lane % boxes), looked up before the slot is free.
-        const int run = lane % boxes, pos = c0 + run * box;
-        int page = a.num_pages, slot = 0;  // outside the pool: zeros
-        if (pos + box > it.begin && pos < it.end) {
-          page = page_of(a.batch, it.s, pos / a.page_size, a.num_pages);
-          slot = pos % a.page_size;
-          if (page < 0) {
-            atomicExch(a.err, kErrPage);
-            page = a.num_pages;
-          }
-        }
-        const int sl = count % kSlots;
-        wait(&bar.empty[sl], ((count / kSlots) & 1u) ^ 1u);
+  // 168 registers a thread at launch: 88 for the last warpgroup and 208 for the two of the softmax.
+  if (warp >= 8) {
+    sm100::reg_give<88>();
+    Walk walk;
+    walk.start(a, group, misc.part);
+    Item it;
+    if (warp == 8) {
+      // ------------------------------------------------------------ TMA producer
+      const int boxes = kTile / box;           // page runs of a tile
+      unsigned count = 0;                      // loads issued so far
+      while (walk.next(a, group, it)) {
         if (__any_sync(0xffffffffu, *s_err)) break;
-        if (lane == 0) sm100::mbar_arrive_expect_tx(&bar.full[sl], C::kTileBytes);
-        __syncwarp();
-        uint8_t* dst = ring + sl * C::kTileBytes + run * box * 128;
-        for (int j = lane; j < boxes * C::kHalves; j += 32)  // 32 lanes are a multiple of the runs
-          sm100::tma_load_4d(dst + (j / boxes) * C::kHalfBytes, load & 1 ? &tv : &tk, &bar.full[sl],
-                             (j / boxes) * 64, it.h, slot, page);
-        __syncwarp();
-      }
-    }
-    // Never leave while a copy into this CTA's shared memory is in flight.
-    if (lane == 0)
-      for (unsigned i = count > kSlots ? count - kSlots : 0; i < count; ++i)
-        sm100::mbar_wait(&bar.full[i % kSlots], (i / kSlots) & 1u);
-  } else if (warp == 9) {
-    // ------------------------------------------------------------ MMA issue
-    if (sm100::elect_one()) {
-      unsigned base = 0;                   // loads of the items before
-      unsigned nq[2] = {0, 0}, np[2] = {0, 0};
-      auto slot_of = [&](int i) { return (base + i) % kSlots; };
-      auto phase_of = [&](int i) { return ((base + i) / kSlots) & 1u; };
-      while (walk.next(a, group, it) && !*s_err) {
         const Steps st(it);
-        const int steps = st.count();
-        wait(&bar.qready[0], nq[0]++ & 1u);
-        if (st.wide) wait(&bar.qready[1], nq[1]++ & 1u);
-        auto scores = [&](int k) {
-          const int t = k & 1, at = st.k_at(st.tile(k));
-          wait(&bar.full[slot_of(at)], phase_of(at));
-          sm100::tc_fence_after();
-          const uint8_t* qt = smem + C::kQ + (st.wide ? t : 0) * C::kTileBytes;
-          const uint8_t* kt = ring + slot_of(at) * C::kTileBytes;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            const uint64_t da = sm100::smem_desc_sw128(qt + (i >> 2) * C::kHalfBytes) + 2 * (i & 3);
-            const uint64_t db = sm100::smem_desc_sw128(kt + (i >> 2) * C::kHalfBytes) + 2 * (i & 3);
-            sm100::mma_bf16(tmem + t * 128, da, db, idesc<T>(128, false), i > 0 ? 1u : 0u);
+        if (it.over && lane == 0) atomicExch(a.err, kErrPage);
+        for (int i = 0; i < 2 * st.nt; ++i, ++count) {
+          const int load = st.load(i);
+          const int c0 = (it.tile0 + it.t0 + (load >> 1)) * kTile;
+          // Page and slot of this lane's run (lane % boxes), looked up before the slot is free.
+          const int run = lane % boxes, pos = c0 + run * box;
+          int page = a.num_pages, slot = 0;  // outside the pool: zeros
+          if (pos + box > it.begin && pos < it.end) {
+            page = page_of(a.batch, it.s, pos / a.page_size, a.num_pages);
+            slot = pos % a.page_size;
+            if (page < 0) {
+              atomicExch(a.err, kErrPage);
+              page = a.num_pages;
+            }
           }
-          sm100::mma_commit(&bar.sfull[t]);
-          if (!st.wide || t == 1) sm100::mma_commit(&bar.empty[slot_of(at)]);
-        };
-        scores(0);
-        if (steps > 1) scores(1);
-        for (int k = 0; k < steps && !*s_err; ++k) {
-          const int t = k & 1, at = st.v_at(st.tile(k));
-          wait(&bar.full[slot_of(at)], phase_of(at));
-          wait(&bar.pready[t], np[t]++ & 1u);
-          sm100::tc_fence_after();
-          const uint8_t* vt = ring + slot_of(at) * C::kTileBytes;
-#pragma unroll
-          for (int i = 0; i < kTile / 16; ++i)  // 16 tokens: 2048 bytes further in V, 8 columns in P
-            sm100::mma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + i * 8,
-                              sm100::smem_desc_mn_sw128(vt + i * 2048, C::kHalfBytes, 1024), idesc<T>(D, true),
-                              (k > 1 || i > 0) ? 1u : 0u);
-          if (!st.wide || t == 1) sm100::mma_commit(&bar.empty[slot_of(at)]);
-          if (k + 2 < steps)
-            scores(k + 2);
-          else
-            sm100::mma_commit(&bar.ofull[t]);
+          const int sl = count % kSlots;
+          wait(&bar.empty[sl], ((count / kSlots) & 1u) ^ 1u);
+          if (__any_sync(0xffffffffu, *s_err)) break;
+          if (lane == 0) sm100::mbar_arrive_expect_tx(&bar.full[sl], C::kTileBytes);
+          __syncwarp();
+          uint8_t* dst = ring + sl * C::kTileBytes + run * box * 128;
+          for (int j = lane; j < boxes * C::kHalves; j += 32)  // 32 lanes are a multiple of the runs
+            sm100::tma_load_4d(dst + (j / boxes) * C::kHalfBytes, load & 1 ? &tv : &tk, &bar.full[sl],
+                               (j / boxes) * 64, it.h, slot, page);
+          __syncwarp();
         }
-        base += 2 * st.nt;
       }
-      // Tensor memory is freed only after every product is done.
-      sm100::mma_commit(&bar.drained);
-      if (!sm100::mbar_wait(&bar.drained, 0)) *s_err = 1;
+      // Never leave while a copy into this CTA's shared memory is in flight.
+      if (lane == 0)
+        for (unsigned i = count > kSlots ? count - kSlots : 0; i < count; ++i)
+          sm100::mbar_wait(&bar.full[i % kSlots], (i / kSlots) & 1u);
+    } else if (warp == 9) {
+      // ------------------------------------------------------------ MMA issue
+      if (sm100::elect_one()) {
+        unsigned base = 0;                   // loads of the items before
+        unsigned nq[2] = {0, 0}, np[2] = {0, 0};
+        auto slot_of = [&](int i) { return (base + i) % kSlots; };
+        auto phase_of = [&](int i) { return ((base + i) / kSlots) & 1u; };
+        while (walk.next(a, group, it) && !*s_err) {
+          const Steps st(it);
+          const int steps = st.count();
+          wait(&bar.qready[0], nq[0]++ & 1u);
+          if (st.wide) wait(&bar.qready[1], nq[1]++ & 1u);
+          auto scores = [&](int k) {
+            const int t = k & 1, at = st.k_at(st.tile(k));
+            wait(&bar.full[slot_of(at)], phase_of(at));
+            sm100::tc_fence_after();
+            const uint8_t* qt = smem + C::kQ + (st.wide ? t : 0) * C::kTileBytes;
+            const uint8_t* kt = ring + slot_of(at) * C::kTileBytes;
+  #pragma unroll
+            for (int i = 0; i < D / 16; ++i) {
+              const uint64_t da = sm100::smem_desc_sw128(qt + (i >> 2) * C::kHalfBytes) + 2 * (i & 3);
+              const uint64_t db = sm100::smem_desc_sw128(kt + (i >> 2) * C::kHalfBytes) + 2 * (i & 3);
+              sm100::mma_bf16(tmem + t * 128, da, db, idesc<T>(128, false), i > 0 ? 1u : 0u);
+            }
+            sm100::mma_commit(&bar.sfull[t]);
+            if (!st.wide || t == 1) sm100::mma_commit(&bar.empty[slot_of(at)]);
+          };
+          scores(0);
+          if (steps > 1) scores(1);
+          for (int k = 0; k < steps && !*s_err; ++k) {
+            const int t = k & 1, at = st.v_at(st.tile(k));
+            wait(&bar.full[slot_of(at)], phase_of(at));
+            wait(&bar.pready[t], np[t]++ & 1u);
+            sm100::tc_fence_after();
+            const uint8_t* vt = ring + slot_of(at) * C::kTileBytes;
+  #pragma unroll
+            for (int i = 0; i < kTile / 16; ++i)  // 16 tokens: 2048 bytes further in V, 8 columns in P
+              sm100::mma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + i * 8,
+                                sm100::smem_desc_mn_sw128(vt + i * 2048, C::kHalfBytes, 1024), idesc<T>(D, true),
+                                (k > 1 || i > 0) ? 1u : 0u);
+            if (!st.wide || t == 1) sm100::mma_commit(&bar.empty[slot_of(at)]);
+            if (k + 2 < steps)
+              scores(k + 2);
+            else
+              sm100::mma_commit(&bar.ofull[t]);
+          }
+          base += 2 * st.nt;
+        }
+        // Tensor memory is freed only after every product is done.
+        sm100::mma_commit(&bar.drained);
+        if (!sm100::mbar_wait(&bar.drained, 0)) *s_err = 1;
+      }
+      __syncwarp();
     }
-    __syncwarp();
-  } else if (warp < 8) {
+  } else {
     // ------------------------------------------------------------ softmax
+    sm100::reg_take<208>();
+    Walk walk;
+    walk.start(a, group, misc.part);
+    Item it;
     const int t = warp >> 2, w4 = warp & 3;
     const int row = w4 * 32 + lane;  // row of the group's tile
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
