@@ -211,18 +211,20 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
     const bool mine = id < MP && m0 + id < a.M;
     const float* sx = a.sx + m0 + id;
     const float* sw = a.sw + static_cast<int64_t>(block) * a.kblocks;
-    auto scale = [&](int i) {  // of the i-th K block
+    // The factors of the i-th K block; multiplied where they are used, so that no load is waited for before.
+    auto scale = [&](int i) {
       const int kb = kb0 + i;
-      return mine && i < nkb ? __ldg(sx + kb * a.lds) * __ldg(sw + kb) : 0.f;
+      return mine && i < nkb ? make_float2(__ldg(sx + kb * a.lds), __ldg(sw + kb)) : make_float2(0.f, 0.f);
     };
-    float s2 = scale(2), s3 = scale(3);
+    const float2 s0 = scale(0), s1 = scale(1);
+    float2 s2 = scale(2), s3 = scale(3);
     if (id < MP) {
-      scales[id] = scale(0);
-      scales[MP + id] = scale(1);
+      scales[id] = s0.x * s0.y;
+      scales[MP + id] = s1.x * s1.y;
     }
     for (int i = 0; i < nkb; ++i) {
       const int bf = i % C::kBufs;
-      if (id < MP) scales[((i + 2) % C::kScales) * MP + id] = s2;
+      if (id < MP) scales[((i + 2) % C::kScales) * MP + id] = s2.x * s2.y;
       s2 = s3;
       s3 = scale(i + 4);
       // Orders the writes of block i + 2 against its reads, and all reads of block i - 2 (whose place the
@@ -390,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t tmem = *tmem_slot;
   auto wait = [&](uint64_t* b, uint32_t parity) {
     if (*s_err) return;
-    if (!sm100::mbar_wait_cluster(b, parity)) *s_err = 1;
+    if (!sm100::mbar_wait(b, parity)) *s_err = 1;
   };
   pdl_wait();
   pdl_trigger();
@@ -413,7 +415,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (leader)
         for (unsigned i = n > kStages ? n - kStages : 0; i < n; ++i)
-          sm100::mbar_wait_cluster(&full[i % kStages], (i / kStages) & 1u);
+          sm100::mbar_wait(&full[i % kStages], (i / kStages) & 1u);
     }
     if (warp == 9 && leader && sm100::elect_one()) {
       // -------------------------------------------------------- MMA issue (leader)
@@ -433,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (uint32_t r = 0; r < 2; ++r) sm100::mma_commit_pair(sm100::mapa_shared(sm100::smem_u32(&tfull[bf]), r));
       }
       sm100::mma_commit_pair(sm100::mapa_shared(sm100::smem_u32(drained), 0));
-      if (!sm100::mbar_wait_cluster(drained, 0)) *s_err = 1;
+      if (!sm100::mbar_wait(drained, 0)) *s_err = 1;
     }
   } else {
     // ---------------------------------------------------------- scale, add, store: 8 warps
@@ -450,14 +452,18 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int m = tm * BM + static_cast<int>(rank) * 128 + row, n0 = tn * BN + g * 128;
       const float* sx = a.sx + min(m, a.M - 1);
       const float* sw = a.sw + static_cast<int64_t>(min(n0, a.N - 1) / kBlock) * a.kblocks;
-      auto scale = [&](int kb) { return kb < k1 ? __ldg(sx + kb * a.lds) * __ldg(sw + kb) : 0.f; };
-      float s0 = scale(k0), s1 = scale(k0 + 1);
+      // Loaded two blocks ahead, multiplied where they are used.
+      auto scale = [&](int kb) {
+        return kb < k1 ? make_float2(__ldg(sx + kb * a.lds), __ldg(sw + kb)) : make_float2(0.f, 0.f);
+      };
+      float2 s0 = scale(k0), s1 = scale(k0 + 1);
       uint64_t acc[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) acc[i] = 0;
       for (int kb = k0; kb < k1; ++kb, ++n) {
         const int bf = n & 1;
-        const uint64_t s = pack64(__float_as_uint(s0), __float_as_uint(s0));
+        const float sf = s0.x * s0.y;
+        const uint64_t s = pack64(__float_as_uint(sf), __float_as_uint(sf));
         s0 = s1;
         s1 = scale(kb + 2);
         wait(&tfull[bf], (n >> 1) & 1u);
@@ -471,7 +477,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (c == 64) {  // the accumulator is read: the next block but one may overwrite it
             sm100::tc_fence_before();
             __syncwarp();
-            if (lane == 0) sm100::mbar_arrive_cluster(free_bar[bf]);
+            if (lane == 0) sm100::mbar_arrive_remote(free_bar[bf]);
           }
 #pragma unroll
           for (int e = 0; e < 64; e += 2) acc[(c + e) / 2] = fma2(pack64(r[e], r[e + 1]), s, acc[(c + e) / 2]);

@@ -247,6 +247,12 @@ SM100_DEV bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, uint64_t limit_
 SM100_DEV void mbar_arrive_cluster(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
+// The same with the ordering of this CTA only: enough where the arrival hands over
+// tensor memory (ordered by tcgen05.fence) and no shared or global data. The
+// form above waits for the thread's outstanding global accesses at each arrival.
+SM100_DEV void mbar_arrive_remote(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
 // Tiled load into this CTA's shared memory whose completion is counted on the
 // barrier at `bar_cluster_addr` (the pair leader's); no multicast.
 SM100_DEV void tma_load_2d_pair(void* smem_dst, const CUtensorMap* map, uint32_t bar_cluster_addr, int x, int y) {

@@ -16,6 +16,7 @@
 //                   O_t in tensor memory; a thread owns one row
 //   warp 8          TMA producer: a lane loads one run of tokens of one page
 //   warp 9          TMEM allocation and MMA issue (one thread)
+//   warp 10         walks the CTA's items and hands them to the others
 //
 // Steps alternate between the two groups, so that one's products run during
 // the other's softmax. What the groups work on depends on the block's rows:
@@ -140,7 +141,7 @@ struct Cfg {
   static constexpr uint32_t kQ = 0;                         // two tiles of queries
   static constexpr uint32_t kRing = 2 * kTileBytes;
   static constexpr uint32_t kMisc = kRing + kSlots * kTileBytes;
-  static constexpr size_t kSmem = 1024 + kMisc + 768;
+  static constexpr size_t kSmem = 1024 + kMisc + 1024;
 };
 
 constexpr int kThreads = 384;
@@ -153,17 +154,21 @@ struct Barriers {
   uint64_t sfull[2];           // S_t computed (and the O_t of the step before)
   uint64_t pready[2];          // P_t written, O_t rescaled
   uint64_t ofull[2];           // last P V of group t in a block done
+  uint64_t gsync;              // the eight softmax warps
+  uint64_t ifull[4], iempty[4];  // ring of items
   uint64_t drained;
 };
+constexpr int kItems = 4;
 struct Misc {
   Barriers bar;
+  Item item[kItems];  // rows == 0: no more
   int64_t red[33];
   Part part;
   uint32_t tmem;
   int err;
   unsigned bad;  // rows of a 32-row block that came out as NaN
 };
-static_assert(sizeof(Misc) <= 768, "miscellaneous shared memory");
+static_assert(sizeof(Misc) <= 1024, "miscellaneous shared memory");
 
 // exp2 of the arguments that a softmax makes: 0 below the normal numbers.
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -171,7 +176,27 @@ __device__ __forceinline__ float fast_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void group_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t pack64(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(__float_as_uint(lo)), "r"(__float_as_uint(hi)));
+  return r;
+}
+__device__ __forceinline__ float2 unpack64(uint64_t v) {
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+  return make_float2(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
 
 template <typename T>
 struct Weights;
@@ -236,6 +261,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::mbar_init(&bar.pready[i], 4);
       sm100::mbar_init(&bar.ofull[i], 1);
     }
+    for (int i = 0; i < kItems; ++i) {
+      sm100::mbar_init(&bar.ifull[i], 1);
+      sm100::mbar_init(&bar.iempty[i], 10);  // producer, MMA issue, eight softmax warps
+    }
+    sm100::mbar_init(&bar.gsync, 8);
     sm100::mbar_init(&bar.drained, 1);
     misc.err = 0;
     misc.bad = 0;
@@ -263,15 +293,30 @@ __global__ void __launch_bounds__(kThreads, 1)
   // 168 registers a thread at launch: 88 for the last warpgroup and 208 for the two of the softmax.
   if (warp >= 8) {
     sm100::reg_give<88>();
-    Walk walk;
-    walk.start(a, group, misc.part);
-    Item it;
+    if (warp == 10) {
+      // ---------------------------------------------------------- items
+      if (lane == 0) {
+        Walk walk;
+        walk.start(a, group, misc.part);
+        for (unsigned i = 0;; ++i) {
+          Item it;
+          const bool more = walk.next(a, group, it) && !*s_err;
+          if (!more) it.rows = 0;
+          wait(&bar.iempty[i % kItems], ((i / kItems) & 1u) ^ 1u);
+          misc.item[i % kItems] = it;
+          sm100::mbar_arrive(&bar.ifull[i % kItems]);
+          if (!more) break;
+        }
+      }
+    }
     if (warp == 8) {
       // ------------------------------------------------------------ TMA producer
       const int boxes = kTile / box;           // page runs of a tile
       unsigned count = 0;                      // loads issued so far
-      while (walk.next(a, group, it)) {
-        if (__any_sync(0xffffffffu, *s_err)) break;
+      for (unsigned item = 0;; ++item) {
+        wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
+        const Item& it = misc.item[item % kItems];
+        if (__any_sync(0xffffffffu, *s_err || it.rows == 0)) break;
         const Steps st(it);
         if (it.over && lane == 0) atomicExch(a.err, kErrPage);
         for (int i = 0; i < 2 * st.nt; ++i, ++count) {
@@ -299,6 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                (j / boxes) * 64, it.h, slot, page);
           __syncwarp();
         }
+        if (lane == 0) sm100::mbar_arrive(&bar.iempty[item % kItems]);
       }
       // Never leave while a copy into this CTA's shared memory is in flight.
       if (lane == 0)
@@ -311,8 +357,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         unsigned nq[2] = {0, 0}, np[2] = {0, 0};
         auto slot_of = [&](int i) { return (base + i) % kSlots; };
         auto phase_of = [&](int i) { return ((base + i) / kSlots) & 1u; };
-        while (walk.next(a, group, it) && !*s_err) {
+        for (unsigned item = 0;; ++item) {
+          wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
+          const Item& it = misc.item[item % kItems];
+          if (*s_err || it.rows == 0) break;
           const Steps st(it);
+          sm100::mbar_arrive(&bar.iempty[item % kItems]);
           const int steps = st.count();
           wait(&bar.qready[0], nq[0]++ & 1u);
           if (st.wide) wait(&bar.qready[1], nq[1]++ & 1u);
@@ -361,16 +411,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   } else {
     // ------------------------------------------------------------ softmax
     sm100::reg_take<208>();
-    Walk walk;
-    walk.start(a, group, misc.part);
-    Item it;
     const int t = warp >> 2, w4 = warp & 3;
     const int row = w4 * 32 + lane;  // row of the group's tile
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
     const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + kColO + t * 128;
-    unsigned ns = 0, no = 0, base = 0;  // steps, blocks ends and loads so far
-    bool have = walk.next(a, group, it);
+    unsigned ns = 0, no = 0, ng = 0, base = 0;  // steps, block ends, group syncs and loads so far
     bool q_loaded = false;
+    // All softmax warps (not a barrier that a warp which gave up would leave the others at).
+    auto group_sync = [&] {
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&bar.gsync);
+      wait(&bar.gsync, ng++ & 1u);
+    };
+    auto more = [&](unsigned i) {
+      wait(&bar.ifull[i % kItems], (i / kItems) & 1u);
+      return !__any_sync(0xffffffffu, *s_err || misc.item[i % kItems].rows == 0);
+    };
 
     // Writes the queries of an item into this group's tile (or, with at most
     // 128 rows, group 0 into its own).
@@ -401,7 +457,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) sm100::mbar_arrive(&bar.qready[t]);
     };
 
-    while (have) {
+    for (unsigned item = 0; more(item); ++item) {
+      const Item& it = misc.item[item % kItems];
       const Steps st(it);
       const int steps = st.count();
       const bool wide = st.wide, quad = it.rows <= 32;
@@ -467,21 +524,23 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
             const float shift = m == -INFINITY ? 0.f : Weights<T>::kBias - m * scale_log2;
-            float sum[4] = {0.f, 0.f, 0.f, 0.f};
+            const uint64_t scale2 = pack64(scale_log2, scale_log2), shift2 = pack64(shift, shift);
+            uint64_t sum[2] = {0, 0};
 #pragma unroll
             for (int c = 0; c < kCols; c += 32) {
               uint32_t p[16];
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
-                const float p0 = fast_exp2(fmaf(__uint_as_float(x[c + e]), scale_log2, shift));
-                const float p1 = fast_exp2(fmaf(__uint_as_float(x[c + e + 1]), scale_log2, shift));
-                sum[e & 2] += p0;
-                sum[(e & 2) + 1] += p1;
+                const float2 y = unpack64(
+                    fma2(pack64(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1])), scale2, shift2));
+                const float p0 = fast_exp2(y.x), p1 = fast_exp2(y.y);
+                sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], pack64(p0, p1));
                 p[e / 2] = pack2<T>(p0, p1);
               }
               sm100::tmem_st_32x32b_x16(tS + (first + c) / 2, p);
             }
-            l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+            const float2 all = unpack64(add2(sum[0], sum[1]));
+            l += all.x + all.y;
             if constexpr (kCols < 128) {
               // The other quarters' tokens have no weight in this warp's rows.
               const uint32_t zero[16] = {};
@@ -520,10 +579,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       base += 2 * st.nt;
 
       // ---------------------------------------------------------- end of the block's part
-      Item next = it;
-      const bool more = walk.next(a, group, next);
-      if (more && wide) {  // this group's last S is done: its queries are free
-        load_q(next);
+      if (wide && more(item + 1)) {  // this group's last S is done: its queries are free
+        load_q(misc.item[(item + 1) % kItems]);
         q_loaded = true;
       }
       if (mine > 0) {
@@ -715,8 +772,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         group_sync();  // the queries' memory is free again
       }
       sm100::tc_fence_before();
-      it = next;
-      have = more;
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(&bar.iempty[item % kItems]);
     }
   }
 
