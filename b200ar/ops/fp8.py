@@ -33,15 +33,6 @@ def _blocks(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def _rows_2d(x: torch.Tensor) -> torch.Tensor:
-    """[rows, K] with contiguous rows on 16-byte boundaries (copied if x has none)."""
-    x2 = x.reshape(-1, x.shape[-1])
-    step = 16 // x2.element_size()
-    if (x2.shape[1] > 1 and x2.stride(1) != 1) or x2.stride(0) % step or x2.data_ptr() % 16:
-        x2 = x2.clone(memory_format=torch.contiguous_format)
-    return x2
-
-
 def _check_input(t: torch.Tensor, name: str) -> None:
     if t.dim() < 1 or t.dtype not in _FLOATS:
         raise TypeError(f"{name} must be bfloat16, float16 or float32")
@@ -54,33 +45,22 @@ def quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
     The scales are a view of storage that keeps the rows of a block together,
     which is what ``linear_fp8`` reads."""
+    if x.is_cuda:
+        return _C.quantize_fp8(x)
     _check_input(x, "x")
-    x2 = _rows_2d(x)
-    m, k = x2.shape
-    codes = torch.empty(m, k, dtype=torch.float8_e4m3fn, device=x.device)
-    scale = torch.empty(_blocks(k), m, dtype=torch.float32, device=x.device)
-    if x.device.type == "cpu":
-        ref_codes, ref_scale = ref_quantize_fp8(x2)
-        codes.copy_(ref_codes)
-        scale.copy_(ref_scale.t())
-    else:
-        _C.quantize_fp8(x2, codes, scale)
-    return codes.view(x.shape), scale.t().unflatten(0, x.shape[:-1]) if x.dim() > 1 else scale.t()[0]
+    codes, scale = ref_quantize_fp8(x.reshape(-1, x.shape[-1]))
+    return codes.view(x.shape), scale.t().contiguous().t().view(*x.shape[:-1], -1)
 
 
 def quantize_fp8_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """``w`` [N, K] -> (codes float8_e4m3fn [N, K], scales fp32 [ceil(N / 128), ceil(K / 128)])."""
+    if w.is_cuda:
+        error_word(w.device)  # exists before a graph that uses it is captured
+        return _C.quantize_fp8_weight(w)
     if w.dim() != 2:
         raise ValueError("w must be [N, K]")
     _check_input(w, "w")
-    n, k = w.shape
-    if w.device.type == "cpu":
-        return ref_quantize_fp8_weight(w)
-    error_word(w.device)  # exists before a graph that uses it is captured
-    codes = torch.empty(n, k, dtype=torch.float8_e4m3fn, device=w.device)
-    scale = torch.empty(_blocks(n), _blocks(k), dtype=torch.float32, device=w.device)
-    _C.quantize_fp8_weight(_rows_2d(w), codes, scale)
-    return codes, scale
+    return ref_quantize_fp8_weight(w)
 
 
 def linear_fp8(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor, out: Optional[torch.Tensor] = None,
@@ -92,6 +72,9 @@ def linear_fp8(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor, out: O
     is of ``dtype`` (bf16 or fp16). K must be a multiple of 16 and N of 8.
     Products are exact, sums fp32, and each block of 128 along K is scaled
     before it is added."""
+    if x.is_cuda:  # checked there
+        like = None if x_scale is None else _like(dtype)
+        return _C.linear_fp8(x, w_q, w_scale, out, x_scale, like, error_word(x.device))
     if w_q.dim() != 2 or w_q.dtype != torch.float8_e4m3fn or not w_q.is_contiguous():
         raise TypeError("w_q must be contiguous float8_e4m3fn [N, K]")
     n, k = w_q.shape
@@ -121,22 +104,20 @@ def linear_fp8(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor, out: O
         out = torch.empty(shape, dtype=dtype, device=x.device)
     elif tuple(out.shape) != shape or out.dtype != dtype or out.device != x.device:
         raise ValueError(f"out must be {dtype} {list(shape)} on {x.device}")
-    out2 = out.view(-1, n)
-    if x_scale is None:
-        x2, scale = _rows_2d(x), None
-    else:
-        x2 = x.reshape(-1, k).contiguous()
-        if x2.data_ptr() % 16:
-            x2 = x2.clone()
-        scale = x_scale.reshape(-1, _blocks(k)).t()
-        if (x2.shape[0] > 1 and scale.stride(1) != 1) or scale.stride(0) < x2.shape[0]:
-            scale = scale.contiguous()
-    if x.device.type == "cpu":
-        codes, scale = ref_quantize_fp8(x2) if scale is None else (x2, scale.t())
-        out2.copy_(ref_linear_fp8(codes, scale, w_q, w_scale).to(dtype))
-        return out
-    _C.linear_fp8(x2, scale, w_q, w_scale, out2, error_word(x.device))
+    x2 = x.reshape(-1, k)
+    codes, scale = ref_quantize_fp8(x2) if x_scale is None else (x2, x_scale.reshape(-1, _blocks(k)))
+    out.view(-1, n).copy_(ref_linear_fp8(codes, scale, w_q, w_scale).to(dtype))
     return out
+
+
+_LIKE = {}
+
+
+def _like(dtype: torch.dtype) -> torch.Tensor:
+    """An empty tensor that carries a type into the native call."""
+    if dtype not in _LIKE:
+        _LIKE[dtype] = torch.empty(0, dtype=dtype)
+    return _LIKE[dtype]
 
 
 # ------------------------------------------------------------------ references

@@ -19,10 +19,12 @@ _ERR: Dict[int, torch.Tensor] = {}
 
 def error_word(device) -> torch.Tensor:
     """Per-device int32 that a kernel sets when one of its bounded waits expires."""
-    idx = torch.device(device).index or 0
-    if idx not in _ERR:
-        _ERR[idx] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-    return _ERR[idx]
+    idx = device.index if isinstance(device, torch.device) else torch.device(device).index
+    idx = idx or 0
+    word = _ERR.get(idx)
+    if word is None:
+        word = _ERR[idx] = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
+    return word
 
 
 # What the codes of the error word above the bounded waits' say.

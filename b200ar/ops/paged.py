@@ -122,6 +122,9 @@ def qk_norm_rope_paged(qkv: torch.Tensor, batch: PagedBatch, rot: RotaryTable, k
     (``qkv[:, :hq * d].view(rows, hq, d)``). fp32 inside, rounded once.
     A row whose position has no page, or is outside ``rot``, is skipped.
     """
+    if qkv.is_cuda:  # checked there
+        return _C.qk_norm_rope_paged(qkv, batch.page_table, batch.kv_len, batch.q_start, rot.cos, rot.sin, k_pages,
+                                     v_pages, hq, hkv, q_gamma, k_gamma, q_out, error_word(qkv.device), eps)
     d = rot.head_dim
     if hq < 1 or hkv < 1:
         raise ValueError("hq and hkv must be positive")
@@ -147,11 +150,7 @@ def qk_norm_rope_paged(qkv: torch.Tensor, batch: PagedBatch, rot: RotaryTable, k
     for t, name in ((q_out, "q_out"), (k_pages, "k_pages"), (v_pages, "v_pages")):
         if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
             raise ValueError(f"{name} is written and must not be expanded")
-    if qkv.device.type == "cpu":
-        ref_qk_norm_rope_paged(qkv, batch, rot, k_pages, v_pages, hq, hkv, q_gamma, k_gamma, eps, q_out)
-        return q_out
-    _C.qk_norm_rope_paged(qkv, batch.page_table, batch.kv_len, batch.q_start, rot.cos, rot.sin, k_pages, v_pages,
-                          q_gamma, k_gamma, q_out, error_word(qkv.device), float(eps))
+    ref_qk_norm_rope_paged(qkv, batch, rot, k_pages, v_pages, hq, hkv, q_gamma, k_gamma, eps, q_out)
     return q_out
 
 
@@ -168,6 +167,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Nothing behind a sequence's length, and nothing that a row's mask hides,
     reaches its output, whatever the pages hold there.
     """
+    if q.is_cuda:  # checked there
+        return _C.paged_attention(q, k_pages, v_pages, batch.page_table, batch.kv_len, batch.q_start, out,
+                                  error_word(q.device), scale, causal, window)
     if q.dim() != 3:
         raise ValueError("q must be [rows, heads, d]")
     rows, hq, d = q.shape
@@ -194,12 +196,7 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     for t, name in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages")):
         if _overlaps(out3, t):
             raise ValueError(f"out overlaps {name}")
-    if q.device.type == "cpu":
-        ref_paged_attention(q, k_pages, v_pages, batch, scale, causal, window, out3)
-        return out
-    window = min(int(window), 2**31 - 1)
-    _C.paged_attention(q, k_pages, v_pages, batch.page_table, batch.kv_len, batch.q_start, out3,
-                       error_word(q.device), float(scale), bool(causal), window)
+    ref_paged_attention(q, k_pages, v_pages, batch, scale, causal, window, out3)
     return out
 
 

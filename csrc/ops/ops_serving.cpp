@@ -1,14 +1,18 @@
 // Binds the serving operators: paged rotary step, paged attention, 8-bit linear.
 //
-// Every check of types, sizes, strides and devices that keeps a kernel inside
-// its tensors is made here; what only the device knows (lengths, offsets,
-// pages) is checked by the kernels, which leave a code in the error word.
+// Every check of types, sizes, strides and devices of a CUDA call is made here,
+// in one native call (the Python side would take longer than a small kernel);
+// what only the device knows (lengths, offsets, pages) is checked by the
+// kernels, which leave a code in the error word.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
 #include <algorithm>
+#include <cmath>
 #include <optional>
+#include <utility>
+#include <vector>
 
 #include "../fp8/fp8.h"
 #include "../paged/paged.h"
@@ -21,64 +25,82 @@ namespace {
 using b200ar::paged::Batch;
 using b200ar::paged::Half;
 using b200ar::paged::Pool;
+using OptTensor = std::optional<at::Tensor>;
 
 constexpr int64_t kInt = 0x7fffffff;
 
+#define VALUE_CHECK(cond, ...) \
+  if (!(cond)) throw py::value_error(c10::str(__VA_ARGS__))
+#define TYPE_CHECK(cond, ...) \
+  if (!(cond)) throw py::type_error(c10::str(__VA_ARGS__))
+
 cudaStream_t stream_of() { return at::cuda::getCurrentCUDAStream().stream(); }
 
+bool aligned(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+
 void check_device(const at::Tensor& t, const at::Tensor& like, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), name, " must be on ", like.device(), ", got ", t.device());
+  VALUE_CHECK(t.device() == like.device(), name, " must be on ", like.device(), ", got ", t.device());
 }
 
-// [rows, heads, d] with any strides that keep 16-byte packets aligned.
-void check_rows(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.dim() == 3 && t.size(0) <= kInt && t.size(1) <= 65535, name, " must be [rows, heads, d]");
-  TORCH_CHECK(t.stride(2) == 1 && t.stride(1) % 8 == 0 && t.stride(0) % 8 == 0 && t.stride(0) >= 0 && t.stride(1) >= 0 &&
-                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              name, " must have contiguous heads that start on 16-byte boundaries");
+// Heads of d contiguous elements on 16-byte boundaries in every dimension before them; `written` ones must not
+// share memory among themselves.
+void check_heads(const at::Tensor& t, const char* name, bool written) {
+  bool ok = t.stride(-1) == 1 && aligned(t);
+  for (int64_t i = 0; i + 1 < t.dim(); ++i) {
+    ok = ok && (t.size(i) <= 1 || (t.stride(i) % 8 == 0 && t.stride(i) >= 0));
+    VALUE_CHECK(!written || t.size(i) <= 1 || t.stride(i) != 0, name, " is written and must not be expanded");
+  }
+  VALUE_CHECK(ok, name, " must have contiguous heads that start on 16-byte boundaries");
 }
 
-Half half_of(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf, name, " must be bfloat16 or float16");
+// Whether the address ranges of two tensors meet.
+bool overlaps(const at::Tensor& a, const at::Tensor& b) {
+  if (a.numel() == 0 || b.numel() == 0) return false;
+  const auto span = [](const at::Tensor& t) {
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    const uintptr_t p = reinterpret_cast<uintptr_t>(t.data_ptr());
+    return std::make_pair(p, p + (last + 1) * t.element_size());
+  };
+  const auto x = span(a), y = span(b);
+  return x.first < y.second && y.first < x.second;
+}
+
+Half half_of(const at::Tensor& t) {
+  TYPE_CHECK(t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf,
+             "paged ops take bfloat16 or float16, got ", t.scalar_type());
   return t.scalar_type() == at::kBFloat16 ? Half::kBf16 : Half::kFp16;
 }
 
 Pool pool_of(const at::Tensor& t, const at::Tensor& like, const at::Tensor& first, int64_t hkv, int64_t d,
-             const char* name) {
+             const char* name, bool written) {
+  VALUE_CHECK(t.dim() == 4 && t.sizes() == first.sizes() && t.size(2) == hkv && t.size(3) == d, name,
+              " must be [pages, page_size, ", hkv, ", ", d, "]");
+  TYPE_CHECK(t.scalar_type() == like.scalar_type(), name, " must have the type of the input, ", like.scalar_type());
   check_device(t, like, name);
-  TORCH_CHECK(t.scalar_type() == like.scalar_type(), name, " must have the type of the queries");
-  TORCH_CHECK(t.dim() == 4 && t.size(2) == hkv && t.size(3) == d && t.sizes() == first.sizes(), name,
-              " must be [pages, page_size, kv_heads, d]");
-  TORCH_CHECK(t.size(0) >= 1 && t.size(0) < kInt && t.size(1) >= 1 && t.size(1) <= 65536, name,
+  VALUE_CHECK(t.size(0) >= 1 && t.size(0) < kInt && t.size(1) >= 1 && t.size(1) <= 65536, name,
               " must have pages of 1 to 65536 tokens");
-  TORCH_CHECK(t.stride(3) == 1 && t.stride(2) % 8 == 0 && t.stride(1) % 8 == 0 && t.stride(0) % 8 == 0 &&
-                  t.stride(0) >= 0 && t.stride(1) >= 0 && t.stride(2) >= 0 &&
-                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              name, " must have contiguous heads that start on 16-byte boundaries");
-  for (int i = 0; i < 3; ++i) TORCH_CHECK(t.size(i) == 1 || t.stride(i) > 0, name, " must not be expanded");
+  check_heads(t, name, written);
+  for (int i = 0; i < 3; ++i) VALUE_CHECK(t.size(i) == 1 || t.stride(i) > 0, name, " must not be expanded");
   return Pool{t.data_ptr(), t.stride(0), t.stride(1), t.stride(2)};
 }
 
-Batch batch_of(const at::Tensor& table, const at::Tensor& kv_len, const std::optional<at::Tensor>& q_start,
-               const at::Tensor& like, int64_t rows) {
-  check_device(table, like, "page_table");
-  check_device(kv_len, like, "kv_len");
-  TORCH_CHECK(table.scalar_type() == at::kInt && table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1) &&
-                  table.stride(0) >= 0 && table.size(0) < kInt && table.size(1) < kInt,
-              "page_table must be int32 [sequences, pages] with contiguous rows");
+// Types and shapes of the batch were checked when it was made (PagedBatch).
+Batch batch_of(const at::Tensor& table, const at::Tensor& kv_len, const OptTensor& q_start, const at::Tensor& like,
+               int64_t rows) {
+  check_device(table, like, "the batch");
   const int64_t seqs = table.size(0);
-  TORCH_CHECK(kv_len.scalar_type() == at::kInt && kv_len.dim() == 1 && kv_len.size(0) == seqs &&
-                  kv_len.is_contiguous(),
-              "kv_len must be int32 [sequences]");
+  TORCH_CHECK(table.scalar_type() == at::kInt && kv_len.scalar_type() == at::kInt && kv_len.numel() == seqs &&
+                  kv_len.device() == table.device() && table.size(1) < kInt && seqs < kInt && rows < kInt,
+              "bad batch");
   Batch b{};
   if (q_start.has_value()) {
-    check_device(*q_start, like, "q_start");
-    TORCH_CHECK(q_start->scalar_type() == at::kInt && q_start->dim() == 1 && q_start->size(0) == seqs + 1 &&
-                    q_start->is_contiguous(),
-                "q_start must be int32 [sequences + 1]");
+    TORCH_CHECK(q_start->scalar_type() == at::kInt && q_start->numel() == seqs + 1 &&
+                    q_start->device() == table.device(),
+                "bad batch");
     b.q_start = q_start->data_ptr<int>();
   } else {
-    TORCH_CHECK(rows == seqs, "without q_start every sequence has one new token: ", seqs, " sequences, ", rows,
+    VALUE_CHECK(rows == seqs, "without q_start every sequence has one new token: ", seqs, " sequences, ", rows,
                 " rows");
   }
   b.page_table = table.data_ptr<int>();
@@ -90,29 +112,29 @@ Batch batch_of(const at::Tensor& table, const at::Tensor& kv_len, const std::opt
 }
 
 int* err_of(const at::Tensor& err, const at::Tensor& like) {
-  check_device(err, like, "err");
-  TORCH_CHECK(err.scalar_type() == at::kInt && err.numel() >= 1, "err must be a CUDA int32");
+  TORCH_CHECK(err.device() == like.device() && err.scalar_type() == at::kInt && err.numel() >= 1,
+              "err must be a CUDA int32");
   return err.data_ptr<int>();
 }
 
-b200ar::fp8::Type fp8_type(const at::Tensor& t, bool wide, const char* name) {
-  if (t.scalar_type() == at::kBFloat16) return b200ar::fp8::Type::kBf16;
-  if (t.scalar_type() == at::kHalf) return b200ar::fp8::Type::kFp16;
-  TORCH_CHECK(wide && t.scalar_type() == at::kFloat, name, " must be bfloat16", wide ? ", float16 or float32" : " or float16");
+void check_head_dim(int64_t d) { VALUE_CHECK(d == 64 || d == 128, "head dimension must be 64 or 128, got ", d); }
+
+b200ar::fp8::Type fp8_type(at::ScalarType t, bool wide, const char* name) {
+  if (t == at::kBFloat16) return b200ar::fp8::Type::kBf16;
+  if (t == at::kHalf) return b200ar::fp8::Type::kFp16;
+  TYPE_CHECK(wide && t == at::kFloat, name, " must be bfloat16", wide ? ", float16 or float32" : " or float16");
   return b200ar::fp8::Type::kFp32;
 }
 
-void check_rows_2d(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) &&
-                  t.stride(0) * t.element_size() % 16 == 0 && t.stride(0) >= 0 &&
-                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              name, " must be a 2-D CUDA tensor with contiguous rows that start on 16-byte boundaries");
-}
+void check_k(int64_t k) { VALUE_CHECK(k >= 1 && k % 16 == 0, "K must be a positive multiple of 16, got ", k); }
 
-void check_codes(const at::Tensor& t, const char* name) {
-  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && t.is_contiguous() && t.scalar_type() == at::kFloat8_e4m3fn &&
-                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              name, " must be a contiguous 2-D float8_e4m3fn CUDA tensor");
+// [rows, K] with contiguous rows on 16-byte boundaries; copied if x is not laid out like that.
+at::Tensor rows_2d(const at::Tensor& x) {
+  const at::Tensor t = x.dim() == 2 ? x : x.reshape({-1, x.size(-1)});
+  if ((t.size(1) <= 1 || t.stride(1) == 1) && aligned(t) && t.stride(0) >= 0 &&
+      (t.size(0) <= 1 || t.stride(0) * t.element_size() % 16 == 0))
+    return t;
+  return t.clone(at::MemoryFormat::Contiguous);
 }
 
 }  // namespace
@@ -120,92 +142,115 @@ void check_codes(const at::Tensor& t, const char* name) {
 void register_serving_ops(py::module& m) {
   m.def(
       "qk_norm_rope_paged",
-      [](const at::Tensor& qkv, const at::Tensor& table, const at::Tensor& kv_len,
-         const std::optional<at::Tensor>& q_start, const at::Tensor& cos_t, const at::Tensor& sin_t,
-         at::Tensor& k_pages, at::Tensor& v_pages, const std::optional<at::Tensor>& q_gamma,
-         const std::optional<at::Tensor>& k_gamma, at::Tensor& q_out, at::Tensor& err, double eps) {
-        TORCH_CHECK(qkv.is_cuda() && qkv.dim() == 2, "qkv must be a CUDA tensor [rows, (hq + 2 hkv) * d]");
-        const Half type = half_of(qkv, "qkv");
-        check_rows(q_out, "q_out");
-        check_device(q_out, qkv, "q_out");
-        TORCH_CHECK(q_out.scalar_type() == qkv.scalar_type() && q_out.size(0) == qkv.size(0),
-                    "q_out must have the type and the rows of qkv");
-        TORCH_CHECK(k_pages.dim() == 4, "k_pages must be [pages, page_size, kv_heads, d]");
-        const int64_t hq = q_out.size(1), d = q_out.size(2), hkv = k_pages.size(2);
-        TORCH_CHECK(hq >= 1 && hkv >= 1 && qkv.size(1) == (hq + 2 * hkv) * d, "qkv must be [rows, (hq + 2 hkv) * d]");
-        TORCH_CHECK((qkv.stride(1) == 1) && qkv.stride(0) % 8 == 0 && qkv.stride(0) >= 0 &&
-                        reinterpret_cast<uintptr_t>(qkv.data_ptr()) % 16 == 0,
-                    "qkv must have contiguous rows that start on 16-byte boundaries");
+      [](const at::Tensor& qkv, const at::Tensor& table, const at::Tensor& kv_len, const OptTensor& q_start,
+         const at::Tensor& cos_t, const at::Tensor& sin_t, const at::Tensor& k_pages, const at::Tensor& v_pages,
+         int64_t hq, int64_t hkv, const OptTensor& q_gamma, const OptTensor& k_gamma, const OptTensor& q_out,
+         const at::Tensor& err, double eps) {
+        VALUE_CHECK(cos_t.dim() == 2, "the rotary table must be fp32 [positions, d / 2]");
+        const int64_t d = 2 * cos_t.size(1);
+        VALUE_CHECK(hq >= 1 && hkv >= 1 && hq <= 65535 && hkv <= 65535, "hq and hkv must be positive");
+        VALUE_CHECK(qkv.dim() == 2 && qkv.size(1) == (hq + 2 * hkv) * d, "qkv must be [rows, (hq + 2 hkv) * ", d,
+                    "]");
+        const Half type = half_of(qkv);
+        check_head_dim(d);
         b200ar::paged::RopeArgs a{};
-        a.k = pool_of(k_pages, qkv, k_pages, hkv, d, "k_pages");
-        a.v = pool_of(v_pages, qkv, k_pages, hkv, d, "v_pages");
-        a.batch = batch_of(table, kv_len, q_start, qkv, qkv.size(0));
-        for (const at::Tensor* t : {&cos_t, &sin_t}) {
-          check_device(*t, qkv, "the rotary table");
-          TORCH_CHECK(t->scalar_type() == at::kFloat && t->dim() == 2 && t->size(1) == d / 2 && t->is_contiguous() &&
-                          t->size(0) < kInt && t->sizes() == cos_t.sizes(),
-                      "the rotary table must be fp32 [positions, d / 2]");
-        }
-        TORCH_CHECK(q_gamma.has_value() == k_gamma.has_value(), "give the norm weights of both q and k, or neither");
+        a.k = pool_of(k_pages, qkv, k_pages, hkv, d, "k_pages", true);
+        a.v = pool_of(v_pages, qkv, k_pages, hkv, d, "v_pages", true);
+        check_heads(qkv, "qkv", false);
+        const int64_t rows = qkv.size(0);
+        a.batch = batch_of(table, kv_len, q_start, qkv, rows);
+        for (const at::Tensor* t : {&cos_t, &sin_t})
+          VALUE_CHECK(t->scalar_type() == at::kFloat && t->sizes() == cos_t.sizes() && t->is_contiguous() &&
+                          t->device() == qkv.device() && t->size(0) < kInt && aligned(*t),
+                      "the rotary table must be contiguous fp32 [positions, d / 2] on ", qkv.device());
+        VALUE_CHECK(q_gamma.has_value() == k_gamma.has_value(), "give the norm weights of both q and k, or neither");
         if (q_gamma.has_value())
-          for (const at::Tensor* t : {&*q_gamma, &*k_gamma}) {
-            check_device(*t, qkv, "the norm weights");
-            TORCH_CHECK(t->scalar_type() == qkv.scalar_type() && t->numel() == d && t->is_contiguous() &&
-                            reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
-                        "the norm weights must be [d], of the type of qkv");
-          }
+          for (const at::Tensor* t : {&*q_gamma, &*k_gamma})
+            VALUE_CHECK(t->scalar_type() == qkv.scalar_type() && t->dim() == 1 && t->size(0) == d &&
+                            t->is_contiguous() && t->device() == qkv.device() && aligned(*t),
+                        "the norm weights must be [", d, "], of the type and on the device of qkv");
+        const at::cuda::OptionalCUDAGuard guard(device_of(qkv));
+        at::Tensor q;
+        if (q_out.has_value()) {
+          q = *q_out;
+          VALUE_CHECK(q.dim() == 3 && q.size(0) == rows && q.size(1) == hq && q.size(2) == d &&
+                          q.scalar_type() == qkv.scalar_type() && q.device() == qkv.device(),
+                      "q_out must be [rows, hq, d], of the type and on the device of qkv");
+          check_heads(q, "q_out", true);
+          const bool in_place = q.data_ptr() == qkv.data_ptr() && (rows <= 1 || q.stride(0) == qkv.stride(0)) &&
+                                (hq == 1 || q.stride(1) == d);
+          VALUE_CHECK(in_place || !overlaps(q, qkv), "q_out overlaps qkv but is not its q part");
+        } else {
+          q = at::empty({rows, hq, d}, qkv.options());
+        }
         a.qkv = qkv.data_ptr();
         a.q_gamma = q_gamma.has_value() ? q_gamma->data_ptr() : nullptr;
         a.k_gamma = k_gamma.has_value() ? k_gamma->data_ptr() : nullptr;
         a.cos_t = cos_t.data_ptr<float>();
         a.sin_t = sin_t.data_ptr<float>();
-        a.q_out = q_out.data_ptr();
+        a.q_out = q.data_ptr();
         a.qkv_stride = qkv.stride(0);
-        a.q_tok = q_out.stride(0);
-        a.q_head = q_out.stride(1);
+        a.q_tok = q.stride(0);
+        a.q_head = q.stride(1);
         a.err = err_of(err, qkv);
-        a.rows = static_cast<int>(qkv.size(0));
+        a.rows = static_cast<int>(rows);
         a.hq = static_cast<int>(hq);
         a.hkv = static_cast<int>(hkv);
         a.positions = static_cast<int>(cos_t.size(0));
         a.num_pages = static_cast<int>(k_pages.size(0));
         a.page_size = static_cast<int>(k_pages.size(1));
         a.eps = static_cast<float>(eps);
-        const at::cuda::OptionalCUDAGuard guard(device_of(qkv));
         b200ar::paged::qk_norm_rope_paged(a, static_cast<int>(d), type, stream_of());
+        return q;
       },
       "norms of q and k, rotary embedding and the write into a paged KV cache", py::arg("qkv"), py::arg("page_table"),
       py::arg("kv_len"), py::arg("q_start"), py::arg("cos_t"), py::arg("sin_t"), py::arg("k_pages"),
-      py::arg("v_pages"), py::arg("q_gamma"), py::arg("k_gamma"), py::arg("q_out"), py::arg("err"), py::arg("eps"));
+      py::arg("v_pages"), py::arg("hq"), py::arg("hkv"), py::arg("q_gamma"), py::arg("k_gamma"), py::arg("q_out"),
+      py::arg("err"), py::arg("eps"));
   m.def(
       "paged_attention",
       [](const at::Tensor& q, const at::Tensor& k_pages, const at::Tensor& v_pages, const at::Tensor& table,
-         const at::Tensor& kv_len, const std::optional<at::Tensor>& q_start, at::Tensor& out, at::Tensor& err,
-         double scale, bool causal, int64_t window) {
-        TORCH_CHECK(q.is_cuda(), "q must be a CUDA tensor");
-        const Half type = half_of(q, "q");
-        check_rows(q, "q");
-        check_rows(out, "out");
-        check_device(out, q, "out");
-        TORCH_CHECK(out.scalar_type() == q.scalar_type() && out.sizes() == q.sizes(), "out must be like q");
-        TORCH_CHECK(k_pages.dim() == 4, "k_pages must be [pages, page_size, kv_heads, d]");
-        const int64_t hq = q.size(1), d = q.size(2), hkv = k_pages.size(2);
-        TORCH_CHECK(hkv >= 1 && hq >= hkv && hq % hkv == 0, "query heads must be a multiple of the KV heads");
-        TORCH_CHECK(k_pages.size(1) % 8 == 0, "the page size must be a multiple of 8");
-        TORCH_CHECK(window >= 0 && window <= kInt && (causal || window == 0),
+         const at::Tensor& kv_len, const OptTensor& q_start, const OptTensor& out_opt, const at::Tensor& err,
+         std::optional<double> scale, bool causal, int64_t window) {
+        VALUE_CHECK(q.dim() == 3, "q must be [rows, heads, d]");
+        const int64_t rows = q.size(0), hq = q.size(1), d = q.size(2);
+        const Half type = half_of(q);
+        check_head_dim(d);
+        VALUE_CHECK(k_pages.dim() == 4, "k_pages must be [pages, page_size, kv_heads, d]");
+        const int64_t hkv = k_pages.size(2);
+        VALUE_CHECK(hkv >= 1 && hq >= hkv && hq <= 65535 && hq % hkv == 0,
+                    "query heads must be a multiple of the KV heads");
+        VALUE_CHECK(k_pages.size(1) % 8 == 0, "the page size must be a multiple of 8, got ", k_pages.size(1));
+        VALUE_CHECK(window >= 0 && (causal || window == 0),
                     "window must be 0 (all) or a number of positions, with causal attention");
         b200ar::paged::AttnArgs a{};
-        a.k = pool_of(k_pages, q, k_pages, hkv, d, "k_pages");
-        a.v = pool_of(v_pages, q, k_pages, hkv, d, "v_pages");
-        a.batch = batch_of(table, kv_len, q_start, q, q.size(0));
+        a.scale = static_cast<float>(scale.has_value() ? *scale : 1.0 / std::sqrt(static_cast<double>(d)));
+        VALUE_CHECK(std::isfinite(a.scale), "scale must be finite");
+        a.k = pool_of(k_pages, q, k_pages, hkv, d, "k_pages", false);
+        a.v = pool_of(v_pages, q, k_pages, hkv, d, "v_pages", false);
+        check_heads(q, "q", false);
+        a.batch = batch_of(table, kv_len, q_start, q, rows);
+        const at::cuda::OptionalCUDAGuard guard(device_of(q));
+        at::Tensor out;
+        a.o_head = d;
+        if (out_opt.has_value()) {
+          out = *out_opt;
+          VALUE_CHECK(out.dim() == 2 && out.size(0) == rows && out.size(1) == hq * d &&
+                          out.scalar_type() == q.scalar_type() && out.device() == q.device(),
+                      "out must be [rows, hq * d], of the type and on the device of q");
+          check_heads(out, "out", true);
+          VALUE_CHECK(!overlaps(out, q) && !overlaps(out, k_pages) && !overlaps(out, v_pages),
+                      "out overlaps an input");
+        } else {
+          out = at::empty({rows, hq * d}, q.options());
+        }
         a.q = q.data_ptr();
         a.out = out.data_ptr();
         a.q_tok = q.stride(0);
         a.q_head = q.stride(1);
         a.o_tok = out.stride(0);
-        a.o_head = out.stride(1);
         a.err = err_of(err, q);
-        a.rows = static_cast<int>(q.size(0));
+        a.rows = static_cast<int>(rows);
         a.hq = static_cast<int>(hq);
         a.hkv = static_cast<int>(hkv);
         a.num_pages = static_cast<int>(k_pages.size(0));
@@ -214,110 +259,139 @@ void register_serving_ops(py::module& m) {
         a.capacity = static_cast<int>(capacity);
         a.window = window >= capacity ? 0 : static_cast<int>(window);  // a window over every position hides nothing
         a.causal = causal;
-        a.scale = static_cast<float>(scale);
-        const at::cuda::OptionalCUDAGuard guard(device_of(q));
         // From the caching allocator on this stream: concurrent calls, eager or captured, never share it.
         const at::Tensor workspace =
-            at::empty({b200ar::paged::paged_attention_workspace(q.size(0), a.hq, a.hkv, static_cast<int>(d))},
+            at::empty({b200ar::paged::paged_attention_workspace(rows, a.hq, a.hkv, static_cast<int>(d))},
                       q.options().dtype(at::kFloat));
         b200ar::paged::paged_attention(a, static_cast<int>(d), type, workspace.data_ptr<float>(), stream_of());
+        return out;
       },
       "attention of new tokens over a paged KV cache", py::arg("q"), py::arg("k_pages"), py::arg("v_pages"),
       py::arg("page_table"), py::arg("kv_len"), py::arg("q_start"), py::arg("out"), py::arg("err"), py::arg("scale"),
       py::arg("causal"), py::arg("window"));
   m.def(
       "quantize_fp8",
-      [](const at::Tensor& x, at::Tensor& q, at::Tensor& scale) {
-        check_rows_2d(x, "x");
-        check_codes(q, "q");
-        check_device(q, x, "q");
-        check_device(scale, x, "scale");
-        const int64_t M = x.size(0), K = x.size(1), blocks = (K + 127) / 128;
-        TORCH_CHECK(q.sizes() == x.sizes(), "q must have the shape of x");
-        TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.dim() == 2 && scale.size(0) == blocks &&
-                        scale.size(1) == M && (M <= 1 || scale.stride(1) == 1) && scale.stride(0) >= M,
-                    "scale must be fp32 [ceil(K / 128), M]");
+      [](const at::Tensor& x) {
+        const b200ar::fp8::Type type = fp8_type(x.scalar_type(), true, "x");
+        VALUE_CHECK(x.dim() >= 1, "x must be [..., K]");
+        check_k(x.size(-1));
         const at::cuda::OptionalCUDAGuard guard(device_of(x));
-        b200ar::fp8::quantize(x.data_ptr(), x.stride(0), static_cast<uint8_t*>(q.data_ptr()),
-                              scale.data_ptr<float>(), scale.stride(0), M, K, fp8_type(x, true, "x"), nullptr, 0,
-                              stream_of());
+        const at::Tensor x2 = rows_2d(x);
+        const int64_t M = x2.size(0), K = x2.size(1), blocks = (K + 127) / 128;
+        at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kFloat8_e4m3fn));
+        at::Tensor scale = at::empty({blocks, M}, x.options().dtype(at::kFloat));
+        b200ar::fp8::quantize(x2.data_ptr(), x2.stride(0), static_cast<uint8_t*>(q.data_ptr()),
+                              scale.data_ptr<float>(), M, M, K, type, nullptr, 0, stream_of());
+        std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+        shape.back() = blocks;
+        std::vector<int64_t> strides(shape.size());
+        strides.back() = M;
+        for (int64_t i = static_cast<int64_t>(shape.size()) - 2, n = 1; i >= 0; --i) {
+          strides[i] = n;
+          n *= shape[i];
+        }
+        return std::make_pair(q, scale.as_strided(shape, strides));
       },
-      "e4m3 values and a scale for each row and block of 128", py::arg("x"), py::arg("q"), py::arg("scale"));
+      "e4m3 values and a scale for each row and block of 128", py::arg("x"));
   m.def(
       "quantize_fp8_weight",
-      [](const at::Tensor& w, at::Tensor& q, at::Tensor& scale) {
-        check_rows_2d(w, "w");
-        check_codes(q, "q");
-        check_device(q, w, "q");
-        check_device(scale, w, "scale");
-        TORCH_CHECK(q.sizes() == w.sizes(), "q must have the shape of w");
-        TORCH_CHECK(scale.scalar_type() == at::kFloat && scale.is_contiguous() && scale.dim() == 2 &&
-                        scale.size(0) == (w.size(0) + 127) / 128 && scale.size(1) == (w.size(1) + 127) / 128,
-                    "scale must be fp32 [ceil(N / 128), ceil(K / 128)]");
+      [](const at::Tensor& w) {
+        const b200ar::fp8::Type type = fp8_type(w.scalar_type(), true, "w");
+        VALUE_CHECK(w.dim() == 2, "w must be [N, K]");
+        check_k(w.size(1));
         const at::cuda::OptionalCUDAGuard guard(device_of(w));
-        b200ar::fp8::quantize_weight(w.data_ptr(), w.stride(0), static_cast<uint8_t*>(q.data_ptr()),
-                                     scale.data_ptr<float>(), w.size(0), w.size(1), fp8_type(w, true, "w"),
-                                     stream_of());
+        const at::Tensor w2 = rows_2d(w);
+        const int64_t N = w2.size(0), K = w2.size(1);
+        at::Tensor q = at::empty({N, K}, w.options().dtype(at::kFloat8_e4m3fn));
+        at::Tensor scale = at::empty({(N + 127) / 128, (K + 127) / 128}, w.options().dtype(at::kFloat));
+        b200ar::fp8::quantize_weight(w2.data_ptr(), w2.stride(0), static_cast<uint8_t*>(q.data_ptr()),
+                                     scale.data_ptr<float>(), N, K, type, stream_of());
+        return std::make_pair(q, scale);
       },
-      "e4m3 values and a scale for each 128 x 128 block", py::arg("w"), py::arg("q"), py::arg("scale"));
+      "e4m3 values and a scale for each 128 x 128 block", py::arg("w"));
   m.def(
       "linear_fp8",
-      [](const at::Tensor& x, const std::optional<at::Tensor>& x_scale, const at::Tensor& w,
-         const at::Tensor& w_scale, at::Tensor& out, at::Tensor& err) {
-        check_codes(w, "w_q");
-        TORCH_CHECK(x.dim() == 2, "x must be [M, K]");
-        const int64_t M = x.size(0), K = x.size(1), N = w.size(0), blocks = (K + 127) / 128;
-        check_device(w, x, "w_q");
-        check_device(out, x, "out");
-        check_device(w_scale, x, "w_scale");
-        TORCH_CHECK(w.size(1) == K, "x and w_q must have the same K");
-        TORCH_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.is_contiguous() && w_scale.dim() == 2 &&
+      [](const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale, const OptTensor& out_opt,
+         const OptTensor& x_scale, const OptTensor& like, const at::Tensor& err) {
+        TYPE_CHECK(w.dim() == 2 && w.scalar_type() == at::kFloat8_e4m3fn && w.is_contiguous() && aligned(w),
+                   "w_q must be contiguous float8_e4m3fn [N, K]");
+        const int64_t N = w.size(0), K = w.size(1), blocks = (K + 127) / 128;
+        check_k(K);
+        VALUE_CHECK(N >= 1 && N % 8 == 0, "N must be a positive multiple of 8, got ", N);
+        VALUE_CHECK(x.dim() >= 1 && x.size(-1) == K, "x must be [..., ", K, "]");
+        VALUE_CHECK(w_scale.scalar_type() == at::kFloat && w_scale.is_contiguous() && w_scale.dim() == 2 &&
                         w_scale.size(0) == (N + 127) / 128 && w_scale.size(1) == blocks,
-                    "w_scale must be fp32 [ceil(N / 128), ceil(K / 128)]");
-        check_rows_2d(out, "out");
-        TORCH_CHECK(out.size(0) == M && out.size(1) == N, "out must be [M, N]");
-        const b200ar::fp8::Type type = fp8_type(out, false, "out");
+                    "w_scale must be contiguous fp32 [", (N + 127) / 128, ", ", blocks, "]");
+        check_device(w, x, "w_q");
+        check_device(w_scale, x, "w_scale");
+        // The output's type: that of x, or with x_scale that of the empty tensor `like`.
+        const at::ScalarType dtype = x_scale.has_value() ? like->scalar_type() : x.scalar_type();
+        const b200ar::fp8::Type type = fp8_type(dtype, false, x_scale.has_value() ? "dtype" : "x");
         const at::cuda::OptionalCUDAGuard guard(device_of(x));
         const cudaStream_t s = stream_of();
+        const int64_t M = x.numel() / K;
+        at::Tensor out;
+        if (out_opt.has_value()) {
+          out = *out_opt;
+          bool same = out.dim() == x.dim() && out.scalar_type() == dtype && out.size(-1) == N;
+          for (int64_t i = 0; same && i + 1 < x.dim(); ++i) same = out.size(i) == x.size(i);
+          VALUE_CHECK(same && out.device() == x.device(), "out must be ", dtype, " [..., ", N, "] on ", x.device());
+        } else {
+          std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
+          shape.back() = N;
+          out = at::empty(shape, x.options().dtype(dtype));
+        }
+        const at::Tensor out2 = out.dim() == 2 ? out : out.view({M, N});
+        check_heads(out2, "out", true);
+        VALUE_CHECK(!overlaps(out, x) && !overlaps(out, w) && !overlaps(out, w_scale), "out overlaps an input");
         b200ar::fp8::LinearArgs a{};
         a.w = static_cast<const uint8_t*>(w.data_ptr());
         a.sw = w_scale.data_ptr<float>();
-        a.out = out.data_ptr();
-        a.ldo = out.stride(0);
+        a.out = out2.data_ptr();
+        a.ldo = out2.stride(0);
         a.M = M;
         a.N = N;
         a.K = K;
         a.err = err_of(err, x);
         // Scratch from the caching allocator on this stream: concurrent calls, eager or captured, never share it.
+        // Codes and scales of x, then the product's own.
         const b200ar::fp8::Scratch need = b200ar::fp8::linear_scratch(a);
-        const auto bytes = x.options().dtype(at::kByte);
-        const at::Tensor scratch = at::empty({need.floats * 4 + need.counters * 4}, bytes);
-        a.workspace = static_cast<float*>(scratch.data_ptr());
-        a.counters = reinterpret_cast<unsigned*>(a.workspace + need.floats);
-        at::Tensor codes, scales;
-        if (x_scale.has_value()) {
-          check_codes(x, "x");
-          check_device(*x_scale, x, "x_scale");
-          TORCH_CHECK(x_scale->scalar_type() == at::kFloat && x_scale->dim() == 2 && x_scale->size(0) == blocks &&
-                          x_scale->size(1) == M && (M <= 1 || x_scale->stride(1) == 1) && x_scale->stride(0) >= M,
-                      "x_scale must be fp32 [ceil(K / 128), M]");
-          a.x = static_cast<const uint8_t*>(x.data_ptr());
-          a.sx = x_scale->data_ptr<float>();
-          a.lds = x_scale->stride(0);
-          if (M > 0 && need.counters) C10_CUDA_CHECK(cudaMemsetAsync(a.counters, 0, need.counters * 4, s));
-        } else {
-          check_rows_2d(x, "x");
-          codes = at::empty({M, K}, bytes);
-          scales = at::empty({blocks, M}, x.options().dtype(at::kFloat));
-          a.x = codes.data_ptr<uint8_t>();
-          a.sx = scales.data_ptr<float>();
+        const bool quantize = !x_scale.has_value();
+        const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+        const int64_t codes_at = up(need.floats * 4) + up(need.counters * 4);
+        const int64_t scales_at = codes_at + (quantize ? up(M * K) : 0);
+        const at::Tensor scratch =
+            at::empty({scales_at + (quantize ? blocks * M * 4 : 0)}, x.options().dtype(at::kByte));
+        uint8_t* mem = static_cast<uint8_t*>(scratch.data_ptr());
+        a.workspace = reinterpret_cast<float*>(mem);
+        a.counters = reinterpret_cast<unsigned*>(mem + up(need.floats * 4));
+        at::Tensor x2, sx;
+        if (quantize) {
+          x2 = rows_2d(x);
+          a.x = mem + codes_at;
+          a.sx = reinterpret_cast<float*>(mem + scales_at);
           a.lds = M;
           a.early = true;
-          b200ar::fp8::quantize(x.data_ptr(), x.stride(0), codes.data_ptr<uint8_t>(), scales.data_ptr<float>(), M, M,
-                                K, fp8_type(x, false, "x"), a.counters, need.counters, s);
+          b200ar::fp8::quantize(x2.data_ptr(), x2.stride(0), mem + codes_at, reinterpret_cast<float*>(mem + scales_at),
+                                M, M, K, fp8_type(dtype, false, "x"), a.counters, need.counters, s);
+        } else {
+          TYPE_CHECK(x.scalar_type() == at::kFloat8_e4m3fn, "with x_scale, x must be float8_e4m3fn");
+          bool same = x_scale->dim() == x.dim() && x_scale->scalar_type() == at::kFloat && x_scale->size(-1) == blocks;
+          for (int64_t i = 0; same && i + 1 < x.dim(); ++i) same = x_scale->size(i) == x.size(i);
+          VALUE_CHECK(same && x_scale->device() == x.device(), "x_scale must be fp32 [..., ", blocks, "] on ",
+                      x.device());
+          x2 = x.reshape({M, K}).contiguous();
+          if (!aligned(x2)) x2 = x2.clone();
+          sx = x_scale->reshape({M, blocks}).t();
+          if ((M > 1 && sx.stride(1) != 1) || sx.stride(0) < M) sx = sx.contiguous();
+          a.x = static_cast<const uint8_t*>(x2.data_ptr());
+          a.sx = sx.data_ptr<float>();
+          a.lds = sx.stride(0);
+          if (M > 0 && need.counters) C10_CUDA_CHECK(cudaMemsetAsync(a.counters, 0, need.counters * 4, s));
         }
         b200ar::fp8::linear(a, type, s);
+        return out;
       },
       "product of e4m3 operands with block scales; x is quantized unless it comes with its scales", py::arg("x"),
-      py::arg("x_scale"), py::arg("w"), py::arg("w_scale"), py::arg("out"), py::arg("err"));
+      py::arg("w_q"), py::arg("w_scale"), py::arg("out"), py::arg("x_scale"), py::arg("like"), py::arg("err"));
 }

@@ -238,7 +238,8 @@ struct Steps {
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
-                     const __grid_constant__ AttnArgs a, const Workspace ws, int group, int box, float q_sign, float scale_log2) {
+                     const __grid_constant__ AttnArgs a, const Workspace ws, int group, int box, float q_sign,
+                     float scale_log2) {
   using C = Cfg<D>;
   constexpr int kSlots = C::kSlots;
   extern __shared__ __align__(1024) uint8_t attention_smem[];

@@ -18,6 +18,7 @@ of the type, t its smallest normal number, below which the steps stay the same.
 
 import math
 
+import pytest
 import torch
 
 from b200ar.ops.paged import PagedBatch
@@ -185,3 +186,93 @@ def check_linear(out, x_codes, x_scale, w_codes, w_scale):
     err = (got - want).abs()
     bound = rounding(want, out.dtype) + 2.0 ** -17 * mag
     assert (err <= bound).all(), (err - bound).max().item()
+
+
+# ------------------------------------------------------------------ refusals
+def _paged_setup(device, dtype=torch.bfloat16, d=64, hq=4, hkv=2, page=16):
+    from b200ar.ops.layers import RotaryTable
+
+    batch, pool = make_batch([2, 1], [5, 3], page, device)
+    k, v = (torch.zeros(pool, page, hkv, d, dtype=dtype, device=device) for _ in range(2))
+    return {"batch": batch, "k_pages": k, "v_pages": v, "rot": RotaryTable(d, 32, 500000.0, device),
+            "qkv": torch.zeros(3, (hq + 2 * hkv) * d, dtype=dtype, device=device),
+            "q": torch.zeros(3, hq, d, dtype=dtype, device=device)}
+
+
+def refuse_rope(device):
+    """Every call that the rotary step must refuse; the first two it must take."""
+    from b200ar.ops.layers import RotaryTable
+    from b200ar.ops.paged import PagedBatch, qk_norm_rope_paged
+
+    a = _paged_setup(device)
+
+    def call(**kw):
+        b = {**a, **kw}
+        return qk_norm_rope_paged(b["qkv"], b["batch"], b["rot"], b["k_pages"], b["v_pages"], b.get("hq", 4),
+                                  b.get("hkv", 2), q_gamma=b.get("q_gamma"), k_gamma=b.get("k_gamma"),
+                                  q_out=b.get("q_out"))
+
+    assert call().shape == (3, 4, 64)
+    own = a["qkv"][:, :256].view(3, 4, 64)
+    assert call(q_out=own).data_ptr() == own.data_ptr()  # in place
+    g = torch.ones(64, dtype=torch.bfloat16, device=device)
+    bad = [dict(hq=5), dict(hkv=0), dict(qkv=a["qkv"][0]), dict(v_pages=a["v_pages"][1:]), dict(q_gamma=g),
+           dict(q_gamma=g, k_gamma=g.float()), dict(q_gamma=g, k_gamma=g[:32]),
+           dict(rot=RotaryTable(128, 8, 1e4, device)), dict(q_out=own[:2]), dict(q_out=own.float()),
+           dict(q_out=a["qkv"][:, 64:320].view(3, 4, 64)),
+           dict(q_out=torch.zeros(1, 4, 64, device=device).bfloat16().expand(3, 4, 64)),
+           dict(batch=PagedBatch(a["batch"].page_table, a["batch"].kv_len)),
+           dict(k_pages=a["k_pages"][:1].expand(5, 16, 2, 64), v_pages=a["v_pages"][:1].expand(5, 16, 2, 64))]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            call(**kw)
+    for kw in (dict(k_pages=a["k_pages"].float(), v_pages=a["v_pages"].float()), dict(qkv=a["qkv"].half()),
+               dict(qkv=a["qkv"].float(), k_pages=a["k_pages"].float(), v_pages=a["v_pages"].float())):
+        with pytest.raises(TypeError):
+            call(**kw)
+
+
+def refuse_attention(device):
+    from b200ar.ops.paged import PagedBatch, paged_attention
+
+    a = _paged_setup(device)
+
+    def call(**kw):
+        b = {**a, **kw}
+        return paged_attention(b["q"], b["k_pages"], b["v_pages"], b["batch"], scale=b.get("scale"),
+                               causal=b.get("causal", True), window=b.get("window", 0), out=b.get("out"))
+
+    assert call().shape == (3, 256)
+    for kw in (dict(q=a["q"][0]), dict(q=torch.zeros(3, 3, 64, device=device).bfloat16()),
+               dict(q=torch.zeros(3, 4, 32, device=device).bfloat16()),
+               dict(window=-1), dict(window=4, causal=False), dict(scale=float("nan")),
+               dict(out=torch.zeros(3, 255, device=device).bfloat16()), dict(out=torch.zeros(3, 256, device=device)),
+               dict(out=a["q"].view(3, 256)), dict(out=torch.zeros(1, 256, device=device).bfloat16().expand(3, 256)),
+               dict(batch=PagedBatch(a["batch"].page_table, a["batch"].kv_len)),
+               dict(k_pages=a["k_pages"][:, :12], v_pages=a["v_pages"][:, :12])):
+        with pytest.raises(ValueError):
+            call(**kw)
+    with pytest.raises(TypeError):
+        call(q=a["q"].half())
+
+
+def refuse_linear_fp8(device):
+    from b200ar.ops.fp8 import linear_fp8, quantize_fp8, quantize_fp8_weight
+
+    x, w = torch.zeros(3, 32, device=device).bfloat16(), torch.zeros(16, 32, device=device).bfloat16()
+    w_q, w_s = quantize_fp8_weight(w)
+    x_q, x_s = quantize_fp8(x)
+    for f in (lambda: quantize_fp8(x[:, :20]), lambda: quantize_fp8_weight(w[0]),
+              lambda: linear_fp8(x[:, :16], w_q, w_s),
+              lambda: linear_fp8(x, w_q[:12], w_s), lambda: linear_fp8(x, w_q, w_s[:, :0]),
+              lambda: linear_fp8(x, w_q, w_s.double()),
+              lambda: linear_fp8(x, w_q, w_s, out=torch.zeros(3, 16, device=device)),
+              lambda: linear_fp8(x, w_q, w_s, out=torch.zeros(3, 8, device=device).bfloat16()),
+              lambda: linear_fp8(x_q, w_q, w_s, x_scale=x_s[:2])):
+        with pytest.raises(ValueError):
+            f()
+    for f in (lambda: quantize_fp8(x.long()), lambda: linear_fp8(x.float(), w_q, w_s), lambda: linear_fp8(x, w, w_s),
+              lambda: linear_fp8(x, w_q, w_s, x_scale=x_s), lambda: linear_fp8(x_q, w_q, w_s),
+              lambda: linear_fp8(x_q, w_q, w_s, x_scale=x_s, dtype=torch.float32)):
+        with pytest.raises(TypeError):
+            f()

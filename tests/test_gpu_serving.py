@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from serving_util import (check_attention, check_linear, check_rope, make_batch, plain_quantize, plain_rope, randn,
-                          starts_of)
+                          refuse_attention, refuse_linear_fp8, refuse_rope, starts_of)
 
 pytestmark = pytest.mark.gpu
 
@@ -29,6 +29,23 @@ def _attention_inputs(new, total, page, hq, hkv, d, dtype, seed=0, pad=0, decode
     q = randn((rows, hq, d), dtype, "cuda", seed + 1)
     k, v = (randn((pool, page, hkv, d), dtype, "cuda", seed + i) for i in (2, 3))
     return q, k, v, batch
+
+
+def test_refusals():
+    from b200ar.ops.fp8 import linear_fp8, quantize_fp8_weight
+    from b200ar.ops.paged import PagedBatch, paged_attention
+
+    refuse_rope("cuda")
+    refuse_attention("cuda")
+    refuse_linear_fp8("cuda")
+    # Tensors of two devices.
+    q, k, v, batch = _attention_inputs([2], [20], 16, 4, 1, 64, BF)
+    there = PagedBatch(batch.page_table.cpu(), batch.kv_len.cpu(), batch.q_start.cpu())
+    w_q, w_s = quantize_fp8_weight(torch.zeros(16, 32, dtype=BF))
+    for f in (lambda: paged_attention(q, k, v, there), lambda: paged_attention(q, k.cpu(), v.cpu(), batch),
+              lambda: paged_attention(q.cpu(), k, v, there), lambda: linear_fp8(q[0, :, :32], w_q, w_s)):
+        with pytest.raises(ValueError):
+            f()
 
 
 # ------------------------------------------------------------------ attention
