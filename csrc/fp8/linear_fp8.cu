@@ -469,18 +469,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         wait(&tfull[bf], (n >> 1) & 1u);
         sm100::tc_fence_after();
 #pragma unroll
-        for (int c = 0; c < 128; c += 64) {
-          uint32_t r[64];
+        for (int c = 0; c < 128; c += 32) {
+          uint32_t r[32];
           sm100::tmem_ld_32x32b_x32(td + bf * BN + c, r);
-          sm100::tmem_ld_32x32b_x32(td + bf * BN + c + 32, r + 32);
           sm100::tmem_ld_wait();
-          if (c == 64) {  // the accumulator is read: the next block but one may overwrite it
+          if (c == 96) {  // the accumulator is read: the next block but one may overwrite it
             sm100::tc_fence_before();
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive_remote(free_bar[bf]);
           }
 #pragma unroll
-          for (int e = 0; e < 64; e += 2) acc[(c + e) / 2] = fma2(pack64(r[e], r[e + 1]), s, acc[(c + e) / 2]);
+          for (int e = 0; e < 32; e += 2) acc[(c + e) / 2] = fma2(pack64(r[e], r[e + 1]), s, acc[(c + e) / 2]);
         }
       }
       u += k1 - k0;

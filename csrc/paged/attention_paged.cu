@@ -121,7 +121,7 @@ __device__ __noinline__ void attention_row(const AttnArgs& a, int s, int row, in
 // and its last item (slots 2 c and 2 c + 1).
 struct PartDesc {
   int s, h, b, rows;
-  int t0, t1, tiles, used;
+  int t0, t1, tiles, q0;  // q0 < 0: not used
 };
 
 struct Workspace {
@@ -146,13 +146,14 @@ struct Cfg {
 
 constexpr int kThreads = 384;
 constexpr uint32_t kTmemCols = 512;
+constexpr int kEarly = 96;       // tokens of P after which its product may start
 constexpr uint32_t kColO = 256;  // S_0, S_1 at columns 0 and 128, O_0, O_1 at 256 and 384
 
 struct Barriers {
   uint64_t full[8], empty[8];  // ring slots
   uint64_t qready[2];          // queries of group t written
   uint64_t sfull[2];           // S_t computed (and the O_t of the step before)
-  uint64_t pready[2];          // P_t written, O_t rescaled
+  uint64_t pready[2][2];       // O_t rescaled and the first kEarly tokens of P_t written; the rest written
   uint64_t ofull[2];           // last P V of group t in a block done
   uint64_t gsync;              // the eight softmax warps
   uint64_t ifull[4], iempty[4];  // ring of items
@@ -259,7 +260,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&bar.qready[i], 4);
       sm100::mbar_init(&bar.sfull[i], 1);
-      sm100::mbar_init(&bar.pready[i], 4);
+      sm100::mbar_init(&bar.pready[i][0], 4);
+      sm100::mbar_init(&bar.pready[i][1], 4);
       sm100::mbar_init(&bar.ofull[i], 1);
     }
     for (int i = 0; i < kItems; ++i) {
@@ -279,7 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     sm100::tmem_relinquish();
   }
   pdl_wait();  // lengths, offsets, pages, queries and the cache may come from the kernel before
-  if (threadIdx.x == 0) desc[0].used = desc[1].used = 0;
+  if (threadIdx.x == 0) desc[0].q0 = desc[1].q0 = -1;
   find_part<kThreads>(a, group, misc.red, &misc.part);
   pdl_trigger();  // after a barrier: this CTA holds its tensor memory
   sm100::tc_fence_before();
@@ -291,9 +293,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (*s_err) return;
     if (!sm100::mbar_wait(b, parity)) *s_err = 1;
   };
-  // 168 registers a thread at launch: 88 for the last warpgroup and 208 for the two of the softmax.
+  // 168 registers a thread at launch: 72 for the last warpgroup and 216 for the two of the softmax.
   if (warp >= 8) {
-    sm100::reg_give<88>();
+    sm100::reg_give<72>();
     if (warp == 10) {
       // ---------------------------------------------------------- items
       if (lane == 0) {
@@ -312,37 +314,53 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (warp == 8) {
       // ------------------------------------------------------------ TMA producer
-      const int boxes = kTile / box;           // page runs of a tile
-      unsigned count = 0;                      // loads issued so far
+      const int boxes = kTile / box;    // page runs of a tile
+      const int ahead = 32 / boxes;     // tiles whose runs the warp's lanes look up together
+      const int run = lane % boxes;
+      unsigned count = 0;               // loads issued so far
       for (unsigned item = 0;; ++item) {
         wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
         const Item& it = misc.item[item % kItems];
         if (__any_sync(0xffffffffu, *s_err || it.rows == 0)) break;
         const Steps st(it);
+        const int first = (it.tile0 + it.t0) * kTile, nt = st.nt, s = it.s, begin = it.begin, end = it.end, h = it.h;
         if (it.over && lane == 0) atomicExch(a.err, kErrPage);
-        for (int i = 0; i < 2 * st.nt; ++i, ++count) {
-          const int load = st.load(i);
-          const int c0 = (it.tile0 + it.t0 + (load >> 1)) * kTile;
-          // Page and slot of this lane's run (lane % boxes), looked up before the slot is free.
-          const int run = lane % boxes, pos = c0 + run * box;
-          int page = a.num_pages, slot = 0;  // outside the pool: zeros
-          if (pos + box > it.begin && pos < it.end) {
-            page = page_of(a.batch, it.s, pos / a.page_size, a.num_pages);
-            slot = pos % a.page_size;
+        // Page of this lane's run in the tiles [ahead g, ahead (g + 1)); runs that no row sees lie outside the pool.
+        auto pages_of = [&](int g) {
+          const int j = g * ahead + lane / boxes, pos = first + j * kTile + run * box;
+          int page = a.num_pages;
+          if (j < nt && pos + box > begin && pos < end) {
+            page = page_of(a.batch, s, pos / a.page_size, a.num_pages);
             if (page < 0) {
               atomicExch(a.err, kErrPage);
               page = a.num_pages;
             }
           }
+          return page;
+        };
+        // Even and odd groups. The next one is looked up at a group's second tile: the tile before the group is
+        // done with its register then (its V comes after the K of the group's first), and the loads of one tile
+        // at least cover the latency.
+        int even = pages_of(0), odd = a.num_pages;
+        for (int i = 0; i < 2 * nt; ++i, ++count) {
+          const int load = st.load(i), j = load >> 1, g = j / ahead;
+          if (!(load & 1) && j % ahead == 1) {
+            if (g & 1)
+              even = pages_of(g + 1);
+            else
+              odd = pages_of(g + 1);
+          }
+          const int page = __shfl_sync(0xffffffffu, g & 1 ? odd : even, (j % ahead) * boxes + run);
+          const int slot = (first + j * kTile + run * box) % a.page_size;
           const int sl = count % kSlots;
           wait(&bar.empty[sl], ((count / kSlots) & 1u) ^ 1u);
           if (__any_sync(0xffffffffu, *s_err)) break;
           if (lane == 0) sm100::mbar_arrive_expect_tx(&bar.full[sl], C::kTileBytes);
           __syncwarp();
           uint8_t* dst = ring + sl * C::kTileBytes + run * box * 128;
-          for (int j = lane; j < boxes * C::kHalves; j += 32)  // 32 lanes are a multiple of the runs
-            sm100::tma_load_4d(dst + (j / boxes) * C::kHalfBytes, load & 1 ? &tv : &tk, &bar.full[sl],
-                               (j / boxes) * 64, it.h, slot, page);
+          for (int x = lane; x < boxes * C::kHalves; x += 32)  // 32 lanes are a multiple of the runs
+            sm100::tma_load_4d(dst + (x / boxes) * C::kHalfBytes, load & 1 ? &tv : &tk, &bar.full[sl],
+                               (x / boxes) * 64, h, slot, page);
           __syncwarp();
         }
         if (lane == 0) sm100::mbar_arrive(&bar.iempty[item % kItems]);
@@ -367,17 +385,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int steps = st.count();
           wait(&bar.qready[0], nq[0]++ & 1u);
           if (st.wide) wait(&bar.qready[1], nq[1]++ & 1u);
-          auto scores = [&](int k) {
+            auto scores = [&](int k) {
             const int t = k & 1, at = st.k_at(st.tile(k));
             wait(&bar.full[slot_of(at)], phase_of(at));
             sm100::tc_fence_after();
-            const uint8_t* qt = smem + C::kQ + (st.wide ? t : 0) * C::kTileBytes;
-            const uint8_t* kt = ring + slot_of(at) * C::kTileBytes;
-  #pragma unroll
+            const uint64_t dq = sm100::smem_desc_sw128(smem + C::kQ + (st.wide ? t : 0) * C::kTileBytes);
+            const uint64_t dk = sm100::smem_desc_sw128(ring + slot_of(at) * C::kTileBytes);
+#pragma unroll
             for (int i = 0; i < D / 16; ++i) {
-              const uint64_t da = sm100::smem_desc_sw128(qt + (i >> 2) * C::kHalfBytes) + 2 * (i & 3);
-              const uint64_t db = sm100::smem_desc_sw128(kt + (i >> 2) * C::kHalfBytes) + 2 * (i & 3);
-              sm100::mma_bf16(tmem + t * 128, da, db, idesc<T>(128, false), i > 0 ? 1u : 0u);
+              const uint64_t off = (i >> 2) * (C::kHalfBytes >> 4) + 2 * (i & 3);
+              sm100::mma_bf16(tmem + t * 128, dq + off, dk + off, idesc<T>(128, false), i > 0 ? 1u : 0u);
             }
             sm100::mma_commit(&bar.sfull[t]);
             if (!st.wide || t == 1) sm100::mma_commit(&bar.empty[slot_of(at)]);
@@ -386,15 +403,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (steps > 1) scores(1);
           for (int k = 0; k < steps && !*s_err; ++k) {
             const int t = k & 1, at = st.v_at(st.tile(k));
+            const uint32_t parity = np[t]++ & 1u;
             wait(&bar.full[slot_of(at)], phase_of(at));
-            wait(&bar.pready[t], np[t]++ & 1u);
+            const uint64_t dv = sm100::smem_desc_mn_sw128(ring + slot_of(at) * C::kTileBytes, C::kHalfBytes, 1024);
+            wait(&bar.pready[t][0], parity);
             sm100::tc_fence_after();
-            const uint8_t* vt = ring + slot_of(at) * C::kTileBytes;
-  #pragma unroll
-            for (int i = 0; i < kTile / 16; ++i)  // 16 tokens: 2048 bytes further in V, 8 columns in P
-              sm100::mma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + i * 8,
-                                sm100::smem_desc_mn_sw128(vt + i * 2048, C::kHalfBytes, 1024), idesc<T>(D, true),
-                                (k > 1 || i > 0) ? 1u : 0u);
+#pragma unroll
+            for (int i = 0; i < kTile / 16; ++i) {  // 16 tokens: 2048 bytes further in V, 8 columns in P
+              if (i == kEarly / 16) {
+                wait(&bar.pready[t][1], parity);
+                sm100::tc_fence_after();
+              }
+              sm100::mma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + i * 8, dv + i * (2048 >> 4),
+                                idesc<T>(D, true), (k > 1 || i > 0) ? 1u : 0u);
+            }
             if (!st.wide || t == 1) sm100::mma_commit(&bar.empty[slot_of(at)]);
             if (k + 2 < steps)
               scores(k + 2);
@@ -411,7 +433,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ softmax
-    sm100::reg_take<208>();
+    sm100::reg_take<216>();
     const int t = warp >> 2, w4 = warp & 3;
     const int row = w4 * 32 + lane;  // row of the group's tile
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
@@ -429,6 +451,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       return !__any_sync(0xffffffffu, *s_err || misc.item[i % kItems].rows == 0);
     };
 
+    // Hands this warp's part of tensor memory to the MMA issue.
+    auto arrive = [&](uint64_t* b) {
+      sm100::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) sm100::mbar_arrive(b);
+    };
     // Writes the queries of an item into this group's tile (or, with at most
     // 128 rows, group 0 into its own).
     auto load_q = [&](const Item& i) {
@@ -477,11 +505,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int hi_all = __reduce_min_sync(0xffffffffu, valid ? hi : 0x7fffffff);
       const int lo_all = __reduce_max_sync(0xffffffffu, valid ? lo : -0x7fffffff);
 
+      const int first_pos = (it.tile0 + it.t0) * kTile, len = it.len, begin = it.begin;
       float m = -INFINITY, l = 0.f;  // bound on the maximum, in units of S; sum of P
       int mine = 0;                  // steps of this group
       for (int k = t; k < steps; k += 2, ++mine) {
         const int j = st.tile(k);
-        const int c0 = (it.tile0 + it.t0 + j) * kTile;
+        const int c0 = first_pos + j * kTile;
+        // Tokens behind the sequence and before every row's window may hold anything: zeros in V, since
+        // zero times NaN is NaN.
+        if (c0 + kTile > len || c0 < begin) {
+          const unsigned at = base + st.v_at(j);
+          wait(&bar.full[at % kSlots], (at / kSlots) & 1u);
+          if (c0 + row >= len || c0 + row < begin) {
+            uint8_t* vt = ring + (at % kSlots) * C::kTileBytes + row * 128;
+#pragma unroll
+            for (int c = 0; c < 8 * C::kHalves; ++c)
+              *reinterpret_cast<uint4*>(vt + (c >> 3) * C::kHalfBytes + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+          }
+          sm100::fence_proxy_async_smem();
+        }
         wait(&bar.sfull[t], ns++ & 1u);
         sm100::tc_fence_after();
         if (!idle) {
@@ -492,7 +534,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int first = kCols == 128 ? 0 : w4 * 32;
             uint32_t x[kCols];
 #pragma unroll
-            for (int c = 0; c < kCols; c += 32) sm100::tmem_ld_32x32b_x32(tS + first + c, x + c);
+            for (int c = 0; c < kCols; c += 32)
+              sm100::tmem_ld_32x32b_x32(tS + first + c, x + c);
             sm100::tmem_ld_wait();
             if constexpr (kMasked) {
               const int from = lo - c0 - first, to = hi - c0 - first;
@@ -528,7 +571,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const uint64_t scale2 = pack64(scale_log2, scale_log2), shift2 = pack64(shift, shift);
             uint64_t sum[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < kCols; c += 32) {
+            for (int c = 0; c < kCols; c += 32) {  // P of columns c .. c + 31 goes where S was
               uint32_t p[16];
 #pragma unroll
               for (int e = 0; e < 32; e += 2) {
@@ -539,6 +582,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 p[e / 2] = pack2<T>(p0, p1);
               }
               sm100::tmem_st_32x32b_x16(tS + (first + c) / 2, p);
+              if (c + 32 == kEarly) {
+                sm100::tmem_st_wait();
+                arrive(&bar.pready[t][0]);
+              }
             }
             const float2 all = unpack64(add2(sum[0], sum[1]));
             l += all.x + all.y;
@@ -560,22 +607,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             softmax(std::integral_constant<int, 128>{}, Yes{});
           }
         }
-        // Tokens behind the sequence and before every row's window may hold anything: zeros in V, since
-        // zero times NaN is NaN.
-        if (c0 + kTile > it.len || c0 < it.begin) {
-          const unsigned at = base + st.v_at(j);
-          wait(&bar.full[at % kSlots], (at / kSlots) & 1u);
-          if (c0 + row >= it.len || c0 + row < it.begin) {
-            uint8_t* vt = ring + (at % kSlots) * C::kTileBytes + row * 128;
-#pragma unroll
-            for (int c = 0; c < 8 * C::kHalves; ++c)
-              *reinterpret_cast<uint4*>(vt + (c >> 3) * C::kHalfBytes + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          }
-          sm100::fence_proxy_async_smem();
-        }
-        sm100::tc_fence_before();
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&bar.pready[t]);
+        if (idle || quad) arrive(&bar.pready[t][0]);
+        arrive(&bar.pready[t][1]);
       }
       base += 2 * st.nt;
 
@@ -593,7 +626,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int which = it.t0 > 0 ? 0 : 1, slot = 2 * blockIdx.x + which;
       float* acc = ws.acc + static_cast<int64_t>(slot) * ws.row_cap * D;
       float* ml = ws.ml + static_cast<int64_t>(slot) * ws.row_cap * 2;
-      if (!whole && threadIdx.x == 0) desc[which] = PartDesc{it.s, it.h, it.b, it.rows, it.t0, it.t1, it.tiles, 1};
+      if (!whole && threadIdx.x == 0) desc[which] = PartDesc{it.s, it.h, it.b, it.rows, it.t0, it.t1, it.tiles, it.q0};
       auto out_of = [&](int r2) {
         const int x = it.row0 + r2;
         return static_cast<T*>(a.out) + (it.q0 + x / group) * a.o_tok + (it.h * group + x % group) * a.o_head;
@@ -792,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // attention kernel, row groups); the CTA whose part starts such a block owns it.
 // Parts are added in the order of the tiles, so results do not depend on timing.
 constexpr int kMergeThreads = 256;
-constexpr int kMergeGroups = 8;
+constexpr int kMergeGroups = 32;
 constexpr int kMaxParts = 1024;
 
 template <typename T, int D>
@@ -803,7 +836,7 @@ __global__ void __launch_bounds__(kMergeThreads)
   pdl_wait();
   pdl_trigger();
   const PartDesc first = ws.desc[2 * blockIdx.x + 1];
-  if (!first.used || first.t1 == first.tiles) return;
+  if (first.q0 < 0 || first.t1 == first.tiles || blockIdx.y * (kMergeThreads / 32) >= first.rows) return;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (warp == 0) {
     // Continuations follow in the order of the CTAs; one that reaches the last tile is the last.
@@ -812,8 +845,9 @@ __global__ void __launch_bounds__(kMergeThreads)
     for (int c0 = blockIdx.x + 1; c0 < ctas; c0 += 32) {
       const int c = c0 + lane;
       PartDesc d{};
+      d.q0 = -1;
       if (c < ctas) d = ws.desc[2 * c];
-      const bool on = d.used && d.s == first.s && d.h == first.h && d.b == first.b;
+      const bool on = d.q0 >= 0 && d.s == first.s && d.h == first.h && d.b == first.b;
       const unsigned who = __ballot_sync(0xffffffffu, on);
       if (on) part[n + __popc(who & ((1u << lane) - 1u))] = 2 * c;
       n += __popc(who);
@@ -823,24 +857,34 @@ __global__ void __launch_bounds__(kMergeThreads)
   }
   __syncthreads();
   const int n = parts;
-  const int q0 = q_begin(a.batch, first.s), cnt = q_begin(a.batch, first.s + 1) - q0;
-  const int len = __ldg(a.batch.kv_len + first.s);
   for (int r = blockIdx.y * (kMergeThreads / 32) + warp; r < first.rows; r += kMergeGroups * (kMergeThreads / 32)) {
-    float m = -INFINITY, l = 0.f;
-    for (int i = 0; i < n; ++i) m = fmaxf(m, __ldcg(ws.ml + (static_cast<int64_t>(part[i]) * ws.row_cap + r) * 2));
-    float o[D / 32] = {};
+    // A lane has the states of parts lane, lane + 32, ...
+    auto state = [&](int i) {
+      return i < n ? __ldcg(reinterpret_cast<const float2*>(ws.ml + (static_cast<int64_t>(part[i]) * ws.row_cap + r) * 2))
+                   : make_float2(-INFINITY, 0.f);
+    };
+    const float2 mine = state(lane);
+    float m = mine.x;
+    for (int i = lane + 32; i < n; i += 32) m = fmaxf(m, state(i).x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    float l = 0.f, o[D / 32] = {};
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      const float2 v = i0 == 0 ? mine : state(i0 + lane);
+      const float f_mine = v.x == -INFINITY ? 0.f : fast_exp2(v.x - m), l_mine = v.y * f_mine;
+      const int cnt = min(32, n - i0);
 #pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const int64_t at = static_cast<int64_t>(part[i]) * ws.row_cap + r;
-      const float2 v = __ldcg(reinterpret_cast<const float2*>(ws.ml + at * 2));
-      const float f = v.x == -INFINITY ? 0.f : fast_exp2(v.x - m);
-      l += v.y * f;
-      if constexpr (D == 128) {
-        const float4 x = __ldcg(reinterpret_cast<const float4*>(ws.acc + at * D) + lane);
-        if (f != 0.f) o[0] += x.x * f, o[1] += x.y * f, o[2] += x.z * f, o[3] += x.w * f;
-      } else {
-        const float2 x = __ldcg(reinterpret_cast<const float2*>(ws.acc + at * D) + lane);
-        if (f != 0.f) o[0] += x.x * f, o[1] += x.y * f;
+      for (int i = 0; i < cnt; ++i) {
+        const int64_t at = static_cast<int64_t>(part[i0 + i]) * ws.row_cap + r;
+        const float f = __shfl_sync(0xffffffffu, f_mine, i);
+        l += __shfl_sync(0xffffffffu, l_mine, i);
+        if constexpr (D == 128) {
+          const float4 x = __ldcg(reinterpret_cast<const float4*>(ws.acc + at * D) + lane);
+          if (f != 0.f) o[0] += x.x * f, o[1] += x.y * f, o[2] += x.z * f, o[3] += x.w * f;
+        } else {
+          const float2 x = __ldcg(reinterpret_cast<const float2*>(ws.acc + at * D) + lane);
+          if (f != 0.f) o[0] += x.x * f, o[1] += x.y * f;
+        }
       }
     }
     const float inv = l == 0.f ? 0.f : 1.f / l;
@@ -850,8 +894,9 @@ __global__ void __launch_bounds__(kMergeThreads)
       o[e] = inv == 0.f ? 0.f : o[e] * inv;
       odd += o[e] * 0.f;
     }
-    const int x = first.b * kBlock + r, tok = x / group, h = first.h * group + x % group;
+    const int x = first.b * kBlock + r, tok = x / group, h = first.h * group + x % group, q0 = first.q0;
     if (__any_sync(0xffffffffu, odd != 0.f)) {
+      const int cnt = q_begin(a.batch, first.s + 1) - q0, len = __ldg(a.batch.kv_len + first.s);
       attention_row<T, D>(a, first.s, q0 + tok, len - cnt + tok, len, h, first.h);
       continue;
     }

@@ -43,16 +43,29 @@ __device__ __forceinline__ uint4 pack8(const float* v) {
   return make_uint4(pack2<T>(v[0], v[1]), pack2<T>(v[2], v[3]), pack2<T>(v[4], v[5]), pack2<T>(v[6], v[7]));
 }
 
-// Grid (rows, head chunks); a block handles `per_block` consecutive heads of
-// [q heads | k heads | v heads] of one row.
-template <typename T, int D>
-__global__ void __launch_bounds__(kThreads) rope_paged_kernel(const RopeArgs a, int per_block) {
-  constexpr int kLanes = D / 16;             // lanes of a head
+// Grid (rows, head chunks); a block handles kIters * kGroups consecutive heads
+// of [q heads | k heads | v heads] of one row.
+template <typename T, int D, int kIters>
+__global__ void __launch_bounds__(kThreads) rope_paged_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int kLanes = D / 16;              // lanes of a head
   constexpr int kGroups = kThreads / kLanes;  // heads in flight in a block
   const int row = blockIdx.x;
-  const int lane = threadIdx.x % kLanes, group = threadIdx.x / kLanes;
+  const int lane = threadIdx.x % kLanes;
+  const int h0 = blockIdx.y * (kIters * kGroups) + threadIdx.x / kLanes;
+  const int heads = a.hq + 2 * a.hkv;
   pdl_wait();
   pdl_trigger();
+  // The values first: their loads run beside the chain of loads that finds the page.
+  uint4 w0[kIters], w1[kIters];
+  const T* in = static_cast<const T*>(a.qkv) + row * a.qkv_stride + lane * 8;
+#pragma unroll
+  for (int i = 0; i < kIters; ++i) {
+    w0[i] = w1[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (h0 + i * kGroups < heads) {
+      w0[i] = *reinterpret_cast<const uint4*>(in + (h0 + i * kGroups) * D);
+      w1[i] = *reinterpret_cast<const uint4*>(in + (h0 + i * kGroups) * D + D / 2);
+    }
+  }
   const int s = sequence_of_row(a.batch, row);
   if (s < 0) return;
   const int first = q_begin(a.batch, s), n = q_begin(a.batch, s + 1) - first;
@@ -77,74 +90,75 @@ __global__ void __launch_bounds__(kThreads) rope_paged_kernel(const RopeArgs a, 
     *reinterpret_cast<float4*>(sn) = __ldg(sp);
     *reinterpret_cast<float4*>(sn + 4) = __ldg(sp + 1);
   }
-  const T* in = static_cast<const T*>(a.qkv) + row * a.qkv_stride;
-  const int heads = a.hq + 2 * a.hkv;
-  const int h_end = min(heads, (static_cast<int>(blockIdx.y) + 1) * per_block);
-  // Uniform trip count: the shuffles below need every lane of the warp.
-  for (int h0 = blockIdx.y * per_block; h0 < h_end; h0 += kGroups) {
-    const int h = h0 + group;
-    const bool on = h < h_end;
-    float x0[8], x1[8];
-    uint4 w0 = make_uint4(0u, 0u, 0u, 0u), w1 = w0;
-    if (on) {
-      const T* src = in + h * D + lane * 8;
-      w0 = *reinterpret_cast<const uint4*>(src);
-      w1 = *reinterpret_cast<const uint4*>(src + D / 2);
-    }
-    unpack8<T>(w0, x0);
-    unpack8<T>(w1, x1);
+#pragma unroll
+  for (int i = 0; i < kIters; ++i) {
+    const int h = h0 + i * kGroups;
     const bool is_q = h < a.hq, is_v = h >= a.hq + a.hkv;
-    const T* gamma = static_cast<const T*>(is_q ? a.q_gamma : a.k_gamma);
+    float x0[8], x1[8];
+    unpack8<T>(w0[i], x0);
+    unpack8<T>(w1[i], x1);
     float ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss += x0[i] * x0[i] + x1[i] * x1[i];
+    for (int e = 0; e < 8; ++e) ss += x0[e] * x0[e] + x1[e] * x1[e];
 #pragma unroll
     for (int o = kLanes / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (!on) continue;
+    if (h >= heads) continue;
     T* dst;
     if (is_q) {
       dst = static_cast<T*>(a.q_out) + row * a.q_tok + h * a.q_head;
     } else {
       const Pool& p = is_v ? a.v : a.k;
-      const int kh = h - a.hq - (is_v ? a.hkv : 0);
-      dst = static_cast<T*>(p.base) + page * p.page + slot * p.tok + kh * p.head;
+      dst = static_cast<T*>(p.base) + page * p.page + slot * p.tok + (h - a.hq - (is_v ? a.hkv : 0)) * p.head;
     }
     dst += lane * 8;
     if (is_v) {
-      *reinterpret_cast<uint4*>(dst) = w0;
-      *reinterpret_cast<uint4*>(dst + D / 2) = w1;
+      *reinterpret_cast<uint4*>(dst) = w0[i];
+      *reinterpret_cast<uint4*>(dst + D / 2) = w1[i];
       continue;
     }
+    const T* gamma = static_cast<const T*>(is_q ? a.q_gamma : a.k_gamma);
     if (gamma) {
       const float inv = rsqrtf(ss * (1.f / D) + a.eps);
       float g0[8], g1[8];
       unpack8<T>(__ldg(reinterpret_cast<const uint4*>(gamma + lane * 8)), g0);
       unpack8<T>(__ldg(reinterpret_cast<const uint4*>(gamma + D / 2 + lane * 8)), g1);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        x0[i] = x0[i] * inv * g0[i];
-        x1[i] = x1[i] * inv * g1[i];
+      for (int e = 0; e < 8; ++e) {
+        x0[e] = x0[e] * inv * g0[e];
+        x1[e] = x1[e] * inv * g1[e];
       }
     }
     float y0[8], y1[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      y0[i] = x0[i] * c[i] - x1[i] * sn[i];
-      y1[i] = x1[i] * c[i] + x0[i] * sn[i];
+    for (int e = 0; e < 8; ++e) {
+      y0[e] = x0[e] * c[e] - x1[e] * sn[e];
+      y1[e] = x1[e] * c[e] + x0[e] * sn[e];
     }
     *reinterpret_cast<uint4*>(dst) = pack8<T>(y0);
     *reinterpret_cast<uint4*>(dst + D / 2) = pack8<T>(y1);
   }
 }
 
+template <typename T, int D, int kIters>
+void launch_iters(const RopeArgs& a, cudaStream_t s) {
+  constexpr int kHeads = kIters * (kThreads / (D / 16));  // heads of a block
+  const int heads = a.hq + 2 * a.hkv;
+  const dim3 grid(static_cast<unsigned>(a.rows), static_cast<unsigned>((heads + kHeads - 1) / kHeads));
+  launch_pdl(rope_paged_kernel<T, D, kIters>, grid, dim3(kThreads), 0, s, 1, a);
+}
+
 template <typename T, int D>
 void launch(const RopeArgs& a, cudaStream_t s) {
   constexpr int kGroups = kThreads / (D / 16);
   const int heads = a.hq + 2 * a.hkv;
-  // Few rows: one pass of the block over its heads, so that more SMs share the call.
-  const int per_block = kGroups;
-  const dim3 grid(static_cast<unsigned>(a.rows), static_cast<unsigned>((heads + per_block - 1) / per_block));
-  launch_pdl(rope_paged_kernel<T, D>, grid, dim3(kThreads), 0, s, 1, a, per_block);
+  // Many rows: up to three heads a thread, so that a block's fixed chain of loads serves more values. Few rows:
+  // one, so that more SMs share the call.
+  if (a.rows < 512 || heads <= kGroups)
+    launch_iters<T, D, 1>(a, s);
+  else if (heads <= 2 * kGroups)
+    launch_iters<T, D, 2>(a, s);
+  else
+    launch_iters<T, D, 3>(a, s);
 }
 
 }  // namespace
