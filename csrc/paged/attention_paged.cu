@@ -14,7 +14,7 @@
 //
 //   warps 0-3, 4-7  softmax: group t owns S_t, P_t (in the columns of S_t) and
 //                   O_t in tensor memory; a thread owns one row
-//   warp 8          TMA producer: a lane loads one run of tokens of one page
+//   warps 8, 11     TMA producers of K and of V
 //   warp 9          TMEM allocation and MMA issue (one thread)
 //   warp 10         walks the CTA's items and hands them to the others
 //
@@ -135,13 +135,14 @@ struct Workspace {
 template <int D>
 struct Cfg {
   static constexpr int kHalves = D / 64;                    // 128-byte wide halves of a row
+  static constexpr uint32_t kGroupBytes = kHalves * 1024;   // 8 tokens of K or V: [half][token][128 bytes]
   static constexpr uint32_t kHalfBytes = 128 * 128;         // 128 rows x 128 bytes
   static constexpr uint32_t kTileBytes = kHalves * kHalfBytes;
   static constexpr int kSlots = D == 128 ? 5 : 8;           // ring of K and V tiles
   static constexpr uint32_t kQ = 0;                         // two tiles of queries
   static constexpr uint32_t kRing = 2 * kTileBytes;
   static constexpr uint32_t kMisc = kRing + kSlots * kTileBytes;
-  static constexpr size_t kSmem = 1024 + kMisc + 1024;
+  static constexpr size_t kSmem = 1024 + kMisc + 1280;
 };
 
 constexpr int kThreads = 384;
@@ -151,7 +152,7 @@ constexpr uint32_t kColO = 256;  // S_0, S_1 at columns 0 and 128, O_0, O_1 at 2
 
 struct Barriers {
   uint64_t full[8], empty[8];  // ring slots
-  uint64_t qready[2];          // queries of group t written
+  uint64_t qready[2];          // queries of tile t written
   uint64_t sfull[2];           // S_t computed (and the O_t of the step before)
   uint64_t pready[2][2];       // O_t rescaled and the first kEarly tokens of P_t written; the rest written
   uint64_t ofull[2];           // last P V of group t in a block done
@@ -167,9 +168,11 @@ struct Misc {
   Part part;
   uint32_t tmem;
   int err;
-  unsigned bad;  // rows of a 32-row block that came out as NaN
+  unsigned bad;      // rows of a 32-row block that came out as NaN
+  float sum[32];     // sums of P of such a block's rows
+  int last[2][8];    // last load of K and of V into each slot of the ring, or -1
 };
-static_assert(sizeof(Misc) <= 1024, "miscellaneous shared memory");
+static_assert(sizeof(Misc) <= 1280, "miscellaneous shared memory");
 
 // exp2 of the arguments that a softmax makes: 0 below the normal numbers.
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -218,6 +221,10 @@ constexpr uint32_t idesc(int n, bool bt) {
          (static_cast<uint32_t>(n >> 3) << 17) | (128u >> 4 << 24);
 }
 
+__device__ __forceinline__ void wait_slow(uint64_t* b, uint32_t parity, volatile int* err) {
+  if (!*err && !sm100::mbar_wait(b, parity)) *err = 1;
+}
+
 // Steps of an item: step k belongs to group k & 1.
 struct Steps {
   bool wide;  // over 128 rows: both groups use every tile
@@ -228,12 +235,6 @@ struct Steps {
   // Place of tile j's K and V in the ring's order of loads: the order of first use.
   __device__ __forceinline__ int k_at(int j) const { return wide ? 2 * j : (j == 0 ? 0 : 2 * j - 1); }
   __device__ __forceinline__ int v_at(int j) const { return wide ? 2 * j + 1 : (j + 1 < nt ? 2 * j + 2 : 2 * nt - 1); }
-  // The inverse: the i-th load is K (even result) or V (odd) of tile result / 2.
-  __device__ __forceinline__ int load(int i) const {
-    if (wide || i == 0) return i;
-    if (i == 2 * nt - 1) return 2 * (nt - 1) + 1;
-    return i & 1 ? i + 1 : i - 1;
-  }
 };
 
 template <typename T, int D>
@@ -266,12 +267,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int i = 0; i < kItems; ++i) {
       sm100::mbar_init(&bar.ifull[i], 1);
-      sm100::mbar_init(&bar.iempty[i], 10);  // producer, MMA issue, eight softmax warps
+      sm100::mbar_init(&bar.iempty[i], 11);  // two producers, MMA issue, eight softmax warps
     }
     sm100::mbar_init(&bar.gsync, 8);
     sm100::mbar_init(&bar.drained, 1);
     misc.err = 0;
     misc.bad = 0;
+    for (int i = 0; i < 8; ++i) misc.last[0][i] = misc.last[1][i] = -1;
     sm100::fence_barrier_init();
     sm100::prefetch_tmap(&tk);
     sm100::prefetch_tmap(&tv);
@@ -288,10 +290,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = misc.tmem;
-  // A wait that does nothing once any role of the CTA has given up.
+  // A wait that ends early once any role of the CTA has given up.
   auto wait = [&](uint64_t* b, uint32_t parity) {
-    if (*s_err) return;
-    if (!sm100::mbar_wait(b, parity)) *s_err = 1;
+    if (!sm100::mbar_try_wait(b, parity)) wait_slow(b, parity, s_err);
   };
   // 168 registers a thread at launch: 72 for the last warpgroup and 216 for the two of the softmax.
   if (warp >= 8) {
@@ -312,118 +313,145 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
     }
-    if (warp == 8) {
-      // ------------------------------------------------------------ TMA producer
-      const int boxes = kTile / box;    // page runs of a tile
-      const int ahead = 32 / boxes;     // tiles whose runs the warp's lanes look up together
-      const int run = lane % boxes;
-      unsigned count = 0;               // loads issued so far
+    if (warp == 8 || warp == 11) {
+      // ------------------------------------------------------------ TMA producers
+      const bool is_v = warp == 11;
+      const CUtensorMap* map = is_v ? &tv : &tk;
+      const int boxes = kTile / box;  // page runs of a tile
+      const int ahead = 32 / boxes;   // tiles whose runs the warp's lanes look up together
+      const int unit = is_v ? a.unit_v : a.unit_k;  // of 64 values from head to head
+      unsigned base = 0;              // loads of the items before, K and V
       for (unsigned item = 0;; ++item) {
         wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
         const Item& it = misc.item[item % kItems];
         if (__any_sync(0xffffffffu, *s_err || it.rows == 0)) break;
         const Steps st(it);
-        const int first = (it.tile0 + it.t0) * kTile, nt = st.nt, s = it.s, begin = it.begin, end = it.end, h = it.h;
+        const int first = (it.tile0 + it.t0) * kTile, nt = st.nt, s = it.s, begin = it.begin, end = it.end;
+        const int head = it.h * unit;
         if (it.over && lane == 0) atomicExch(a.err, kErrPage);
-        // Page of this lane's run in the tiles [ahead g, ahead (g + 1)); runs that no row sees lie outside the pool.
-        auto pages_of = [&](int g) {
-          const int j = g * ahead + lane / boxes, pos = first + j * kTile + run * box;
-          int page = a.num_pages;
+        // Page and token of this lane's run in the tiles [ahead g, ahead (g + 1)). Runs that no row sees lie
+        // outside the pool: zeros.
+        auto look_up = [&](int g) {
+          const int j = g * ahead + lane / boxes, pos = first + j * kTile + lane % boxes * box;
+          int2 at = make_int2(a.num_pages, 0);
           if (j < nt && pos + box > begin && pos < end) {
-            page = page_of(a.batch, s, pos / a.page_size, a.num_pages);
-            if (page < 0) {
+            at.x = page_of(a.batch, s, pos / a.page_size, a.num_pages);
+            at.y = pos % a.page_size / 8;
+            if (at.x < 0) {
               atomicExch(a.err, kErrPage);
-              page = a.num_pages;
+              at.x = a.num_pages;
             }
           }
-          return page;
+          return at;
         };
-        // Even and odd groups. The next one is looked up at a group's second tile: the tile before the group is
-        // done with its register then (its V comes after the K of the group's first), and the loads of one tile
-        // at least cover the latency.
-        int even = pages_of(0), odd = a.num_pages;
-        for (int i = 0; i < 2 * nt; ++i, ++count) {
-          const int load = st.load(i), j = load >> 1, g = j / ahead;
-          if (!(load & 1) && j % ahead == 1) {
-            if (g & 1)
-              even = pages_of(g + 1);
-            else
-              odd = pages_of(g + 1);
+        int2 cur = make_int2(0, 0), next = look_up(0);
+        for (int j = 0; j < nt; ++j) {
+          if (j % ahead == 0) {
+            cur = next;
+            next = look_up(j / ahead + 1);
           }
-          const int page = __shfl_sync(0xffffffffu, g & 1 ? odd : even, (j % ahead) * boxes + run);
-          const int slot = (first + j * kTile + run * box) % a.page_size;
-          const int sl = count % kSlots;
-          wait(&bar.empty[sl], ((count / kSlots) & 1u) ^ 1u);
+          const unsigned n = base + (is_v ? st.v_at(j) : st.k_at(j)), sl = n % kSlots, ph = (n / kSlots) & 1u;
+          wait(&bar.empty[sl], ph ^ 1u);
           if (__any_sync(0xffffffffu, *s_err)) break;
           if (lane == 0) sm100::mbar_arrive_expect_tx(&bar.full[sl], C::kTileBytes);
-          __syncwarp();
-          uint8_t* dst = ring + sl * C::kTileBytes + run * box * 128;
-          for (int x = lane; x < boxes * C::kHalves; x += 32)  // 32 lanes are a multiple of the runs
-            sm100::tma_load_4d(dst + (x / boxes) * C::kHalfBytes, load & 1 ? &tv : &tk, &bar.full[sl],
-                               (x / boxes) * 64, h, slot, page);
-          __syncwarp();
+          uint8_t* dst = ring + sl * C::kTileBytes;
+          for (int run = 0; run < boxes; ++run) {
+            const int page = __shfl_sync(0xffffffffu, cur.x, j % ahead * boxes + run);
+            const int tok8 = __shfl_sync(0xffffffffu, cur.y, j % ahead * boxes + run);
+            if (lane == 0)
+              sm100::tma_load_5d(dst + run * (box / 8) * C::kGroupBytes, map, &bar.full[sl], 0, 0, head, tok8, page);
+          }
+          if (lane == 0) misc.last[is_v][sl] = static_cast<int>(n);
         }
+        base += 2 * nt;
         if (lane == 0) sm100::mbar_arrive(&bar.iempty[item % kItems]);
       }
-      // Never leave while a copy into this CTA's shared memory is in flight.
-      if (lane == 0)
-        for (unsigned i = count > kSlots ? count - kSlots : 0; i < count; ++i)
-          sm100::mbar_wait(&bar.full[i % kSlots], (i / kSlots) & 1u);
     } else if (warp == 9) {
       // ------------------------------------------------------------ MMA issue
       if (sm100::elect_one()) {
-        unsigned base = 0;                   // loads of the items before
-        unsigned nq[2] = {0, 0}, np[2] = {0, 0};
-        auto slot_of = [&](int i) { return (base + i) % kSlots; };
-        auto phase_of = [&](int i) { return ((base + i) / kSlots) & 1u; };
+        // This thread's waits are on the critical path: it polls before it lets itself be suspended.
+        auto poll = [&](uint64_t* b, uint32_t parity) {
+          for (int i = 0; i < 256; ++i)
+            if (sm100::mbar_test_wait(b, parity)) return;
+          wait_slow(b, parity, s_err);
+        };
+        // A place in the ring.
+        struct Place {
+          int slot;
+          uint32_t phase;
+          __device__ __forceinline__ void operator+=(int n) {
+            slot += n;
+            if (slot >= kSlots) slot -= kSlots, phase ^= 1u;
+          }
+        };
+        unsigned base = 0;             // loads of the items before
+        uint32_t qphase = 0, pphase = 0;  // bit t: parity of the next qready[t], pready[t]
+        int qt = 0;                    // tile of the queries of an item of at most 128 rows
+        bool narrow_before = false;
         for (unsigned item = 0;; ++item) {
           wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
           const Item& it = misc.item[item % kItems];
           if (*s_err || it.rows == 0) break;
           const Steps st(it);
           sm100::mbar_arrive(&bar.iempty[item % kItems]);
-          const int steps = st.count();
-          wait(&bar.qready[0], nq[0]++ & 1u);
-          if (st.wide) wait(&bar.qready[1], nq[1]++ & 1u);
-            auto scores = [&](int k) {
-            const int t = k & 1, at = st.k_at(st.tile(k));
-            wait(&bar.full[slot_of(at)], phase_of(at));
+          const int steps = st.count(), nt = st.nt;
+          const bool wide = st.wide;
+          qt = !wide && narrow_before ? qt ^ 1 : 0;
+          narrow_before = !wide;
+          poll(&bar.qready[qt], qphase >> qt & 1u);
+          qphase ^= 1u << qt;
+          if (wide) {
+            poll(&bar.qready[1], qphase >> 1 & 1u);
+            qphase ^= 2u;
+          }
+          Place kp{static_cast<int>(base % kSlots), (base / kSlots) & 1u}, vp = kp;
+          vp += wide || nt == 1 ? 1 : 2;
+          // S of step k: its tile is the next in K's order. With `wide` both groups use it: the first waits for
+          // it and the second frees it.
+          auto scores = [&](int k) {
+            const int t = k & 1;
+            if (!wide || t == 0) poll(&bar.full[kp.slot], kp.phase);
             sm100::tc_fence_after();
-            const uint64_t dq = sm100::smem_desc_sw128(smem + C::kQ + (st.wide ? t : 0) * C::kTileBytes);
-            const uint64_t dk = sm100::smem_desc_sw128(ring + slot_of(at) * C::kTileBytes);
+            const uint64_t dq = sm100::smem_desc_sw128(smem + C::kQ + (wide ? t : qt) * C::kTileBytes);
+            const uint64_t dk = sm100::smem_desc_mn_sw128(ring + kp.slot * C::kTileBytes, 16, C::kGroupBytes);
 #pragma unroll
-            for (int i = 0; i < D / 16; ++i) {
-              const uint64_t off = (i >> 2) * (C::kHalfBytes >> 4) + 2 * (i & 3);
-              sm100::mma_bf16(tmem + t * 128, dq + off, dk + off, idesc<T>(128, false), i > 0 ? 1u : 0u);
-            }
+            for (int i = 0; i < D / 16; ++i)
+              sm100::mma_bf16(tmem + t * 128, dq + (i >> 2) * (C::kHalfBytes >> 4) + 2 * (i & 3),
+                              dk + (i >> 2) * (1024 >> 4) + 2 * (i & 3), idesc<T>(128, false), i > 0 ? 1u : 0u);
             sm100::mma_commit(&bar.sfull[t]);
-            if (!st.wide || t == 1) sm100::mma_commit(&bar.empty[slot_of(at)]);
+            if (!wide || t == 1) {
+              sm100::mma_commit(&bar.empty[kp.slot]);
+              kp += wide || k > 0 ? 2 : 1;
+            }
           };
           scores(0);
           if (steps > 1) scores(1);
           for (int k = 0; k < steps && !*s_err; ++k) {
-            const int t = k & 1, at = st.v_at(st.tile(k));
-            const uint32_t parity = np[t]++ & 1u;
-            wait(&bar.full[slot_of(at)], phase_of(at));
-            const uint64_t dv = sm100::smem_desc_mn_sw128(ring + slot_of(at) * C::kTileBytes, C::kHalfBytes, 1024);
-            wait(&bar.pready[t][0], parity);
+            const int t = k & 1;
+            const uint32_t parity = pphase >> t & 1u;
+            pphase ^= 1u << t;
+            if (!wide || t == 0) poll(&bar.full[vp.slot], vp.phase);
+            const uint64_t dv = sm100::smem_desc_mn_sw128(ring + vp.slot * C::kTileBytes, 1024, C::kGroupBytes);
+            poll(&bar.pready[t][0], parity);
             sm100::tc_fence_after();
 #pragma unroll
-            for (int i = 0; i < kTile / 16; ++i) {  // 16 tokens: 2048 bytes further in V, 8 columns in P
+            for (int i = 0; i < kTile / 16; ++i) {  // 16 tokens: two groups further in V, 8 columns in P
               if (i == kEarly / 16) {
-                wait(&bar.pready[t][1], parity);
+                poll(&bar.pready[t][1], parity);
                 sm100::tc_fence_after();
               }
-              sm100::mma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + i * 8, dv + i * (2048 >> 4),
+              sm100::mma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + i * 8, dv + i * (2 * C::kGroupBytes >> 4),
                                 idesc<T>(D, true), (k > 1 || i > 0) ? 1u : 0u);
             }
-            if (!st.wide || t == 1) sm100::mma_commit(&bar.empty[slot_of(at)]);
+            const int v_slot = vp.slot;
+            if (!wide || t == 1) vp += wide || k + 2 < nt ? 2 : 1;
             if (k + 2 < steps)
               scores(k + 2);
             else
               sm100::mma_commit(&bar.ofull[t]);
+            if (!wide || t == 1) sm100::mma_commit(&bar.empty[v_slot]);
           }
-          base += 2 * st.nt;
+          base += 2 * nt;
         }
         // Tensor memory is freed only after every product is done.
         sm100::mma_commit(&bar.drained);
@@ -439,7 +467,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
     const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + kColO + t * 128;
     unsigned ns = 0, no = 0, ng = 0, base = 0;  // steps, block ends, group syncs and loads so far
-    bool q_loaded = false;
+    bool q_loaded = false, narrow_before = false;
+    int qt = 0;  // tile of the queries of an item of at most 128 rows
     // All softmax warps (not a barrier that a warp which gave up would leave the others at).
     auto group_sync = [&] {
       __syncwarp();
@@ -457,13 +486,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) sm100::mbar_arrive(b);
     };
-    // Writes the queries of an item into this group's tile (or, with at most
-    // 128 rows, group 0 into its own).
-    auto load_q = [&](const Item& i) {
-      const bool wide = i.rows > 128;
-      if (!wide && t == 1) return;
-      const int r = wide ? t * 128 + row : (i.rows <= 32 ? lane : row);
-      uint8_t* dst = smem + C::kQ + t * C::kTileBytes + row * 128;
+    // Writes the queries of an item into a tile: those of this group's 128 rows, or all of an item of at most 128.
+    auto load_q = [&](const Item& i, int tile) {
+      const int r = i.rows > 128 ? t * 128 + row : (i.rows <= 32 ? lane : row);
+      uint8_t* dst = smem + C::kQ + tile * C::kTileBytes + row * 128;
       const bool valid = r < i.rows;
       const int tok = (i.row0 + r) / group, g = (i.row0 + r) % group;
       const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (i.q0 + tok) * a.q_tok +
@@ -483,7 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       sm100::fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&bar.qready[t]);
+      if (lane == 0) sm100::mbar_arrive(&bar.qready[tile]);
     };
 
     for (unsigned item = 0; more(item); ++item) {
@@ -491,8 +517,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Steps st(it);
       const int steps = st.count();
       const bool wide = st.wide, quad = it.rows <= 32;
-      if (!q_loaded) load_q(it);
-      q_loaded = false;
+      // The queries of a narrow item alternate between the tiles, so that those of the next are loaded now; the
+      // item's own tile takes the joining of its states at the end.
+      qt = !wide && narrow_before ? qt ^ 1 : 0;
+      narrow_before = !wide;
+      if (!q_loaded && (wide || t == 1)) load_q(it, wide ? t : qt);
+      const bool next_narrow = !wide && more(item + 1) && misc.item[(item + 1) % kItems].rows <= 128;
+      if (next_narrow && t == 1) load_q(misc.item[(item + 1) % kItems], qt ^ 1);
+      q_loaded = next_narrow;
       // This thread's row of the block and what it sees.
       const int r = wide ? t * 128 + row : (quad ? lane : row);
       const bool valid = r < it.rows;
@@ -511,21 +543,21 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int k = t; k < steps; k += 2, ++mine) {
         const int j = st.tile(k);
         const int c0 = first_pos + j * kTile;
+        wait(&bar.sfull[t], ns++ & 1u);
+        sm100::tc_fence_after();
         // Tokens behind the sequence and before every row's window may hold anything: zeros in V, since
-        // zero times NaN is NaN.
+        // zero times NaN is NaN. (After S of the step: its K, and what the slot of V held before, are consumed.)
         if (c0 + kTile > len || c0 < begin) {
           const unsigned at = base + st.v_at(j);
           wait(&bar.full[at % kSlots], (at / kSlots) & 1u);
           if (c0 + row >= len || c0 + row < begin) {
-            uint8_t* vt = ring + (at % kSlots) * C::kTileBytes + row * 128;
+            uint8_t* vt = ring + (at % kSlots) * C::kTileBytes + (row >> 3) * C::kGroupBytes + (row & 7) * 128;
 #pragma unroll
             for (int c = 0; c < 8 * C::kHalves; ++c)
-              *reinterpret_cast<uint4*>(vt + (c >> 3) * C::kHalfBytes + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(vt + (c >> 3) * 1024 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
           }
           sm100::fence_proxy_async_smem();
         }
-        wait(&bar.sfull[t], ns++ & 1u);
-        sm100::tc_fence_after();
         if (!idle) {
           // Columns of this thread: all, or the warp's quarter.
           auto softmax = [&](auto cols_tag, auto masked_tag) {
@@ -614,7 +646,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 
       // ---------------------------------------------------------- end of the block's part
       if (wide && more(item + 1)) {  // this group's last S is done: its queries are free
-        load_q(misc.item[(item + 1) % kItems]);
+        const Item& next = misc.item[(item + 1) % kItems];
+        if (next.rows > 128 || t == 0) load_q(next, t);
         q_loaded = true;
       }
       if (mine > 0) {
@@ -637,9 +670,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                             it.h);
       };
       // Stores 32 columns of a row: rounded with the factor inv, or as fp32 to the workspace.
-      auto store32 = [&](int r2, int c, const float* o, float inv, float& odd) {
+      T* const out = out_of(min(r, it.rows - 1));
+      auto store32 = [&](int c, const float* o, float inv, float& odd) {
         if (whole) {
-          uint4* dst = reinterpret_cast<uint4*>(out_of(r2) + c);
+          uint4* dst = reinterpret_cast<uint4*>(out + c);
 #pragma unroll
           for (int e = 0; e < 32; e += 8) {
             float y[8];
@@ -652,7 +686,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     pack2<T>(y[6], y[7]));
           }
         } else {
-          float4* dst = reinterpret_cast<float4*>(acc + static_cast<int64_t>(r2) * D + c);
+          float4* dst = reinterpret_cast<float4*>(acc + static_cast<int64_t>(r) * D + c);
 #pragma unroll
           for (int e = 0; e < 32; e += 4) dst[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
         }
@@ -668,28 +702,36 @@ __global__ void __launch_bounds__(kThreads, 1)
             uint32_t o[32];
             sm100::tmem_ld_32x32b_x32(tO + c, o);
             sm100::tmem_ld_wait();
-            if (valid) store32(r, c, reinterpret_cast<const float*>(o), inv, odd);
+            if (valid) store32(c, reinterpret_cast<const float*>(o), inv, odd);
           }
           if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(m2, l);
           unsigned redo = __ballot_sync(0xffffffffu, whole && valid && odd != 0.f);
           for (; redo; redo &= redo - 1) again(t * 128 + w4 * 32 + __ffs(redo) - 1);
         }
       } else {
-        // Join the states of each row through shared memory that the queries held.
-        float2* sml = reinterpret_cast<float2*>(smem + C::kQ);
-        float* buf = reinterpret_cast<float*>(smem + C::kQ + C::kTileBytes);
+        // Join the states of each row through the memory that the item's queries held.
+        float* buf = reinterpret_cast<float*>(smem + C::kQ + qt * C::kTileBytes);
+        float2* sml = reinterpret_cast<float2*>(buf);
         constexpr int kBuf = C::kTileBytes / 4;
         group_sync();  // every S of the block is done in both groups
         sml[t * 128 + row] = make_float2(m2, l);
         group_sync();
         const int states = quad ? 8 : 2;
+        float2 state[8];
         float mj = -INFINITY, lj = 0.f;
-        for (int i = 0; i < states; ++i) mj = fmaxf(mj, sml[quad ? i * 32 + lane : i * 128 + row].x);
-        auto factor = [&](float mm) { return mm == -INFINITY ? 0.f : fast_exp2(mm - mj); };
-        for (int i = 0; i < states; ++i) {
-          const float2 v = sml[quad ? i * 32 + lane : i * 128 + row];
-          lj += v.y * factor(v.x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          state[i] = i < states ? sml[quad ? i * 32 + lane : i * 128 + row] : make_float2(-INFINITY, 0.f);
+          mj = fmaxf(mj, state[i].x);
         }
+        auto factor = [&](float mm) { return mm == -INFINITY ? 0.f : fast_exp2(mm - mj); };
+#pragma unroll
+        for (int i = 0; i < 8; ++i) lj += state[i].y * factor(state[i].x);
+        if (quad && warp == 0) {
+          misc.sum[lane] = lj;
+          if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
+        }
+        group_sync();
         const float f = factor(m2);
         if (!quad) {
           const float inv = lj == 0.f ? 0.f : 1.f / lj;
@@ -731,7 +773,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                   y[4 * e + 2] = __uint_as_float(o[4 * e + 2]) * f + other.z;
                   y[4 * e + 3] = __uint_as_float(o[4 * e + 3]) * f + other.w;
                 }
-                if (valid) store32(r, c0 + c, y, inv, odd);
+                if (valid) store32(c0 + c, y, inv, odd);
               }
             }
           }
@@ -770,18 +812,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int i = threadIdx.x; i < it.rows * (pass / 4); i += 256) {
               const int r2 = i / (pass / 4), c = i % (pass / 4);
               float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-              float mr = -INFINITY, lr = 0.f;
-              for (int q = 0; q < 8; ++q) mr = fmaxf(mr, sml[q * 32 + r2].x);
 #pragma unroll
               for (int q = 0; q < 8; ++q) {
                 const float4 v = reinterpret_cast<const float4*>(buf + (q * it.rows + r2) * pass)[c ^ (r2 & 3)];
-                y.x += v.x;
-                y.y += v.y;
-                y.z += v.z;
-                y.w += v.w;
-                const float2 s = sml[q * 32 + r2];
-                lr += s.x == -INFINITY ? 0.f : s.y * fast_exp2(s.x - mr);
+                y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
               }
+              const float lr = misc.sum[r2];
               if (whole) {
                 const float inv = lr == 0.f ? 0.f : 1.f / lr;
                 if (inv == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -790,7 +826,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                 *reinterpret_cast<uint2*>(out_of(r2) + c0 + 4 * c) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
               } else {
                 *reinterpret_cast<float4*>(acc + static_cast<int64_t>(r2) * D + c0 + 4 * c) = y;
-                if (c0 == 0 && c == 0) *reinterpret_cast<float2*>(ml + r2 * 2) = make_float2(mr, lr);
               }
             }
           }
@@ -803,7 +838,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (threadIdx.x == 0) misc.bad = 0;
           }
         }
-        group_sync();  // the queries' memory is free again
+        group_sync();  // the item's memory is free again
       }
       sm100::tc_fence_before();
       __syncwarp();
@@ -817,7 +852,15 @@ __global__ void __launch_bounds__(kThreads, 1)
     sm100::tc_fence_after();
     sm100::tmem_dealloc(tmem, kTmemCols);
   }
-  if (threadIdx.x == 0 && *s_err) atomicExch(a.err, kErrTimeout);
+  if (threadIdx.x == 0 && *s_err) {
+    // Every load was waited for by its product, unless a role gave up: then it is here, so that none is in flight
+    // when the CTA's memory goes.
+    for (int sl = 0; sl < kSlots; ++sl) {
+      const int n = max(misc.last[0][sl], misc.last[1][sl]);
+      if (n >= 0) sm100::mbar_wait(&bar.full[sl], (n / kSlots) & 1);
+    }
+    atomicExch(a.err, kErrTimeout);
+  }
 }
 
 // ------------------------------------------------------------------ merge
@@ -924,19 +967,22 @@ EncodeFn encode() {
   return fn;
 }
 
-// 4-D map over a pool [pages, page_size, kv_heads, d] with its strides; box of
-// 64 dims x 1 head x `box` tokens x 1 page, 128-byte swizzle.
-CUtensorMap pool_map(const Pool& p, int d, int hkv, int page_size, int num_pages, int box, Half type) {
+// Map over a pool [pages, page_size, kv_heads, d] with its strides, in 64-value
+// units: (64 values, 8 tokens, unit, tokens / 8, page). Units of 64 values from
+// a token's first on hold all its heads, so a head is `unit` of them further
+// and its halves are neighbours. A box is 64 values x 8 tokens x the halves x
+// `box` / 8 x 1: runs of 8 tokens in the layout [half][token][128 bytes].
+CUtensorMap pool_map(const Pool& p, int d, int hkv, int unit, int page_size, int num_pages, int box, Half type) {
   CUtensorMap m;
-  const cuuint64_t dims[4] = {static_cast<cuuint64_t>(d), static_cast<cuuint64_t>(hkv),
-                              static_cast<cuuint64_t>(page_size), static_cast<cuuint64_t>(num_pages)};
+  const cuuint64_t dims[5] = {64, 8, static_cast<cuuint64_t>((hkv - 1) * static_cast<int64_t>(unit) + d / 64),
+                              static_cast<cuuint64_t>(page_size / 8), static_cast<cuuint64_t>(num_pages)};
   // The stride of a dimension of one is never used; any valid one serves.
-  const auto bytes = [](int64_t n, int64_t stride) { return static_cast<cuuint64_t>(n == 1 ? 16 : stride * 2); };
-  const cuuint64_t strides[3] = {bytes(hkv, p.head), bytes(page_size, p.tok), bytes(num_pages, p.page)};
-  const cuuint32_t boxes[4] = {64, 1, static_cast<cuuint32_t>(box), 1};
-  const cuuint32_t estr[4] = {1, 1, 1, 1};
+  const cuuint64_t strides[4] = {static_cast<cuuint64_t>(p.tok) * 2, 128, static_cast<cuuint64_t>(p.tok) * 16,
+                                 num_pages == 1 ? 16 : static_cast<cuuint64_t>(p.page) * 2};
+  const cuuint32_t boxes[5] = {64, 8, static_cast<cuuint32_t>(d / 64), static_cast<cuuint32_t>(box / 8), 1};
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   const CUresult r = encode()(
-      &m, type == Half::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, p.base, dims,
+      &m, type == Half::kBf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5, p.base, dims,
       strides, boxes, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
       CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) throw std::runtime_error("cuTensorMapEncodeTiled (paged cache) failed: " + std::to_string(r));
@@ -953,12 +999,21 @@ int sm_count() {
 int row_cap(int64_t rows, int group) { return static_cast<int>(std::min<int64_t>(kBlock, rows * group)); }
 
 template <typename T, int D>
-void launch(const AttnArgs& a, Half type, float* workspace, cudaStream_t s) {
+void launch(const AttnArgs& args, Half type, float* workspace, cudaStream_t s) {
+  AttnArgs a = args;
+  const auto unit = [&](const Pool& p) {
+    if (a.hkv == 1) return D / 64;
+    B200AR_CHECK(p.head % 64 == 0 && p.head / 64 * a.hkv < (1ll << 31),
+                 "the pools' heads must be a multiple of 64 values apart");
+    return static_cast<int>(p.head / 64);
+  };
+  a.unit_k = unit(a.k);
+  a.unit_v = unit(a.v);
   const int group = a.hq / a.hkv, ctas = sm_count();
   int box = kTile;
   while (a.page_size % box) box /= 2;
-  const CUtensorMap tk = pool_map(a.k, D, a.hkv, a.page_size, a.num_pages, box, type);
-  const CUtensorMap tv = pool_map(a.v, D, a.hkv, a.page_size, a.num_pages, box, type);
+  const CUtensorMap tk = pool_map(a.k, D, a.hkv, a.unit_k, a.page_size, a.num_pages, box, type);
+  const CUtensorMap tv = pool_map(a.v, D, a.hkv, a.unit_v, a.page_size, a.num_pages, box, type);
   Workspace ws{};
   ws.row_cap = row_cap(a.rows, group);
   ws.desc = reinterpret_cast<PartDesc*>(workspace);

@@ -63,6 +63,7 @@ struct AttnArgs {
   int rows, hq, hkv, num_pages, page_size;
   int capacity;  // positions of a row of the page table
   int window;    // positions that a row sees, its own included; 0: all
+  int unit_k, unit_v;  // set by paged_attention(): 64-value units from KV head to KV head
   bool causal;
   float scale;
 };
