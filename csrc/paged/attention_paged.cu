@@ -25,7 +25,10 @@
 //   up to 32   as before, and the 32 rows are held four times: warp w of a
 //              group takes the tokens 32 w .. 32 w + 31 of a tile. The products
 //              cost the same, the softmax of a tile a quarter
-// and the states of a row (its maximum, sum and O) are joined at the end.
+// and the states of a row (its maximum, sum and O) are joined at the end. Calls
+// with one token for each sequence and at most 32 heads to a KV head have only
+// the last kind: they run an instance of the kernel without the others' code
+// (kTokens), which a short call fetches faster.
 //
 // S(k + 2) is issued after P V(k), in the order of which the tensor core
 // works, so a group that sees S(k + 2) knows that O holds step k: it may
@@ -156,7 +159,7 @@ struct Barriers {
   uint64_t sfull[2];           // S_t computed (and the O_t of the step before)
   uint64_t pready[2][2];       // O_t rescaled and the first kEarly tokens of P_t written; the rest written
   uint64_t ofull[2];           // last P V of group t in a block done
-  uint64_t gsync;              // the eight softmax warps
+  uint64_t gsync, gfree;       // the eight softmax warps: states written; their memory read
   uint64_t ifull[4], iempty[4];  // ring of items
   uint64_t drained;
 };
@@ -226,10 +229,11 @@ __device__ __forceinline__ void wait_slow(uint64_t* b, uint32_t parity, volatile
 }
 
 // Steps of an item: step k belongs to group k & 1.
+template <bool kTokens>
 struct Steps {
   bool wide;  // over 128 rows: both groups use every tile
   int nt;     // tiles
-  __device__ __forceinline__ Steps(const Item& it) : wide(it.rows > 128), nt(it.t1 - it.t0) {}
+  __device__ __forceinline__ Steps(const Item& it) : wide(!kTokens && it.rows > 128), nt(it.t1 - it.t0) {}
   __device__ __forceinline__ int count() const { return wide ? 2 * nt : nt; }
   __device__ __forceinline__ int tile(int k) const { return wide ? k >> 1 : k; }
   // Place of tile j's K and V in the ring's order of loads: the order of first use.
@@ -237,7 +241,7 @@ struct Steps {
   __device__ __forceinline__ int v_at(int j) const { return wide ? 2 * j + 1 : (j + 1 < nt ? 2 * j + 2 : 2 * nt - 1); }
 };
 
-template <typename T, int D>
+template <typename T, int D, bool kTokens>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                      const __grid_constant__ AttnArgs a, const Workspace ws, int group, int box, float q_sign,
@@ -270,6 +274,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::mbar_init(&bar.iempty[i], 11);  // two producers, MMA issue, eight softmax warps
     }
     sm100::mbar_init(&bar.gsync, 8);
+    sm100::mbar_init(&bar.gfree, 8);
     sm100::mbar_init(&bar.drained, 1);
     misc.err = 0;
     misc.bad = 0;
@@ -294,9 +299,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait = [&](uint64_t* b, uint32_t parity) {
     if (!sm100::mbar_try_wait(b, parity)) wait_slow(b, parity, s_err);
   };
-  // 168 registers a thread at launch: 72 for the last warpgroup and 216 for the two of the softmax.
+  // 168 registers a thread at launch: 72 for the last warpgroup and 216 for the two of the softmax, where whole
+  // rows of S are held.
   if (warp >= 8) {
-    sm100::reg_give<72>();
+    if constexpr (!kTokens) sm100::reg_give<72>();
     if (warp == 10) {
       // ---------------------------------------------------------- items
       if (lane == 0) {
@@ -325,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
         const Item& it = misc.item[item % kItems];
         if (__any_sync(0xffffffffu, *s_err || it.rows == 0)) break;
-        const Steps st(it);
+        const Steps<kTokens> st(it);
         const int first = (it.tile0 + it.t0) * kTile, nt = st.nt, s = it.s, begin = it.begin, end = it.end;
         const int head = it.h * unit;
         if (it.over && lane == 0) atomicExch(a.err, kErrPage);
@@ -392,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
           const Item& it = misc.item[item % kItems];
           if (*s_err || it.rows == 0) break;
-          const Steps st(it);
+          const Steps<kTokens> st(it);
           sm100::mbar_arrive(&bar.iempty[item % kItems]);
           const int steps = st.count(), nt = st.nt;
           const bool wide = st.wide;
@@ -461,12 +467,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ------------------------------------------------------------ softmax
-    sm100::reg_take<216>();
+    if constexpr (!kTokens) sm100::reg_take<216>();
     const int t = warp >> 2, w4 = warp & 3;
     const int row = w4 * 32 + lane;  // row of the group's tile
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
     const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + kColO + t * 128;
-    unsigned ns = 0, no = 0, ng = 0, base = 0;  // steps, block ends, group syncs and loads so far
+    unsigned ns = 0, no = 0, ng = 0, nf = 0, base = 0;  // steps, block ends, joins, frees and loads so far
     bool q_loaded = false, narrow_before = false;
     int qt = 0;  // tile of the queries of an item of at most 128 rows
     // All softmax warps (not a barrier that a warp which gave up would leave the others at).
@@ -488,7 +494,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     // Writes the queries of an item into a tile: those of this group's 128 rows, or all of an item of at most 128.
     auto load_q = [&](const Item& i, int tile) {
-      const int r = i.rows > 128 ? t * 128 + row : (i.rows <= 32 ? lane : row);
+      const int r = !kTokens && i.rows > 128 ? t * 128 + row : (kTokens || i.rows <= 32 ? lane : row);
       uint8_t* dst = smem + C::kQ + tile * C::kTileBytes + row * 128;
       const bool valid = r < i.rows;
       const int tok = (i.row0 + r) / group, g = (i.row0 + r) % group;
@@ -514,11 +520,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     for (unsigned item = 0; more(item); ++item) {
       const Item& it = misc.item[item % kItems];
-      const Steps st(it);
+      const Steps<kTokens> st(it);
       const int steps = st.count();
-      const bool wide = st.wide, quad = it.rows <= 32;
+      const bool wide = st.wide, quad = kTokens || it.rows <= 32;
       // The queries of a narrow item alternate between the tiles, so that those of the next are loaded now; the
       // item's own tile takes the joining of its states at the end.
+      if (narrow_before) wait(&bar.gfree, nf++ & 1u);  // the memory of the item before is read
       qt = !wide && narrow_before ? qt ^ 1 : 0;
       narrow_before = !wide;
       if (!q_loaded && (wide || t == 1)) load_q(it, wide ? t : qt);
@@ -631,7 +638,9 @@ __global__ void __launch_bounds__(kThreads, 1)
           };
           using Yes = std::integral_constant<bool, true>;
           using No = std::integral_constant<bool, false>;
-          if (quad) {
+          if constexpr (kTokens) {
+            softmax(std::integral_constant<int, 32>{}, Yes{});
+          } else if (quad) {
             softmax(std::integral_constant<int, 32>{}, Yes{});
           } else if (c0 >= lo_all && c0 + kTile <= hi_all) {
             softmax(std::integral_constant<int, 128>{}, No{});
@@ -693,119 +702,89 @@ __global__ void __launch_bounds__(kThreads, 1)
       };
       const float m2 = m == -INFINITY ? -INFINITY : m * scale_log2;
 
-      if (wide) {
-        const float inv = l == 0.f ? 0.f : 1.f / l;
+      // Rows computed by one thread each: 128 of a wide block by each group, or a narrow block's by group 0, which
+      // adds the state of group 1: the same rows in the same lanes of tensor memory.
+      auto finish_rows = [&](float mj, float lj, float f0, float f1, bool add) {
+        const float inv = lj == 0.f ? 0.f : 1.f / lj;
         float odd = 0.f;
-        if (!idle) {
 #pragma unroll 1
-          for (int c = 0; c < D; c += 32) {
-            uint32_t o[32];
-            sm100::tmem_ld_32x32b_x32(tO + c, o);
+        for (int c = 0; c < D; c += 32) {
+          uint32_t o[32];
+          sm100::tmem_ld_32x32b_x32(tO + c, o);
+          sm100::tmem_ld_wait();
+          float y[32];
+#pragma unroll
+          for (int e = 0; e < 32; ++e) y[e] = __uint_as_float(o[e]) * f0;
+          if (add) {
+            sm100::tmem_ld_32x32b_x32(tO + 128 + c, o);
             sm100::tmem_ld_wait();
-            if (valid) store32(c, reinterpret_cast<const float*>(o), inv, odd);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) y[e] += __uint_as_float(o[e]) * f1;
           }
-          if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(m2, l);
-          unsigned redo = __ballot_sync(0xffffffffu, whole && valid && odd != 0.f);
-          for (; redo; redo &= redo - 1) again(t * 128 + w4 * 32 + __ffs(redo) - 1);
+          if (valid) store32(c, y, inv, odd);
         }
+        if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
+        unsigned redo = __ballot_sync(0xffffffffu, whole && valid && odd != 0.f);
+        for (; redo; redo &= redo - 1) again((wide ? t * 128 : 0) + w4 * 32 + __ffs(redo) - 1);
+      };
+      float* buf = reinterpret_cast<float*>(smem + C::kQ + qt * C::kTileBytes);
+      if (wide) {
+        if (!idle) finish_rows(m2, l, 1.f, 0.f, false);
       } else {
-        // Join the states of each row through the memory that the item's queries held.
-        float* buf = reinterpret_cast<float*>(smem + C::kQ + qt * C::kTileBytes);
-        float2* sml = reinterpret_cast<float2*>(buf);
-        constexpr int kBuf = C::kTileBytes / 4;
-        group_sync();  // every S of the block is done in both groups
-        sml[t * 128 + row] = make_float2(m2, l);
+        // The states of all warps, through the memory of the item's queries: every S is done, since it was issued
+        // before the last but one product with V, which each group with a step has waited for.
+        float2* sml = reinterpret_cast<float2*>(buf);  // [8 warps][32 lanes]
+        const bool two = steps > 1;                    // group 1 had a tile
+        if (mine > 0) sml[threadIdx.x] = make_float2(m2, l);
+        sm100::tc_fence_before();
         group_sync();
-        const int states = quad ? 8 : 2;
-        float2 state[8];
-        float mj = -INFINITY, lj = 0.f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          state[i] = i < states ? sml[quad ? i * 32 + lane : i * 128 + row] : make_float2(-INFINITY, 0.f);
-          mj = fmaxf(mj, state[i].x);
-        }
-        auto factor = [&](float mm) { return mm == -INFINITY ? 0.f : fast_exp2(mm - mj); };
-#pragma unroll
-        for (int i = 0; i < 8; ++i) lj += state[i].y * factor(state[i].x);
-        if (quad && warp == 0) {
-          misc.sum[lane] = lj;
-          if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
-        }
-        group_sync();
-        const float f = factor(m2);
+        auto factor = [](float mm, float top) { return mm == -INFINITY ? 0.f : fast_exp2(mm - top); };
         if (!quad) {
-          const float inv = lj == 0.f ? 0.f : 1.f / lj;
-          float odd = 0.f;
-          // Group 1 hands over half of its columns at a time; its float4 c sits at place c ^ (row & 7).
-          constexpr int kPass = kBuf / 128;
-          const bool two = steps > 1;  // group 1 had a tile
-#pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += kPass) {
-            if (c0) group_sync();
-            if (t == 1 && two && !idle) {
-#pragma unroll 1
-              for (int c = 0; c < kPass; c += 32) {
-                uint32_t o[32];
-                sm100::tmem_ld_32x32b_x32(tO + c0 + c, o);
-                sm100::tmem_ld_wait();
-                float4* dst = reinterpret_cast<float4*>(buf + row * kPass);
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                  dst[(c / 4 + e) ^ (row & 7)] =
-                      make_float4(__uint_as_float(o[4 * e]) * f, __uint_as_float(o[4 * e + 1]) * f,
-                                  __uint_as_float(o[4 * e + 2]) * f, __uint_as_float(o[4 * e + 3]) * f);
-              }
-            }
-            group_sync();
-            if (t == 0 && !idle) {
-#pragma unroll 1
-              for (int c = 0; c < kPass; c += 32) {
-                uint32_t o[32];
-                sm100::tmem_ld_32x32b_x32(tO + c0 + c, o);
-                sm100::tmem_ld_wait();
-                float y[32];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                  float4 other = make_float4(0.f, 0.f, 0.f, 0.f);
-                  if (two) other = reinterpret_cast<const float4*>(buf + row * kPass)[(c / 4 + e) ^ (row & 7)];
-                  y[4 * e] = __uint_as_float(o[4 * e]) * f + other.x;
-                  y[4 * e + 1] = __uint_as_float(o[4 * e + 1]) * f + other.y;
-                  y[4 * e + 2] = __uint_as_float(o[4 * e + 2]) * f + other.z;
-                  y[4 * e + 3] = __uint_as_float(o[4 * e + 3]) * f + other.w;
-                }
-                if (valid) store32(c0 + c, y, inv, odd);
-              }
-            }
-          }
           if (t == 0 && !idle) {
-            if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
-            unsigned redo = __ballot_sync(0xffffffffu, whole && valid && odd != 0.f);
-            for (; redo; redo &= redo - 1) again(w4 * 32 + __ffs(redo) - 1);
+            const float2 other = two ? sml[128 + row] : make_float2(-INFINITY, 0.f);
+            const float mj = fmaxf(m2, other.x), f0 = factor(m2, mj), f1 = factor(other.x, mj);
+            sm100::tc_fence_after();
+            finish_rows(mj, l * f0 + other.y * f1, f0, f1, two);
           }
         } else {
-          // Eight states a row. A pass takes as many columns as fit: state-row i * rows + r, float4 c at
-          // place c ^ (r & 7); then a thread adds the states of four columns of a row.
+          // Lane = row. The two groups' states of a quarter lie in the same lanes: warp (t, w) adds them for the
+          // half t of the columns and writes the quarter's sum; then a thread adds the quarters of four columns
+          // of a row. A pass takes as many columns as fit; float4 c sits at place c ^ (r & 3).
+          float* part = buf + 512;
+          constexpr int kPart = C::kTileBytes / 4 - 512;
+          float mj = -INFINITY, lj = 0.f;
+          for (int i = 0; i < (two ? 8 : 4); ++i) mj = fmaxf(mj, sml[i * 32 + lane].x);
+          for (int i = 0; i < (two ? 8 : 4); ++i) lj += sml[i * 32 + lane].y * factor(sml[i * 32 + lane].x, mj);
+          const float f0 = factor(sml[w4 * 32 + lane].x, mj);
+          const float f1 = two ? factor(sml[(4 + w4) * 32 + lane].x, mj) : 0.f;
+          if (warp == 0) {
+            misc.sum[lane] = lj;
+            if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
+          }
+          sm100::tc_fence_after();
+          const uint32_t tO0 = tmem + lanes + kColO;
           int pass = D;
-          while (8 * it.rows * pass > kBuf) pass /= 2;  // 32 rows: D / 4 columns
-          const int state = t * 4 + w4;
+          while (4 * it.rows * pass > kPart) pass /= 2;  // 32 rows: 32 columns of 128, 16 of 64
 #pragma unroll 1
           for (int c0 = 0; c0 < D; c0 += pass) {
             if (c0) group_sync();
 #pragma unroll 1
-            for (int c = 0; c < pass; c += 16) {
-              uint32_t o[16];
-              sm100::tmem_ld_32x32b_x16(tO + c0 + c, o);
+            for (int c = t * (pass / 2); c < (t + 1) * (pass / 2); c += 8) {
+              uint32_t o0[8], o1[8];
+              sm100::tmem_ld_32x32b_x8(tO0 + c0 + c, o0);
+              if (two) sm100::tmem_ld_32x32b_x8(tO0 + 128 + c0 + c, o1);
               sm100::tmem_ld_wait();
-              if (valid) {
-                float4* dst = reinterpret_cast<float4*>(buf + (state * it.rows + r) * pass);
+              float y[8];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                  const float4 v = make_float4(__uint_as_float(o[4 * e]), __uint_as_float(o[4 * e + 1]),
-                                               __uint_as_float(o[4 * e + 2]), __uint_as_float(o[4 * e + 3]));
-                  // A state that saw nothing holds no numbers yet, or zeros times whatever V holds.
-                  dst[(c / 4 + e) ^ (r & 3)] = f == 0.f ? make_float4(0.f, 0.f, 0.f, 0.f)
-                                                        : make_float4(v.x * f, v.y * f, v.z * f, v.w * f);
-                }
+              for (int e = 0; e < 8; ++e) {
+                // A state that saw nothing holds zeros times whatever V holds.
+                y[e] = f0 == 0.f ? 0.f : __uint_as_float(o0[e]) * f0;
+                if (two && f1 != 0.f) y[e] += __uint_as_float(o1[e]) * f1;
+              }
+              if (valid) {
+                float4* dst = reinterpret_cast<float4*>(part + (w4 * it.rows + r) * pass);
+                dst[(c / 4) ^ (r & 3)] = make_float4(y[0], y[1], y[2], y[3]);
+                dst[(c / 4 + 1) ^ (r & 3)] = make_float4(y[4], y[5], y[6], y[7]);
               }
             }
             group_sync();
@@ -813,13 +792,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               const int r2 = i / (pass / 4), c = i % (pass / 4);
               float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-              for (int q = 0; q < 8; ++q) {
-                const float4 v = reinterpret_cast<const float4*>(buf + (q * it.rows + r2) * pass)[c ^ (r2 & 3)];
+              for (int q = 0; q < 4; ++q) {
+                const float4 v = reinterpret_cast<const float4*>(part + (q * it.rows + r2) * pass)[c ^ (r2 & 3)];
                 y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
               }
-              const float lr = misc.sum[r2];
               if (whole) {
-                const float inv = lr == 0.f ? 0.f : 1.f / lr;
+                const float lr = misc.sum[r2], inv = lr == 0.f ? 0.f : 1.f / lr;
                 if (inv == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
                 y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
                 if ((y.x + y.y + y.z + y.w) * 0.f != 0.f) atomicOr(&misc.bad, 1u << r2);
@@ -829,16 +807,18 @@ __global__ void __launch_bounds__(kThreads, 1)
               }
             }
           }
-          group_sync();
-          const unsigned bad = *reinterpret_cast<volatile unsigned*>(&misc.bad);
-          if (bad) {
-            for (int r2 = warp; r2 < it.rows; r2 += 8)
-              if (bad >> r2 & 1u) again(r2);
-            group_sync();
-            if (threadIdx.x == 0) misc.bad = 0;
+          if (whole) {
+            group_sync();  // all rows are written: those that came out as NaN are computed again
+            const unsigned bad = *reinterpret_cast<volatile unsigned*>(&misc.bad);
+            if (bad) {
+              for (int r2 = warp; r2 < it.rows; r2 += 8)
+                if (bad >> r2 & 1u) again(r2);
+              group_sync();
+              if (threadIdx.x == 0) misc.bad = 0;
+            }
           }
         }
-        group_sync();  // the item's memory is free again
+        arrive(&bar.gfree);
       }
       sm100::tc_fence_before();
       __syncwarp();
@@ -1019,11 +999,12 @@ void launch(const AttnArgs& args, Half type, float* workspace, cudaStream_t s) {
   ws.desc = reinterpret_cast<PartDesc*>(workspace);
   ws.ml = workspace + 2ll * ctas * (sizeof(PartDesc) / 4);
   ws.acc = ws.ml + 2ll * ctas * ws.row_cap * 2;
-  auto kern = attention_kernel<T, D>;
+  const bool tokens = a.batch.q_start == nullptr && group <= 32;
+  auto kern = tokens ? attention_kernel<T, D, true> : attention_kernel<T, D, false>;
   static PerDeviceOnce attr;
   attr([&] {
-    B200AR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                     static_cast<int>(Cfg<D>::kSmem)));
+    for (auto k : {attention_kernel<T, D, true>, attention_kernel<T, D, false>})
+      B200AR_CUDA(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(Cfg<D>::kSmem)));
   });
   const float sign = a.scale > 0.f ? 1.f : (a.scale < 0.f ? -1.f : 0.f);
   const float scale_log2 = (sign == 0.f ? 1.f : a.scale * sign) * kLog2e;

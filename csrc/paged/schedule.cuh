@@ -23,10 +23,16 @@ namespace paged {
 constexpr int kTile = 128;   // tokens of a K or V tile
 constexpr int kBlock = 256;  // rows of a block
 
+// Quotients of numbers that are nearly always below 2^32.
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+  return a / b;
+}
+
 struct SeqWork {
   int n, len, q0, blocks;
   int64_t a, cap, head;  // weight of block 0, limit of a weight, weight of all blocks of one head
-  int step;              // growth from block to block
+  bool grows;            // by kBlock from block to block, up to the limit
 
   __device__ __forceinline__ void load(const AttnArgs& p, int group, int s) {
     q0 = q_begin(p.batch, s);
@@ -36,23 +42,23 @@ struct SeqWork {
     const int64_t g = group, fixed = kTile * g;
     if (p.causal) {
       a = g * max(len - n, 0) + kBlock + fixed;
-      step = kBlock;
+      grows = true;
       cap = p.window > 0 ? g * p.window + kBlock + 2 * fixed : (1ll << 60);
     } else {
       a = g * max(len, 0) + fixed;
-      step = 0;
+      grows = false;
       cap = 1ll << 60;
     }
     head = before(blocks);
   }
   __device__ __forceinline__ int64_t weight(int b) const {
-    return min(a + static_cast<int64_t>(step) * b, cap);
+    return min(a + (grows ? static_cast<int64_t>(kBlock) * b : 0), cap);
   }
   // Weight of the blocks before b.
   __device__ __forceinline__ int64_t before(int b) const {
-    int64_t ramp = a >= cap ? 0 : b;
-    if (step > 0 && a < cap) ramp = min(ramp, (cap - a + step - 1) / step);
-    return a * ramp + step * (ramp * (ramp - 1) / 2) + (b - ramp) * (step > 0 || a >= cap ? cap : 0);
+    if (!grows) return a * b;
+    const int64_t ramp = a >= cap ? 0 : min(static_cast<int64_t>(b), (cap - a + kBlock - 1) / kBlock);
+    return a * ramp + kBlock * (ramp * (ramp - 1) / 2) + (b - ramp) * (b > ramp ? cap : 0);
   }
 };
 
@@ -89,7 +95,7 @@ struct Walk {
     s = pt.s0;
     if (!pt.active) return;
     w.load(p, group, s);
-    h = static_cast<int>(pt.off0 / w.head);
+    h = static_cast<int>(quotient(pt.off0, w.head));
     const int64_t rest = pt.off0 - h * w.head;
     int lo = 0, hi = w.blocks - 1;  // the last block with before(b) <= rest
     while (lo < hi) {
@@ -137,8 +143,8 @@ struct Walk {
       it.tiles = it.end > it.begin ? (it.end + kTile - 1) / kTile - it.tile0 : 1;
       const int64_t x0 = s == part.s0 ? max(part.off0 - at, static_cast<int64_t>(0)) : 0;
       const int64_t x1 = s == part.s1 ? min(part.off1 - at, weight) : weight;
-      it.t0 = static_cast<int>(x0 * it.tiles / weight);
-      it.t1 = static_cast<int>(x1 * it.tiles / weight);
+      it.t0 = x0 == 0 ? 0 : static_cast<int>(quotient(x0 * it.tiles, weight));
+      it.t1 = x1 == weight ? it.tiles : static_cast<int>(quotient(x1 * it.tiles, weight));
       at += weight;
       ++b;
       if (it.t0 < it.t1) return true;
@@ -175,14 +181,11 @@ __device__ __forceinline__ void find_part(const AttnArgs& p, int group, int64_t*
     if (i < warp) base += red[i];
     total += red[i];
   }
-  // Every part holds the weight of one tile at least (its tokens and its block's constant).
+  // Equal parts, none below the weight of one tile (its tokens and its block's constant).
   const int64_t least = static_cast<int64_t>(kTile) * group;
-  const int64_t ctas = min(static_cast<int64_t>(gridDim.x), max((total + least - 1) / least, static_cast<int64_t>(1)));
-  const int64_t c = blockIdx.x;
-  if (c < ctas && total > 0) {
-    // total is below 2^60 / 2^10: the products stay inside 64 bits for any batch that fits memory.
-    const int64_t x0 = total / ctas * c + total % ctas * c / ctas;
-    const int64_t x1 = total / ctas * (c + 1) + total % ctas * (c + 1) / ctas;
+  const int64_t part_weight = max(quotient(total + gridDim.x - 1, gridDim.x), least);
+  const int64_t x0 = part_weight * blockIdx.x, x1 = min(x0 + part_weight, total);
+  if (x0 < total) {
     int64_t off = base + inc - mine;  // the line's position of sequence lo
     if (mine > 0 && x1 > off && x0 < off + mine)
       for (int s = lo; s < hi; ++s) {
