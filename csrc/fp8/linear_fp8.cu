@@ -12,8 +12,13 @@
 //   rows of x (16 to 128) its N, so a product moves each weight once whatever
 //   the number of rows. The K blocks are split over the CTAs of a cluster,
 //   which add their sums through distributed shared memory: no workspace.
-// pair_kernel (many rows). CTA pairs (cta_group::2) compute 256 x 256 tiles. All
-//   tiles' K blocks form one line that is cut into equal parts for the pairs,
+// pair_kernel (many rows). CTA pairs (cta_group::2) compute 256 x 256 tiles. A K
+//   block's sums go to one of two buffers in tensor memory, each in two halves
+//   of 128 columns with a warpgroup and barriers of its own: handing a buffer
+//   over and back takes about as long as its products (signals between the CTAs
+//   included), so four half buffers keep more of them in flight than two whole
+//   ones. Scales come by cp.async through shared memory: read straight from
+//   global memory they made every block wait for them. All tiles' K blocks form one line that is cut into equal parts for the pairs,
 //   so no pair idles in a last partial wave. A tile that a cut falls into is
 //   finished by the pair that arrives last, which adds the parts in the order
 //   of K.
@@ -147,8 +152,8 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
   sm100::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   auto wait = [&](uint64_t* b, uint32_t parity) {
-    if (*s_err) return;
-    if (!sm100::mbar_wait(b, parity)) *s_err = 1;
+    if (sm100::mbar_try_wait(b, parity)) return;
+    if (!*s_err && !sm100::mbar_wait(b, parity)) *s_err = 1;
   };
 
   float acc[MP];
@@ -308,8 +313,10 @@ constexpr int BM = 256, BN = 256;
 constexpr int kStages = 6;
 constexpr int kThreads = 384;  // three warpgroups of 168 registers a thread: 56 and twice 224 after the split
 constexpr uint32_t kA = 128 * 128, kB = 128 * 128, kStage = kA + kB;  // a CTA's halves
-constexpr size_t kSmem = 1024 + kStages * kStage + 256;
-constexpr uint32_t kCols = 512;
+constexpr int kScales = 8;           // ring of K blocks' scales: 128 of the CTA's rows, 2 of the tile's columns
+constexpr int kScaleFloats = 132;
+constexpr size_t kSmem = 1024 + kStages * kStage + kScales * kScaleFloats * 4 + 512;
+constexpr uint32_t kCols = 512;      // [2 buffers][2 halves of the tile's columns][128]
 constexpr int64_t kPartFloats = 128 * 256;  // a CTA's sums of a tile
 
 struct Line {
@@ -337,6 +344,14 @@ __device__ __forceinline__ void unpack64(uint64_t v, float& lo, float& hi) {
   lo = __uint_as_float(a);
   hi = __uint_as_float(b);
 }
+// Four bytes to shared memory, and the arrival on a barrier once all of the thread's copies so far are there.
+__device__ __forceinline__ void cp_async4(void* smem, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sm100::smem_u32(smem)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // Two fp32 sums in one instruction.
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
@@ -352,11 +367,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pair_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* sA = smem;
   uint8_t* sB = smem + kStages * kA;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kStages * kStage);
+  float* scales = reinterpret_cast<float*>(smem + kStages * kStage);  // [kScales][kScaleFloats]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + kScales * kScaleFloats);
   uint64_t* empty = full + kStages;
-  uint64_t* tfull = empty + kStages;  // [2]
-  uint64_t* tempty = tfull + 2;       // [2] (the leader's: 8 warps of each CTA)
-  uint64_t* drained = tempty + 2;
+  uint64_t* tfull = empty + kStages;  // [2 buffers][2 halves]
+  uint64_t* tempty = tfull + 4;       // the same (the leader's: four warps of each CTA)
+  uint64_t* sfull = tempty + 4;       // [kScales]
+  uint64_t* sempty = sfull + kScales;
+  uint64_t* drained = sempty + kScales;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* s_err = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* s_last = const_cast<int*>(s_err) + 1;
@@ -371,9 +389,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       sm100::mbar_init(&full[i], 1);
       sm100::mbar_init(&empty[i], 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       sm100::mbar_init(&tfull[i], 1);
-      sm100::mbar_init(&tempty[i], 16);
+      sm100::mbar_init(&tempty[i], 8);
+    }
+    for (int i = 0; i < kScales; ++i) {
+      sm100::mbar_init(&sfull[i], 64);
+      sm100::mbar_init(&sempty[i], 8);
     }
     sm100::mbar_init(drained, 1);
     *s_err = 0;
@@ -391,89 +413,122 @@ __global__ void __launch_bounds__(kThreads, 1)
   sm100::tc_fence_after();
   const uint32_t tmem = *tmem_slot;
   auto wait = [&](uint64_t* b, uint32_t parity) {
-    if (*s_err) return;
-    if (!sm100::mbar_wait(b, parity)) *s_err = 1;
+    if (sm100::mbar_try_wait(b, parity)) return;
+    if (!*s_err && !sm100::mbar_wait(b, parity)) *s_err = 1;
   };
   pdl_wait();
   pdl_trigger();
   const int64_t u0 = line.start(p), u1 = line.start(p + 1);
+  const int count = static_cast<int>(u1 - u0);
 
   if (warp >= 8) {
     sm100::reg_give<56>();
+    int tile = static_cast<int>(u0 / a.kblocks), kb = static_cast<int>(u0 - int64_t(tile) * a.kblocks);
     if (warp == 8 && sm100::elect_one()) {
       // -------------------------------------------------------- TMA producer
-      unsigned n = 0;
-      for (int64_t u = u0; u < u1; ++u, ++n) {
-        const int tile = static_cast<int>(u / a.kblocks), kb = static_cast<int>(u - int64_t(tile) * a.kblocks);
-        const int tm = tile % line.tiles_m, tn = tile / line.tiles_m, st = n % kStages;
-        wait(&empty[st], ((n / kStages) & 1u) ^ 1u);
+      int st = 0, n = 0;
+      uint32_t phase = 0;
+      const uint32_t fbar = sm100::mapa_shared(sm100::smem_u32(full), 0);
+      for (; n < count; ++n) {
+        const int ym = tile % line.tiles_m * BM + static_cast<int>(rank) * 128;
+        const int yn = tile / line.tiles_m * BN + static_cast<int>(rank) * 64;
+        wait(&empty[st], phase ^ 1u);
         if (*s_err) break;
-        const uint32_t fbar = sm100::mapa_shared(sm100::smem_u32(&full[st]), 0);
         if (leader) sm100::mbar_arrive_expect_tx(&full[st], 2 * kStage);  // both CTAs' bytes
-        sm100::tma_load_2d_pair(sA + st * kA, &tx, fbar, kb * kBlock, tm * BM + static_cast<int>(rank) * 128);
-        sm100::tma_load_2d_pair(sB + st * kB, &tw, fbar, kb * kBlock, tn * BN + static_cast<int>(rank) * 128);
+        sm100::tma_load_2d_pair(sA + st * kA, &tx, fbar + st * 8, kb * kBlock, ym);
+        // Half of each half of the tile's columns: a product of one half reads 64 rows of W from either CTA.
+        sm100::tma_load_2d_pair(sB + st * kB, &tw, fbar + st * 8, kb * kBlock, yn);
+        sm100::tma_load_2d_pair(sB + st * kB + kB / 2, &tw, fbar + st * 8, kb * kBlock, yn + 128);
+        if (++st == kStages) st = 0, phase ^= 1u;
+        if (++kb == a.kblocks) kb = 0, ++tile;
       }
       if (leader)
-        for (unsigned i = n > kStages ? n - kStages : 0; i < n; ++i)
-          sm100::mbar_wait(&full[i % kStages], (i / kStages) & 1u);
+        for (int i = max(0, n - kStages); i < n; ++i) sm100::mbar_wait(&full[i % kStages], (i / kStages) & 1);
     }
     if (warp == 9 && leader && sm100::elect_one()) {
       // -------------------------------------------------------- MMA issue (leader)
-      unsigned n = 0;
-      for (int64_t u = u0; u < u1 && !*s_err; ++u, ++n) {
-        const int st = n % kStages, bf = n & 1;
-        wait(&tempty[bf], ((n >> 1) & 1u) ^ 1u);
-        wait(&full[st], (n / kStages) & 1u);
-        if (*s_err) break;
-        sm100::tc_fence_after();
-        const uint64_t da = sm100::smem_desc_sw128(sA + st * kA);
-        const uint64_t db = sm100::smem_desc_sw128(sB + st * kB);
+      int st = 0;
+      uint32_t phase = 0;
+      uint32_t empty_at[2], tfull_at[2];
+      for (uint32_t r = 0; r < 2; ++r) {
+        empty_at[r] = sm100::mapa_shared(sm100::smem_u32(empty), r);
+        tfull_at[r] = sm100::mapa_shared(sm100::smem_u32(tfull), r);
+      }
+      const uint64_t da0 = sm100::smem_desc_sw128(sA), db0 = sm100::smem_desc_sw128(sB);
+      for (int i = 0; i < count && !*s_err; ++i) {
+        const int bf = i & 1;
+        const uint64_t da = da0 + st * (kA >> 4);
+        wait(&full[st], phase);
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-          mma_e4m3_pair(tmem + bf * BN, da + 2 * k, db + 2 * k, idesc_e4m3(BM, BN), k > 0 ? 1u : 0u);
-        for (uint32_t r = 0; r < 2; ++r) sm100::mma_commit_pair(sm100::mapa_shared(sm100::smem_u32(&empty[st]), r));
-        for (uint32_t r = 0; r < 2; ++r) sm100::mma_commit_pair(sm100::mapa_shared(sm100::smem_u32(&tfull[bf]), r));
+        for (int h = 0; h < 2; ++h) {
+          wait(&tempty[bf * 2 + h], ((i >> 1) & 1u) ^ 1u);
+          if (*s_err) break;
+          sm100::tc_fence_after();
+          const uint64_t db = db0 + st * (kB >> 4) + h * (kB >> 5);
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            mma_e4m3_pair(tmem + bf * 256 + h * 128, da + 2 * k, db + 2 * k, idesc_e4m3(BM, 128), k > 0 ? 1u : 0u);
+          sm100::mma_commit_pair(tfull_at[0] + (bf * 2 + h) * 8);
+          sm100::mma_commit_pair(tfull_at[1] + (bf * 2 + h) * 8);
+        }
+        sm100::mma_commit_pair(empty_at[0] + st * 8);
+        sm100::mma_commit_pair(empty_at[1] + st * 8);
+        if (++st == kStages) st = 0, phase ^= 1u;
       }
       sm100::mma_commit_pair(sm100::mapa_shared(sm100::smem_u32(drained), 0));
       if (!sm100::mbar_wait(drained, 0)) *s_err = 1;
     }
+    if (warp >= 10) {
+      // -------------------------------------------------------- scales: two rows a lane
+      const int id = (warp - 10) * 32 + lane, nblocks = (a.N + kBlock - 1) / kBlock;
+      for (int i = 0; i < count; ++i) {
+        const int sl = i % kScales;
+        wait(&sempty[sl], ((i / kScales) & 1u) ^ 1u);
+        const int m = tile % line.tiles_m * BM + static_cast<int>(rank) * 128 + id;
+        float* dst = scales + sl * kScaleFloats + id;
+        const float* src = a.sx + kb * a.lds;
+        cp_async4(dst, src + min(m, a.M - 1));
+        cp_async4(dst + 64, src + min(m + 64, a.M - 1));
+        if (id < 2) {
+          const int nb = min(tile / line.tiles_m * 2 + id, nblocks - 1);
+          cp_async4(dst + 128, a.sw + static_cast<int64_t>(nb) * a.kblocks + kb);
+        }
+        cp_async_arrive(&sfull[sl]);
+        if (++kb == a.kblocks) kb = 0, ++tile;
+      }
+      cp_async_wait_all();
+    }
   } else {
     // ---------------------------------------------------------- scale, add, store: 8 warps
     sm100::reg_take<224>();
-    const int g = warp >> 2, row = (warp & 3) * 32 + lane;  // 128 columns of the tile, row of the CTA
+    const int g = warp >> 2, row = (warp & 3) * 32 + lane;  // half of the tile's columns, row of the CTA
     const uint32_t td = tmem + (static_cast<uint32_t>((warp & 3) * 32) << 16) + g * 128;
-    const uint32_t free_bar[2] = {sm100::mapa_shared(sm100::smem_u32(&tempty[0]), 0),
-                                  sm100::mapa_shared(sm100::smem_u32(&tempty[1]), 0)};
+    const uint32_t free_bar[2] = {sm100::mapa_shared(sm100::smem_u32(&tempty[g]), 0),
+                                  sm100::mapa_shared(sm100::smem_u32(&tempty[2 + g]), 0)};
     unsigned n = 0;
     for (int64_t u = u0; u < u1;) {
       const int tile = static_cast<int>(u / a.kblocks), k0 = static_cast<int>(u - int64_t(tile) * a.kblocks);
       const int k1 = static_cast<int>(min(static_cast<int64_t>(a.kblocks), k0 + u1 - u));
       const int tm = tile % line.tiles_m, tn = tile / line.tiles_m;
       const int m = tm * BM + static_cast<int>(rank) * 128 + row, n0 = tn * BN + g * 128;
-      const float* sx = a.sx + min(m, a.M - 1);
-      const float* sw = a.sw + static_cast<int64_t>(min(n0, a.N - 1) / kBlock) * a.kblocks;
-      // Loaded two blocks ahead, multiplied where they are used.
-      auto scale = [&](int kb) {
-        return kb < k1 ? make_float2(__ldg(sx + kb * a.lds), __ldg(sw + kb)) : make_float2(0.f, 0.f);
-      };
-      float2 s0 = scale(k0), s1 = scale(k0 + 1);
       uint64_t acc[64];
 #pragma unroll
       for (int i = 0; i < 64; ++i) acc[i] = 0;
       for (int kb = k0; kb < k1; ++kb, ++n) {
-        const int bf = n & 1;
-        const float sf = s0.x * s0.y;
+        const int bf = n & 1, sl = n % kScales;
+        wait(&sfull[sl], (n / kScales) & 1u);
+        const float sf = scales[sl * kScaleFloats + row] * scales[sl * kScaleFloats + 128 + g];
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&sempty[sl]);
         const uint64_t s = pack64(__float_as_uint(sf), __float_as_uint(sf));
-        s0 = s1;
-        s1 = scale(kb + 2);
-        wait(&tfull[bf], (n >> 1) & 1u);
+        wait(&tfull[bf * 2 + g], (n >> 1) & 1u);
         sm100::tc_fence_after();
 #pragma unroll
         for (int c = 0; c < 128; c += 32) {
           uint32_t r[32];
           sm100::tmem_ld_32x32b_x32(td + bf * BN + c, r);
           sm100::tmem_ld_wait();
-          if (c == 96) {  // the accumulator is read: the next block but one may overwrite it
+          if (c == 96) {  // the half buffer is read: the next block but one may overwrite it
             sm100::tc_fence_before();
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive_remote(free_bar[bf]);
@@ -612,7 +667,7 @@ int pairs_of(const LinearArgs& l) {
 
 template <typename T>
 void launch_pair(const LinearArgs& l, const Args& a, cudaStream_t s) {
-  const CUtensorMap tx = codes_map(l.x, l.M, l.K, 128), tw = codes_map(l.w, l.N, l.K, 128);
+  const CUtensorMap tx = codes_map(l.x, l.M, l.K, 128), tw = codes_map(l.w, l.N, l.K, 64);
   pair::Line line{};
   line.tiles_m = static_cast<int>((l.M + pair::BM - 1) / pair::BM);
   line.tiles = line.tiles_m * static_cast<int>((l.N + pair::BN - 1) / pair::BN);
