@@ -28,25 +28,26 @@ void quantize_weight(const void* w, int64_t ldw, uint8_t* q, float* scale, int64
                      cudaStream_t s);
 
 struct LinearArgs {
-  const uint8_t* x;   // [M, K]
-  const float* sx;    // [ceil(K / 128), M], row stride lds
+  // x as codes [M, K] with scales [ceil(K / 128), M], row stride lds; or raw: [M, K] of the output's type, row
+  // stride ldx, quantized here.
+  const uint8_t* x;
+  const float* sx;
+  int64_t lds;
+  const void* raw;
+  int64_t ldx;
   const uint8_t* w;   // [N, K]
   const float* sw;    // [ceil(N / 128), ceil(K / 128)]
   void* out;          // [M, N], row stride ldo
-  int64_t lds, ldo;
+  int64_t ldo;
   int64_t M, N, K;
   int* err;
-  float* workspace;    // linear_scratch().floats
-  unsigned* counters;  // linear_scratch().counters words, zero
-  bool early;          // the kernel before is quantize() of x: the weights need no wait
+  float* workspace;    // set by linear()
+  unsigned* counters;
 };
-// What a product needs besides its tensors; not kept from call to call.
-struct Scratch {
-  int64_t floats, counters;
-};
-Scratch linear_scratch(const LinearArgs& a);
+// Bytes of scratch of a call; not kept from call to call.
+int64_t linear_scratch(const LinearArgs& a);
 // out = sum over blocks b of sx[b, m] sw[n / 128, b] (x[m, b] . w[n, b])
-void linear(const LinearArgs& a, Type out, cudaStream_t s);
+void linear(const LinearArgs& a, Type out, void* scratch, cudaStream_t s);
 
 }  // namespace fp8
 }  // namespace b200ar

@@ -80,6 +80,15 @@ __device__ __forceinline__ void mma_e4m3_pair(uint32_t d, uint64_t a, uint64_t b
       : "memory");
 }
 
+// Four bytes to shared memory, and the arrival on a barrier once all of the thread's copies so far are there.
+__device__ __forceinline__ void cp_async4(void* smem, const void* global) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sm100::smem_u32(smem)), "l"(global) : "memory");
+}
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
 struct Args {
   const float* sx;  // [kblocks, M], row stride lds
   const float* sw;  // [ceil(N / 128), kblocks]
@@ -92,14 +101,15 @@ struct Args {
 // ------------------------------------------------------------------ few rows
 template <int MP>  // rows of x in a tile
 struct RowsCfg {
-  static constexpr int kThreads = 192;
+  static constexpr int kThreads = 224;
   static constexpr uint32_t kW = 128 * 128, kX = MP * 128, kStage = kW + kX;
   // Two CTAs fit an SM, or one at 128 rows, whose sums need the space once the ring is done.
   static constexpr int kStages = (100 * 1024) / kStage;
   static constexpr int kBufs = MP == 128 ? 2 : 4;  // accumulators in tensor memory
   static constexpr uint32_t kCols = kBufs * MP;    // a power of two from 64 to 256
-  static constexpr int kScales = 4;                // ring of K blocks' scales
-  static constexpr size_t kSmem = 1024 + kStages * kStage + kScales * MP * 4 + 256;
+  static constexpr int kScales = 8;                // ring of K blocks' scales: of the rows of x, of those of W
+  static constexpr int kScaleFloats = MP + 4;
+  static constexpr size_t kSmem = 1024 + kStages * kStage + kScales * kScaleFloats * 4 + 512;
   static_assert(MP * 128 * 4 <= kStages * kStage, "the sums of a CTA reuse the ring");
 };
 
@@ -113,15 +123,17 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(rows_smem) + 1023) & ~uintptr_t(1023));
   uint8_t* sW = smem;
   uint8_t* sX = smem + C::kStages * C::kW;
-  float* scales = reinterpret_cast<float*>(smem + C::kStages * C::kStage);  // [kScales][MP]
-  uint64_t* full = reinterpret_cast<uint64_t*>(scales + C::kScales * MP);
+  float* scales = reinterpret_cast<float*>(smem + C::kStages * C::kStage);  // [kScales][kScaleFloats]
+  uint64_t* full = reinterpret_cast<uint64_t*>(scales + C::kScales * C::kScaleFloats);
   uint64_t* empty = full + C::kStages;
   uint64_t* tfull = empty + C::kStages;
   uint64_t* tempty = tfull + C::kBufs;
-  uint64_t* drained = tempty + C::kBufs;
+  uint64_t* sfull = tempty + C::kBufs;
+  uint64_t* sempty = sfull + C::kScales;
+  uint64_t* drained = sempty + C::kScales;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drained + 1);
   volatile int* s_err = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  static_assert((2 * C::kStages + 2 * C::kBufs + 2) * 8 <= 256, "barriers");
+  static_assert((2 * C::kStages + 2 * C::kBufs + 2 * C::kScales + 2) * 8 <= 512, "barriers");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int block = blockIdx.x / splits, rank = blockIdx.x % splits;
@@ -136,6 +148,10 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
     for (int i = 0; i < C::kBufs; ++i) {
       sm100::mbar_init(&tfull[i], 1);
       sm100::mbar_init(&tempty[i], 4);
+    }
+    for (int i = 0; i < C::kScales; ++i) {
+      sm100::mbar_init(&sfull[i], 32);
+      sm100::mbar_init(&sempty[i], 4);
     }
     sm100::mbar_init(drained, 1);
     *s_err = 0;
@@ -207,37 +223,33 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
     }
     __syncwarp();
     pdl_wait();
-  } else {
-    // Thread = row of W. The scales of a K block, sx sw, are the same for all rows: 128 threads load them two
-    // blocks ahead and share them.
+  } else if (warp == 6) {
+    // Scales, up to eight K blocks ahead: read straight from global memory by the warps below they would be waited
+    // for with every block.
     pdl_wait();
-    const int q4 = warp & 3, id = q4 * 32 + lane;
-    const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
-    const bool mine = id < MP && m0 + id < a.M;
-    const float* sx = a.sx + m0 + id;
-    const float* sw = a.sw + static_cast<int64_t>(block) * a.kblocks;
-    // The factors of the i-th K block; multiplied where they are used, so that no load is waited for before.
-    auto scale = [&](int i) {
-      const int kb = kb0 + i;
-      return mine && i < nkb ? make_float2(__ldg(sx + kb * a.lds), __ldg(sw + kb)) : make_float2(0.f, 0.f);
-    };
-    const float2 s0 = scale(0), s1 = scale(1);
-    float2 s2 = scale(2), s3 = scale(3);
-    if (id < MP) {
-      scales[id] = s0.x * s0.y;
-      scales[MP + id] = s1.x * s1.y;
-    }
+    const float* sw = a.sw + static_cast<int64_t>(block) * a.kblocks + kb0;
     for (int i = 0; i < nkb; ++i) {
-      const int bf = i % C::kBufs;
-      if (id < MP) scales[((i + 2) % C::kScales) * MP + id] = s2.x * s2.y;
-      s2 = s3;
-      s3 = scale(i + 4);
-      // Orders the writes of block i + 2 against its reads, and all reads of block i - 2 (whose place the
-      // next step reuses) before them.
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+      const int sl = i % C::kScales;
+      wait(&sempty[sl], ((i / C::kScales) & 1) ^ 1);
+      float* dst = scales + sl * C::kScaleFloats;
+      const float* sx = a.sx + (kb0 + i) * a.lds + m0;
+#pragma unroll
+      for (int m = lane; m < MP; m += 32) cp_async4(dst + m, sx + min(m, a.M - 1 - m0));
+      if (lane == 0) cp_async4(dst + MP, sw + i);
+      cp_async_arrive(&sfull[sl]);
+    }
+    cp_async_wait_all();
+  } else {
+    // Thread = row of W.
+    pdl_wait();
+    const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    for (int i = 0; i < nkb; ++i) {
+      const int bf = i % C::kBufs, sl = i % C::kScales;
+      wait(&sfull[sl], (i / C::kScales) & 1);
+      const float* sc = scales + sl * C::kScaleFloats;
+      const float sw = sc[MP];
       wait(&tfull[bf], (i / C::kBufs) & 1);
       sm100::tc_fence_after();
-      const float4* sc = reinterpret_cast<const float4*>(scales + (i % C::kScales) * MP);
       constexpr int kStep = MP < 32 ? MP : 32;
 #pragma unroll
       for (int c = 0; c < MP; c += kStep) {
@@ -249,16 +261,19 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
         sm100::tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < kStep; e += 4) {
-          const float4 s = sc[(c + e) / 4];
-          acc[c + e] = fmaf(__uint_as_float(r[e]), s.x, acc[c + e]);
-          acc[c + e + 1] = fmaf(__uint_as_float(r[e + 1]), s.y, acc[c + e + 1]);
-          acc[c + e + 2] = fmaf(__uint_as_float(r[e + 2]), s.z, acc[c + e + 2]);
-          acc[c + e + 3] = fmaf(__uint_as_float(r[e + 3]), s.w, acc[c + e + 3]);
+          const float4 s = *reinterpret_cast<const float4*>(sc + c + e);
+          acc[c + e] = fmaf(__uint_as_float(r[e]) * s.x, sw, acc[c + e]);
+          acc[c + e + 1] = fmaf(__uint_as_float(r[e + 1]) * s.y, sw, acc[c + e + 1]);
+          acc[c + e + 2] = fmaf(__uint_as_float(r[e + 2]) * s.z, sw, acc[c + e + 2]);
+          acc[c + e + 3] = fmaf(__uint_as_float(r[e + 3]) * s.w, sw, acc[c + e + 3]);
         }
       }
       sm100::tc_fence_before();
       __syncwarp();
-      if (lane == 0) sm100::mbar_arrive(&tempty[bf]);
+      if (lane == 0) {
+        sm100::mbar_arrive(&tempty[bf]);
+        sm100::mbar_arrive(&sempty[sl]);
+      }
     }
   }
   pdl_trigger();
@@ -270,7 +285,7 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
   }
   // Sums of the cluster: [row of x][row of W] in each CTA, added in the order of K.
   float* sums = reinterpret_cast<float*>(smem);
-  if (warp >= 2) {
+  if (warp >= 2 && warp < 6) {
     const int id = (warp & 3) * 32 + lane;
 #pragma unroll
     for (int i = 0; i < MP; ++i)
@@ -344,14 +359,6 @@ __device__ __forceinline__ void unpack64(uint64_t v, float& lo, float& hi) {
   lo = __uint_as_float(a);
   hi = __uint_as_float(b);
 }
-// Four bytes to shared memory, and the arrival on a barrier once all of the thread's copies so far are there.
-__device__ __forceinline__ void cp_async4(void* smem, const void* global) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(sm100::smem_u32(smem)), "l"(global) : "memory");
-}
-__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
-  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(sm100::smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 // Two fp32 sums in one instruction.
 __device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
   uint64_t d;
@@ -656,7 +663,7 @@ void launch_rows(const LinearArgs& l, const Args& a, int splits, cudaStream_t s)
     B200AR_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(C::kSmem)));
   });
   const dim3 grid(static_cast<unsigned>((l.N + 127) / 128 * splits), static_cast<unsigned>((l.M + MP - 1) / MP));
-  launch_pdl(kern, grid, dim3(C::kThreads), C::kSmem, s, splits, tw, tx, a, splits, l.early ? 1 : 0);
+  launch_pdl(kern, grid, dim3(C::kThreads), C::kSmem, s, splits, tw, tx, a, splits, l.raw ? 1 : 0);
 }
 
 int pairs_of(const LinearArgs& l) {
@@ -686,22 +693,24 @@ void launch_pair(const LinearArgs& l, const Args& a, cudaStream_t s) {
 }
 
 // Rows up to which rows_kernel is taken.
-bool few_rows(const LinearArgs& l) { return l.M <= 512; }
+constexpr int64_t kFewRows = 512;
+
+template <typename T, int MP>
+void dispatch_rows(const LinearArgs& l, const Args& a, cudaStream_t s) {
+  // Cluster size: the most CTAs that two to an SM hold, with two K blocks each at least.
+  const int64_t ctas = (l.N + 127) / 128 * ((l.M + MP - 1) / MP);
+  int splits = 1;
+  while (splits < 8 && ctas * splits * 2 <= 2 * sm_count() && a.kblocks >= splits * 4) splits *= 2;
+  launch_rows<T, MP>(l, a, splits, s);
+}
 
 template <typename T>
 void dispatch(const LinearArgs& l, const Args& a, cudaStream_t s) {
-  if (!few_rows(l)) return launch_pair<T>(l, a, s);
-  const int mp = l.M <= 16 ? 16 : l.M <= 32 ? 32 : l.M <= 64 ? 64 : 128;
-  // Cluster size: the most CTAs that two to an SM hold, with two K blocks each at least.
-  const int64_t ctas = (l.N + 127) / 128 * ((l.M + mp - 1) / mp);
-  int splits = 1;
-  while (splits < 8 && ctas * splits * 2 <= 2 * sm_count() && a.kblocks >= splits * 4) splits *= 2;
-  switch (mp) {
-    case 16: return launch_rows<T, 16>(l, a, splits, s);
-    case 32: return launch_rows<T, 32>(l, a, splits, s);
-    case 64: return launch_rows<T, 64>(l, a, splits, s);
-    default: return launch_rows<T, 128>(l, a, splits, s);
-  }
+  if (l.M > kFewRows) return launch_pair<T>(l, a, s);
+  if (l.M <= 16) return dispatch_rows<T, 16>(l, a, s);
+  if (l.M <= 32) return dispatch_rows<T, 32>(l, a, s);
+  if (l.M <= 64) return dispatch_rows<T, 64>(l, a, s);
+  dispatch_rows<T, 128>(l, a, s);
 }
 
 void check(const LinearArgs& l) {
@@ -712,17 +721,55 @@ void check(const LinearArgs& l) {
 
 }  // namespace
 
-Scratch linear_scratch(const LinearArgs& l) {
-  check(l);
-  if (l.M == 0 || few_rows(l)) return {0, 0};
-  const int64_t tiles = (l.M + pair::BM - 1) / pair::BM * ((l.N + pair::BN - 1) / pair::BN);
-  return {pairs_of(l) * 4 * pair::kPartFloats, 2 * tiles};
+namespace {
+
+// Places of a call's scratch, in bytes: parts of cut tiles, their counters, codes and scales of x.
+struct Layout {
+  int64_t counters, zeros, codes, scales, bytes;
+};
+Layout layout(const LinearArgs& l) {
+  const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+  Layout o{};
+  if (l.M > kFewRows) {
+    const int64_t tiles = (l.M + pair::BM - 1) / pair::BM * ((l.N + pair::BN - 1) / pair::BN);
+    o.counters = up(pairs_of(l) * 4 * pair::kPartFloats * 4);
+    o.zeros = 2 * tiles;
+  }
+  o.codes = o.counters + up(o.zeros * 4);
+  o.scales = o.codes;
+  o.bytes = o.codes;
+  if (l.raw) {
+    o.scales += up(l.M * l.K);
+    o.bytes = o.scales + (l.K + kBlock - 1) / kBlock * l.M * 4;
+  }
+  return o;
 }
 
-void linear(const LinearArgs& l, Type out, cudaStream_t s) {
+}  // namespace
+
+int64_t linear_scratch(const LinearArgs& l) {
+  check(l);
+  return l.M == 0 ? 0 : layout(l).bytes;
+}
+
+void linear(const LinearArgs& args, Type out, void* scratch, cudaStream_t s) {
   const TraceRange trace("b200ar::linear_fp8");
+  LinearArgs l = args;
   check(l);
   if (l.M == 0) return;
+  const Layout at = layout(l);
+  uint8_t* mem = static_cast<uint8_t*>(scratch);
+  l.workspace = reinterpret_cast<float*>(mem);
+  l.counters = reinterpret_cast<unsigned*>(mem + at.counters);
+  if (l.raw) {
+    float* scales = reinterpret_cast<float*>(mem + at.scales);
+    quantize(l.raw, l.ldx, mem + at.codes, scales, l.M, l.M, l.K, out, l.counters, at.zeros, s);
+    l.x = mem + at.codes;
+    l.sx = scales;
+    l.lds = l.M;
+  } else if (at.zeros) {
+    B200AR_CUDA(cudaMemsetAsync(l.counters, 0, at.zeros * 4, s));
+  }
   Args a{};
   a.sx = l.sx;
   a.sw = l.sw;

@@ -3,20 +3,19 @@
 //   scale = amax / 448 (1 for a block of zeros),  q = e4m3(x / scale)
 //
 // Both quotients are the correctly rounded fp32 ones, so the codes are those
-// of the formula and not an approximation of it. The maximum is taken over the
+// of the formula and not an approximation of it. (A product with 1 / scale is
+// off by less than 2 units in the last place, so it has the same code unless
+// it is that near to the middle between two e4m3 numbers; only then, and for
+// subnormal codes and scales, the division is made.) The maximum is taken over the
 // bit patterns of |x|, in which NaN is above infinity: a block that holds a
 // NaN gets the scale NaN, one that holds an infinity the scale infinity, and
 // either reaches the outputs of its row.
 //
-// Memory bounds both kernels: 3 bytes a value move, and a division costs about
-// ten instructions of the forty that the SM issues in the time of those bytes.
-#include <cuda_bf16.h>
-#include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
+// Memory bounds both kernels: 3 bytes a value move.
 #include "../common/check.h"
 #include "../common/pdl.h"
 #include "../common/trace.h"
+#include "encode.cuh"
 #include "fp8.h"
 
 namespace b200ar {
@@ -24,81 +23,39 @@ namespace fp8 {
 
 namespace {
 
-constexpr float kMax = 448.f;
 constexpr int kThreads = 256;
 
-// Eight consecutive values as fp32.
-template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* v);
-template <>
-__device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float* v) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&w);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __bfloat1622float2(h[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-template <>
-__device__ __forceinline__ void load8<__half>(const __half* p, float* v) {
-  const uint4 w = *reinterpret_cast<const uint4*>(p);
-  const __half2* h = reinterpret_cast<const __half2*>(&w);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(h[i]);
-    v[2 * i] = f.x;
-    v[2 * i + 1] = f.y;
-  }
-}
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float* v) {
-  *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
-  *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
-}
-
-__device__ __forceinline__ unsigned abs_max8(const float* v) {
-  unsigned m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  return m;
-}
-__device__ __forceinline__ float scale_of(unsigned amax_bits) {
-  return amax_bits == 0u ? 1.f : __fdiv_rn(__uint_as_float(amax_bits), kMax);
-}
-__device__ __forceinline__ uint2 encode8(const float* v, float scale) {
-  uint32_t w[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(v[2 * i], scale), __fdiv_rn(v[2 * i + 1], scale)),
-                                    __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
-}
-
-// Sixteen lanes share a block of 128 values; grid (row, 16 blocks of the row).
-template <typename T>
+// Sixteen lanes share a block of 128 values; grid (groups of kRows rows, 16 blocks of them).
+template <typename T, int kRows>
 __global__ void __launch_bounds__(kThreads)
     quantize_kernel(const T* __restrict__ x, int64_t ldx, uint8_t* __restrict__ q, float* __restrict__ scale,
                     int64_t lds, int64_t M, int K, unsigned* __restrict__ zero, int64_t zeros) {
-  const int64_t m = blockIdx.x;
+  const int64_t m0 = static_cast<int64_t>(blockIdx.x) * kRows;
   const int lane = threadIdx.x & 15;
   const int b = blockIdx.y * (kThreads / 16) + (threadIdx.x >> 4);
   const int k = b * kBlock + lane * 8;
-  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float v[kRows][8];
   pdl_wait();
   pdl_trigger();
-  for (int64_t i = (m * gridDim.y + blockIdx.y) * kThreads + threadIdx.x; i < zeros;
+  for (int64_t i = (static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * kThreads + threadIdx.x; i < zeros;
        i += static_cast<int64_t>(gridDim.x) * gridDim.y * kThreads)
     zero[i] = 0u;
-  if (k < K) load8<T>(x + m * ldx + k, v);
-  unsigned amax = abs_max8(v);
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  const float s = scale_of(amax);
-  if (k >= K) return;
-  *reinterpret_cast<uint2*>(q + m * K + k) = encode8(v, s);
-  if (lane == 0) scale[b * lds + m] = s;
+  for (int r = 0; r < kRows; ++r) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[r][e] = 0.f;
+    if (k < K && m0 + r < M) load8<T>(x + (m0 + r) * ldx + k, v[r]);
+  }
+#pragma unroll
+  for (int r = 0; r < kRows; ++r) {
+    unsigned amax = abs_max8(v[r]);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    const float s = scale_of(amax);
+    if (k >= K || m0 + r >= M) continue;
+    *reinterpret_cast<uint2*>(q + (m0 + r) * K + k) = encode8(v[r], s, inverse_of(s));
+    if (lane == 0) scale[b * lds + m0 + r] = s;
+  }
 }
 
 // One CTA for each 128 x 128 block: 16 lanes on a row, 8 rows a thread.
@@ -128,11 +85,11 @@ __global__ void __launch_bounds__(kThreads)
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kThreads / 32; ++i) amax = max(amax, part[i]);
-  const float s = scale_of(amax);
+  const float s = scale_of(amax), inverse = inverse_of(s);
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t n = n0 + r0 + 16 * i;
-    if (n < N && k < K) *reinterpret_cast<uint2*>(q + n * K + k) = encode8(v[i], s);
+    if (n < N && k < K) *reinterpret_cast<uint2*>(q + n * K + k) = encode8(v[i], s, inverse);
   }
   if (threadIdx.x == 0) scale[blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x] = s;
 }
@@ -140,10 +97,15 @@ __global__ void __launch_bounds__(kThreads)
 template <typename T>
 void launch_rows(const void* x, int64_t ldx, uint8_t* q, float* scale, int64_t lds, int64_t M, int64_t K,
                  unsigned* zero, int64_t zeros, cudaStream_t s) {
-  const int64_t blocks = (K + kBlock - 1) / kBlock;
-  const dim3 grid(static_cast<unsigned>(M), static_cast<unsigned>((blocks + kThreads / 16 - 1) / (kThreads / 16)));
-  launch_pdl(quantize_kernel<T>, grid, dim3(kThreads), 0, s, 1, static_cast<const T*>(x), ldx, q, scale, lds, M,
-             static_cast<int>(K), zero, zeros);
+  const unsigned blocks = static_cast<unsigned>(((K + kBlock - 1) / kBlock + kThreads / 16 - 1) / (kThreads / 16));
+  const T* xt = static_cast<const T*>(x);
+  // Many rows: four loads of a thread under way at once.
+  if (M >= 512)
+    launch_pdl(quantize_kernel<T, 4>, dim3(static_cast<unsigned>((M + 3) / 4), blocks), dim3(kThreads), 0, s, 1, xt,
+               ldx, q, scale, lds, M, static_cast<int>(K), zero, zeros);
+  else
+    launch_pdl(quantize_kernel<T, 1>, dim3(static_cast<unsigned>(M), blocks), dim3(kThreads), 0, s, 1, xt, ldx, q,
+               scale, lds, M, static_cast<int>(K), zero, zeros);
 }
 template <typename T>
 void launch_weight(const void* w, int64_t ldw, uint8_t* q, float* scale, int64_t N, int64_t K, cudaStream_t s) {

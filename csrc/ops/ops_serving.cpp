@@ -353,28 +353,8 @@ void register_serving_ops(py::module& m) {
         a.N = N;
         a.K = K;
         a.err = err_of(err, x);
-        // Scratch from the caching allocator on this stream: concurrent calls, eager or captured, never share it.
-        // Codes and scales of x, then the product's own.
-        const b200ar::fp8::Scratch need = b200ar::fp8::linear_scratch(a);
-        const bool quantize = !x_scale.has_value();
-        const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
-        const int64_t codes_at = up(need.floats * 4) + up(need.counters * 4);
-        const int64_t scales_at = codes_at + (quantize ? up(M * K) : 0);
-        const at::Tensor scratch =
-            at::empty({scales_at + (quantize ? blocks * M * 4 : 0)}, x.options().dtype(at::kByte));
-        uint8_t* mem = static_cast<uint8_t*>(scratch.data_ptr());
-        a.workspace = reinterpret_cast<float*>(mem);
-        a.counters = reinterpret_cast<unsigned*>(mem + up(need.floats * 4));
         at::Tensor x2, sx;
-        if (quantize) {
-          x2 = rows_2d(x);
-          a.x = mem + codes_at;
-          a.sx = reinterpret_cast<float*>(mem + scales_at);
-          a.lds = M;
-          a.early = true;
-          b200ar::fp8::quantize(x2.data_ptr(), x2.stride(0), mem + codes_at, reinterpret_cast<float*>(mem + scales_at),
-                                M, M, K, fp8_type(dtype, false, "x"), a.counters, need.counters, s);
-        } else {
+        if (x_scale.has_value()) {
           TYPE_CHECK(x.scalar_type() == at::kFloat8_e4m3fn, "with x_scale, x must be float8_e4m3fn");
           bool same = x_scale->dim() == x.dim() && x_scale->scalar_type() == at::kFloat && x_scale->size(-1) == blocks;
           for (int64_t i = 0; same && i + 1 < x.dim(); ++i) same = x_scale->size(i) == x.size(i);
@@ -387,9 +367,16 @@ void register_serving_ops(py::module& m) {
           a.x = static_cast<const uint8_t*>(x2.data_ptr());
           a.sx = sx.data_ptr<float>();
           a.lds = sx.stride(0);
-          if (M > 0 && need.counters) C10_CUDA_CHECK(cudaMemsetAsync(a.counters, 0, need.counters * 4, s));
+        } else {
+          x2 = rows_2d(x);
+          a.raw = x2.data_ptr();
+          a.ldx = x2.stride(0);
         }
-        b200ar::fp8::linear(a, type, s);
+        // From the caching allocator on this stream: concurrent calls, eager or captured, never share it.
+        const int64_t bytes = b200ar::fp8::linear_scratch(a);
+        at::Tensor scratch;
+        if (bytes > 0) scratch = at::empty({bytes}, x.options().dtype(at::kByte));
+        b200ar::fp8::linear(a, type, bytes > 0 ? scratch.data_ptr() : nullptr, s);
         return out;
       },
       "product of e4m3 operands with block scales; x is quantized unless it comes with its scales", py::arg("x"),
