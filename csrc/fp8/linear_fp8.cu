@@ -348,6 +348,7 @@ struct Line {
   }
 };
 
+__device__ __forceinline__ void sum_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 __device__ __forceinline__ uint64_t pack64(uint32_t lo, uint32_t hi) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
@@ -546,16 +547,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       u += k1 - k0;
 
-      bool store = true;
-      int first = p, last = p;
       if (k1 - k0 < a.kblocks) {
-        // A cut tile: whoever arrives last has all parts. Each CTA of the pair has its own rows.
-        first = line.owner(int64_t(tile) * a.kblocks);
-        last = line.owner(int64_t(tile + 1) * a.kblocks - 1);
+        // A cut tile: whoever arrives last has all parts and adds them in the order of K. (Of two parts it adds the
+        // other to its own: the sum of two numbers has no order.) Each CTA of the pair has its own rows.
+        const int first = line.owner(int64_t(tile) * a.kblocks);
+        const int last = line.owner(int64_t(tile + 1) * a.kblocks - 1);
+        const unsigned others = static_cast<unsigned>(last - first);
         unsigned* done = line.done + tile * 2 + rank;
-        if (threadIdx.x == 0) *s_last = atomicAdd(done, 0u) == static_cast<unsigned>(last - first);
-        asm volatile("bar.sync 1, 256;" ::: "memory");
-        if (!*reinterpret_cast<volatile int*>(s_last)) {
+        volatile int* is_last = s_last;
+        if (threadIdx.x == 0) *is_last = others == 1 && atomicAdd(done, 0u) == others;
+        sum_sync();
+        if (!*is_last) {
           float4* dst = reinterpret_cast<float4*>(line.part(p, k0 > 0 ? 0 : 1, rank)) + g * 32 * 128 + row;
 #pragma unroll
           for (int i = 0; i < 32; ++i) {
@@ -565,38 +567,43 @@ __global__ void __launch_bounds__(kThreads, 1)
             __stcg(dst + i * 128, v);
           }
           __threadfence();
-          asm volatile("bar.sync 1, 256;" ::: "memory");
-          if (threadIdx.x == 0) *s_last = atomicAdd(done, 1u) == static_cast<unsigned>(last - first);
-          asm volatile("bar.sync 1, 256;" ::: "memory");
+          sum_sync();
+          if (threadIdx.x == 0) *is_last = atomicAdd(done, 1u) == others;
+          sum_sync();
         }
-        store = *reinterpret_cast<volatile int*>(s_last) != 0;
+        const bool finish = *is_last != 0;
         __threadfence();
-        asm volatile("bar.sync 1, 256;" ::: "memory");  // s_last may be written again
+        sum_sync();  // s_last may be written again
+        if (!finish) continue;
+        if (others > 1) {
+#pragma unroll
+          for (int i = 0; i < 64; ++i) acc[i] = 0;
+        }
+        for (int o = first; o <= last; ++o) {
+          if (others == 1 && o == p) continue;
+          const float4* src = reinterpret_cast<const float4*>(line.part(o, o > first ? 0 : 1, rank)) + g * 32 * 128 + row;
+#pragma unroll
+          for (int i = 0; i < 32; i += 8) {  // eight loads under way
+            float4 v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] = __ldcg(src + (i + e) * 128);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float x, y;
+              unpack64(acc[2 * (i + e)], x, y);
+              acc[2 * (i + e)] = pack64(__float_as_uint(x + v[e].x), __float_as_uint(y + v[e].y));
+              unpack64(acc[2 * (i + e) + 1], x, y);
+              acc[2 * (i + e) + 1] = pack64(__float_as_uint(x + v[e].z), __float_as_uint(y + v[e].w));
+            }
+          }
+        }
       }
-      if (!store) continue;
       T* out = static_cast<T*>(a.out) + static_cast<int64_t>(m) * a.ldo + n0;
 #pragma unroll
       for (int c = 0; c < 128; c += 8) {
         float y[8];
 #pragma unroll
         for (int e = 0; e < 4; ++e) unpack64(acc[c / 2 + e], y[2 * e], y[2 * e + 1]);
-        if (first < last) {
-          float own[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) own[e] = y[e], y[e] = 0.f;
-          for (int q = first; q <= last; ++q) {
-            if (q == p) {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) y[e] += own[e];
-            } else {
-              const float4* src =
-                  reinterpret_cast<const float4*>(line.part(q, q > first ? 0 : 1, rank)) + g * 32 * 128 + row;
-              const float4 v0 = __ldcg(src + (c / 4) * 128), v1 = __ldcg(src + (c / 4 + 1) * 128);
-              y[0] += v0.x, y[1] += v0.y, y[2] += v0.z, y[3] += v0.w;
-              y[4] += v1.x, y[5] += v1.y, y[6] += v1.z, y[7] += v1.w;
-            }
-          }
-        }
         if (m < a.M && n0 + c < a.N)  // N is a multiple of 8
           *reinterpret_cast<uint4*>(out + c) =
               make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
@@ -666,10 +673,22 @@ void launch_rows(const LinearArgs& l, const Args& a, int splits, cudaStream_t s)
   launch_pdl(kern, grid, dim3(C::kThreads), C::kSmem, s, splits, tw, tx, a, splits, l.raw ? 1 : 0);
 }
 
+// K blocks of a pair's part at least: shorter parts take longer to add than to compute.
+constexpr int64_t kPartUnits = 12;
+
+int64_t pair_tiles(const LinearArgs& l) {
+  return (l.M + pair::BM - 1) / pair::BM * ((l.N + pair::BN - 1) / pair::BN);
+}
+int64_t pair_units(const LinearArgs& l) { return pair_tiles(l) * ((l.K + kBlock - 1) / kBlock); }
 int pairs_of(const LinearArgs& l) {
-  const int64_t tiles = (l.M + pair::BM - 1) / pair::BM * ((l.N + pair::BN - 1) / pair::BN);
-  const int64_t units = tiles * ((l.K + kBlock - 1) / kBlock);
-  return static_cast<int>(std::min<int64_t>(sm_count() / 2, units));
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count() / 2, pair_units(l) / kPartUnits)));
+}
+
+// Whether pair_kernel takes a call: above one tile of rows_kernel, if there is a part for every pair. Measured
+// (rows_kernel, pair_kernel): 128 x 7168 x 8192 43, 45 us; 256 x 7168 x 8192 67, 45 us (1792 K blocks of tiles);
+// 512 x 1280 x 8192 41, 39 us (640); 300 x 4096 x 2048 29, 35 us (512); 333 x 1288 x 1040 14, 27 us (108).
+bool many_rows(const LinearArgs& l) {
+  return l.M > 128 && (pair_units(l) >= sm_count() / 2 * kPartUnits || l.M > 65535 * 128);
 }
 
 template <typename T>
@@ -677,8 +696,8 @@ void launch_pair(const LinearArgs& l, const Args& a, cudaStream_t s) {
   const CUtensorMap tx = codes_map(l.x, l.M, l.K, 128), tw = codes_map(l.w, l.N, l.K, 64);
   pair::Line line{};
   line.tiles_m = static_cast<int>((l.M + pair::BM - 1) / pair::BM);
-  line.tiles = line.tiles_m * static_cast<int>((l.N + pair::BN - 1) / pair::BN);
-  line.units = static_cast<int64_t>(line.tiles) * a.kblocks;
+  line.tiles = static_cast<int>(pair_tiles(l));
+  line.units = pair_units(l);
   line.pairs = pairs_of(l);
   line.parts = l.workspace;
   line.done = l.counters;
@@ -692,9 +711,6 @@ void launch_pair(const LinearArgs& l, const Args& a, cudaStream_t s) {
              line);
 }
 
-// Rows up to which rows_kernel is taken.
-constexpr int64_t kFewRows = 512;
-
 template <typename T, int MP>
 void dispatch_rows(const LinearArgs& l, const Args& a, cudaStream_t s) {
   // Cluster size: the most CTAs that two to an SM hold, with two K blocks each at least.
@@ -706,7 +722,7 @@ void dispatch_rows(const LinearArgs& l, const Args& a, cudaStream_t s) {
 
 template <typename T>
 void dispatch(const LinearArgs& l, const Args& a, cudaStream_t s) {
-  if (l.M > kFewRows) return launch_pair<T>(l, a, s);
+  if (many_rows(l)) return launch_pair<T>(l, a, s);
   if (l.M <= 16) return dispatch_rows<T, 16>(l, a, s);
   if (l.M <= 32) return dispatch_rows<T, 32>(l, a, s);
   if (l.M <= 64) return dispatch_rows<T, 64>(l, a, s);
@@ -730,10 +746,9 @@ struct Layout {
 Layout layout(const LinearArgs& l) {
   const auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
   Layout o{};
-  if (l.M > kFewRows) {
-    const int64_t tiles = (l.M + pair::BM - 1) / pair::BM * ((l.N + pair::BN - 1) / pair::BN);
+  if (many_rows(l)) {
     o.counters = up(pairs_of(l) * 4 * pair::kPartFloats * 4);
-    o.zeros = 2 * tiles;
+    o.zeros = 2 * pair_tiles(l);
   }
   o.codes = o.counters + up(o.zeros * 4);
   o.scales = o.codes;

@@ -430,7 +430,8 @@ def test_rope_paged_far_positions_and_large_pools():
 
 # ------------------------------------------------------------------ 8-bit linear
 SHAPES = [(1, 8, 16), (1, 7168, 1024), (3, 136, 144), (16, 256, 128), (17, 264, 400), (48, 8192, 512), (64, 1280, 2048),
-          (65, 512, 272), (128, 128, 128), (129, 392, 656), (333, 1288, 1040), (513, 1024, 384), (1000, 72, 48)]
+          (65, 512, 272), (128, 128, 128), (129, 392, 656), (333, 1288, 1040), (513, 1024, 384), (1000, 72, 48),
+          (140, 7168, 4096), (257, 3592, 7184), (900, 2056, 2832), (1025, 1280, 2048)]
 
 
 @pytest.mark.parametrize("m,n,k", SHAPES)
@@ -457,7 +458,7 @@ def test_linear_fp8(m, n, k, dtype):
 def test_linear_fp8_long_sums():
     from b200ar.ops.fp8 import linear_fp8, quantize_fp8, quantize_fp8_weight
 
-    for m, n, k in ((2, 128, 28672), (300, 256, 28672)):
+    for m, n, k in ((2, 128, 28672), (300, 256, 28672), (300, 1024, 28672)):
         x, w = randn((m, k), BF, "cuda", 1).abs(), randn((n, k), BF, "cuda", 2).abs()
         w_q, w_s = quantize_fp8_weight(w)
         check_linear(linear_fp8(x, w_q, w_s), *quantize_fp8(x), w_q, w_s)
