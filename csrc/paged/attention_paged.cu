@@ -130,7 +130,7 @@ struct PartDesc {
 struct Workspace {
   PartDesc* desc;  // [2 CTAs]
   float* ml;       // [2 CTAs][row_cap][2]: bound on the maximum (log2 units), sum
-  float* acc;      // [2 CTAs][row_cap][d]
+  float* acc;      // [2 CTAs][d / 4][row_cap][4]
   int row_cap;
 };
 
@@ -493,25 +493,36 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) sm100::mbar_arrive(b);
     };
     // Writes the queries of an item into a tile: those of this group's 128 rows, or all of an item of at most 128.
+    // D / 8 lanes read a row, so that a load touches whole lines.
     auto load_q = [&](const Item& i, int tile) {
-      const int r = !kTokens && i.rows > 128 ? t * 128 + row : (kTokens || i.rows <= 32 ? lane : row);
-      uint8_t* dst = smem + C::kQ + tile * C::kTileBytes + row * 128;
-      const bool valid = r < i.rows;
-      const int tok = (i.row0 + r) / group, g = (i.row0 + r) % group;
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.q) + (i.q0 + tok) * a.q_tok +
-                                                        (i.h * group + g) * a.q_head);
+      constexpr int kLanes = D / 8, kRows = 32 / kLanes;
+      const int chunk = lane % kLanes;
+      const int first = !kTokens && i.rows > 128 ? t * 128 + w4 * 32 : (kTokens || i.rows <= 32 ? 0 : w4 * 32);
+      uint8_t* dst = smem + C::kQ + tile * C::kTileBytes + (chunk >> 3) * C::kHalfBytes + w4 * 32 * 128;
+      int r = first + lane / kLanes;
+      int tok = (i.row0 + r) / group, g = (i.row0 + r) % group;
+      const T* q = static_cast<const T*>(a.q) + i.q0 * a.q_tok + i.h * group * a.q_head + chunk * 8;
+      const int rows = i.rows;
+      uint4 v[kLanes];
 #pragma unroll
-      for (int c = 0; c < D / 8; ++c) {
-        uint4 v = valid ? __ldg(src + c) : make_uint4(0u, 0u, 0u, 0u);
+      for (int j = 0; j < kLanes; ++j) {
+        v[j] = make_uint4(0u, 0u, 0u, 0u);
+        if (r < rows) v[j] = __ldg(reinterpret_cast<const uint4*>(q + tok * a.q_tok + g * a.q_head));
+        r += kRows;
+        for (g += kRows; g >= group; g -= group) ++tok;
+      }
+#pragma unroll
+      for (int j = 0; j < kLanes; ++j) {
         if (q_sign != 1.f) {  // a negative or zero scale moves into the queries
-          uint32_t* u = reinterpret_cast<uint32_t*>(&v);
+          uint32_t* u = reinterpret_cast<uint32_t*>(&v[j]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const float2 f = to_float2<T>(u[e]);
             u[e] = pack2<T>(f.x * q_sign, f.y * q_sign);
           }
         }
-        *reinterpret_cast<uint4*>(dst + (c >> 3) * C::kHalfBytes + (((c & 7) ^ (row & 7)) << 4)) = v;
+        const int lr = j * kRows + lane / kLanes;
+        *reinterpret_cast<uint4*>(dst + lr * 128 + (((chunk & 7) ^ (lr & 7)) << 4)) = v[j];
       }
       sm100::fence_proxy_async_smem();
       __syncwarp();
@@ -678,26 +689,53 @@ __global__ void __launch_bounds__(kThreads, 1)
         attention_row<T, D>(a, it.s, it.q0 + x / group, it.len - it.n + x / group, it.len, it.h * group + x % group,
                             it.h);
       };
-      // Stores 32 columns of a row: rounded with the factor inv, or as fp32 to the workspace.
-      T* const out = out_of(min(r, it.rows - 1));
+      // Stores 32 columns of each of the warp's rows. As fp32 to the workspace: float4 c of row r at place
+      // c row_cap + r, so that lanes write side by side. Or rounded with the factor inv: four lanes exchange their
+      // 16-byte parts, so that each store writes 64 bytes of a row.
+      const int64_t my_out = out_of(min(r, it.rows - 1)) - static_cast<T*>(a.out);
       auto store32 = [&](int c, const float* o, float inv, float& odd) {
-        if (whole) {
-          uint4* dst = reinterpret_cast<uint4*>(out + c);
+        if (!whole) {
+          if (!valid) return;
+          float4* dst = reinterpret_cast<float4*>(acc) + static_cast<int64_t>(c / 4) * ws.row_cap + r;
 #pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            float y[8];
+          for (int e = 0; e < 8; ++e)
+            dst[static_cast<int64_t>(e) * ws.row_cap] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+          return;
+        }
+        uint4 part[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              y[i] = inv == 0.f ? 0.f : o[e + i] * inv;
-              odd += y[i] * 0.f;  // NaN if any is not finite
-            }
-            dst[e / 8] = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]),
-                                    pack2<T>(y[6], y[7]));
+        for (int e = 0; e < 4; ++e) {
+          float y[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            y[i] = inv == 0.f ? 0.f : o[8 * e + i] * inv;
+            odd += y[i] * 0.f;  // NaN if any is not finite
           }
-        } else {
-          float4* dst = reinterpret_cast<float4*>(acc + static_cast<int64_t>(r) * D + c);
+          part[e] = make_uint4(pack2<T>(y[0], y[1]), pack2<T>(y[2], y[3]), pack2<T>(y[4], y[5]), pack2<T>(y[6], y[7]));
+        }
+        auto exchange = [&](uint4& keep_low, uint4& keep_high, int mask) {
+          const bool high = lane & mask;
+          const uint4 send = high ? keep_low : keep_high;
+          uint4 got;
+          got.x = __shfl_xor_sync(0xffffffffu, send.x, mask);
+          got.y = __shfl_xor_sync(0xffffffffu, send.y, mask);
+          got.z = __shfl_xor_sync(0xffffffffu, send.z, mask);
+          got.w = __shfl_xor_sync(0xffffffffu, send.w, mask);
+          if (high)
+            keep_low = got;
+          else
+            keep_high = got;
+        };
+        exchange(part[0], part[1], 1);
+        exchange(part[2], part[3], 1);
+        exchange(part[0], part[2], 2);
+        exchange(part[1], part[3], 2);
 #pragma unroll
-          for (int e = 0; e < 32; e += 4) dst[e / 4] = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+        for (int e = 0; e < 4; ++e) {  // part e of this lane: columns 8 (lane & 3) of row 4 (lane / 4) + e of the warp
+          const int from = (lane & ~3) + e;
+          const int64_t off = __shfl_sync(0xffffffffu, my_out, from);
+          if (__shfl_sync(0xffffffffu, static_cast<int>(valid), from))
+            *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + off + c + (lane & 3) * 8) = part[e];
         }
       };
       const float m2 = m == -INFINITY ? -INFINITY : m * scale_log2;
@@ -721,7 +759,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
             for (int e = 0; e < 32; ++e) y[e] += __uint_as_float(o[e]) * f1;
           }
-          if (valid) store32(c, y, inv, odd);
+          store32(c, y, inv, odd);
         }
         if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
         unsigned redo = __ballot_sync(0xffffffffu, whole && valid && odd != 0.f);
@@ -803,7 +841,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if ((y.x + y.y + y.z + y.w) * 0.f != 0.f) atomicOr(&misc.bad, 1u << r2);
                 *reinterpret_cast<uint2*>(out_of(r2) + c0 + 4 * c) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
               } else {
-                *reinterpret_cast<float4*>(acc + static_cast<int64_t>(r2) * D + c0 + 4 * c) = y;
+                reinterpret_cast<float4*>(acc)[static_cast<int64_t>(c0 / 4 + c) * ws.row_cap + r2] = y;
               }
             }
           }
@@ -847,20 +885,21 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the parts of the blocks that a cut fell into. Grid (CTAs of the
 // attention kernel, row groups); the CTA whose part starts such a block owns it.
 // Parts are added in the order of the tiles, so results do not depend on timing.
-constexpr int kMergeThreads = 256;
-constexpr int kMergeGroups = 32;
+// A lane has a row, a warp 16 columns of 32 rows.
 constexpr int kMaxParts = 1024;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(kMergeThreads)
+__global__ void __launch_bounds__(D * 2)
     merge_kernel(const __grid_constant__ AttnArgs a, const Workspace ws, int group, int ctas) {
   __shared__ int part[kMaxParts];
   __shared__ int parts;
+  __shared__ unsigned odd_rows;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) odd_rows = 0;
   pdl_wait();
   pdl_trigger();
   const PartDesc first = ws.desc[2 * blockIdx.x + 1];
-  if (first.q0 < 0 || first.t1 == first.tiles || blockIdx.y * (kMergeThreads / 32) >= first.rows) return;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (first.q0 < 0 || first.t1 == first.tiles || static_cast<int>(blockIdx.y) * 32 >= first.rows) return;
   if (warp == 0) {
     // Continuations follow in the order of the CTAs; one that reaches the last tile is the last.
     int n = 1;
@@ -880,54 +919,58 @@ __global__ void __launch_bounds__(kMergeThreads)
   }
   __syncthreads();
   const int n = parts;
-  for (int r = blockIdx.y * (kMergeThreads / 32) + warp; r < first.rows; r += kMergeGroups * (kMergeThreads / 32)) {
-    // A lane has the states of parts lane, lane + 32, ...
-    auto state = [&](int i) {
-      return i < n ? __ldcg(reinterpret_cast<const float2*>(ws.ml + (static_cast<int64_t>(part[i]) * ws.row_cap + r) * 2))
-                   : make_float2(-INFINITY, 0.f);
-    };
-    const float2 mine = state(lane);
-    float m = mine.x;
-    for (int i = lane + 32; i < n; i += 32) m = fmaxf(m, state(i).x);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    float l = 0.f, o[D / 32] = {};
-    for (int i0 = 0; i0 < n; i0 += 32) {
-      const float2 v = i0 == 0 ? mine : state(i0 + lane);
-      const float f_mine = v.x == -INFINITY ? 0.f : fast_exp2(v.x - m), l_mine = v.y * f_mine;
-      const int cnt = min(32, n - i0);
+  const int r = blockIdx.y * 32 + lane, rc = min(r, first.rows - 1);
+  auto state = [&](int i) {
+    return __ldcg(reinterpret_cast<const float2*>(ws.ml + (static_cast<int64_t>(part[i]) * ws.row_cap + rc) * 2));
+  };
+  float m = -INFINITY;
+#pragma unroll 8
+  for (int i = 0; i < n; ++i) m = fmaxf(m, state(i).x);
+  float l = 0.f, o[16] = {};
 #pragma unroll 4
-      for (int i = 0; i < cnt; ++i) {
-        const int64_t at = static_cast<int64_t>(part[i0 + i]) * ws.row_cap + r;
-        const float f = __shfl_sync(0xffffffffu, f_mine, i);
-        l += __shfl_sync(0xffffffffu, l_mine, i);
-        if constexpr (D == 128) {
-          const float4 x = __ldcg(reinterpret_cast<const float4*>(ws.acc + at * D) + lane);
-          if (f != 0.f) o[0] += x.x * f, o[1] += x.y * f, o[2] += x.z * f, o[3] += x.w * f;
-        } else {
-          const float2 x = __ldcg(reinterpret_cast<const float2*>(ws.acc + at * D) + lane);
-          if (f != 0.f) o[0] += x.x * f, o[1] += x.y * f;
-        }
+  for (int i = 0; i < n; ++i) {
+    const float2 v = state(i);
+    const float f = v.x == -INFINITY ? 0.f : fast_exp2(v.x - m);
+    l += v.y * f;
+    const float4* src = reinterpret_cast<const float4*>(ws.acc + static_cast<int64_t>(part[i]) * ws.row_cap * D) +
+                        static_cast<int64_t>(warp * 4) * ws.row_cap + rc;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float4 x = __ldcg(src + static_cast<int64_t>(e) * ws.row_cap);
+      if (f != 0.f) {
+        o[4 * e] += x.x * f;
+        o[4 * e + 1] += x.y * f;
+        o[4 * e + 2] += x.z * f;
+        o[4 * e + 3] += x.w * f;
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    float odd = 0.f;
+  }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  float odd = 0.f;
 #pragma unroll
-    for (int e = 0; e < D / 32; ++e) {
-      o[e] = inv == 0.f ? 0.f : o[e] * inv;
-      odd += o[e] * 0.f;
-    }
-    const int x = first.b * kBlock + r, tok = x / group, h = first.h * group + x % group, q0 = first.q0;
-    if (__any_sync(0xffffffffu, odd != 0.f)) {
-      const int cnt = q_begin(a.batch, first.s + 1) - q0, len = __ldg(a.batch.kv_len + first.s);
-      attention_row<T, D>(a, first.s, q0 + tok, len - cnt + tok, len, h, first.h);
-      continue;
-    }
-    T* dst = static_cast<T*>(a.out) + (q0 + tok) * a.o_tok + h * a.o_head;
-    if constexpr (D == 128)
-      *reinterpret_cast<uint2*>(dst + lane * 4) = make_uint2(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]));
-    else
-      *reinterpret_cast<uint32_t*>(dst + lane * 2) = pack2<T>(o[0], o[1]);
+  for (int e = 0; e < 16; ++e) {
+    o[e] = inv == 0.f ? 0.f : o[e] * inv;
+    odd += o[e] * 0.f;
+  }
+  const int x = first.b * kBlock + rc, tok = x / group, h = first.h * group + x % group;
+  const bool valid = r < first.rows;
+  if (valid) {
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (first.q0 + tok) * a.o_tok + h * a.o_head + warp * 16);
+    dst[0] = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
+    dst[1] = make_uint4(pack2<T>(o[8], o[9]), pack2<T>(o[10], o[11]), pack2<T>(o[12], o[13]), pack2<T>(o[14], o[15]));
+  }
+  // Rows that came out as NaN are computed again, after every warp has stored its columns.
+  const unsigned bad = __ballot_sync(0xffffffffu, valid && odd != 0.f);
+  if (lane == 0 && bad) atomicOr(&odd_rows, bad);
+  __syncthreads();
+  const unsigned redo = odd_rows;
+  if (!redo) return;
+  const int cnt = q_begin(a.batch, first.s + 1) - first.q0, len = __ldg(a.batch.kv_len + first.s);
+  for (int i = warp; i < 32; i += D / 16) {
+    if (!(redo >> i & 1u)) continue;
+    const int y = first.b * kBlock + blockIdx.y * 32 + i;
+    attention_row<T, D>(a, first.s, first.q0 + y / group, len - cnt + y / group, len, first.h * group + y % group,
+                        first.h);
   }
 }
 
@@ -1010,8 +1053,8 @@ void launch(const AttnArgs& args, Half type, float* workspace, cudaStream_t s) {
   const float scale_log2 = (sign == 0.f ? 1.f : a.scale * sign) * kLog2e;
   launch_pdl(kern, dim3(static_cast<unsigned>(ctas)), dim3(kThreads), Cfg<D>::kSmem, s, 1, tk, tv, a, ws, group, box,
              sign, scale_log2);
-  launch_pdl(merge_kernel<T, D>, dim3(static_cast<unsigned>(ctas), kMergeGroups), dim3(kMergeThreads), 0, s, 1, a, ws,
-             group, ctas);
+  launch_pdl(merge_kernel<T, D>, dim3(static_cast<unsigned>(ctas), static_cast<unsigned>((ws.row_cap + 31) / 32)),
+             dim3(D * 2), 0, s, 1, a, ws, group, ctas);
 }
 
 }  // namespace
