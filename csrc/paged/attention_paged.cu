@@ -14,9 +14,10 @@
 //
 //   warps 0-3, 4-7  softmax: group t owns S_t, P_t (in the columns of S_t) and
 //                   O_t in tensor memory; a thread owns one row
-//   warps 8, 11     TMA producers of K and of V
-//   warp 9          TMEM allocation and MMA issue (one thread)
-//   warp 10         walks the CTA's items and hands them to the others
+//   warps 8, 11     TMA producers of K and of V; warp 8 walks the CTA's items and
+//                   hands them to the others
+//   warps 9, 10     MMA issue for group 0 and 1 (one thread each: one for both took
+//                   longer to issue the products than they take)
 //
 // Steps alternate between the two groups, so that one's products run during
 // the other's softmax. What the groups work on depends on the block's rows:
@@ -30,12 +31,16 @@
 // the last kind: they run an instance of the kernel without the others' code
 // (kTokens), which a short call fetches faster.
 //
-// S(k + 2) is issued after P V(k), in the order of which the tensor core
-// works, so a group that sees S(k + 2) knows that O holds step k: it may
-// rescale O then. It does so only when the row's maximum has grown by 2^8 or
-// more over the bound m in use (2^6 for fp16, whose P has a factor 2^8 to keep
-// small weights out of the subnormals): P stays in the type's range, and
-// numerator and denominator have the same factor.
+// A step takes 64 tokens of a tile, and S has two buffers for each group, so that
+// the next S of a group is there when its softmax of this one is done. (With one
+// buffer of 128 tokens the softmax waited for P V and S of its own group in every
+// step: 735 us instead of the present time for 4096 tokens over 4096 with 64
+// heads.) P takes the place of S; S(k + 4) is issued after P V(k), in the order of
+// which the tensor core works. O is rescaled only when the row's maximum has grown
+// by 2^8 or more over the bound m in use (2^6 for fp16, whose P has a factor 2^8
+// to keep small weights out of the subnormals), after the product before is done:
+// P stays in the type's range, and numerator and denominator have the same factor.
+// Calls with single tokens take steps of 128: their softmax is short.
 //
 // Pages are read by TMA boxes of the largest power of two of tokens (8 to
 // 128) that divides the page size. Runs that no row sees are not looked up:
@@ -150,18 +155,18 @@ struct Cfg {
 
 constexpr int kThreads = 384;
 constexpr uint32_t kTmemCols = 512;
-constexpr int kEarly = 96;       // tokens of P after which its product may start
-constexpr uint32_t kColO = 256;  // S_0, S_1 at columns 0 and 128, O_0, O_1 at 256 and 384
+constexpr uint32_t kColO = 256;  // S_0, S_1 at columns 0 and 128 (two buffers of 64 each), O_0, O_1 at 256 and 384
 
 struct Barriers {
   uint64_t full[8], empty[8];  // ring slots
   uint64_t qready[2];          // queries of tile t written
-  uint64_t sfull[2];           // S_t computed (and the O_t of the step before)
-  uint64_t pready[2][2];       // O_t rescaled and the first kEarly tokens of P_t written; the rest written
-  uint64_t ofull[2];           // last P V of group t in a block done
+  uint64_t sfull[2][2];        // S computed in buffer b of group t
+  uint64_t pready[2][2];       // P written in its place, O_t rescaled if need be
+  uint64_t odone[2];           // a product P V of group t done
+  uint64_t ofull[2];           // the last one in a block
   uint64_t gsync, gfree;       // the eight softmax warps: states written; their memory read
   uint64_t ifull[4], iempty[4];  // ring of items
-  uint64_t drained;
+  uint64_t drained[2];
 };
 constexpr int kItems = 4;
 struct Misc {
@@ -217,6 +222,34 @@ struct Weights<__half> {
   static constexpr float kBias = 8.f, kSlack = 6.f;
   static constexpr uint32_t kFormat = 0;
 };
+
+// Products with shared-memory descriptors given by their low words: the high word of a layout is a constant, and
+// the issuing thread, whose pace bounds the kernel otherwise, has one register to hand over instead of two.
+constexpr uint32_t desc_high(uint32_t stride_bytes) { return (stride_bytes >> 4) | 1u << 14 | 2u << 29; }
+__device__ __forceinline__ uint32_t desc_low(const void* tile, uint32_t lead_bytes) {
+  return ((sm100::smem_u32(tile) >> 4) & 0x3fffu) | (lead_bytes >> 4) << 16;
+}
+template <uint32_t kHighA, uint32_t kHighB, uint32_t kIdesc>
+__device__ __forceinline__ void mma_ss(uint32_t d, uint32_t a_low, uint32_t b_low, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"
+      "mov.b64 da, {%1, %4};\n\tmov.b64 db, {%2, %5};\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %6, p;\n\t}" ::"r"(d),
+      "r"(a_low), "r"(b_low), "r"(static_cast<uint32_t>(accumulate)), "n"(kHighA), "n"(kHighB), "n"(kIdesc)
+      : "memory");
+}
+template <uint32_t kHighB, uint32_t kIdesc>
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint32_t b_low, bool accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %4};\n\t"
+      "setp.ne.b32 p, %3, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %5, p;\n\t}" ::"r"(d),
+      "r"(a), "r"(b_low), "r"(static_cast<uint32_t>(accumulate)), "n"(kHighB), "n"(kIdesc)
+      : "memory");
+}
+
 // Instruction descriptor: D fp32, A and B of type T, shape 128 x n; B MN-major if `bt`.
 template <typename T>
 constexpr uint32_t idesc(int n, bool bt) {
@@ -228,14 +261,18 @@ __device__ __forceinline__ void wait_slow(uint64_t* b, uint32_t parity, volatile
   if (!*err && !sm100::mbar_wait(b, parity)) *err = 1;
 }
 
-// Steps of an item: step k belongs to group k & 1.
+// Steps of an item: step k belongs to group k & 1 and takes kStep tokens of a
+// tile, its kSub parts in turn, each in a buffer of its own.
 template <bool kTokens>
 struct Steps {
-  bool wide;  // over 128 rows: both groups use every tile
+  static constexpr int kStep = kTokens ? 128 : 64, kSub = kTile / kStep;
+  bool wide;  // over 128 rows: both groups use every tile, else every other one
   int nt;     // tiles
   __device__ __forceinline__ Steps(const Item& it) : wide(!kTokens && it.rows > 128), nt(it.t1 - it.t0) {}
-  __device__ __forceinline__ int count() const { return wide ? 2 * nt : nt; }
-  __device__ __forceinline__ int tile(int k) const { return wide ? k >> 1 : k; }
+  __device__ __forceinline__ int count() const { return 2 * kSub * (wide ? nt : (nt + 1) / 2); }
+  __device__ __forceinline__ int tile(int k) const { return wide ? k / (2 * kSub) : k / (2 * kSub) * 2 + (k & 1); }
+  __device__ __forceinline__ static int part(int k) { return (k >> 1) & (kSub - 1); }
+  __device__ __forceinline__ bool valid(int k) const { return k < count() && (wide || tile(k) < nt); }
   // Place of tile j's K and V in the ring's order of loads: the order of first use.
   __device__ __forceinline__ int k_at(int j) const { return wide ? 2 * j : (j == 0 ? 0 : 2 * j - 1); }
   __device__ __forceinline__ int v_at(int j) const { return wide ? 2 * j + 1 : (j + 1 < nt ? 2 * j + 2 : 2 * nt - 1); }
@@ -260,22 +297,24 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
       sm100::mbar_init(&bar.full[i], 1);
-      sm100::mbar_init(&bar.empty[i], 1);
+      sm100::mbar_init(&bar.empty[i], 2);  // both issuers
     }
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&bar.qready[i], 4);
-      sm100::mbar_init(&bar.sfull[i], 1);
-      sm100::mbar_init(&bar.pready[i][0], 4);
-      sm100::mbar_init(&bar.pready[i][1], 4);
+      sm100::mbar_init(&bar.drained[i], 1);
+      for (int b = 0; b < 2; ++b) {
+        sm100::mbar_init(&bar.sfull[i][b], 1);
+        sm100::mbar_init(&bar.pready[i][b], 4);
+      }
+      sm100::mbar_init(&bar.odone[i], 1);
       sm100::mbar_init(&bar.ofull[i], 1);
     }
     for (int i = 0; i < kItems; ++i) {
       sm100::mbar_init(&bar.ifull[i], 1);
-      sm100::mbar_init(&bar.iempty[i], 11);  // two producers, MMA issue, eight softmax warps
+      sm100::mbar_init(&bar.iempty[i], 12);  // the producers, two issuers, eight softmax warps
     }
     sm100::mbar_init(&bar.gsync, 8);
     sm100::mbar_init(&bar.gfree, 8);
-    sm100::mbar_init(&bar.drained, 1);
     misc.err = 0;
     misc.bad = 0;
     for (int i = 0; i < 8; ++i) misc.last[0][i] = misc.last[1][i] = -1;
@@ -299,26 +338,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto wait = [&](uint64_t* b, uint32_t parity) {
     if (!sm100::mbar_try_wait(b, parity)) wait_slow(b, parity, s_err);
   };
-  // 168 registers a thread at launch: 72 for the last warpgroup and 216 for the two of the softmax, where whole
-  // rows of S are held.
+  // 168 registers a thread at launch: 104 for the last warpgroup and 200 for the two of the softmax.
   if (warp >= 8) {
-    if constexpr (!kTokens) sm100::reg_give<72>();
-    if (warp == 10) {
-      // ---------------------------------------------------------- items
-      if (lane == 0) {
-        Walk walk;
-        walk.start(a, group, misc.part);
-        for (unsigned i = 0;; ++i) {
-          Item it;
-          const bool more = walk.next(a, group, it) && !*s_err;
-          if (!more) it.rows = 0;
-          wait(&bar.iempty[i % kItems], ((i / kItems) & 1u) ^ 1u);
-          misc.item[i % kItems] = it;
-          sm100::mbar_arrive(&bar.ifull[i % kItems]);
-          if (!more) break;
-        }
-      }
-    }
+    if constexpr (!kTokens) sm100::reg_give<104>();
     if (warp == 8 || warp == 11) {
       // ------------------------------------------------------------ TMA producers
       const bool is_v = warp == 11;
@@ -327,6 +349,22 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int ahead = 32 / boxes;   // tiles whose runs the warp's lanes look up together
       const int unit = is_v ? a.unit_v : a.unit_k;  // of 64 values from head to head
       unsigned base = 0;              // loads of the items before, K and V
+      Walk walk;
+      auto publish = [&](unsigned i) {  // the next item, or that there is none
+        Item it;
+        const bool more = walk.next(a, group, it);
+        wait(&bar.iempty[i % kItems], ((i / kItems) & 1u) ^ 1u);
+        if (lane == 0) {
+          if (!more || *s_err) it.rows = 0;
+          misc.item[i % kItems] = it;
+          sm100::mbar_arrive(&bar.ifull[i % kItems]);
+        }
+        __syncwarp();
+      };
+      if (!is_v) {
+        walk.start(a, group, misc.part);
+        publish(0);
+      }
       for (unsigned item = 0;; ++item) {
         wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
         const Item& it = misc.item[item % kItems];
@@ -368,111 +406,106 @@ __global__ void __launch_bounds__(kThreads, 1)
               sm100::tma_load_5d(dst + run * (box / 8) * C::kGroupBytes, map, &bar.full[sl], 0, 0, head, tok8, page);
           }
           if (lane == 0) misc.last[is_v][sl] = static_cast<int>(n);
+          if (j == 0 && !is_v) publish(item + 1);  // behind the first load, which is waited for
         }
         base += 2 * nt;
         if (lane == 0) sm100::mbar_arrive(&bar.iempty[item % kItems]);
       }
-    } else if (warp == 9) {
-      // ------------------------------------------------------------ MMA issue
+    } else {
+      // ------------------------------------------------------------ MMA issue for group t
+      const int t = warp - 9;
       if (sm100::elect_one()) {
-        // This thread's waits are on the critical path: it polls before it lets itself be suspended.
-        auto poll = [&](uint64_t* b, uint32_t parity) {
-          for (int i = 0; i < 256; ++i)
-            if (sm100::mbar_test_wait(b, parity)) return;
-          wait_slow(b, parity, s_err);
-        };
-        // A place in the ring.
-        struct Place {
-          int slot;
-          uint32_t phase;
-          __device__ __forceinline__ void operator+=(int n) {
-            slot += n;
-            if (slot >= kSlots) slot -= kSlots, phase ^= 1u;
+        using S = Steps<kTokens>;
+        constexpr int kStep = S::kStep, kSub = S::kSub;
+        constexpr uint32_t kHighQ = desc_high(1024), kHighKV = desc_high(C::kGroupBytes);
+        const uint32_t tmem_s = tmem + t * 128, tmem_o = tmem + kColO + t * 128;
+        unsigned base = 0, seen = 0;      // loads of the items before; loads waited for
+        uint32_t qphase = 0, pphase = 0;  // parity of the next qready[tile] (bit tile), pready[t][b] (bit b)
+        // Waits for load n. The loads before it that the other group alone uses are waited for and given back: a slot
+        // is filled again only when both issuers have seen it full, so a parity never stands for two phases.
+        auto loaded = [&](unsigned n) {
+          for (; seen < n; ++seen) {
+            wait(&bar.full[seen % kSlots], (seen / kSlots) & 1u);
+            sm100::mbar_arrive(&bar.empty[seen % kSlots]);
           }
+          wait(&bar.full[n % kSlots], (n / kSlots) & 1u);
+          seen = n + 1;
         };
-        unsigned base = 0;             // loads of the items before
-        uint32_t qphase = 0, pphase = 0;  // bit t: parity of the next qready[t], pready[t]
-        int qt = 0;                    // tile of the queries of an item of at most 128 rows
+        int qt = 0;                       // tile of the queries of an item of at most 128 rows
         bool narrow_before = false;
         for (unsigned item = 0;; ++item) {
           wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
           const Item& it = misc.item[item % kItems];
           if (*s_err || it.rows == 0) break;
-          const Steps<kTokens> st(it);
+          const S st(it);
           sm100::mbar_arrive(&bar.iempty[item % kItems]);
-          const int steps = st.count(), nt = st.nt;
           const bool wide = st.wide;
           qt = !wide && narrow_before ? qt ^ 1 : 0;
           narrow_before = !wide;
-          poll(&bar.qready[qt], qphase >> qt & 1u);
+          const int my_q = wide ? t : qt;
+          // Every phase of a barrier is waited for in turn, also of queries that are not this group's.
+          wait(&bar.qready[qt], qphase >> qt & 1u);
           qphase ^= 1u << qt;
           if (wide) {
-            poll(&bar.qready[1], qphase >> 1 & 1u);
+            wait(&bar.qready[1], qphase >> 1 & 1u);
             qphase ^= 2u;
           }
-          Place kp{static_cast<int>(base % kSlots), (base / kSlots) & 1u}, vp = kp;
-          vp += wide || nt == 1 ? 1 : 2;
-          // S of step k: its tile is the next in K's order. With `wide` both groups use it: the first waits for
-          // it and the second frees it.
+          const uint32_t q_low = desc_low(smem + C::kQ + my_q * C::kTileBytes, 16);
           auto scores = [&](int k) {
-            const int t = k & 1;
-            if (!wide || t == 0) poll(&bar.full[kp.slot], kp.phase);
+            const int b = S::part(k);
+            const unsigned n = base + st.k_at(st.tile(k)), sl = n % kSlots;
+            if (b == 0) loaded(n);
             sm100::tc_fence_after();
-            const uint64_t dq = sm100::smem_desc_sw128(smem + C::kQ + (wide ? t : qt) * C::kTileBytes);
-            const uint64_t dk = sm100::smem_desc_mn_sw128(ring + kp.slot * C::kTileBytes, 16, C::kGroupBytes);
+            const uint32_t k_low = desc_low(ring + sl * C::kTileBytes + b * (kStep / 8) * C::kGroupBytes, 16);
 #pragma unroll
             for (int i = 0; i < D / 16; ++i)
-              sm100::mma_bf16(tmem + t * 128, dq + (i >> 2) * (C::kHalfBytes >> 4) + 2 * (i & 3),
-                              dk + (i >> 2) * (1024 >> 4) + 2 * (i & 3), idesc<T>(128, false), i > 0 ? 1u : 0u);
-            sm100::mma_commit(&bar.sfull[t]);
-            if (!wide || t == 1) {
-              sm100::mma_commit(&bar.empty[kp.slot]);
-              kp += wide || k > 0 ? 2 : 1;
-            }
+              mma_ss<kHighQ, kHighKV, idesc<T>(kStep, false)>(
+                  tmem_s + b * kStep, q_low + (i >> 2) * (C::kHalfBytes >> 4) + 2 * (i & 3),
+                  k_low + (i >> 2) * (1024 >> 4) + 2 * (i & 3), i > 0);
+            sm100::mma_commit(&bar.sfull[t][b]);
+            if (b == kSub - 1) sm100::mma_commit(&bar.empty[sl]);
           };
-          scores(0);
-          if (steps > 1) scores(1);
-          for (int k = 0; k < steps && !*s_err; ++k) {
-            const int t = k & 1;
-            const uint32_t parity = pphase >> t & 1u;
-            pphase ^= 1u << t;
-            if (!wide || t == 0) poll(&bar.full[vp.slot], vp.phase);
-            const uint64_t dv = sm100::smem_desc_mn_sw128(ring + vp.slot * C::kTileBytes, 1024, C::kGroupBytes);
-            poll(&bar.pready[t][0], parity);
+          for (int k = t; k < 2 * kSub; k += 2)
+            if (st.valid(k)) scores(k);
+          for (int k = t; st.valid(k) && !*s_err; k += 2) {
+            const int b = S::part(k);
+            const unsigned n = base + st.v_at(st.tile(k)), sl = n % kSlots;
+            if (b == 0) loaded(n);
+            const uint32_t v_low = desc_low(ring + sl * C::kTileBytes + b * (kStep / 8) * C::kGroupBytes, 1024);
+            wait(&bar.pready[t][b], pphase >> b & 1u);
+            pphase ^= 1u << b;
             sm100::tc_fence_after();
 #pragma unroll
-            for (int i = 0; i < kTile / 16; ++i) {  // 16 tokens: two groups further in V, 8 columns in P
-              if (i == kEarly / 16) {
-                poll(&bar.pready[t][1], parity);
-                sm100::tc_fence_after();
-              }
-              sm100::mma_f16_ts(tmem + kColO + t * 128, tmem + t * 128 + i * 8, dv + i * (2 * C::kGroupBytes >> 4),
-                                idesc<T>(D, true), (k > 1 || i > 0) ? 1u : 0u);
-            }
-            const int v_slot = vp.slot;
-            if (!wide || t == 1) vp += wide || k + 2 < nt ? 2 : 1;
-            if (k + 2 < steps)
-              scores(k + 2);
-            else
-              sm100::mma_commit(&bar.ofull[t]);
-            if (!wide || t == 1) sm100::mma_commit(&bar.empty[v_slot]);
+            for (int i = 0; i < kStep / 16; ++i)  // 16 tokens: two groups further in V, 8 columns in P
+              mma_ts<kHighKV, idesc<T>(D, true)>(tmem_o, tmem_s + b * kStep + i * 8,
+                                                 v_low + i * (2 * C::kGroupBytes >> 4), k > 1 || i > 0);
+            sm100::mma_commit(&bar.odone[t]);
+            if (st.valid(k + 2 * kSub)) scores(k + 2 * kSub);
+            if (b == kSub - 1) sm100::mma_commit(&bar.empty[sl]);
+            if (!st.valid(k + 2)) sm100::mma_commit(&bar.ofull[t]);
           }
-          base += 2 * nt;
+          base += 2 * st.nt;
+          for (; seen < base && !*s_err; ++seen) {
+            wait(&bar.full[seen % kSlots], (seen / kSlots) & 1u);
+            sm100::mbar_arrive(&bar.empty[seen % kSlots]);
+          }
         }
         // Tensor memory is freed only after every product is done.
-        sm100::mma_commit(&bar.drained);
-        if (!sm100::mbar_wait(&bar.drained, 0)) *s_err = 1;
+        sm100::mma_commit(&bar.drained[t]);
+        if (!sm100::mbar_wait(&bar.drained[t], 0)) *s_err = 1;
       }
       __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ softmax
-    if constexpr (!kTokens) sm100::reg_take<216>();
+    if constexpr (!kTokens) sm100::reg_take<200>();
     const int t = warp >> 2, w4 = warp & 3;
     const int row = w4 * 32 + lane;  // row of the group's tile
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
-    const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + kColO + t * 128;
-    unsigned ns = 0, no = 0, ng = 0, nf = 0, base = 0;  // steps, block ends, joins, frees and loads so far
+    constexpr int kStep = Steps<kTokens>::kStep;
+    const uint32_t tS0 = tmem + lanes + t * 128, tO = tmem + lanes + kColO + t * 128;
+    unsigned no = 0, nb = 0, ng = 0, nf = 0, base = 0;  // products P V, blocks, joins, frees and loads so far
+    uint32_t sphase = 0;                        // bit b: parity of the next sfull[t][b]
     bool q_loaded = false, narrow_before = false;
     int qt = 0;  // tile of the queries of an item of at most 128 rows
     // All softmax warps (not a barrier that a warp which gave up would leave the others at).
@@ -503,26 +536,30 @@ __global__ void __launch_bounds__(kThreads, 1)
       int tok = (i.row0 + r) / group, g = (i.row0 + r) % group;
       const T* q = static_cast<const T*>(a.q) + i.q0 * a.q_tok + i.h * group * a.q_head + chunk * 8;
       const int rows = i.rows;
-      uint4 v[kLanes];
+      // Four loads under way; a short loop, since code that runs once per block is fetched anew each time.
+#pragma unroll 1
+      for (int j = 0; j < kLanes; j += 4) {
+        uint4 v[4];
 #pragma unroll
-      for (int j = 0; j < kLanes; ++j) {
-        v[j] = make_uint4(0u, 0u, 0u, 0u);
-        if (r < rows) v[j] = __ldg(reinterpret_cast<const uint4*>(q + tok * a.q_tok + g * a.q_head));
-        r += kRows;
-        for (g += kRows; g >= group; g -= group) ++tok;
-      }
-#pragma unroll
-      for (int j = 0; j < kLanes; ++j) {
-        if (q_sign != 1.f) {  // a negative or zero scale moves into the queries
-          uint32_t* u = reinterpret_cast<uint32_t*>(&v[j]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const float2 f = to_float2<T>(u[e]);
-            u[e] = pack2<T>(f.x * q_sign, f.y * q_sign);
-          }
+        for (int e = 0; e < 4; ++e) {
+          v[e] = make_uint4(0u, 0u, 0u, 0u);
+          if (r < rows) v[e] = __ldg(reinterpret_cast<const uint4*>(q + tok * a.q_tok + g * a.q_head));
+          r += kRows;
+          for (g += kRows; g >= group; g -= group) ++tok;
         }
-        const int lr = j * kRows + lane / kLanes;
-        *reinterpret_cast<uint4*>(dst + lr * 128 + (((chunk & 7) ^ (lr & 7)) << 4)) = v[j];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (q_sign != 1.f) {  // a negative or zero scale moves into the queries
+            uint32_t* u = reinterpret_cast<uint32_t*>(&v[e]);
+#pragma unroll
+            for (int x = 0; x < 4; ++x) {
+              const float2 f = to_float2<T>(u[x]);
+              u[x] = pack2<T>(f.x * q_sign, f.y * q_sign);
+            }
+          }
+          const int lr = (j + e) * kRows + lane / kLanes;
+          *reinterpret_cast<uint4*>(dst + lr * 128 + (((chunk & 7) ^ (lr & 7)) << 4)) = v[e];
+        }
       }
       sm100::fence_proxy_async_smem();
       __syncwarp();
@@ -532,7 +569,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (unsigned item = 0; more(item); ++item) {
       const Item& it = misc.item[item % kItems];
       const Steps<kTokens> st(it);
-      const int steps = st.count();
       const bool wide = st.wide, quad = kTokens || it.rows <= 32;
       // The queries of a narrow item alternate between the tiles, so that those of the next are loaded now; the
       // item's own tile takes the joining of its states at the end.
@@ -558,14 +594,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int first_pos = (it.tile0 + it.t0) * kTile, len = it.len, begin = it.begin;
       float m = -INFINITY, l = 0.f;  // bound on the maximum, in units of S; sum of P
       int mine = 0;                  // steps of this group
-      for (int k = t; k < steps; k += 2, ++mine) {
-        const int j = st.tile(k);
-        const int c0 = first_pos + j * kTile;
-        wait(&bar.sfull[t], ns++ & 1u);
+      for (int k = t; st.valid(k); k += 2, ++mine, ++no) {
+        const int j = st.tile(k), b = st.part(k);
+        const int c0 = first_pos + j * kTile, cs = c0 + b * kStep;  // positions of the tile and of the step
+        const uint32_t tS = tS0 + b * kStep;
+        wait(&bar.sfull[t][b], sphase >> b & 1u);
+        sphase ^= 1u << b;
         sm100::tc_fence_after();
         // Tokens behind the sequence and before every row's window may hold anything: zeros in V, since
-        // zero times NaN is NaN. (After S of the step: its K, and what the slot of V held before, are consumed.)
-        if (c0 + kTile > len || c0 < begin) {
+        // zero times NaN is NaN. (After S of the step: what the slot of V held before is consumed or still waited
+        // for by this load.)
+        if (b == 0 && (c0 + kTile > len || c0 < begin)) {
           const unsigned at = base + st.v_at(j);
           wait(&bar.full[at % kSlots], (at / kSlots) & 1u);
           if (c0 + row >= len || c0 + row < begin) {
@@ -581,14 +620,17 @@ __global__ void __launch_bounds__(kThreads, 1)
           auto softmax = [&](auto cols_tag, auto masked_tag) {
             constexpr int kCols = decltype(cols_tag)::value;
             constexpr bool kMasked = decltype(masked_tag)::value;
-            const int first = kCols == 128 ? 0 : w4 * 32;
+            const int first = kCols == kStep ? 0 : w4 * kCols;
             uint32_t x[kCols];
+            if constexpr (kCols == 16) {
+              sm100::tmem_ld_32x32b_x16(tS + first, x);
+            } else {
 #pragma unroll
-            for (int c = 0; c < kCols; c += 32)
-              sm100::tmem_ld_32x32b_x32(tS + first + c, x + c);
+              for (int c = 0; c < kCols; c += 32) sm100::tmem_ld_32x32b_x32(tS + first + c, x + c);
+            }
             sm100::tmem_ld_wait();
             if constexpr (kMasked) {
-              const int from = lo - c0 - first, to = hi - c0 - first;
+              const int from = lo - cs - first, to = hi - cs - first;
 #pragma unroll
               for (int c = 0; c < kCols; ++c)
                 if (c < from || c >= to) x[c] = 0xff800000u;  // -inf
@@ -605,6 +647,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               m = top;
               l *= f;
               if (mine > 0) {
+                wait(&bar.odone[t], (no - 1) & 1u);  // the product of the step before; those before it are done
+                sm100::tc_fence_after();
 #pragma unroll
                 for (int c = 0; c < D; c += 32) {
                   uint32_t o[32];
@@ -620,47 +664,51 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float shift = m == -INFINITY ? 0.f : Weights<T>::kBias - m * scale_log2;
             const uint64_t scale2 = pack64(scale_log2, scale_log2), shift2 = pack64(shift, shift);
             uint64_t sum[2] = {0, 0};
+            constexpr int kChunk = kCols < 32 ? kCols : 32;
 #pragma unroll
-            for (int c = 0; c < kCols; c += 32) {  // P of columns c .. c + 31 goes where S was
-              uint32_t p[16];
+            for (int c = 0; c < kCols; c += kChunk) {  // P of columns c .. goes where S was
+              uint32_t p[kChunk / 2];
 #pragma unroll
-              for (int e = 0; e < 32; e += 2) {
+              for (int e = 0; e < kChunk; e += 2) {
                 const float2 y = unpack64(
                     fma2(pack64(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1])), scale2, shift2));
-                const float p0 = fast_exp2(y.x), p1 = fast_exp2(y.y);
-                sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], pack64(p0, p1));
-                p[e / 2] = pack2<T>(p0, p1);
+                const float2 w = make_float2(fast_exp2(y.x), fast_exp2(y.y));
+                sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], pack64(w.x, w.y));
+                p[e / 2] = pack2<T>(w.x, w.y);
               }
-              sm100::tmem_st_32x32b_x16(tS + (first + c) / 2, p);
-              if (c + 32 == kEarly) {
-                sm100::tmem_st_wait();
-                arrive(&bar.pready[t][0]);
-              }
+              if constexpr (kChunk == 16)
+                sm100::tmem_st_32x32b_x8(tS + (first + c) / 2, p);
+              else
+                sm100::tmem_st_32x32b_x16(tS + (first + c) / 2, p);
             }
             const float2 all = unpack64(add2(sum[0], sum[1]));
             l += all.x + all.y;
-            if constexpr (kCols < 128) {
+            if constexpr (kCols < kStep) {
               // The other quarters' tokens have no weight in this warp's rows.
-              const uint32_t zero[16] = {};
+              const uint32_t zero[kCols / 2] = {};
 #pragma unroll
-              for (int q = 1; q < 4; ++q) sm100::tmem_st_32x32b_x16(tS + ((w4 + q) & 3) * 16, zero);
+              for (int q = 1; q < 4; ++q) {
+                if constexpr (kCols == 16)
+                  sm100::tmem_st_32x32b_x8(tS + ((w4 + q) & 3) * 8, zero);
+                else
+                  sm100::tmem_st_32x32b_x16(tS + ((w4 + q) & 3) * 16, zero);
+              }
             }
             sm100::tmem_st_wait();
           };
           using Yes = std::integral_constant<bool, true>;
           using No = std::integral_constant<bool, false>;
           if constexpr (kTokens) {
-            softmax(std::integral_constant<int, 32>{}, Yes{});
+            softmax(std::integral_constant<int, kStep / 4>{}, Yes{});
           } else if (quad) {
-            softmax(std::integral_constant<int, 32>{}, Yes{});
-          } else if (c0 >= lo_all && c0 + kTile <= hi_all) {
-            softmax(std::integral_constant<int, 128>{}, No{});
+            softmax(std::integral_constant<int, kStep / 4>{}, Yes{});
+          } else if (cs >= lo_all && cs + kStep <= hi_all) {
+            softmax(std::integral_constant<int, kStep>{}, No{});
           } else {
-            softmax(std::integral_constant<int, 128>{}, Yes{});
+            softmax(std::integral_constant<int, kStep>{}, Yes{});
           }
         }
-        if (idle || quad) arrive(&bar.pready[t][0]);
-        arrive(&bar.pready[t][1]);
+        arrive(&bar.pready[t][b]);
       }
       base += 2 * st.nt;
 
@@ -671,7 +719,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         q_loaded = true;
       }
       if (mine > 0) {
-        wait(&bar.ofull[t], no++ & 1u);
+        wait(&bar.ofull[t], nb++ & 1u);
         sm100::tc_fence_after();
       }
       const bool whole = it.whole();
@@ -769,12 +817,13 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (wide) {
         if (!idle) finish_rows(m2, l, 1.f, 0.f, false);
       } else {
-        // The states of all warps, through the memory of the item's queries: every S is done, since it was issued
-        // before the last but one product with V, which each group with a step has waited for.
+        // The states of all warps, through the memory of the item's queries, which both groups have used up once
+        // their last products with V are done.
         float2* sml = reinterpret_cast<float2*>(buf);  // [8 warps][32 lanes]
-        const bool two = steps > 1;                    // group 1 had a tile
-        if (mine > 0) sml[threadIdx.x] = make_float2(m2, l);
+        const bool two = st.nt > 1;                    // group 1 had a tile
         sm100::tc_fence_before();
+        group_sync();
+        if (mine > 0) sml[threadIdx.x] = make_float2(m2, l);
         group_sync();
         auto factor = [](float mm, float top) { return mm == -INFINITY ? 0.f : fast_exp2(mm - top); };
         if (!quad) {
@@ -885,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the parts of the blocks that a cut fell into. Grid (CTAs of the
 // attention kernel, row groups); the CTA whose part starts such a block owns it.
 // Parts are added in the order of the tiles, so results do not depend on timing.
-// A lane has a row, a warp 16 columns of 32 rows.
+// A lane has a row, a warp 16 columns of 32 rows; with fewer rows several lanes share a row's parts.
 constexpr int kMaxParts = 1024;
 
 template <typename T, int D>
@@ -919,16 +968,17 @@ __global__ void __launch_bounds__(D * 2)
   }
   __syncthreads();
   const int n = parts;
-  const int r = blockIdx.y * 32 + lane, rc = min(r, first.rows - 1);
+  // Lanes to a row: 1, 2 or 4, `width` lanes apart.
+  const int width = first.rows <= 8 ? 8 : (first.rows <= 16 ? 16 : 32);
+  const int r = blockIdx.y * 32 + lane % width, rc = min(r, first.rows - 1);
+  float m = -INFINITY, l = 0.f, o[16] = {};
   auto state = [&](int i) {
     return __ldcg(reinterpret_cast<const float2*>(ws.ml + (static_cast<int64_t>(part[i]) * ws.row_cap + rc) * 2));
   };
-  float m = -INFINITY;
 #pragma unroll 8
-  for (int i = 0; i < n; ++i) m = fmaxf(m, state(i).x);
-  float l = 0.f, o[16] = {};
+  for (int i = lane / width; i < n; i += 32 / width) m = fmaxf(m, state(i).x);
 #pragma unroll 4
-  for (int i = 0; i < n; ++i) {
+  for (int i = lane / width; i < n; i += 32 / width) {
     const float2 v = state(i);
     const float f = v.x == -INFINITY ? 0.f : fast_exp2(v.x - m);
     l += v.y * f;
@@ -937,13 +987,21 @@ __global__ void __launch_bounds__(D * 2)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float4 x = __ldcg(src + static_cast<int64_t>(e) * ws.row_cap);
-      if (f != 0.f) {
+      if (f != 0.f) {  // a part that saw nothing has no numbers, or zeros times whatever V holds
         o[4 * e] += x.x * f;
         o[4 * e + 1] += x.y * f;
         o[4 * e + 2] += x.z * f;
         o[4 * e + 3] += x.w * f;
       }
     }
+  }
+  for (int w = width; w < 32; w *= 2) {
+    const float other = __shfl_xor_sync(0xffffffffu, m, w), top = fmaxf(m, other);
+    const float f0 = m == -INFINITY ? 0.f : fast_exp2(m - top), f1 = other == -INFINITY ? 0.f : fast_exp2(other - top);
+    m = top;
+    l = l * f0 + __shfl_xor_sync(0xffffffffu, l, w) * f1;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) o[e] = o[e] * f0 + __shfl_xor_sync(0xffffffffu, o[e], w) * f1;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   float odd = 0.f;
@@ -953,7 +1011,7 @@ __global__ void __launch_bounds__(D * 2)
     odd += o[e] * 0.f;
   }
   const int x = first.b * kBlock + rc, tok = x / group, h = first.h * group + x % group;
-  const bool valid = r < first.rows;
+  const bool valid = r < first.rows && lane < width;
   if (valid) {
     uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (first.q0 + tok) * a.o_tok + h * a.o_head + warp * 16);
     dst[0] = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
