@@ -14,10 +14,9 @@
 //
 //   warps 0-3, 4-7  softmax: group t owns S_t, P_t (in the columns of S_t) and
 //                   O_t in tensor memory; a thread owns one row
-//   warps 8, 11     TMA producers of K and of V; warp 8 walks the CTA's items and
-//                   hands them to the others
-//   warps 9, 10     MMA issue for group 0 and 1 (one thread each: one for both took
-//                   longer to issue the products than they take)
+//   warps 8, 11     TMA producers of K and of V
+//   warp 9          TMEM allocation and MMA issue (one thread)
+//   warp 10         walks the CTA's items and hands them to the others
 //
 // Steps alternate between the two groups, so that one's products run during
 // the other's softmax. What the groups work on depends on the block's rows:
@@ -31,16 +30,21 @@
 // the last kind: they run an instance of the kernel without the others' code
 // (kTokens), which a short call fetches faster.
 //
-// A step takes 64 tokens of a tile, and S has two buffers for each group, so that
-// the next S of a group is there when its softmax of this one is done. (With one
-// buffer of 128 tokens the softmax waited for P V and S of its own group in every
-// step: 735 us instead of the present time for 4096 tokens over 4096 with 64
-// heads.) P takes the place of S; S(k + 4) is issued after P V(k), in the order of
-// which the tensor core works. O is rescaled only when the row's maximum has grown
-// by 2^8 or more over the bound m in use (2^6 for fp16, whose P has a factor 2^8
-// to keep small weights out of the subnormals), after the product before is done:
-// P stays in the type's range, and numerator and denominator have the same factor.
-// Calls with single tokens take steps of 128: their softmax is short.
+// P takes the place of S; S of a group's next step is issued behind its P V, in
+// which order the tensor core works. (Measured: steps of 64 tokens with two
+// buffers for S, which hide the products of the step before, take 873 us where
+// whole tiles take 723, for 4096 tokens over 4096 with 64 heads of 128: S of 64
+// columns takes the tensor core nearly as long as of 128. With heads of 64: 764
+// and 714 us.) O is rescaled only when the row's maximum has grown by 2^8 or more
+// over the bound m in use (2^6 for fp16, whose P has a factor 2^8 to keep small
+// weights out of the subnormals), after the product before is done: P stays in
+// the type's range, and numerator and denominator have the same factor.
+//
+// What bounds it: with many rows the softmax, whose exponentials alone (8 clocks
+// for a warp's 32) take the time of both products, next to the conversions and
+// maxima in the same schedulers; with single tokens over long caches the stream of
+// K and V (64 tokens over 1 to 4095 with 8 KV heads of 128: 102 us for 0.5 GB),
+// and over short ones the way of a block through the pipeline, about 3 us.
 //
 // Pages are read by TMA boxes of the largest power of two of tokens (8 to
 // 128) that divides the page size. Runs that no row sees are not looked up:
@@ -90,6 +94,7 @@ __device__ __noinline__ void attention_row(const AttnArgs& a, int s, int row, in
     o[i] = make_float2(0.f, 0.f);
   }
   float m = -INFINITY, l = 0.f;
+#pragma unroll 1
   for (int p = begin; p < end; ++p) {
     const int page = page_of(a.batch, s, p / a.page_size, a.num_pages);
     if (page < 0) continue;  // reported by the producer
@@ -155,18 +160,18 @@ struct Cfg {
 
 constexpr int kThreads = 384;
 constexpr uint32_t kTmemCols = 512;
-constexpr uint32_t kColO = 256;  // S_0, S_1 at columns 0 and 128 (two buffers of 64 each), O_0, O_1 at 256 and 384
+constexpr uint32_t kColO = 256;  // S_0, S_1 at columns 0 and 128 O_0, O_1 at 256 and 384
 
 struct Barriers {
   uint64_t full[8], empty[8];  // ring slots
   uint64_t qready[2];          // queries of tile t written
-  uint64_t sfull[2][2];        // S computed in buffer b of group t
-  uint64_t pready[2][2];       // P written in its place, O_t rescaled if need be
+  uint64_t sfull[2];           // S of group t computed
+  uint64_t pready[2];          // P written in its place, O_t rescaled if need be
   uint64_t odone[2];           // a product P V of group t done
   uint64_t ofull[2];           // the last one in a block
   uint64_t gsync, gfree;       // the eight softmax warps: states written; their memory read
   uint64_t ifull[4], iempty[4];  // ring of items
-  uint64_t drained[2];
+  uint64_t drained;
 };
 constexpr int kItems = 4;
 struct Misc {
@@ -257,22 +262,14 @@ constexpr uint32_t idesc(int n, bool bt) {
          (static_cast<uint32_t>(n >> 3) << 17) | (128u >> 4 << 24);
 }
 
-__device__ __forceinline__ void wait_slow(uint64_t* b, uint32_t parity, volatile int* err) {
-  if (!*err && !sm100::mbar_wait(b, parity)) *err = 1;
-}
-
-// Steps of an item: step k belongs to group k & 1 and takes kStep tokens of a
-// tile, its kSub parts in turn, each in a buffer of its own.
+// Steps of an item: step k belongs to group k & 1 and takes a tile.
 template <bool kTokens>
 struct Steps {
-  static constexpr int kStep = kTokens ? 128 : 64, kSub = kTile / kStep;
   bool wide;  // over 128 rows: both groups use every tile, else every other one
   int nt;     // tiles
   __device__ __forceinline__ Steps(const Item& it) : wide(!kTokens && it.rows > 128), nt(it.t1 - it.t0) {}
-  __device__ __forceinline__ int count() const { return 2 * kSub * (wide ? nt : (nt + 1) / 2); }
-  __device__ __forceinline__ int tile(int k) const { return wide ? k / (2 * kSub) : k / (2 * kSub) * 2 + (k & 1); }
-  __device__ __forceinline__ static int part(int k) { return (k >> 1) & (kSub - 1); }
-  __device__ __forceinline__ bool valid(int k) const { return k < count() && (wide || tile(k) < nt); }
+  __device__ __forceinline__ int count() const { return wide ? 2 * nt : nt; }
+  __device__ __forceinline__ int tile(int k) const { return wide ? k / 2 : k; }
   // Place of tile j's K and V in the ring's order of loads: the order of first use.
   __device__ __forceinline__ int k_at(int j) const { return wide ? 2 * j : (j == 0 ? 0 : 2 * j - 1); }
   __device__ __forceinline__ int v_at(int j) const { return wide ? 2 * j + 1 : (j + 1 < nt ? 2 * j + 2 : 2 * nt - 1); }
@@ -297,24 +294,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int i = 0; i < kSlots; ++i) {
       sm100::mbar_init(&bar.full[i], 1);
-      sm100::mbar_init(&bar.empty[i], 2);  // both issuers
+      sm100::mbar_init(&bar.empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&bar.qready[i], 4);
-      sm100::mbar_init(&bar.drained[i], 1);
-      for (int b = 0; b < 2; ++b) {
-        sm100::mbar_init(&bar.sfull[i][b], 1);
-        sm100::mbar_init(&bar.pready[i][b], 4);
-      }
+      sm100::mbar_init(&bar.sfull[i], 1);
+      sm100::mbar_init(&bar.pready[i], 4);
       sm100::mbar_init(&bar.odone[i], 1);
       sm100::mbar_init(&bar.ofull[i], 1);
     }
     for (int i = 0; i < kItems; ++i) {
       sm100::mbar_init(&bar.ifull[i], 1);
-      sm100::mbar_init(&bar.iempty[i], 12);  // the producers, two issuers, eight softmax warps
+      sm100::mbar_init(&bar.iempty[i], 11);  // two producers, MMA issue, eight softmax warps
     }
     sm100::mbar_init(&bar.gsync, 8);
     sm100::mbar_init(&bar.gfree, 8);
+    sm100::mbar_init(&bar.drained, 1);
     misc.err = 0;
     misc.bad = 0;
     for (int i = 0; i < 8; ++i) misc.last[0][i] = misc.last[1][i] = -1;
@@ -334,14 +329,37 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   sm100::tc_fence_after();
   const uint32_t tmem = misc.tmem;
-  // A wait that ends early once any role of the CTA has given up.
+  // A wait that ends early once any role of the CTA has given up. A failed try is suspended for a microsecond or
+  // two, so the limit is seconds (and a tenth of one if it never were). Small on purpose: it is inlined at many
+  // places, and code that does not stay in the instruction cache is what a short call spends its time on.
   auto wait = [&](uint64_t* b, uint32_t parity) {
-    if (!sm100::mbar_try_wait(b, parity)) wait_slow(b, parity, s_err);
+#pragma unroll 1
+    for (int i = 0; !sm100::mbar_try_wait(b, parity); ++i)
+      if ((i & 63) == 63 && (*s_err || i > (1 << 22))) {
+        *s_err = 1;
+        break;
+      }
   };
-  // 168 registers a thread at launch: 104 for the last warpgroup and 200 for the two of the softmax.
+  // 168 registers a thread at launch: 72 for the last warpgroup and 216 for the two of the softmax.
   if (warp >= 8) {
-    if constexpr (!kTokens) sm100::reg_give<104>();
-    if (warp == 8 || warp == 11) {
+    if constexpr (!kTokens) sm100::reg_give<72>();
+    if (warp == 10) {
+      // ------------------------------------------------------------ items
+      if (lane == 0) {
+        Walk walk;
+        walk.start(a, group, misc.part);
+#pragma unroll 1
+        for (unsigned i = 0;; ++i) {
+          Item it;
+          const bool more = walk.next(a, group, it) && !*s_err;
+          if (!more) it.rows = 0;
+          wait(&bar.iempty[i % kItems], ((i / kItems) & 1u) ^ 1u);
+          misc.item[i % kItems] = it;
+          sm100::mbar_arrive(&bar.ifull[i % kItems]);
+          if (!more) break;
+        }
+      }
+    } else if (warp == 8 || warp == 11) {
       // ------------------------------------------------------------ TMA producers
       const bool is_v = warp == 11;
       const CUtensorMap* map = is_v ? &tv : &tk;
@@ -349,22 +367,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int ahead = 32 / boxes;   // tiles whose runs the warp's lanes look up together
       const int unit = is_v ? a.unit_v : a.unit_k;  // of 64 values from head to head
       unsigned base = 0;              // loads of the items before, K and V
-      Walk walk;
-      auto publish = [&](unsigned i) {  // the next item, or that there is none
-        Item it;
-        const bool more = walk.next(a, group, it);
-        wait(&bar.iempty[i % kItems], ((i / kItems) & 1u) ^ 1u);
-        if (lane == 0) {
-          if (!more || *s_err) it.rows = 0;
-          misc.item[i % kItems] = it;
-          sm100::mbar_arrive(&bar.ifull[i % kItems]);
-        }
-        __syncwarp();
-      };
-      if (!is_v) {
-        walk.start(a, group, misc.part);
-        publish(0);
-      }
+#pragma unroll 1
       for (unsigned item = 0;; ++item) {
         wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
         const Item& it = misc.item[item % kItems];
@@ -389,6 +392,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           return at;
         };
         int2 cur = make_int2(0, 0), next = look_up(0);
+#pragma unroll 1
         for (int j = 0; j < nt; ++j) {
           if (j % ahead == 0) {
             cur = next;
@@ -399,6 +403,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (__any_sync(0xffffffffu, *s_err)) break;
           if (lane == 0) sm100::mbar_arrive_expect_tx(&bar.full[sl], C::kTileBytes);
           uint8_t* dst = ring + sl * C::kTileBytes;
+#pragma unroll 1
           for (int run = 0; run < boxes; ++run) {
             const int page = __shfl_sync(0xffffffffu, cur.x, j % ahead * boxes + run);
             const int tok8 = __shfl_sync(0xffffffffu, cur.y, j % ahead * boxes + run);
@@ -406,106 +411,91 @@ __global__ void __launch_bounds__(kThreads, 1)
               sm100::tma_load_5d(dst + run * (box / 8) * C::kGroupBytes, map, &bar.full[sl], 0, 0, head, tok8, page);
           }
           if (lane == 0) misc.last[is_v][sl] = static_cast<int>(n);
-          if (j == 0 && !is_v) publish(item + 1);  // behind the first load, which is waited for
         }
         base += 2 * nt;
         if (lane == 0) sm100::mbar_arrive(&bar.iempty[item % kItems]);
       }
     } else {
-      // ------------------------------------------------------------ MMA issue for group t
-      const int t = warp - 9;
+      // ------------------------------------------------------------ MMA issue
       if (sm100::elect_one()) {
-        using S = Steps<kTokens>;
-        constexpr int kStep = S::kStep, kSub = S::kSub;
         constexpr uint32_t kHighQ = desc_high(1024), kHighKV = desc_high(C::kGroupBytes);
-        const uint32_t tmem_s = tmem + t * 128, tmem_o = tmem + kColO + t * 128;
-        unsigned base = 0, seen = 0;      // loads of the items before; loads waited for
-        uint32_t qphase = 0, pphase = 0;  // parity of the next qready[tile] (bit tile), pready[t][b] (bit b)
-        // Waits for load n. The loads before it that the other group alone uses are waited for and given back: a slot
-        // is filled again only when both issuers have seen it full, so a parity never stands for two phases.
-        auto loaded = [&](unsigned n) {
-          for (; seen < n; ++seen) {
-            wait(&bar.full[seen % kSlots], (seen / kSlots) & 1u);
-            sm100::mbar_arrive(&bar.empty[seen % kSlots]);
-          }
-          wait(&bar.full[n % kSlots], (n / kSlots) & 1u);
-          seen = n + 1;
-        };
+        unsigned base = 0;                // loads of the items before
+        uint32_t qphase = 0, pphase = 0;  // parity of the next qready[tile] (bit tile), pready[t] (bit t)
         int qt = 0;                       // tile of the queries of an item of at most 128 rows
         bool narrow_before = false;
+#pragma unroll 1
         for (unsigned item = 0;; ++item) {
           wait(&bar.ifull[item % kItems], (item / kItems) & 1u);
           const Item& it = misc.item[item % kItems];
           if (*s_err || it.rows == 0) break;
-          const S st(it);
+          const Steps<kTokens> st(it);
           sm100::mbar_arrive(&bar.iempty[item % kItems]);
           const bool wide = st.wide;
+          const int steps = st.count();
           qt = !wide && narrow_before ? qt ^ 1 : 0;
           narrow_before = !wide;
-          const int my_q = wide ? t : qt;
-          // Every phase of a barrier is waited for in turn, also of queries that are not this group's.
           wait(&bar.qready[qt], qphase >> qt & 1u);
           qphase ^= 1u << qt;
           if (wide) {
             wait(&bar.qready[1], qphase >> 1 & 1u);
             qphase ^= 2u;
           }
-          const uint32_t q_low = desc_low(smem + C::kQ + my_q * C::kTileBytes, 16);
+          const uint32_t q_low = desc_low(smem + C::kQ, 16), ring_low = desc_low(ring, 0);
+          // S of step k. With `wide` both groups use a tile: the first waits for it and the second frees it.
           auto scores = [&](int k) {
-            const int b = S::part(k);
+            const int t = k & 1;
             const unsigned n = base + st.k_at(st.tile(k)), sl = n % kSlots;
-            if (b == 0) loaded(n);
+            if (!wide || t == 0) wait(&bar.full[sl], (n / kSlots) & 1u);
             sm100::tc_fence_after();
-            const uint32_t k_low = desc_low(ring + sl * C::kTileBytes + b * (kStep / 8) * C::kGroupBytes, 16);
+            const uint32_t q = q_low + (wide ? t : qt) * (C::kTileBytes >> 4);
+            const uint32_t kk = ring_low + sl * (C::kTileBytes >> 4) + (1u << 16);  // leading byte offset, unused
 #pragma unroll
             for (int i = 0; i < D / 16; ++i)
-              mma_ss<kHighQ, kHighKV, idesc<T>(kStep, false)>(
-                  tmem_s + b * kStep, q_low + (i >> 2) * (C::kHalfBytes >> 4) + 2 * (i & 3),
-                  k_low + (i >> 2) * (1024 >> 4) + 2 * (i & 3), i > 0);
-            sm100::mma_commit(&bar.sfull[t][b]);
-            if (b == kSub - 1) sm100::mma_commit(&bar.empty[sl]);
+              mma_ss<kHighQ, kHighKV, idesc<T>(kTile, false)>(
+                  tmem + t * 128, q + (i >> 2) * (C::kHalfBytes >> 4) + 2 * (i & 3),
+                  kk + (i >> 2) * (1024 >> 4) + 2 * (i & 3), i > 0);
+            sm100::mma_commit(&bar.sfull[t]);
+            if (!wide || t == 1) sm100::mma_commit(&bar.empty[sl]);
           };
-          for (int k = t; k < 2 * kSub; k += 2)
-            if (st.valid(k)) scores(k);
-          for (int k = t; st.valid(k) && !*s_err; k += 2) {
-            const int b = S::part(k);
+#pragma unroll 1
+          for (int k = 0; k < 2 && k < steps; ++k) scores(k);
+#pragma unroll 1
+          for (int k = 0; k < steps && !*s_err; ++k) {
+            const int t = k & 1;
             const unsigned n = base + st.v_at(st.tile(k)), sl = n % kSlots;
-            if (b == 0) loaded(n);
-            const uint32_t v_low = desc_low(ring + sl * C::kTileBytes + b * (kStep / 8) * C::kGroupBytes, 1024);
-            wait(&bar.pready[t][b], pphase >> b & 1u);
-            pphase ^= 1u << b;
+            if (!wide || t == 0) wait(&bar.full[sl], (n / kSlots) & 1u);
+            // Leading byte offset: to the second half.
+            const uint32_t v = ring_low + sl * (C::kTileBytes >> 4) + ((1024u >> 4) << 16);
+            wait(&bar.pready[t], pphase >> t & 1u);
+            pphase ^= 1u << t;
             sm100::tc_fence_after();
 #pragma unroll
-            for (int i = 0; i < kStep / 16; ++i)  // 16 tokens: two groups further in V, 8 columns in P
-              mma_ts<kHighKV, idesc<T>(D, true)>(tmem_o, tmem_s + b * kStep + i * 8,
-                                                 v_low + i * (2 * C::kGroupBytes >> 4), k > 1 || i > 0);
+            for (int i = 0; i < kTile / 16; ++i)  // 16 tokens: two groups further in V, 8 columns in P
+              mma_ts<kHighKV, idesc<T>(D, true)>(tmem + kColO + t * 128, tmem + t * 128 + i * 8,
+                                                 v + i * (2 * C::kGroupBytes >> 4), k > 1 || i > 0);
             sm100::mma_commit(&bar.odone[t]);
-            if (st.valid(k + 2 * kSub)) scores(k + 2 * kSub);
-            if (b == kSub - 1) sm100::mma_commit(&bar.empty[sl]);
-            if (!st.valid(k + 2)) sm100::mma_commit(&bar.ofull[t]);
+            if (!wide || t == 1) sm100::mma_commit(&bar.empty[sl]);
+            if (k + 2 < steps)
+              scores(k + 2);
+            else
+              sm100::mma_commit(&bar.ofull[t]);
           }
           base += 2 * st.nt;
-          for (; seen < base && !*s_err; ++seen) {
-            wait(&bar.full[seen % kSlots], (seen / kSlots) & 1u);
-            sm100::mbar_arrive(&bar.empty[seen % kSlots]);
-          }
         }
         // Tensor memory is freed only after every product is done.
-        sm100::mma_commit(&bar.drained[t]);
-        if (!sm100::mbar_wait(&bar.drained[t], 0)) *s_err = 1;
+        sm100::mma_commit(&bar.drained);
+        if (!sm100::mbar_wait(&bar.drained, 0)) *s_err = 1;
       }
       __syncwarp();
     }
   } else {
     // ------------------------------------------------------------ softmax
-    if constexpr (!kTokens) sm100::reg_take<200>();
+    if constexpr (!kTokens) sm100::reg_take<216>();
     const int t = warp >> 2, w4 = warp & 3;
     const int row = w4 * 32 + lane;  // row of the group's tile
     const uint32_t lanes = static_cast<uint32_t>(w4 * 32) << 16;
-    constexpr int kStep = Steps<kTokens>::kStep;
-    const uint32_t tS0 = tmem + lanes + t * 128, tO = tmem + lanes + kColO + t * 128;
+    const uint32_t tS = tmem + lanes + t * 128, tO = tmem + lanes + kColO + t * 128;
     unsigned no = 0, nb = 0, ng = 0, nf = 0, base = 0;  // products P V, blocks, joins, frees and loads so far
-    uint32_t sphase = 0;                        // bit b: parity of the next sfull[t][b]
     bool q_loaded = false, narrow_before = false;
     int qt = 0;  // tile of the queries of an item of at most 128 rows
     // All softmax warps (not a barrier that a warp which gave up would leave the others at).
@@ -545,6 +535,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           v[e] = make_uint4(0u, 0u, 0u, 0u);
           if (r < rows) v[e] = __ldg(reinterpret_cast<const uint4*>(q + tok * a.q_tok + g * a.q_head));
           r += kRows;
+#pragma unroll 1
           for (g += kRows; g >= group; g -= group) ++tok;
         }
 #pragma unroll
@@ -566,6 +557,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) sm100::mbar_arrive(&bar.qready[tile]);
     };
 
+#pragma unroll 1
     for (unsigned item = 0; more(item); ++item) {
       const Item& it = misc.item[item % kItems];
       const Steps<kTokens> st(it);
@@ -584,27 +576,23 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool valid = r < it.rows;
       const int rr = it.row0 + min(r, it.rows - 1);
       const int pos = it.len - it.n + rr / group;
-      const int hi = valid ? (a.causal ? pos + 1 : it.len) : 0;
-      const int lo = a.window > 0 ? pos - a.window + 1 : 0;
-      // What every valid row of the warp sees.
+      const int hi = valid ? (a.causal ? pos + 1 : it.len) : 0x7fffffff;  // rows that are not there hide nothing
+      const int lo = a.window > 0 && valid ? pos - a.window + 1 : 0;
       const bool idle = __all_sync(0xffffffffu, !valid);
-      const int hi_all = __reduce_min_sync(0xffffffffu, valid ? hi : 0x7fffffff);
-      const int lo_all = __reduce_max_sync(0xffffffffu, valid ? lo : -0x7fffffff);
-
+      const int hi_all = __reduce_min_sync(0xffffffffu, hi), lo_all = __reduce_max_sync(0xffffffffu, lo);
       const int first_pos = (it.tile0 + it.t0) * kTile, len = it.len, begin = it.begin;
       float m = -INFINITY, l = 0.f;  // bound on the maximum, in units of S; sum of P
-      int mine = 0;                  // steps of this group
-      for (int k = t; st.valid(k); k += 2, ++mine, ++no) {
-        const int j = st.tile(k), b = st.part(k);
-        const int c0 = first_pos + j * kTile, cs = c0 + b * kStep;  // positions of the tile and of the step
-        const uint32_t tS = tS0 + b * kStep;
-        wait(&bar.sfull[t][b], sphase >> b & 1u);
-        sphase ^= 1u << b;
+      const int steps = st.count();
+      int mine = 0;  // steps of this group
+#pragma unroll 1
+      for (int k = t; k < steps; k += 2, ++mine, ++no) {
+        const int j = st.tile(k), c0 = first_pos + j * kTile;
+        wait(&bar.sfull[t], no & 1u);
         sm100::tc_fence_after();
         // Tokens behind the sequence and before every row's window may hold anything: zeros in V, since
         // zero times NaN is NaN. (After S of the step: what the slot of V held before is consumed or still waited
         // for by this load.)
-        if (b == 0 && (c0 + kTile > len || c0 < begin)) {
+        if (c0 + kTile > len || c0 < begin) {
           const unsigned at = base + st.v_at(j);
           wait(&bar.full[at % kSlots], (at / kSlots) & 1u);
           if (c0 + row >= len || c0 + row < begin) {
@@ -617,23 +605,23 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!idle) {
           // Columns of this thread: all, or the warp's quarter.
-          auto softmax = [&](auto cols_tag, auto masked_tag) {
+          auto softmax = [&](auto cols_tag) {
             constexpr int kCols = decltype(cols_tag)::value;
-            constexpr bool kMasked = decltype(masked_tag)::value;
-            const int first = kCols == kStep ? 0 : w4 * kCols;
+            const int first = kCols == kTile ? 0 : w4 * kCols;
             uint32_t x[kCols];
-            if constexpr (kCols == 16) {
-              sm100::tmem_ld_32x32b_x16(tS + first, x);
-            } else {
 #pragma unroll
-              for (int c = 0; c < kCols; c += 32) sm100::tmem_ld_32x32b_x32(tS + first + c, x + c);
-            }
+            for (int c = 0; c < kCols; c += 32) sm100::tmem_ld_32x32b_x32(tS + first + c, x + c);
             sm100::tmem_ld_wait();
-            if constexpr (kMasked) {
-              const int from = lo - cs - first, to = hi - cs - first;
+            // Hidden columns become -inf, in the tiles where a row of the warp has some.
+            if (kCols < kTile || c0 + kTile > hi_all) {
+              const int to = hi - c0 - first;
 #pragma unroll
-              for (int c = 0; c < kCols; ++c)
-                if (c < from || c >= to) x[c] = 0xff800000u;  // -inf
+              for (int c = 0; c < kCols; ++c) x[c] = c < to ? x[c] : 0xff800000u;
+            }
+            if (c0 < lo_all) {
+              const int from = lo - c0 - first;
+#pragma unroll
+              for (int c = 0; c < kCols; ++c) x[c] = c >= from ? x[c] : 0xff800000u;
             }
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -664,51 +652,38 @@ __global__ void __launch_bounds__(kThreads, 1)
             const float shift = m == -INFINITY ? 0.f : Weights<T>::kBias - m * scale_log2;
             const uint64_t scale2 = pack64(scale_log2, scale_log2), shift2 = pack64(shift, shift);
             uint64_t sum[2] = {0, 0};
-            constexpr int kChunk = kCols < 32 ? kCols : 32;
 #pragma unroll
-            for (int c = 0; c < kCols; c += kChunk) {  // P of columns c .. goes where S was
-              uint32_t p[kChunk / 2];
+            for (int c = 0; c < kCols; c += 32) {  // P of columns c .. goes where S was
+              uint32_t p[32 / 2];
 #pragma unroll
-              for (int e = 0; e < kChunk; e += 2) {
+              for (int e = 0; e < 32; e += 2) {
                 const float2 y = unpack64(
                     fma2(pack64(__uint_as_float(x[c + e]), __uint_as_float(x[c + e + 1])), scale2, shift2));
                 const float2 w = make_float2(fast_exp2(y.x), fast_exp2(y.y));
                 sum[(e / 2) & 1] = add2(sum[(e / 2) & 1], pack64(w.x, w.y));
                 p[e / 2] = pack2<T>(w.x, w.y);
               }
-              if constexpr (kChunk == 16)
-                sm100::tmem_st_32x32b_x8(tS + (first + c) / 2, p);
-              else
-                sm100::tmem_st_32x32b_x16(tS + (first + c) / 2, p);
+              sm100::tmem_st_32x32b_x16(tS + (first + c) / 2, p);
             }
             const float2 all = unpack64(add2(sum[0], sum[1]));
             l += all.x + all.y;
-            if constexpr (kCols < kStep) {
+            if constexpr (kCols < kTile) {
               // The other quarters' tokens have no weight in this warp's rows.
-              const uint32_t zero[kCols / 2] = {};
+              const uint32_t zero[16] = {};
 #pragma unroll
-              for (int q = 1; q < 4; ++q) {
-                if constexpr (kCols == 16)
-                  sm100::tmem_st_32x32b_x8(tS + ((w4 + q) & 3) * 8, zero);
-                else
-                  sm100::tmem_st_32x32b_x16(tS + ((w4 + q) & 3) * 16, zero);
-              }
+              for (int q = 1; q < 4; ++q) sm100::tmem_st_32x32b_x16(tS + ((w4 + q) & 3) * 16, zero);
             }
             sm100::tmem_st_wait();
           };
-          using Yes = std::integral_constant<bool, true>;
-          using No = std::integral_constant<bool, false>;
           if constexpr (kTokens) {
-            softmax(std::integral_constant<int, kStep / 4>{}, Yes{});
+            softmax(std::integral_constant<int, kTile / 4>{});
           } else if (quad) {
-            softmax(std::integral_constant<int, kStep / 4>{}, Yes{});
-          } else if (cs >= lo_all && cs + kStep <= hi_all) {
-            softmax(std::integral_constant<int, kStep>{}, No{});
+            softmax(std::integral_constant<int, kTile / 4>{});
           } else {
-            softmax(std::integral_constant<int, kStep>{}, Yes{});
+            softmax(std::integral_constant<int, kTile>{});
           }
         }
-        arrive(&bar.pready[t][b]);
+        arrive(&bar.pready[t]);
       }
       base += 2 * st.nt;
 
@@ -811,102 +786,108 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
         unsigned redo = __ballot_sync(0xffffffffu, whole && valid && odd != 0.f);
+#pragma unroll 1
         for (; redo; redo &= redo - 1) again((wide ? t * 128 : 0) + w4 * 32 + __ffs(redo) - 1);
       };
       float* buf = reinterpret_cast<float*>(smem + C::kQ + qt * C::kTileBytes);
-      if (wide) {
-        if (!idle) finish_rows(m2, l, 1.f, 0.f, false);
-      } else {
-        // The states of all warps, through the memory of the item's queries, which both groups have used up once
-        // their last products with V are done.
-        float2* sml = reinterpret_cast<float2*>(buf);  // [8 warps][32 lanes]
-        const bool two = st.nt > 1;                    // group 1 had a tile
+      float mj = m2, lj = l, f0 = 1.f, f1 = 0.f;  // the joined state of this thread's row and the factors of both
+      bool joins = false;
+      auto factor = [](float mm, float top) { return mm == -INFINITY ? 0.f : fast_exp2(mm - top); };
+      // The states of all warps, through the memory of the item's queries: every S is done, since it was issued
+      // before the last but one product with V, which each group with a step has waited for.
+      float2* sml = reinterpret_cast<float2*>(buf);  // [8 warps][32 lanes]
+      const bool two = st.nt > 1;                    // group 1 had a tile
+      if (!wide) {
+        if (mine > 0) sml[threadIdx.x] = make_float2(m2, l);
         sm100::tc_fence_before();
         group_sync();
-        if (mine > 0) sml[threadIdx.x] = make_float2(m2, l);
-        group_sync();
-        auto factor = [](float mm, float top) { return mm == -INFINITY ? 0.f : fast_exp2(mm - top); };
-        if (!quad) {
-          if (t == 0 && !idle) {
-            const float2 other = two ? sml[128 + row] : make_float2(-INFINITY, 0.f);
-            const float mj = fmaxf(m2, other.x), f0 = factor(m2, mj), f1 = factor(other.x, mj);
-            sm100::tc_fence_after();
-            finish_rows(mj, l * f0 + other.y * f1, f0, f1, two);
-          }
-        } else {
-          // Lane = row. The two groups' states of a quarter lie in the same lanes: warp (t, w) adds them for the
-          // half t of the columns and writes the quarter's sum; then a thread adds the quarters of four columns
-          // of a row. A pass takes as many columns as fit; float4 c sits at place c ^ (r & 3).
-          float* part = buf + 512;
-          constexpr int kPart = C::kTileBytes / 4 - 512;
-          float mj = -INFINITY, lj = 0.f;
-          for (int i = 0; i < (two ? 8 : 4); ++i) mj = fmaxf(mj, sml[i * 32 + lane].x);
-          for (int i = 0; i < (two ? 8 : 4); ++i) lj += sml[i * 32 + lane].y * factor(sml[i * 32 + lane].x, mj);
-          const float f0 = factor(sml[w4 * 32 + lane].x, mj);
-          const float f1 = two ? factor(sml[(4 + w4) * 32 + lane].x, mj) : 0.f;
-          if (warp == 0) {
-            misc.sum[lane] = lj;
-            if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
-          }
-          sm100::tc_fence_after();
-          const uint32_t tO0 = tmem + lanes + kColO;
-          int pass = D;
-          while (4 * it.rows * pass > kPart) pass /= 2;  // 32 rows: 32 columns of 128, 16 of 64
+        if (!quad && two) {
+          const float2 other = sml[128 + row];
+          mj = fmaxf(m2, other.x), f0 = factor(m2, mj), f1 = factor(other.x, mj);
+          lj = l * f0 + other.y * f1;
+          joins = true;
+        }
+        sm100::tc_fence_after();
+      }
+      if (!quad) {
+        if (!idle && (wide || t == 0)) finish_rows(mj, lj, f0, f1, joins);
+      } else {
+        // Lane = row. The two groups' states of a quarter lie in the same lanes: warp (t, w) adds them for the
+        // half t of the columns and writes the quarter's sum; then a thread adds the quarters of four columns
+        // of a row. A pass takes as many columns as fit; float4 c sits at place c ^ (r & 3).
+        float* part = buf + 512;
+        constexpr int kPart = C::kTileBytes / 4 - 512;
+        mj = -INFINITY, lj = 0.f;
 #pragma unroll 1
-          for (int c0 = 0; c0 < D; c0 += pass) {
-            if (c0) group_sync();
+        for (int i = 0; i < (two ? 8 : 4); ++i) mj = fmaxf(mj, sml[i * 32 + lane].x);
 #pragma unroll 1
-            for (int c = t * (pass / 2); c < (t + 1) * (pass / 2); c += 8) {
-              uint32_t o0[8], o1[8];
-              sm100::tmem_ld_32x32b_x8(tO0 + c0 + c, o0);
-              if (two) sm100::tmem_ld_32x32b_x8(tO0 + 128 + c0 + c, o1);
-              sm100::tmem_ld_wait();
-              float y[8];
+        for (int i = 0; i < (two ? 8 : 4); ++i) lj += sml[i * 32 + lane].y * factor(sml[i * 32 + lane].x, mj);
+        f0 = factor(sml[w4 * 32 + lane].x, mj);
+        f1 = two ? factor(sml[(4 + w4) * 32 + lane].x, mj) : 0.f;
+        if (warp == 0) {
+          misc.sum[lane] = lj;
+          if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
+        }
+        sm100::tc_fence_after();
+        const uint32_t tO0 = tmem + lanes + kColO;
+        int pass = D;
+        while (4 * it.rows * pass > kPart) pass /= 2;  // 32 rows: 32 columns of 128, 16 of 64
+#pragma unroll 1
+        for (int c0 = 0; c0 < D; c0 += pass) {
+          if (c0) group_sync();
+#pragma unroll 1
+          for (int c = t * (pass / 2); c < (t + 1) * (pass / 2); c += 8) {
+            uint32_t o0[8], o1[8];
+            sm100::tmem_ld_32x32b_x8(tO0 + c0 + c, o0);
+            if (two) sm100::tmem_ld_32x32b_x8(tO0 + 128 + c0 + c, o1);
+            sm100::tmem_ld_wait();
+            float y[8];
 #pragma unroll
-              for (int e = 0; e < 8; ++e) {
-                // A state that saw nothing holds zeros times whatever V holds.
-                y[e] = f0 == 0.f ? 0.f : __uint_as_float(o0[e]) * f0;
-                if (two && f1 != 0.f) y[e] += __uint_as_float(o1[e]) * f1;
-              }
-              if (valid) {
-                float4* dst = reinterpret_cast<float4*>(part + (w4 * it.rows + r) * pass);
-                dst[(c / 4) ^ (r & 3)] = make_float4(y[0], y[1], y[2], y[3]);
-                dst[(c / 4 + 1) ^ (r & 3)] = make_float4(y[4], y[5], y[6], y[7]);
-              }
+            for (int e = 0; e < 8; ++e) {
+              // A state that saw nothing holds zeros times whatever V holds.
+              y[e] = f0 == 0.f ? 0.f : __uint_as_float(o0[e]) * f0;
+              if (two && f1 != 0.f) y[e] += __uint_as_float(o1[e]) * f1;
             }
-            group_sync();
-            for (int i = threadIdx.x; i < it.rows * (pass / 4); i += 256) {
-              const int r2 = i / (pass / 4), c = i % (pass / 4);
-              float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-              for (int q = 0; q < 4; ++q) {
-                const float4 v = reinterpret_cast<const float4*>(part + (q * it.rows + r2) * pass)[c ^ (r2 & 3)];
-                y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
-              }
-              if (whole) {
-                const float lr = misc.sum[r2], inv = lr == 0.f ? 0.f : 1.f / lr;
-                if (inv == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
-                y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-                if ((y.x + y.y + y.z + y.w) * 0.f != 0.f) atomicOr(&misc.bad, 1u << r2);
-                *reinterpret_cast<uint2*>(out_of(r2) + c0 + 4 * c) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
-              } else {
-                reinterpret_cast<float4*>(acc)[static_cast<int64_t>(c0 / 4 + c) * ws.row_cap + r2] = y;
-              }
+            if (valid) {
+              float4* dst = reinterpret_cast<float4*>(part + (w4 * it.rows + r) * pass);
+              dst[(c / 4) ^ (r & 3)] = make_float4(y[0], y[1], y[2], y[3]);
+              dst[(c / 4 + 1) ^ (r & 3)] = make_float4(y[4], y[5], y[6], y[7]);
             }
           }
-          if (whole) {
-            group_sync();  // all rows are written: those that came out as NaN are computed again
-            const unsigned bad = *reinterpret_cast<volatile unsigned*>(&misc.bad);
-            if (bad) {
-              for (int r2 = warp; r2 < it.rows; r2 += 8)
-                if (bad >> r2 & 1u) again(r2);
-              group_sync();
-              if (threadIdx.x == 0) misc.bad = 0;
+          group_sync();
+#pragma unroll 1
+          for (int i = threadIdx.x; i < it.rows * (pass / 4); i += 256) {
+            const int r2 = i / (pass / 4), c = i % (pass / 4);
+            float4 y = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              const float4 v = reinterpret_cast<const float4*>(part + (q * it.rows + r2) * pass)[c ^ (r2 & 3)];
+              y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
+            }
+            if (whole) {
+              const float lr = misc.sum[r2], inv = lr == 0.f ? 0.f : 1.f / lr;
+              if (inv == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
+              y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
+              if ((y.x + y.y + y.z + y.w) * 0.f != 0.f) atomicOr(&misc.bad, 1u << r2);
+              *reinterpret_cast<uint2*>(out_of(r2) + c0 + 4 * c) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
+            } else {
+              reinterpret_cast<float4*>(acc)[static_cast<int64_t>(c0 / 4 + c) * ws.row_cap + r2] = y;
             }
           }
         }
-        arrive(&bar.gfree);
+        if (whole) {
+          group_sync();  // all rows are written: those that came out as NaN are computed again
+          const unsigned bad = *reinterpret_cast<volatile unsigned*>(&misc.bad);
+          if (bad) {
+#pragma unroll 1
+            for (int r2 = warp; r2 < it.rows; r2 += 8)
+              if (bad >> r2 & 1u) again(r2);
+            group_sync();
+            if (threadIdx.x == 0) misc.bad = 0;
+          }
+        }
       }
+      if (!wide) arrive(&bar.gfree);
       sm100::tc_fence_before();
       __syncwarp();
       if (lane == 0) sm100::mbar_arrive(&bar.iempty[item % kItems]);
@@ -922,6 +903,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0 && *s_err) {
     // Every load was waited for by its product, unless a role gave up: then it is here, so that none is in flight
     // when the CTA's memory goes.
+#pragma unroll 1
     for (int sl = 0; sl < kSlots; ++sl) {
       const int n = max(misc.last[0][sl], misc.last[1][sl]);
       if (n >= 0) sm100::mbar_wait(&bar.full[sl], (n / kSlots) & 1);
