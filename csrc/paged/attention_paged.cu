@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   pdl_wait();  // lengths, offsets, pages, queries and the cache may come from the kernel before
   if (threadIdx.x == 0) desc[0].q0 = desc[1].q0 = -1;
-  find_part<kThreads>(a, group, misc.red, &misc.part);
+  find_part<kThreads, kTokens>(a, group, misc.red, &misc.part);
   pdl_trigger();  // after a barrier: this CTA holds its tensor memory
   sm100::tc_fence_before();
   __syncthreads();
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (warp == 10) {
       // ------------------------------------------------------------ items
       if (lane == 0) {
-        Walk walk;
+        Walk<kTokens> walk;
         walk.start(a, group, misc.part);
 #pragma unroll 1
         for (unsigned i = 0;; ++i) {

@@ -8,9 +8,9 @@
 // that a cut falls into is computed in parts and merged (merge_kernel).
 //
 // The line is measured in a weight that has a closed form and is near the
-// tiles' number: a block's tokens times G plus a constant for its start and
-// end (kFixed). With causal rows it grows by the same step from block to block up to
-// the window's limit, so the position of any block is a short sum, and a CTA
+// work: a block's tokens times G plus a constant for its start and end (kFixed),
+// times the work of a tile. With causal rows it grows by the same step from block
+// to block up to the window's limit, so the position of any block is a short sum, and a CTA
 // finds its part from one scan over the sequences. Any weight gives a correct
 // cut: only the balance depends on it.
 #pragma once
@@ -26,6 +26,10 @@ constexpr int kBlock = 256;  // rows of a block
 // it, the join and the output. Measured with 1, 2, 3, 4, 5 and 6: 64 tokens over contexts of 1 to 4095 take 137, 116,
 // 111, 107, 102 and 105 us, a first prompt of 2048 takes 155, 128, 120, 118, 121 and 123 us.
 constexpr int kFixed = 5;
+// Work of a tile for a sequence of over 128 rows against one of fewer. Measured 3 to 2 and 1 to 1: 24 prompts' chunks
+// and single tokens over caches of up to 5000 with 32 heads of 128 take 181 and 197 us. (A call with single tokens only,
+// kTokens, has none over 128: the second factor alone costs it 0.8 us of 17.)
+constexpr int kWideTile = 3, kNarrowTile = 2;
 
 // Quotients of numbers that are nearly always below 2^32.
 __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
@@ -33,36 +37,39 @@ __device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
   return a / b;
 }
 
+template <bool kTokens>
 struct SeqWork {
   int n, len, q0, blocks;
   int64_t a, cap, head;  // weight of block 0, limit of a weight, weight of all blocks of one head
-  bool grows;            // by kBlock from block to block, up to the limit
+  static constexpr int64_t kNoLimit = 1ll << 60;
+  int step;              // by which the weight grows from block to block, up to the limit
 
   __device__ __forceinline__ void load(const AttnArgs& p, int group, int s) {
     q0 = q_begin(p.batch, s);
     n = max(q_begin(p.batch, s + 1) - q0, 0);
     len = __ldg(p.batch.kv_len + s);
     blocks = static_cast<int>((static_cast<int64_t>(n) * group + kBlock - 1) / kBlock);
-    const int64_t g = group, fixed = kFixed * kTile * g;
+    const int unit = kTokens ? 1 : static_cast<int64_t>(n) * group > kBlock / 2 ? kWideTile : kNarrowTile;
+    const int fixed = kFixed * kTile * group * unit;
+    cap = kNoLimit;
     if (p.causal) {
-      a = g * max(len - n, 0) + kBlock + fixed;
-      grows = true;
-      cap = p.window > 0 ? g * (p.window + kTile) + kBlock + fixed : (1ll << 60);
+      a = static_cast<int64_t>(unit * group) * max(len - n, 0) + unit * kBlock + fixed;
+      step = unit * kBlock;
+      if (p.window > 0)
+        cap = static_cast<int64_t>(unit * group) * (static_cast<int64_t>(p.window) + kTile) + step + fixed;
     } else {
-      a = g * max(len, 0) + fixed;
-      grows = false;
-      cap = 1ll << 60;
+      a = static_cast<int64_t>(unit * group) * max(len, 0) + fixed;
+      step = 0;
     }
     head = before(blocks);
   }
-  __device__ __forceinline__ int64_t weight(int b) const {
-    return min(a + (grows ? static_cast<int64_t>(kBlock) * b : 0), cap);
-  }
+  __device__ __forceinline__ int64_t weight(int b) const { return min(a + static_cast<int64_t>(step) * b, cap); }
   // Weight of the blocks before b.
   __device__ __forceinline__ int64_t before(int b) const {
-    if (!grows) return a * b;
-    const int64_t ramp = a >= cap ? 0 : min(static_cast<int64_t>(b), (cap - a + kBlock - 1) / kBlock);
-    return a * ramp + kBlock * (ramp * (ramp - 1) / 2) + (b - ramp) * (b > ramp ? cap : 0);
+    if (step == 0) return a * b;
+    if (cap == kNoLimit) return a * b + step * (static_cast<int64_t>(b) * (b - 1) / 2);
+    const int64_t ramp = a >= cap ? 0 : min(static_cast<int64_t>(b), (cap - a + step - 1) / step);
+    return a * ramp + step * (ramp * (ramp - 1) / 2) + (b - ramp) * cap;
   }
 };
 
@@ -88,9 +95,10 @@ struct Item {
 };
 
 // Walks a CTA's items. Every role of the kernel walks them by itself.
+template <bool kTokens>
 struct Walk {
   Part part;
-  SeqWork w;
+  SeqWork<kTokens> w;
   int s, h, b;
   int64_t at;  // offset of block b of head h in its sequence
 
@@ -158,14 +166,14 @@ struct Walk {
 
 // Finds the calling CTA's part. Called by all `kThreads` threads; `red` is
 // shared scratch of 33 int64. One CTA gets at least about one tile.
-template <int kThreads>
+template <int kThreads, bool kTokens>
 __device__ __forceinline__ void find_part(const AttnArgs& p, int group, int64_t* red, Part* part) {
   constexpr int kWarps = kThreads / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int per = (p.batch.seqs + kThreads - 1) / kThreads;
   const int lo = min(static_cast<int>(threadIdx.x) * per, p.batch.seqs), hi = min(lo + per, p.batch.seqs);
   int64_t mine = 0;
-  SeqWork w;
+  SeqWork<kTokens> w;
   for (int s = lo; s < hi; ++s) {
     w.load(p, group, s);
     mine += w.head * p.hkv;
@@ -186,7 +194,7 @@ __device__ __forceinline__ void find_part(const AttnArgs& p, int group, int64_t*
     total += red[i];
   }
   // Equal parts, none below the weight of one tile (its tokens and its block's constant).
-  const int64_t least = static_cast<int64_t>(kTile) * group;
+  const int64_t least = static_cast<int64_t>((kTokens ? 1 : kNarrowTile) * kTile) * group;
   const int64_t part_weight = max(quotient(total + gridDim.x - 1, gridDim.x), least);
   const int64_t x0 = part_weight * blockIdx.x, x1 = min(x0 + part_weight, total);
   if (x0 < total) {
