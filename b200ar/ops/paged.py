@@ -50,7 +50,11 @@ class PagedBatch:
         q_start: int32 ``[S + 1]``, ascending: rows ``q_start[s]`` to
             ``q_start[s + 1]`` of the call's inputs are the last tokens of
             sequence s. Rows from ``q_start[S]`` on are padding and left
-            alone. None: one new token for each sequence (row s).
+            alone; offsets outside the rows are cut to them. None: one new
+            token for each sequence (row s).
+
+    Sequences may share pages (a common prefix) that no call writes while
+    they do: of two new tokens with one slot, either's k and v may stay.
     """
 
     page_table: torch.Tensor
@@ -108,6 +112,16 @@ def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _shares_memory(t: torch.Tensor) -> bool:
+    """Whether two indices of ``t`` may be one element."""
+    span = 1
+    for stride, n in sorted((s, n) for n, s in zip(t.shape, t.stride()) if n > 1):
+        if stride < span:
+            return True
+        span += (n - 1) * stride
+    return False
+
+
 def qk_norm_rope_paged(qkv: torch.Tensor, batch: PagedBatch, rot: RotaryTable, k_pages: torch.Tensor,
                        v_pages: torch.Tensor, hq: int, hkv: int, q_gamma: Optional[torch.Tensor] = None,
                        k_gamma: Optional[torch.Tensor] = None, eps: float = 1e-5,
@@ -148,8 +162,11 @@ def qk_norm_rope_paged(qkv: torch.Tensor, batch: PagedBatch, rot: RotaryTable, k
     if not in_place and _overlaps(q_out, qkv):
         raise ValueError("q_out overlaps qkv but is not its q part")
     for t, name in ((q_out, "q_out"), (k_pages, "k_pages"), (v_pages, "v_pages")):
-        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
-            raise ValueError(f"{name} is written and must not be expanded")
+        if t.numel() and _shares_memory(t):
+            raise ValueError(f"{name} is written and its rows must not share memory")
+    if k_pages.data_ptr() == v_pages.data_ptr() or any(
+            _overlaps(a, b) for a in (qkv, q_out) for b in (k_pages, v_pages)):
+        raise ValueError("the pools overlap each other, qkv or q_out")
     ref_qk_norm_rope_paged(qkv, batch, rot, k_pages, v_pages, hq, hkv, q_gamma, k_gamma, eps, q_out)
     return q_out
 
@@ -190,8 +207,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         out = torch.empty(rows, hq * d, dtype=q.dtype, device=q.device)
     elif tuple(out.shape) != (rows, hq * d) or out.dtype != q.dtype or out.device != q.device:
         raise ValueError("out must be [rows, hq * d], of the type and on the device of q")
-    if any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride())):
-        raise ValueError("out is written and must not be expanded")
+    if out.numel() and _shares_memory(out):
+        raise ValueError("out is written and its rows must not share memory")
     out3 = out.unflatten(1, (hq, d))
     for t, name in ((q, "q"), (k_pages, "k_pages"), (v_pages, "v_pages")):
         if _overlaps(out3, t):
@@ -204,8 +221,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
 def _rows_of(batch: PagedBatch, rows: int):
     """(sequence, first row, rows, cached tokens) of every sequence."""
     lens = batch.kv_len.tolist()
-    starts = list(range(len(lens) + 1)) if batch.q_start is None else batch.q_start.tolist()
-    return [(s, starts[s], starts[s + 1] - starts[s], lens[s]) for s in range(len(lens))]
+    starts = list(range(len(lens) + 1)) if batch.q_start is None else batch.q_start.clamp(0, rows).tolist()
+    return [(s, starts[s], max(starts[s + 1] - starts[s], 0), lens[s]) for s in range(len(lens))]
 
 
 def _pages_of(batch: PagedBatch, s: int, pos: torch.Tensor, page_size: int, pages: int):

@@ -43,7 +43,7 @@ void check_device(const at::Tensor& t, const at::Tensor& like, const char* name)
 }
 
 // Heads of d contiguous elements on 16-byte boundaries in every dimension before them; `written` ones must not
-// share memory among themselves.
+// share memory among themselves (each stride reaches over what the smaller ones span).
 void check_heads(const at::Tensor& t, const char* name, bool written) {
   bool ok = t.stride(-1) == 1 && aligned(t);
   for (int64_t i = 0; i + 1 < t.dim(); ++i) {
@@ -51,6 +51,19 @@ void check_heads(const at::Tensor& t, const char* name, bool written) {
     VALUE_CHECK(!written || t.size(i) <= 1 || t.stride(i) != 0, name, " is written and must not be expanded");
   }
   VALUE_CHECK(ok, name, " must have contiguous heads that start on 16-byte boundaries");
+  if (!written || t.numel() == 0) return;
+  int64_t span = t.size(-1), below = 0;  // elements that the dimensions with strides up to `below` span
+  for (;;) {
+    int64_t next = 0, at = -1;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i)
+      if (t.size(i) > 1 && t.stride(i) > below && (at < 0 || t.stride(i) < next)) next = t.stride(i), at = i;
+    if (at < 0) return;
+    int64_t same = 0;
+    for (int64_t i = 0; i + 1 < t.dim(); ++i) same += t.size(i) > 1 && t.stride(i) == next;
+    VALUE_CHECK(next >= span && same == 1, name, " is written and its rows must not share memory");
+    span += (t.size(at) - 1) * next;
+    below = next;
+  }
 }
 
 // Whether the address ranges of two tensors meet.
@@ -107,6 +120,7 @@ Batch batch_of(const at::Tensor& table, const at::Tensor& kv_len, const OptTenso
   b.kv_len = kv_len.data_ptr<int>();
   b.table_stride = table.stride(0);
   b.seqs = static_cast<int>(seqs);
+  b.rows = static_cast<int>(rows);
   b.max_pages = static_cast<int>(table.size(1));
   return b;
 }
@@ -157,6 +171,8 @@ void register_serving_ops(py::module& m) {
         a.k = pool_of(k_pages, qkv, k_pages, hkv, d, "k_pages", true);
         a.v = pool_of(v_pages, qkv, k_pages, hkv, d, "v_pages", true);
         check_heads(qkv, "qkv", false);
+        VALUE_CHECK(k_pages.data_ptr() != v_pages.data_ptr(), "k_pages and v_pages are the same memory");
+        VALUE_CHECK(!overlaps(qkv, k_pages) && !overlaps(qkv, v_pages), "qkv overlaps the pools");
         const int64_t rows = qkv.size(0);
         a.batch = batch_of(table, kv_len, q_start, qkv, rows);
         for (const at::Tensor* t : {&cos_t, &sin_t})
@@ -180,6 +196,7 @@ void register_serving_ops(py::module& m) {
           const bool in_place = q.data_ptr() == qkv.data_ptr() && (rows <= 1 || q.stride(0) == qkv.stride(0)) &&
                                 (hq == 1 || q.stride(1) == d);
           VALUE_CHECK(in_place || !overlaps(q, qkv), "q_out overlaps qkv but is not its q part");
+          VALUE_CHECK(!overlaps(q, k_pages) && !overlaps(q, v_pages), "q_out overlaps the pools");
         } else {
           q = at::empty({rows, hq, d}, qkv.options());
         }

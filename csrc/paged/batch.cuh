@@ -9,7 +9,10 @@
 namespace b200ar {
 namespace paged {
 
-__device__ __forceinline__ int q_begin(const Batch& b, int s) { return b.q_start ? __ldg(b.q_start + s) : s; }
+// First row of sequence s. No offset leads outside the inputs, whatever q_start holds.
+__device__ __forceinline__ int q_begin(const Batch& b, int s) {
+  return b.q_start ? min(max(__ldg(b.q_start + s), 0), b.rows) : s;
+}
 
 // Sequence of input row `row` (the last s with q_start[s] <= row), or -1 for a
 // row behind the last sequence. Called by whole warps: each step compares

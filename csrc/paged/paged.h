@@ -29,6 +29,7 @@ struct Batch {
   const int* q_start;     // [S + 1] or null
   int64_t table_stride;
   int seqs, max_pages;
+  int rows;  // of the call's inputs: offsets are cut to them
 };
 
 // K and V pools [num_pages, page_size, kv_heads, d], strides in elements.

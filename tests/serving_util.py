@@ -199,6 +199,13 @@ def _paged_setup(device, dtype=torch.bfloat16, d=64, hq=4, hkv=2, page=16):
             "q": torch.zeros(3, hq, d, dtype=dtype, device=device)}
 
 
+def _lapping(pool):
+    """A pool of the same shape whose pages share half their tokens."""
+    n, page, h, d = pool.shape
+    return torch.zeros(n * page * h * d, dtype=pool.dtype, device=pool.device).as_strided(
+        pool.shape, (page * h * d // 2, h * d, d, 1))
+
+
 def refuse_rope(device):
     """Every call that the rotary step must refuse; the first two it must take."""
     from b200ar.ops.layers import RotaryTable
@@ -222,7 +229,11 @@ def refuse_rope(device):
            dict(q_out=a["qkv"][:, 64:320].view(3, 4, 64)),
            dict(q_out=torch.zeros(1, 4, 64, device=device).bfloat16().expand(3, 4, 64)),
            dict(batch=PagedBatch(a["batch"].page_table, a["batch"].kv_len)),
-           dict(k_pages=a["k_pages"][:1].expand(5, 16, 2, 64), v_pages=a["v_pages"][:1].expand(5, 16, 2, 64))]
+           dict(k_pages=a["k_pages"][:1].expand(5, 16, 2, 64), v_pages=a["v_pages"][:1].expand(5, 16, 2, 64)),
+           dict(v_pages=a["k_pages"]), dict(k_pages=_lapping(a["k_pages"])),
+           dict(q_out=torch.zeros(600, device=device).bfloat16().as_strided((3, 4, 64), (128, 64, 1))),
+           dict(q_out=a["v_pages"].flatten()[:768].view(3, 4, 64)),
+           dict(qkv=a["k_pages"].flatten()[:1536].view(3, 512))]
     for kw in bad:
         with pytest.raises(ValueError):
             call(**kw)
@@ -248,6 +259,7 @@ def refuse_attention(device):
                dict(window=-1), dict(window=4, causal=False), dict(scale=float("nan")),
                dict(out=torch.zeros(3, 255, device=device).bfloat16()), dict(out=torch.zeros(3, 256, device=device)),
                dict(out=a["q"].view(3, 256)), dict(out=torch.zeros(1, 256, device=device).bfloat16().expand(3, 256)),
+               dict(out=torch.zeros(800, device=device).bfloat16().as_strided((3, 256), (128, 1))),
                dict(batch=PagedBatch(a["batch"].page_table, a["batch"].kv_len)),
                dict(k_pages=a["k_pages"][:, :12], v_pages=a["v_pages"][:, :12])):
         with pytest.raises(ValueError):

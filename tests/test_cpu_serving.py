@@ -133,3 +133,14 @@ def test_error_texts():
     finally:
         gemm._ERR.clear()
         gemm._ERR.update(old)
+
+
+def test_offsets_outside_the_rows_are_cut():
+    from b200ar.ops.paged import PagedBatch, paged_attention
+
+    batch, pool = make_batch([2, 3], [40, 70], 16, "cpu")
+    q, k, v = (randn(s, torch.bfloat16, "cpu", i) for i, s in enumerate([(5, 4, 64)] + [(pool, 16, 1, 64)] * 2))
+    want = paged_attention(q, k, v, batch)
+    for starts in ([0, 2, 900], [-7, 2, 5]):
+        cut = PagedBatch(batch.page_table, batch.kv_len, torch.tensor(starts, dtype=torch.int32))
+        assert torch.equal(paged_attention(q, k, v, cut), want)

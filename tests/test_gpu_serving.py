@@ -306,6 +306,24 @@ def test_attention_reports_missing_pages(decode):
     assert torch.equal(out[:new[0]], good[:new[0]])
 
 
+def test_offsets_outside_the_rows_are_cut():
+    """Offsets behind the inputs (or before them) lead to no row that is not there."""
+    from b200ar.ops.layers import RotaryTable
+    from b200ar.ops.paged import PagedBatch, paged_attention, qk_norm_rope_paged
+
+    q, k, v, batch = _attention_inputs([2, 3], [40, 70], 16, 4, 1, 64, BF)
+    qkv, rot = randn((5, 6 * 64), BF, "cuda", 9), RotaryTable(64, 128, 1e4, "cuda")
+    for starts, cut in (([0, 2, 900], [0, 2, 5]), ([0, 2, 2**31 - 1], [0, 2, 5]), ([-7, 2, 5], [0, 2, 5]),
+                        ([0, 2**31 - 1, 2**31 - 1], [0, 5, 5]), ([9, 9, 9], [5, 5, 5])):
+        outs = []
+        for s in (starts, cut):
+            b = PagedBatch(batch.page_table, batch.kv_len, torch.tensor(s, dtype=torch.int32, device="cuda"))
+            kp, vp, out, q_out = k.clone(), v.clone(), torch.full_like(q, 3).flatten(1), torch.full_like(q, 3)
+            qk_norm_rope_paged(qkv, b, rot, kp, vp, 4, 1, q_out=q_out)
+            outs.append((paged_attention(q, k, v, b, out=out), kp, vp, q_out))
+        assert all(torch.equal(x, y) for x, y in zip(*outs))
+
+
 def test_attention_of_nothing():
     from b200ar.ops.paged import PagedBatch, paged_attention
 
