@@ -35,48 +35,78 @@ __device__ __forceinline__ void unpack8<__half>(const uint4& w, float* v) {
     v[2 * i + 1] = f.y;
   }
 }
-// Eight consecutive values as fp32.
+// Eight consecutive values as they are loaded, and the maximum of their absolute values as a bit pattern: fp32, or
+// for the 16-bit types a pair of them, since a max of two 16-bit integers is one instruction.
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, float* v) {
-  unpack8<T>(*reinterpret_cast<const uint4*>(p), v);
-}
-template <>
-__device__ __forceinline__ void load8<float>(const float* p, float* v) {
-  *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p);
-  *reinterpret_cast<float4*>(v + 4) = *reinterpret_cast<const float4*>(p + 4);
-}
-
-__device__ __forceinline__ unsigned abs_max8(const float* v) {
-  unsigned m = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-  return m;
-}
-__device__ __forceinline__ float scale_of(unsigned amax_bits) {
-  return amax_bits == 0u ? 1.f : __fdiv_rn(__uint_as_float(amax_bits), kMax);
-}
-// `inverse` is 1 / scale, or NaN where that is not a normal number.
-__device__ __forceinline__ float inverse_of(float scale) {
-  return scale >= 0x1p-120f ? __frcp_rn(scale) : __uint_as_float(0x7fffffffu);
-}
-__device__ __forceinline__ uint2 encode8(const float* v, float scale, float inverse) {
-  float y[8];
-  bool near = !(inverse == inverse);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    y[i] = v[i] * inverse;
-    const uint32_t u = __float_as_uint(y[i]);
-    // Three bits of the mantissa stay: the middle is a one behind them, then zeros. Zero itself has the code zero.
-    near |= ((u & 0xfffffu) - 0x7fffcu <= 8u) | (fabsf(y[i]) < 0x1p-5f && v[i] != 0.f);
+struct Eight {
+  uint4 w;
+  __device__ __forceinline__ void zero() { w = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void load(const T* p) { w = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ unsigned amax() const {
+    constexpr unsigned kAbs = 0x7fff7fffu;
+    return larger(larger(w.x & kAbs, w.y & kAbs), larger(w.z & kAbs, w.w & kAbs));
   }
-  if (near)
+  static __device__ __forceinline__ unsigned larger(unsigned a, unsigned b) { return __vmaxu2(a, b); }
+  static __device__ __forceinline__ unsigned fp32(unsigned m) {  // the pair's maximum as fp32 bits
+    float v[8];
+    unpack8<T>(make_uint4(max(m & 0xffffu, m >> 16), 0u, 0u, 0u), v);
+    return __float_as_uint(v[0]);
+  }
+  __device__ __forceinline__ void get(float* v) const { unpack8<T>(w, v); }
+};
+template <>
+struct Eight<float> {
+  float4 a, b;
+  __device__ __forceinline__ void zero() { a = b = make_float4(0.f, 0.f, 0.f, 0.f); }
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + 4);
+  }
+  __device__ __forceinline__ unsigned amax() const {
+    float v[8];
+    get(v);
+    unsigned m = 0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = __fdiv_rn(v[i], scale);
-  uint32_t w[4];
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+    return m;
+  }
+  static __device__ __forceinline__ unsigned larger(unsigned x, unsigned y) { return max(x, y); }
+  static __device__ __forceinline__ unsigned fp32(unsigned m) { return m; }
+  __device__ __forceinline__ void get(float* v) const {
+    *reinterpret_cast<float4*>(v) = a;
+    *reinterpret_cast<float4*>(v + 4) = b;
+  }
+};
+
+// A block's scale, and factors just below and above 1 / scale. With inverse = rn(1 / scale), each of the two and their
+// products with a value are off by at most three roundings of 2^-24, less than the 2^-21 they were moved by: so
+// v low <= rn(v / scale) <= v high in magnitude, and where both have one code it is the quotient's.
+struct Scale {
+  float scale, low, high;
+  bool divide;  // 1 / scale may not be a normal number
+  __device__ __forceinline__ explicit Scale(unsigned amax_bits) {
+    scale = amax_bits == 0u ? 1.f : __fdiv_rn(__uint_as_float(amax_bits), kMax);
+    const float inverse = __frcp_rn(scale);
+    low = inverse * (1.f - 0x1p-21f);
+    high = inverse * (1.f + 0x1p-21f);
+    divide = scale < 0x1p-120f;
+  }
+};
+__device__ __forceinline__ uint32_t code2(float a, float b) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+}
+__device__ __forceinline__ uint2 encode8(const float* v, const Scale& s) {
+  uint32_t lo[4], hi[4], differ = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    w[i] = __nv_cvt_float2_to_fp8x2(make_float2(y[2 * i], y[2 * i + 1]), __NV_SATFINITE, __NV_E4M3);
-  return make_uint2(w[0] | (w[1] << 16), w[2] | (w[3] << 16));
+  for (int i = 0; i < 4; ++i) {
+    lo[i] = code2(v[2 * i] * s.low, v[2 * i + 1] * s.low);
+    hi[i] = code2(v[2 * i] * s.high, v[2 * i + 1] * s.high);
+    differ |= lo[i] ^ hi[i];
+  }
+  if (differ != 0u || s.divide)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) lo[i] = code2(__fdiv_rn(v[2 * i], s.scale), __fdiv_rn(v[2 * i + 1], s.scale));
+  return make_uint2(lo[0] | (lo[1] << 16), lo[2] | (lo[3] << 16));
 }
 
 }  // namespace fp8

@@ -11,17 +11,23 @@
 // rows_kernel (few rows of x). The weights' 128 rows are the product's M, the
 //   rows of x (16 to 128) its N, so a product moves each weight once whatever
 //   the number of rows. The K blocks are split over the CTAs of a cluster,
-//   which add their sums through distributed shared memory: no workspace.
+//   which add their sums through distributed shared memory: no workspace. The
+//   weights' first tiles are on their way before the kernel waits for the
+//   quantization of x. Bound by the stream of the weights behind two launches:
+//   1 x 7168 x 8192 takes 14.6 us with the quantization (59 MB, 9.0 us at the
+//   copy rate), 48 x 8192 x 3584 13.0 us (30 MB, 4.7 us).
 // pair_kernel (many rows). CTA pairs (cta_group::2) compute 256 x 256 tiles. A K
 //   block's sums go to one of two buffers in tensor memory, each in two halves
 //   of 128 columns with a warpgroup and barriers of its own: handing a buffer
 //   over and back takes about as long as its products (signals between the CTAs
 //   included), so four half buffers keep more of them in flight than two whole
 //   ones. Scales come by cp.async through shared memory: read straight from
-//   global memory they made every block wait for them. All tiles' K blocks form one line that is cut into equal parts for the pairs,
-//   so no pair idles in a last partial wave. A tile that a cut falls into is
-//   finished by the pair that arrives last, which adds the parts in the order
-//   of K.
+//   global memory they made every block wait for them. All tiles' K blocks form
+//   one line that is cut into equal parts for the pairs, so no pair idles in a
+//   last partial wave. A tile that a cut falls into is finished by the pair that
+//   arrives last, which adds the parts in the order of K. Bound by the way of
+//   every block's sums out of tensor memory: 4093 x 7168 x 8192 takes 310 us with
+//   the quantization, 1550 TFLOP/s.
 //
 // Every wait is bounded: on expiry the error word is set and all roles run
 // down without waiting.

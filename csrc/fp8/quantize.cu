@@ -3,10 +3,9 @@
 //   scale = amax / 448 (1 for a block of zeros),  q = e4m3(x / scale)
 //
 // Both quotients are the correctly rounded fp32 ones, so the codes are those
-// of the formula and not an approximation of it. (A product with 1 / scale is
-// off by less than 2 units in the last place, so it has the same code unless
-// it is that near to the middle between two e4m3 numbers; only then, and for
-// subnormal codes and scales, the division is made.) The maximum is taken over the
+// of the formula and not an approximation of it. (The products with a number
+// just below and one just above 1 / scale enclose the quotient: only where their
+// codes differ the division is made.) The maximum is taken over the
 // bit patterns of |x|, in which NaN is above infinity: a block that holds a
 // NaN gets the scale NaN, one that holds an infinity the scale infinity, and
 // either reaches the outputs of its row.
@@ -34,7 +33,7 @@ __global__ void __launch_bounds__(kThreads)
   const int lane = threadIdx.x & 15;
   const int b = blockIdx.y * (kThreads / 16) + (threadIdx.x >> 4);
   const int k = b * kBlock + lane * 8;
-  float v[kRows][8];
+  Eight<T> v[kRows];
   pdl_wait();
   pdl_trigger();
   for (int64_t i = (static_cast<int64_t>(blockIdx.x) * gridDim.y + blockIdx.y) * kThreads + threadIdx.x; i < zeros;
@@ -42,19 +41,20 @@ __global__ void __launch_bounds__(kThreads)
     zero[i] = 0u;
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[r][e] = 0.f;
-    if (k < K && m0 + r < M) load8<T>(x + (m0 + r) * ldx + k, v[r]);
+    v[r].zero();
+    if (k < K && m0 + r < M) v[r].load(x + (m0 + r) * ldx + k);
   }
 #pragma unroll
   for (int r = 0; r < kRows; ++r) {
-    unsigned amax = abs_max8(v[r]);
+    unsigned amax = v[r].amax();
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-    const float s = scale_of(amax);
+    for (int o = 8; o > 0; o >>= 1) amax = Eight<T>::larger(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     if (k >= K || m0 + r >= M) continue;
-    *reinterpret_cast<uint2*>(q + (m0 + r) * K + k) = encode8(v[r], s, inverse_of(s));
-    if (lane == 0) scale[b * lds + m0 + r] = s;
+    const Scale s(Eight<T>::fp32(amax));
+    float f[8];
+    v[r].get(f);
+    *reinterpret_cast<uint2*>(q + (m0 + r) * K + k) = encode8(f, s);
+    if (lane == 0) scale[b * lds + m0 + r] = s.scale;
   }
 }
 
@@ -67,31 +67,33 @@ __global__ void __launch_bounds__(kThreads)
   const int lane = threadIdx.x & 15, r0 = threadIdx.x >> 4;
   const int k = blockIdx.x * kBlock + lane * 8;
   const int64_t n0 = static_cast<int64_t>(blockIdx.y) * kBlock;
-  float v[8][8];
+  Eight<T> v[8];
   unsigned amax = 0;
   pdl_wait();
   pdl_trigger();
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t n = n0 + r0 + 16 * i;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-    if (n < N && k < K) load8<T>(w + n * ldw + k, v[i]);
-    amax = max(amax, abs_max8(v[i]));
+    v[i].zero();
+    if (n < N && k < K) v[i].load(w + n * ldw + k);
+    amax = Eight<T>::larger(amax, v[i].amax());
   }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = max(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  for (int o = 16; o > 0; o >>= 1) amax = Eight<T>::larger(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = amax;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < kThreads / 32; ++i) amax = max(amax, part[i]);
-  const float s = scale_of(amax), inverse = inverse_of(s);
+  for (int i = 0; i < kThreads / 32; ++i) amax = Eight<T>::larger(amax, part[i]);
+  const Scale s(Eight<T>::fp32(amax));
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int64_t n = n0 + r0 + 16 * i;
-    if (n < N && k < K) *reinterpret_cast<uint2*>(q + n * K + k) = encode8(v[i], s, inverse);
+    if (n >= N || k >= K) continue;
+    float f[8];
+    v[i].get(f);
+    *reinterpret_cast<uint2*>(q + n * K + k) = encode8(f, s);
   }
-  if (threadIdx.x == 0) scale[blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x] = s;
+  if (threadIdx.x == 0) scale[blockIdx.y * static_cast<int64_t>(gridDim.x) + blockIdx.x] = s.scale;
 }
 
 template <typename T>
