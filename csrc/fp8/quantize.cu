@@ -10,7 +10,10 @@
 // NaN gets the scale NaN, one that holds an infinity the scale infinity, and
 // either reaches the outputs of its row.
 //
-// Memory bounds both kernels: 3 bytes a value move.
+// Each value is read once and its code written once, 3 bytes: 4096 x 8192 values
+// take 33 us (100 MB, 15 us at the copy rate) and a weight of 7168 x 8192 45 us;
+// the two conversions of each value and the scales' divisions share the rest.
+// (With a test of every product for the middle between two codes: 51 and 76 us.)
 #include "../common/check.h"
 #include "../common/pdl.h"
 #include "../common/trace.h"
