@@ -324,6 +324,23 @@ def test_offsets_outside_the_rows_are_cut():
         assert all(torch.equal(x, y) for x, y in zip(*outs))
 
 
+@pytest.mark.parametrize("decode", [True, False])
+def test_many_sequences(decode):
+    """More sequences than a block of the schedule has threads, and than two searches of 32 cover."""
+    from b200ar.ops.layers import RotaryTable
+    from b200ar.ops.paged import paged_attention, qk_norm_rope_paged
+
+    new = [1 if decode else (5 * i) % 3 for i in range(1500)]
+    total = [n + (7 * i) % 50 for i, n in enumerate(new)]
+    q, k, v, batch = _attention_inputs(new, total, 8, 4, 1, 64, BF, decode=decode)
+    check_attention(paged_attention(q, k, v, batch), q, k, v, batch)
+    qkv, rot = randn((sum(new), 6 * 64), BF, "cuda", 7), RotaryTable(64, 64, 1e4, "cuda")
+    out = torch.zeros_like(q)
+    want = plain_rope(qkv, batch, 1e4, 64, (k, v), 4, 1, None, None)
+    qk_norm_rope_paged(qkv, batch, rot, k, v, 4, 1, q_out=out)
+    check_rope(out, k, v, want, torch.zeros_like(q))
+
+
 def test_attention_of_nothing():
     from b200ar.ops.paged import PagedBatch, paged_attention
 
