@@ -499,6 +499,38 @@ def test_linear_fp8_long_sums():
         check_linear(linear_fp8(x, w_q, w_s), *quantize_fp8(x), w_q, w_s)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("order", ["sorted", "mixed", "exact"])
+def test_quantize_fp8_every_value(dtype, order):
+    """All finite 16-bit values: codes are those of the rounded quotient, ties between two codes included."""
+    from b200ar.ops.fp8 import quantize_fp8, quantize_fp8_weight
+
+    x = torch.arange(65536, dtype=torch.int32).to(torch.int16).view(dtype)
+    x = x[torch.isfinite(x)]
+    if order == "mixed":
+        x = x[torch.randperm(x.numel(), generator=torch.Generator().manual_seed(1))]
+    elif order == "exact":  # a largest value of 448: the scale is 1, and the values themselves lie on the middles
+        x = x[x.abs() <= 448]
+        x = x[: x.numel() // 127 * 127].view(-1, 127)
+        x = torch.cat([x, torch.full((x.shape[0], 1), 448.0, dtype=dtype)], 1).flatten()
+    x = x[: x.numel() // 512 * 512].view(-1, 512)
+    blocks = x.float().view(x.shape[0], 4, 128)
+    top = blocks.abs().amax(-1)
+    scale = torch.where(top > 0, top / 448.0, torch.ones_like(top))
+    want = (blocks / scale[..., None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(x.shape)
+    codes, got = quantize_fp8(x.cuda())
+    assert torch.equal(got.cpu(), scale)
+    assert torch.equal(codes.cpu().float(), want.float())
+    n = x.shape[0] // 128 * 128
+    tiles = x[:n].float().view(-1, 128, 4, 128)
+    top = tiles.abs().amax((1, 3))
+    scale = torch.where(top > 0, top / 448.0, torch.ones_like(top))
+    want = (tiles / scale[:, None, :, None]).clamp(-448, 448).to(torch.float8_e4m3fn).view(n, 512)
+    codes, got = quantize_fp8_weight(x[:n].cuda())
+    assert torch.equal(got.cpu(), scale)
+    assert torch.equal(codes.cpu().float(), want.float())
+
+
 @pytest.mark.parametrize("m", [3, 40, 200])
 def test_linear_fp8_scales_of_all_sizes(m):
     """Blocks whose scales span many orders, zero blocks, and the extremes of the types."""
