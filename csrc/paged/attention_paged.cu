@@ -77,6 +77,12 @@ namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
 
+// 1 / l for a row's sum of weights. A sum of zero is a row that sees nothing, whose output is zero (the factor 0
+// stands for that), or one whose scores are all -inf: NaN, as exp(-inf - max) is.
+__device__ __forceinline__ float inverse(float l, bool sees) {
+  return l != 0.f ? 1.f / l : (sees ? __int_as_float(0x7fffffff) : 0.f);
+}
+
 // ------------------------------------------------------------------ one row
 // One row by one warp, position by position. Every position that the row does
 // not see is left unread.
@@ -122,7 +128,7 @@ __device__ __noinline__ void attention_row(const AttnArgs& a, int s, int row, in
       o[i].y = o[i].y * f + e * v.y;
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = inverse(l, end > begin);
   T* op = static_cast<T*>(a.out) + row * a.o_tok + h * a.o_head;
 #pragma unroll
   for (int i = 0; i < kPairs; ++i)
@@ -182,7 +188,7 @@ struct Misc {
   uint32_t tmem;
   int err;
   unsigned bad;      // rows of a 32-row block that came out as NaN
-  float sum[32];     // sums of P of such a block's rows
+  float inv[32];     // factors of such a block's rows (inverse())
   int last[2][8];    // last load of K and of V into each slot of the ring, or -1
 };
 static_assert(sizeof(Misc) <= 1280, "miscellaneous shared memory");
@@ -766,7 +772,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // Rows computed by one thread each: 128 of a wide block by each group, or a narrow block's by group 0, which
       // adds the state of group 1: the same rows in the same lanes of tensor memory.
       auto finish_rows = [&](float mj, float lj, float f0, float f1, bool add) {
-        const float inv = lj == 0.f ? 0.f : 1.f / lj;
+        const float inv = inverse(lj, valid && hi > max(lo, 0));
         float odd = 0.f;
 #pragma unroll 1
         for (int c = 0; c < D; c += 32) {
@@ -825,7 +831,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         f0 = factor(sml[w4 * 32 + lane].x, mj);
         f1 = two ? factor(sml[(4 + w4) * 32 + lane].x, mj) : 0.f;
         if (warp == 0) {
-          misc.sum[lane] = lj;
+          misc.inv[lane] = inverse(lj, valid && hi > max(lo, 0));
           if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
         }
         sm100::tc_fence_after();
@@ -865,7 +871,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               y = make_float4(y.x + v.x, y.y + v.y, y.z + v.z, y.w + v.w);
             }
             if (whole) {
-              const float lr = misc.sum[r2], inv = lr == 0.f ? 0.f : 1.f / lr;
+              const float inv = misc.inv[r2];
               if (inv == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
               y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
               if ((y.x + y.y + y.z + y.w) * 0.f != 0.f) atomicOr(&misc.bad, 1u << r2);
@@ -985,14 +991,16 @@ __global__ void __launch_bounds__(D * 2)
 #pragma unroll
     for (int e = 0; e < 16; ++e) o[e] = o[e] * f0 + __shfl_xor_sync(0xffffffffu, o[e], w) * f1;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int x = first.b * kBlock + rc, tok = x / group, h = first.h * group + x % group;
+  const int cnt = q_begin(a.batch, first.s + 1) - first.q0, len = __ldg(a.batch.kv_len + first.s);
+  // Of the positions before the row's own some are in every window.
+  const float inv = inverse(l, a.causal ? len - cnt + tok >= 0 : len > 0);
   float odd = 0.f;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     o[e] = inv == 0.f ? 0.f : o[e] * inv;
     odd += o[e] * 0.f;
   }
-  const int x = first.b * kBlock + rc, tok = x / group, h = first.h * group + x % group;
   const bool valid = r < first.rows && lane < width;
   if (valid) {
     uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (first.q0 + tok) * a.o_tok + h * a.o_head + warp * 16);
@@ -1005,7 +1013,6 @@ __global__ void __launch_bounds__(D * 2)
   __syncthreads();
   const unsigned redo = odd_rows;
   if (!redo) return;
-  const int cnt = q_begin(a.batch, first.s + 1) - first.q0, len = __ldg(a.batch.kv_len + first.s);
   for (int i = warp; i < 32; i += D / 16) {
     if (!(redo >> i & 1u)) continue;
     const int y = first.b * kBlock + blockIdx.y * 32 + i;

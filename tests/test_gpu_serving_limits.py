@@ -1,0 +1,71 @@
+"""Serving operators at the limits of their types: scores and values that are
+infinite or NaN, and scales near the ends of fp32."""
+
+import pytest
+import torch
+
+from serving_util import make_batch, randn
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():
+    pytest.skip("needs a GPU", allow_module_level=True)
+
+BF, HF = torch.bfloat16, torch.float16
+NAN, INF = float("nan"), float("inf")
+
+
+@pytest.fixture(autouse=True)
+def _no_reported_errors():
+    yield
+    from b200ar.ops.gemm import check_errors
+
+    torch.cuda.synchronize()
+    check_errors()
+
+
+# Blocks of up to 32, 128 and 256 rows, single tokens, and blocks that several SMs share.
+# new, total, decode
+BLOCKS = [([1], [1], True), ([1, 1], [300, 40], True), ([1], [6000], True), ([4, 1], [300, 40], False),
+          ([16], [300], False), ([32, 9], [300, 200], False), ([40], [6000], False)]
+PAGE = 16
+
+
+def _inputs(new, total, decode, dtype, d, hq=8, hkv=1):
+    batch, pool = make_batch(new, total, PAGE, "cuda", decode=decode)
+    q = randn((sum(new), hq, d), dtype, "cuda", 1)
+    k, v = (randn((pool, PAGE, hkv, d), dtype, "cuda", i) for i in (2, 3))
+    return q, k, v, batch
+
+
+def _slot(batch, s, p):
+    return int(batch.page_table[s, p // PAGE]), p % PAGE
+
+
+@pytest.mark.parametrize("new,total,decode", BLOCKS)
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64)])
+def test_attention_rows_that_see_only_minus_infinity(new, total, decode, dtype, d):
+    """exp(-inf - max) with a maximum of -inf is NaN; a row that sees nothing gives zeros."""
+    from b200ar.ops.paged import paged_attention
+
+    q, k, v, batch = _inputs(new, total, decode, dtype, d)
+    q.abs_().clamp_(min=0.01)
+    k.fill_(-INF)
+    assert torch.isnan(paged_attention(q, k, v, batch)).all()
+    # One finite score, seen by the last token of the first sequence alone: all the weight is its.
+    p = total[0] - 1
+    pg, slot = _slot(batch, 0, p)
+    k[pg, slot] = 1.0
+    out = paged_attention(q, k, v, batch).view(-1, 8, d)
+    assert torch.equal(out[new[0] - 1], v[pg, slot].expand(8, d))
+    rest = torch.arange(out.shape[0]) != new[0] - 1
+    assert torch.isnan(out[rest]).all()
+    if not decode:  # lengths below the number of new tokens: rows before position 0 see nothing
+        batch.kv_len.fill_(2)
+        k.fill_(-INF)
+        out = paged_attention(q, k, v, batch).view(-1, 8, d)
+        at = 0
+        for n in new:
+            nothing = max(n - 2, 0)
+            assert (out[at:at + nothing] == 0).all() and torch.isnan(out[at + nothing:at + n]).all()
+            at += n
