@@ -118,7 +118,7 @@ __device__ __noinline__ void attention_row(const AttnArgs& a, int s, int row, in
     const float x = dot * a.scale * kLog2e;
     const float mn = fmaxf(m, x);
     const float f = m == -INFINITY ? 0.f : exp2f(m - mn);
-    const float e = mn == -INFINITY ? 0.f : exp2f(x - mn);
+    const float e = mn == -INFINITY && x == x ? 0.f : exp2f(x - mn);  // NaN if x is: the maximum passes it over
     m = mn;
     l = l * f + e;
 #pragma unroll

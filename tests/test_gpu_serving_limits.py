@@ -69,3 +69,22 @@ def test_attention_rows_that_see_only_minus_infinity(new, total, decode, dtype, 
             nothing = max(n - 2, 0)
             assert (out[at:at + nothing] == 0).all() and torch.isnan(out[at + nothing:at + n]).all()
             at += n
+
+
+@pytest.mark.parametrize("new,total,decode", BLOCKS)
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64)])
+def test_attention_rows_that_see_a_score_of_nan(new, total, decode, dtype, d):
+    """Wherever it stands, the first position included: all outputs of the row are NaN, and of no other."""
+    from b200ar.ops.paged import paged_attention
+
+    q, k, v, batch = _inputs(new, total, decode, dtype, d)
+    clean = paged_attention(q, k, v, batch)
+    for p in (0, total[0] // 2, total[0] - 1):
+        pg, slot = _slot(batch, 0, p)
+        old = k[pg, slot].clone()
+        k[pg, slot, 0, 3] = NAN
+        out = paged_attention(q, k, v, batch)
+        k[pg, slot] = old
+        sees = torch.zeros(out.shape[0], dtype=torch.bool)
+        sees[:new[0]] = torch.arange(total[0] - new[0], total[0]) >= p
+        assert torch.isnan(out[sees]).all() and torch.equal(out[~sees], clean[~sees])
