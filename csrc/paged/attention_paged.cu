@@ -850,9 +850,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              // A state that saw nothing holds zeros times whatever V holds.
-              y[e] = f0 == 0.f ? 0.f : __uint_as_float(o0[e]) * f0;
-              if (two && f1 != 0.f) y[e] += __uint_as_float(o1[e]) * f1;
+              // A factor of 0 drops no infinity: where a state holds one, seen or not, the row is computed again.
+              y[e] = __uint_as_float(o0[e]) * f0;
+              if (two) y[e] += __uint_as_float(o1[e]) * f1;
             }
             if (valid) {
               float4* dst = reinterpret_cast<float4*>(part + (w4 * it.rows + r) * pass);
@@ -975,12 +975,10 @@ __global__ void __launch_bounds__(D * 2)
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float4 x = __ldcg(src + static_cast<int64_t>(e) * ws.row_cap);
-      if (f != 0.f) {  // a part that saw nothing has no numbers, or zeros times whatever V holds
-        o[4 * e] += x.x * f;
-        o[4 * e + 1] += x.y * f;
-        o[4 * e + 2] += x.z * f;
-        o[4 * e + 3] += x.w * f;
-      }
+      o[4 * e] += x.x * f;  // a factor of 0 drops no infinity
+      o[4 * e + 1] += x.y * f;
+      o[4 * e + 2] += x.z * f;
+      o[4 * e + 3] += x.w * f;
     }
   }
   for (int w = width; w < 32; w *= 2) {

@@ -88,3 +88,28 @@ def test_attention_rows_that_see_a_score_of_nan(new, total, decode, dtype, d):
         sees = torch.zeros(out.shape[0], dtype=torch.bool)
         sees[:new[0]] = torch.arange(total[0] - new[0], total[0]) >= p
         assert torch.isnan(out[sees]).all() and torch.equal(out[~sees], clean[~sees])
+
+
+@pytest.mark.parametrize("new,total,decode", [([1], [300], True), ([1], [6000], True), ([4], [300], False),
+                                              ([16], [300], False), ([40], [6000], False)])
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64)])
+def test_attention_infinite_value_under_a_vanishing_weight(new, total, decode, dtype, d):
+    """An infinite value where a whole part of the positions weighs e^-181 of the rest (nothing in fp32): its column
+    is not finite, the others are what they were."""
+    from b200ar.ops.paged import paged_attention
+
+    q, k, v, batch = _inputs(new, total, decode, dtype, d)
+    q.fill_(4.0 * (128 / d) ** 0.25)
+    k.zero_()
+    low = range(128, 256) if total[0] == 300 else range(3000)
+    for p in low:
+        k[_slot(batch, 0, p)] = -4.0 * (128 / d) ** 0.25  # -16 d sqrt(128 / d) / sqrt(d) = -181 after the scale
+    clean = paged_attention(q, k, v, batch).view(-1, 8, d)
+    pg, slot = _slot(batch, 0, 130)
+    v[pg, slot, 0, 7] = INF
+    out = paged_attention(q, k, v, batch).view(-1, 8, d)
+    assert not torch.isfinite(out[:, :, 7]).any()
+    out[:, :, 7] = clean[:, :, 7]
+    # Recomputed rows round elsewhere: both are within u A + u |o| of the formula, A the mean of |v|, at most 4.
+    u = torch.finfo(dtype).eps / 2
+    assert (out.float() - clean.float()).abs().max() <= 2 * u * (4 + clean.float().abs().max())
