@@ -180,7 +180,9 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
     Row i of the n new rows of a sequence stands at position
     ``kv_len - n + i`` and sees the positions up to its own, with ``window``
     only the last ``window`` of them; with ``causal=False`` all ``kv_len``.
-    A row that sees nothing gets zeros. ``scale`` defaults to 1 / sqrt(d).
+    A row that sees nothing gets zeros, one whose scores are all -inf or hold
+    a NaN gets NaN. Where a row sees infinities or NaN in v, its columns there
+    are their sum, whatever their weights. ``scale`` defaults to 1 / sqrt(d).
     Nothing behind a sequence's length, and nothing that a row's mask hides,
     reaches its output, whatever the pages hold there.
     """
@@ -281,10 +283,10 @@ def ref_paged_attention(q, k_pages, v_pages, batch, scale, causal, window, out) 
         w = torch.where(see[None], torch.exp(w - top), 0.0)
         norm = w.sum(-1, keepdim=True)
         w = w / torch.where(norm == 0, torch.ones_like(norm), norm)
-        # A weight of zero times an infinity that only other rows see would be NaN: add it where it is seen.
+        # A weight of zero times an infinity that only other rows see would be NaN: add it where it is seen, and as it
+        # is, since no weight is zero in the formula.
         bad = ~torch.isfinite(v)
         o = torch.einsum("hnc,chd->nhd", w, torch.where(bad, 0.0, v))
         for c in bad.flatten(1).any(1).nonzero().flatten().tolist():
-            hit = (w[:, :, c].t()[:, :, None] * v[c][None])
-            o = o + torch.where(see[:, c][:, None, None] & bad[c][None], hit, 0.0)
+            o = o + torch.where(see[:, c][:, None, None] & bad[c][None], v[c][None], 0.0)
         out[first:first + n] = o.to(out.dtype)

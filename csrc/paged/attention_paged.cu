@@ -16,7 +16,7 @@
 //                   O_t in tensor memory; a thread owns one row
 //   warps 8, 11     TMA producers of K and of V
 //   warp 9          TMEM allocation and MMA issue (one thread)
-//   warp 10         walks the CTA's items and hands them to the others
+//   warp 10         walks the CTA's items and hands them to the others; clears positions of V (see below)
 //
 // Steps alternate between the two groups, so that one's products run during
 // the other's softmax. What the groups work on depends on the block's rows:
@@ -37,8 +37,9 @@
 // columns takes the tensor core nearly as long as of 128. With heads of 64: 764
 // and 714 us.) O is rescaled only when the row's maximum has grown by 2^8 or more
 // over the bound m in use (2^6 for fp16, whose P has a factor 2^8 to keep small
-// weights out of the subnormals), after the product before is done: P stays in
-// the type's range, and numerator and denominator have the same factor.
+// weights out of the subnormals; bf16's has 2^-8, so that P is at most 1), after
+// the product before is done: P stays in the type's range, and numerator and
+// denominator have the same factor.
 //
 // What bounds it: with many rows the softmax, whose exponentials alone (8 clocks
 // for a warp's 32) take the time of both products, next to the conversions and
@@ -48,13 +49,16 @@
 //
 // Pages are read by TMA boxes of the largest power of two of tokens (8 to
 // 128) that divides the page size. Runs that no row sees are not looked up:
-// their boxes lie outside the pool and read as zeros. The tokens behind a
-// sequence in its last page, and those before the window in its first, hold
-// anything; they are masked in S and zeroed in V, where a zero weight does not
-// hide a NaN. A position that some rows of a
-// tile see and others do not may also hold an infinity or NaN: the rows that
-// come out as NaN are computed again one by one (attention_row), which touches
-// only what they see.
+// their boxes lie outside the pool and read as zeros. What a row must not see is
+// masked in S; in V, where a zero weight does not hide a NaN,
+//   - positions that no row of the block sees (behind the last row's, before the first row's window) become zeros;
+//   - of those that some rows see and others do not (at most 255 at either end of the block's range, in its first
+//     and last tiles) the infinities and NaN become zeros, and their outputs are settled at the end, row by row;
+//   - what all rows see stays, so it reaches only rows that it belongs to.
+// A row with a NaN score is NaN. Other outputs that are not finite, and rows of a block whose V had to be cleared,
+// follow from the values of V alone: a column is inf, -inf or NaN as the sum of what the row sees in it that is not
+// finite (settle, settle_columns). That reads V once more for each warp with such rows, whatever their number: one NaN
+// that 256 tokens over 4096 with 8 heads of 128 see makes 0.14 ms of 0.06. (Rows computed again one by one took 13.)
 //
 // Every wait is bounded: on expiry the error word is set and all roles run
 // down without waiting.
@@ -83,63 +87,94 @@ __device__ __forceinline__ float inverse(float l, bool sees) {
   return l != 0.f ? 1.f / l : (sees ? __int_as_float(0x7fffffff) : 0.f);
 }
 
-// ------------------------------------------------------------------ one row
-// One row by one warp, position by position. Every position that the row does
-// not see is left unread.
+// ------------------------------------------------------------------ infinities and NaN
+// A pair of 16-bit values without the ones that are not finite.
+template <typename T>
+__device__ __forceinline__ uint32_t finite2(uint32_t w) {
+  constexpr uint32_t kExp = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  return w & ~__vcmpeq2(w & kExp, kExp);
+}
+
+// The largest absolute values of both halves, as bit patterns.
+__device__ __forceinline__ uint32_t largest2(const uint4& w) {
+  constexpr uint32_t kAbs = 0x7fff7fffu;
+  return __vmaxu2(__vmaxu2(w.x & kAbs, w.y & kAbs), __vmaxu2(w.z & kAbs, w.w & kAbs));
+}
+
+// Settles the columns that are not finite in rows whose weights are numbers (bits of `rows`, from row `first` of the
+// block on; the calling warp sees their stored outputs). Every weight counts as positive, as in the formula: a column
+// in which a row sees +inf, -inf or both, or a NaN, is that, -that or NaN. `all`: look at what every row sees, too;
+// `some`: at what not every row sees.
 template <typename T, int D>
-__device__ __noinline__ void attention_row(const AttnArgs& a, int s, int row, int pos, int len, int h, int kh) {
-  constexpr int kPairs = D / 64;  // pairs of elements that a lane holds
+__device__ __noinline__ void settle(const AttnArgs& a, const Item& it, int group, int first, unsigned rows, bool all,
+                                    bool some) {
+  constexpr int kPairs = D / 64;  // pairs of columns that a lane looks at
+  constexpr unsigned kPlus = 1, kMinus = 2, kNan = 4;
   const int lane = threadIdx.x & 31;
-  const int end = a.causal ? pos + 1 : len;
-  const int begin = a.window > 0 ? max(0, pos - a.window + 1) : 0;
-  float2 q[kPairs], o[kPairs];
-  const T* qp = static_cast<const T*>(a.q) + row * a.q_tok + h * a.q_head;
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i) {
-    q[i] = to_float2<T>(*reinterpret_cast<const uint32_t*>(qp + i * 64 + lane * 2));
-    o[i] = make_float2(0.f, 0.f);
-  }
-  float m = -INFINITY, l = 0.f;
+  // Which of the three appear in this lane's columns at positions [from, to): three bits for each column.
+  auto scan = [&](int from, int to) {
+    unsigned seen = 0;
 #pragma unroll 1
-  for (int p = begin; p < end; ++p) {
-    const int page = page_of(a.batch, s, p / a.page_size, a.num_pages);
-    if (page < 0) continue;  // reported by the producer
-    const int slot = p % a.page_size;
-    const T* kp = static_cast<const T*>(a.k.base) + page * a.k.page + slot * a.k.tok + kh * a.k.head;
-    const T* vp = static_cast<const T*>(a.v.base) + page * a.v.page + slot * a.v.tok + kh * a.v.head;
-    float dot = 0.f;
+    for (int p = from; p < to;) {
+      const int index = p / a.page_size, page = page_of(a.batch, it.s, index, a.num_pages);
+      const int stop = min(to, (index + 1) * a.page_size);
+      if (page >= 0) {
+        const T* vp = static_cast<const T*>(a.v.base) + page * a.v.page + it.h * a.v.head + lane * 2;
+#pragma unroll 1
+        for (; p < stop; p += 8) {  // eight positions under way
+          uint32_t w[8][kPairs];
 #pragma unroll
-    for (int i = 0; i < kPairs; ++i) {
-      const float2 k = to_float2<T>(*reinterpret_cast<const uint32_t*>(kp + i * 64 + lane * 2));
-      dot += q[i].x * k.x + q[i].y * k.y;
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i)
+              w[e][i] = p + e < stop ? *reinterpret_cast<const uint32_t*>(vp + (p + e - index * a.page_size) * a.v.tok +
+                                                                          i * 64)
+                                     : 0u;
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+#pragma unroll
+            for (int i = 0; i < kPairs; ++i)
+              if (finite2<T>(w[e][i]) != w[e][i]) {
+                const float2 v = to_float2<T>(w[e][i]);
+                seen |= (v.x != v.x ? kNan : v.x == INFINITY ? kPlus : v.x == -INFINITY ? kMinus : 0u) << (6 * i);
+                seen |= (v.y != v.y ? kNan : v.y == INFINITY ? kPlus : v.y == -INFINITY ? kMinus : 0u) << (6 * i + 3);
+              }
+        }
+      }
+      p = stop;
     }
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) dot += __shfl_xor_sync(0xffffffffu, dot, d);
-    const float x = dot * a.scale * kLog2e;
-    const float mn = fmaxf(m, x);
-    const float f = m == -INFINITY ? 0.f : exp2f(m - mn);
-    const float e = mn == -INFINITY && x == x ? 0.f : exp2f(x - mn);  // NaN if x is: the maximum passes it over
-    m = mn;
-    l = l * f + e;
+    return seen;
+  };
+  const bool common = it.see0 < it.hide0;
+  const unsigned every = all && common ? scan(it.see0, it.hide0) : 0u;
+#pragma unroll 1
+  for (; rows; rows &= rows - 1) {
+    const int x = it.row0 + first + __ffs(rows) - 1, tok = x / group, pos = it.len - it.n + tok;
+    unsigned seen = every;
+    if (some) {
+      const int lo = a.window > 0 ? max(it.begin, pos - a.window + 1) : it.begin, hi = a.causal ? pos + 1 : it.end;
+      seen |= scan(lo, min(hi, common ? it.see0 : it.end));
+      if (common) seen |= scan(it.hide0, min(hi, it.end));
+    }
+    T* out = static_cast<T*>(a.out) + (it.q0 + tok) * a.o_tok + (it.h * group + x % group) * a.o_head + lane * 2;
 #pragma unroll
     for (int i = 0; i < kPairs; ++i) {
-      const float2 v = to_float2<T>(*reinterpret_cast<const uint32_t*>(vp + i * 64 + lane * 2));
-      o[i].x = o[i].x * f + e * v.x;
-      o[i].y = o[i].y * f + e * v.y;
+      auto value = [&](unsigned bits, float old) {
+        return bits == 0 ? old : bits == kPlus ? INFINITY : bits == kMinus ? -INFINITY : __int_as_float(0x7fffffff);
+      };
+      uint32_t* at = reinterpret_cast<uint32_t*>(out + i * 64);
+      const float2 old = to_float2<T>(*reinterpret_cast<volatile uint32_t*>(at));
+      if (seen >> (6 * i) & 63u) *at = pack2<T>(value(seen >> (6 * i) & 7u, old.x), value(seen >> (6 * i + 3) & 7u, old.y));
     }
   }
-  const float inv = inverse(l, end > begin);
-  T* op = static_cast<T*>(a.out) + row * a.o_tok + h * a.o_head;
-#pragma unroll
-  for (int i = 0; i < kPairs; ++i)
-    *reinterpret_cast<uint32_t*>(op + i * 64 + lane * 2) = pack2<T>(o[i].x * inv, o[i].y * inv);
 }
 
 // ------------------------------------------------------------------ workspace
 // CTA c leaves at most two parts of blocks that others work on too: its first
 // and its last item (slots 2 c and 2 c + 1).
 struct PartDesc {
-  int s, h, b, rows;
+  int s, h, b;
+  short rows, cleared;    // cleared: of the item
   int t0, t1, tiles, q0;  // q0 < 0: not used
 };
 
@@ -161,7 +196,7 @@ struct Cfg {
   static constexpr uint32_t kQ = 0;                         // two tiles of queries
   static constexpr uint32_t kRing = 2 * kTileBytes;
   static constexpr uint32_t kMisc = kRing + kSlots * kTileBytes;
-  static constexpr size_t kSmem = 1024 + kMisc + 1280;
+  static constexpr size_t kSmem = 1024 + kMisc + 1536;
 };
 
 constexpr int kThreads = 384;
@@ -177,6 +212,7 @@ struct Barriers {
   uint64_t ofull[2];           // the last one in a block
   uint64_t gsync, gfree;       // the eight softmax warps: states written; their memory read
   uint64_t ifull[4], iempty[4];  // ring of items
+  uint64_t vcut[8], vclear[8];   // ring slots: V with positions to clear is on its way; is cleared
   uint64_t drained;
 };
 constexpr int kItems = 4;
@@ -187,11 +223,11 @@ struct Misc {
   Part part;
   uint32_t tmem;
   int err;
-  unsigned bad;      // rows of a 32-row block that came out as NaN
+  unsigned bad;      // rows of a 32-row block with outputs that are not finite, but for those of NaN weights
   float inv[32];     // factors of such a block's rows (inverse())
   int last[2][8];    // last load of K and of V into each slot of the ring, or -1
 };
-static_assert(sizeof(Misc) <= 1280, "miscellaneous shared memory");
+static_assert(sizeof(Misc) <= 1536, "miscellaneous shared memory");
 
 // exp2 of the arguments that a softmax makes: 0 below the normal numbers.
 __device__ __forceinline__ float fast_exp2(float x) {
@@ -225,13 +261,14 @@ template <typename T>
 struct Weights;
 template <>
 struct Weights<__nv_bfloat16> {
-  static constexpr float kBias = 0.f, kSlack = 8.f;
-  static constexpr uint32_t kFormat = 1;
+  // No weight above 1: sums of weights times large values stay in range where those with the row's maximum do.
+  static constexpr float kBias = -8.f, kSlack = 8.f;
+  static constexpr uint32_t kFormat = 1, kInf = 0x7f80u;
 };
 template <>
 struct Weights<__half> {
   static constexpr float kBias = 8.f, kSlack = 6.f;
-  static constexpr uint32_t kFormat = 0;
+  static constexpr uint32_t kFormat = 0, kInf = 0x7c00u;
 };
 
 // Products with shared-memory descriptors given by their low words: the high word of a layout is a constant, and
@@ -281,6 +318,42 @@ struct Steps {
   __device__ __forceinline__ int v_at(int j) const { return wide ? 2 * j + 1 : (j + 1 < nt ? 2 * j + 2 : 2 * nt - 1); }
 };
 
+// Clears the tile of V from position c0 on, by one warp: zeros where no row of the block sees the position, and in
+// place of what is not finite where only some do, which is marked. (A call, so that this rare work lies outside of
+// the kernel's loops: inlined, it made them 3 to 5 % slower.)
+template <typename T, int kHalves, uint32_t kGroupBytes>
+__device__ __noinline__ void clear_hidden(uint8_t* tile, Item& it, int c0) {
+  const int lane = threadIdx.x & 31, see0 = it.see0, hide0 = it.hide0, begin = it.begin, end = it.end;
+  uint8_t* v = tile + (lane & 7) * 16;  // eight lanes on 128 bytes of a row
+  uint32_t top = 0;
+#pragma unroll 2
+  for (int r = lane >> 3; r < kTile; r += 4) {
+    const int p = c0 + r;
+    const bool none = p >= end || p < begin;
+    if (!none && p < hide0 && p >= see0) continue;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      uint4* w = reinterpret_cast<uint4*>(v + (r >> 3) * kGroupBytes + h * 1024 + (r & 7) * 128);
+      if (none)
+        *w = make_uint4(0u, 0u, 0u, 0u);
+      else
+        top = __vmaxu2(top, largest2(*w));
+    }
+  }
+  if (!__any_sync(0xffffffffu, max(top >> 16, top & 0xffffu) >= Weights<T>::kInf)) return;
+  if (lane == 0) *static_cast<volatile int*>(&it.cleared) = 1;
+#pragma unroll 1
+  for (int r = lane >> 3; r < kTile; r += 4) {
+    if (c0 + r < hide0 && c0 + r >= see0) continue;
+#pragma unroll
+    for (int h = 0; h < kHalves; ++h) {
+      uint4* w = reinterpret_cast<uint4*>(v + (r >> 3) * kGroupBytes + h * 1024 + (r & 7) * 128);
+      const uint4 x = *w;
+      *w = make_uint4(finite2<T>(x.x), finite2<T>(x.y), finite2<T>(x.z), finite2<T>(x.w));
+    }
+  }
+}
+
 template <typename T, int D, bool kTokens>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
@@ -301,6 +374,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int i = 0; i < kSlots; ++i) {
       sm100::mbar_init(&bar.full[i], 1);
       sm100::mbar_init(&bar.empty[i], 1);
+      sm100::mbar_init(&bar.vcut[i], 1);
+      sm100::mbar_init(&bar.vclear[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       sm100::mbar_init(&bar.qready[i], 4);
@@ -350,19 +425,45 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp >= 8) {
     if constexpr (!kTokens) sm100::reg_give<72>();
     if (warp == 10) {
-      // ------------------------------------------------------------ items
-      if (lane == 0) {
-        Walk<kTokens> walk;
-        walk.start(a, group, misc.part);
+      // ------------------------------------------------------------ items, and V where rows differ in what they see
+      Walk<kTokens> walk;
+      if (lane == 0) walk.start(a, group, misc.part);
+      bool more = lane == 0;
+      unsigned base = 0;   // loads of the items before, K and V
+      uint32_t phase = 0;  // parity of the next vcut[slot] (bit slot)
 #pragma unroll 1
-        for (unsigned i = 0;; ++i) {
+      for (unsigned i = 0;; ++i) {
+        if (more) {
           Item it;
-          const bool more = walk.next(a, group, it) && !*s_err;
+          more = walk.next(a, group, it) && !*s_err;
           if (!more) it.rows = 0;
           wait(&bar.iempty[i % kItems], ((i / kItems) & 1u) ^ 1u);
           misc.item[i % kItems] = it;
           sm100::mbar_arrive(&bar.ifull[i % kItems]);
-          if (!more) break;
+        }
+        if constexpr (kTokens) {
+          if (!__any_sync(0xffffffffu, more)) break;
+        } else {
+          // Then the item two before that one: the ring's place was free as soon as this item's turn came.
+          __syncwarp();
+          if (i < 2) continue;
+          Item& it = misc.item[(i - 2) % kItems];
+          if (__any_sync(0xffffffffu, *s_err || it.rows == 0)) break;
+          const Steps<kTokens> st(it);
+          const int first = (it.tile0 + it.t0) * kTile;
+#pragma unroll 1
+          for (int j = 0; j < st.nt; ++j) {
+            if (!it.cut(first + j * kTile)) continue;
+            const unsigned n = base + st.v_at(j), sl = n % kSlots;
+            wait(&bar.vcut[sl], phase >> sl & 1u);
+            phase ^= 1u << sl;
+            wait(&bar.full[sl], (n / kSlots) & 1u);
+            clear_hidden<T, C::kHalves, C::kGroupBytes>(ring + sl * C::kTileBytes, it, first + j * kTile);
+            sm100::fence_proxy_async_smem();
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&bar.vclear[sl]);
+          }
+          base += 2 * st.nt;
         }
       }
     } else if (warp == 8 || warp == 11) {
@@ -417,6 +518,8 @@ __global__ void __launch_bounds__(kThreads, 1)
               sm100::tma_load_5d(dst + run * (box / 8) * C::kGroupBytes, map, &bar.full[sl], 0, 0, head, tok8, page);
           }
           if (lane == 0) misc.last[is_v][sl] = static_cast<int>(n);
+          if constexpr (!kTokens)
+            if (lane == 0 && is_v && it.cut(first + j * kTile)) sm100::mbar_arrive(&bar.vcut[sl]);
         }
         base += 2 * nt;
         if (lane == 0) sm100::mbar_arrive(&bar.iempty[item % kItems]);
@@ -427,6 +530,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr uint32_t kHighQ = desc_high(1024), kHighKV = desc_high(C::kGroupBytes);
         unsigned base = 0;                // loads of the items before
         uint32_t qphase = 0, pphase = 0;  // parity of the next qready[tile] (bit tile), pready[t] (bit t)
+        uint32_t cphase = 0;              // of the next vclear[slot]
         int qt = 0;                       // tile of the queries of an item of at most 128 rows
         bool narrow_before = false;
 #pragma unroll 1
@@ -435,6 +539,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const Item& it = misc.item[item % kItems];
           if (*s_err || it.rows == 0) break;
           const Steps<kTokens> st(it);
+          // Positions before `low` and from `high` on, counted from the first tile, are cleared in V.
+          const int first = (it.tile0 + it.t0) * kTile, low = it.see0 - first, high = it.hide0 - first;
           sm100::mbar_arrive(&bar.iempty[item % kItems]);
           const bool wide = st.wide;
           const int steps = st.count();
@@ -469,7 +575,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int k = 0; k < steps && !*s_err; ++k) {
             const int t = k & 1;
             const unsigned n = base + st.v_at(st.tile(k)), sl = n % kSlots;
-            if (!wide || t == 0) wait(&bar.full[sl], (n / kSlots) & 1u);
+            if (!wide || t == 0) {
+              const int c = st.tile(k) * kTile;
+              const bool cut = !kTokens && (c < low || c + kTile > high);  // Item::cut()
+              wait(cut ? &bar.vclear[sl] : &bar.full[sl], cut ? cphase >> sl & 1u : (n / kSlots) & 1u);
+              if (cut) cphase ^= 1u << sl;
+            }
             // Leading byte offset: to the second half.
             const uint32_t v = ring_low + sl * (C::kTileBytes >> 4) + ((1024u >> 4) << 16);
             wait(&bar.pready[t], pphase >> t & 1u);
@@ -565,7 +676,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 
 #pragma unroll 1
     for (unsigned item = 0; more(item); ++item) {
-      const Item& it = misc.item[item % kItems];
+      Item& it = misc.item[item % kItems];
       const Steps<kTokens> st(it);
       const bool wide = st.wide, quad = kTokens || it.rows <= 32;
       // The queries of a narrow item alternate between the tiles, so that those of the next are loaded now; the
@@ -586,7 +697,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int lo = a.window > 0 && valid ? pos - a.window + 1 : 0;
       const bool idle = __all_sync(0xffffffffu, !valid);
       const int hi_all = __reduce_min_sync(0xffffffffu, hi), lo_all = __reduce_max_sync(0xffffffffu, lo);
-      const int first_pos = (it.tile0 + it.t0) * kTile, len = it.len, begin = it.begin;
+      const int first_pos = (it.tile0 + it.t0) * kTile, see0 = it.see0, hide0 = it.hide0;
       float m = -INFINITY, l = 0.f;  // bound on the maximum, in units of S; sum of P
       const int steps = st.count();
       int mine = 0;  // steps of this group
@@ -595,20 +706,21 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int j = st.tile(k), c0 = first_pos + j * kTile;
         wait(&bar.sfull[t], no & 1u);
         sm100::tc_fence_after();
-        // Tokens behind the sequence and before every row's window may hold anything: zeros in V, since
-        // zero times NaN is NaN. (After S of the step: what the slot of V held before is consumed or still waited
-        // for by this load.)
-        if (c0 + kTile > len || c0 < begin) {
-          const unsigned at = base + st.v_at(j);
-          wait(&bar.full[at % kSlots], (at / kSlots) & 1u);
-          if (c0 + row >= len || c0 + row < begin) {
-            uint8_t* vt = ring + (at % kSlots) * C::kTileBytes + (row >> 3) * C::kGroupBytes + (row & 7) * 128;
+        // Single tokens, whose rows all see the same: what they must not see in V becomes zeros here, since zero times NaN is NaN. (After S
+        // of the step: what the slot of V held before is consumed or still waited for by this load.)
+        if constexpr (kTokens)
+          if (c0 + kTile > hide0 || c0 < see0) {
+            const unsigned at = base + st.v_at(j);
+            wait(&bar.full[at % kSlots], (at / kSlots) & 1u);
+            if (c0 + row >= hide0 || c0 + row < see0) {
+              uint8_t* vt = ring + (at % kSlots) * C::kTileBytes + (row >> 3) * C::kGroupBytes + (row & 7) * 128;
+              // From a part of its own on for each of eight rows: their banks differ.
 #pragma unroll
-            for (int c = 0; c < 8 * C::kHalves; ++c)
-              *reinterpret_cast<uint4*>(vt + (c >> 3) * 1024 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+              for (int c = 0; c < 8 * C::kHalves; ++c)
+                *reinterpret_cast<uint4*>(vt + (c >> 3) * 1024 + ((c + row) & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            sm100::fence_proxy_async_smem();
           }
-          sm100::fence_proxy_async_smem();
-        }
         if (!idle) {
           // Columns of this thread: all, or the warp's quarter.
           auto softmax = [&](auto cols_tag) {
@@ -708,15 +820,15 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int which = it.t0 > 0 ? 0 : 1, slot = 2 * blockIdx.x + which;
       float* acc = ws.acc + static_cast<int64_t>(slot) * ws.row_cap * D;
       float* ml = ws.ml + static_cast<int64_t>(slot) * ws.row_cap * 2;
-      if (!whole && threadIdx.x == 0) desc[which] = PartDesc{it.s, it.h, it.b, it.rows, it.t0, it.t1, it.tiles, it.q0};
+      auto cleared = [&] { return *static_cast<volatile int*>(&it.cleared) != 0; };
+      auto describe = [&] {
+        if (!whole && threadIdx.x == 0)
+          desc[which] = PartDesc{it.s, it.h, it.b, static_cast<short>(it.rows), cleared(), it.t0, it.t1, it.tiles, it.q0};
+      };
+      if (wide) describe();
       auto out_of = [&](int r2) {
         const int x = it.row0 + r2;
         return static_cast<T*>(a.out) + (it.q0 + x / group) * a.o_tok + (it.h * group + x % group) * a.o_head;
-      };
-      auto again = [&](int r2) {  // row r2 of the block by this warp
-        const int x = it.row0 + r2;
-        attention_row<T, D>(a, it.s, it.q0 + x / group, it.len - it.n + x / group, it.len, it.h * group + x % group,
-                            it.h);
       };
       // Stores 32 columns of each of the warp's rows. As fp32 to the workspace: float4 c of row r at place
       // c row_cap + r, so that lanes write side by side. Or rounded with the factor inv: four lanes exchange their
@@ -791,9 +903,12 @@ __global__ void __launch_bounds__(kThreads, 1)
           store32(c, y, inv, odd);
         }
         if (!whole && valid) *reinterpret_cast<float2*>(ml + r * 2) = make_float2(mj, lj);
-        unsigned redo = __ballot_sync(0xffffffffu, whole && valid && odd != 0.f);
-#pragma unroll 1
-        for (; redo; redo &= redo - 1) again((wide ? t * 128 : 0) + w4 * 32 + __ffs(redo) - 1);
+        if (whole) {
+          const bool some = cleared(), counts = valid && inv == inv && inv != 0.f;
+          const unsigned not_finite = __ballot_sync(0xffffffffu, counts && odd != 0.f);
+          const unsigned rows = __ballot_sync(0xffffffffu, counts && (odd != 0.f || some));
+          if (rows) settle<T, D>(a, it, group, (wide ? t * 128 : 0) + w4 * 32, rows, not_finite != 0, some);
+        }
       };
       float* buf = reinterpret_cast<float*>(smem + C::kQ + qt * C::kTileBytes);
       float mj = m2, lj = l, f0 = 1.f, f1 = 0.f;  // the joined state of this thread's row and the factors of both
@@ -807,6 +922,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (mine > 0) sml[threadIdx.x] = make_float2(m2, l);
         sm100::tc_fence_before();
         group_sync();
+        describe();
         if (!quad && two) {
           const float2 other = sml[128 + row];
           mj = fmaxf(m2, other.x), f0 = factor(m2, mj), f1 = factor(other.x, mj);
@@ -850,7 +966,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             float y[8];
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-              // A factor of 0 drops no infinity: where a state holds one, seen or not, the row is computed again.
+              // A factor of 0 drops no infinity: where a state holds one, seen or not, the column is settled below.
               y[e] = __uint_as_float(o0[e]) * f0;
               if (two) y[e] += __uint_as_float(o1[e]) * f1;
             }
@@ -874,7 +990,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               const float inv = misc.inv[r2];
               if (inv == 0.f) y = make_float4(0.f, 0.f, 0.f, 0.f);
               y = make_float4(y.x * inv, y.y * inv, y.z * inv, y.w * inv);
-              if ((y.x + y.y + y.z + y.w) * 0.f != 0.f) atomicOr(&misc.bad, 1u << r2);
+              if (inv == inv && (y.x + y.y + y.z + y.w) * 0.f != 0.f) atomicOr(&misc.bad, 1u << r2);
               *reinterpret_cast<uint2*>(out_of(r2) + c0 + 4 * c) = make_uint2(pack2<T>(y.x, y.y), pack2<T>(y.z, y.w));
             } else {
               reinterpret_cast<float4*>(acc)[static_cast<int64_t>(c0 / 4 + c) * ws.row_cap + r2] = y;
@@ -882,12 +998,14 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (whole) {
-          group_sync();  // all rows are written: those that came out as NaN are computed again
+          group_sync();  // all rows are written
           const unsigned bad = *reinterpret_cast<volatile unsigned*>(&misc.bad);
-          if (bad) {
-#pragma unroll 1
-            for (int r2 = warp; r2 < it.rows; r2 += 8)
-              if (bad >> r2 & 1u) again(r2);
+          const bool some = cleared();
+          if (bad != 0 || some) {
+            const float inv = misc.inv[lane];
+            const unsigned rows = __ballot_sync(0xffffffffu, valid && inv == inv && inv != 0.f && (some || bad >> lane & 1u));
+            const unsigned mine8 = rows & (0x01010101u << warp);  // every eighth row
+            if (mine8) settle<T, D>(a, it, group, 0, mine8, (bad & mine8) != 0, some);
             group_sync();
             if (threadIdx.x == 0) misc.bad = 0;
           }
@@ -925,21 +1043,75 @@ __global__ void __launch_bounds__(kThreads, 1)
 // A lane has a row, a warp 16 columns of 32 rows; with fewer rows several lanes share a row's parts.
 constexpr int kMaxParts = 1024;
 
+// What settle() does, to 16 columns (from column c0 on) of a row for each lane; x: its row among the sequence's.
+template <typename T>
+__device__ __forceinline__ void settle_columns(const AttnArgs& a, const PartDesc& p, int group, int x, int c0,
+                                               bool counts, float* o) {
+  const int lane = threadIdx.x & 31;
+  Item it;
+  it.set_block(a, group, p.s, p.h, p.b, q_begin(a.batch, p.s + 1) - p.q0, __ldg(a.batch.kv_len + p.s), p.q0);
+  unsigned plus = 0, minus = 0, nan = 0;  // columns
+  auto look = [&](int pos) {
+    const int page = page_of(a.batch, it.s, pos / a.page_size, a.num_pages);
+    if (page < 0) return;
+    const uint4* v = reinterpret_cast<const uint4*>(static_cast<const T*>(a.v.base) + page * a.v.page +
+                                                    pos % a.page_size * a.v.tok + it.h * a.v.head + c0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint4 w4 = v[i];
+      const uint32_t w[4] = {w4.x, w4.y, w4.z, w4.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        if (finite2<T>(w[e]) == w[e]) continue;
+        const float2 f = to_float2<T>(w[e]);
+        const float two[2] = {f.x, f.y};
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const unsigned bit = 1u << (8 * i + 2 * e + k);
+          nan |= two[k] != two[k] ? bit : 0u;
+          plus |= two[k] == INFINITY ? bit : 0u;
+          minus |= two[k] == -INFINITY ? bit : 0u;
+        }
+      }
+    }
+  };
+  const bool common = it.see0 < it.hide0;
+  if (common) {
+#pragma unroll 1
+    for (int pos = it.see0 + lane; pos < it.hide0; pos += 32) look(pos);
+    plus = __reduce_or_sync(0xffffffffu, plus);
+    minus = __reduce_or_sync(0xffffffffu, minus);
+    nan = __reduce_or_sync(0xffffffffu, nan);
+  }
+  const int at = it.len - it.n + x / group;
+  const int lo = a.window > 0 ? max(it.begin, at - a.window + 1) : it.begin, hi = a.causal ? at + 1 : it.end;
+#pragma unroll 1
+  for (int pos = it.begin; pos < it.end; ++pos) {
+    if (common && pos == it.see0) pos = it.hide0;
+    if (pos >= lo && pos < min(hi, it.end)) look(pos);
+  }
+  if (counts)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const unsigned bits = (plus >> e & 1u) | (minus >> e & 1u) << 1 | (nan >> e & 1u) << 2;
+      if (bits) o[e] = bits == 1u ? INFINITY : bits == 2u ? -INFINITY : __int_as_float(0x7fffffff);
+    }
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(D * 2)
     merge_kernel(const __grid_constant__ AttnArgs a, const Workspace ws, int group, int ctas) {
   __shared__ int part[kMaxParts];
   __shared__ int parts;
-  __shared__ unsigned odd_rows;
+  __shared__ int cleared;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (threadIdx.x == 0) odd_rows = 0;
   pdl_wait();
   pdl_trigger();
   const PartDesc first = ws.desc[2 * blockIdx.x + 1];
   if (first.q0 < 0 || first.t1 == first.tiles || static_cast<int>(blockIdx.y) * 32 >= first.rows) return;
   if (warp == 0) {
     // Continuations follow in the order of the CTAs; one that reaches the last tile is the last.
-    int n = 1;
+    int n = 1, some = first.cleared;
     if (lane == 0) part[0] = 2 * blockIdx.x + 1;
     for (int c0 = blockIdx.x + 1; c0 < ctas; c0 += 32) {
       const int c = c0 + lane;
@@ -949,10 +1121,14 @@ __global__ void __launch_bounds__(D * 2)
       const bool on = d.q0 >= 0 && d.s == first.s && d.h == first.h && d.b == first.b;
       const unsigned who = __ballot_sync(0xffffffffu, on);
       if (on) part[n + __popc(who & ((1u << lane) - 1u))] = 2 * c;
+      some |= __any_sync(0xffffffffu, on && d.cleared != 0);
       n += __popc(who);
       if (__any_sync(0xffffffffu, on && d.t1 == d.tiles)) break;
     }
-    if (lane == 0) parts = n;
+    if (lane == 0) {
+      parts = n;
+      cleared = some;
+    }
   }
   __syncthreads();
   const int n = parts;
@@ -990,32 +1166,29 @@ __global__ void __launch_bounds__(D * 2)
     for (int e = 0; e < 16; ++e) o[e] = o[e] * f0 + __shfl_xor_sync(0xffffffffu, o[e], w) * f1;
   }
   const int x = first.b * kBlock + rc, tok = x / group, h = first.h * group + x % group;
-  const int cnt = q_begin(a.batch, first.s + 1) - first.q0, len = __ldg(a.batch.kv_len + first.s);
-  // Of the positions before the row's own some are in every window.
-  const float inv = inverse(l, a.causal ? len - cnt + tok >= 0 : len > 0);
+  float inv = 1.f / l;
+  if (l == 0.f) {  // (lengths are looked up only here and below: they would be waited for)
+    const int len = __ldg(a.batch.kv_len + first.s), n_new = q_begin(a.batch, first.s + 1) - first.q0;
+    inv = inverse(l, a.causal ? len - n_new + tok >= 0 : len > 0);  // a row's window holds its own position at least
+  }
+  const bool valid = r < first.rows && lane < width;
   float odd = 0.f;
 #pragma unroll
   for (int e = 0; e < 16; ++e) {
     o[e] = inv == 0.f ? 0.f : o[e] * inv;
     odd += o[e] * 0.f;
   }
-  const bool valid = r < first.rows && lane < width;
-  if (valid) {
+  auto store = [&] {
+    if (!valid) return;
     uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (first.q0 + tok) * a.o_tok + h * a.o_head + warp * 16);
     dst[0] = make_uint4(pack2<T>(o[0], o[1]), pack2<T>(o[2], o[3]), pack2<T>(o[4], o[5]), pack2<T>(o[6], o[7]));
     dst[1] = make_uint4(pack2<T>(o[8], o[9]), pack2<T>(o[10], o[11]), pack2<T>(o[12], o[13]), pack2<T>(o[14], o[15]));
-  }
-  // Rows that came out as NaN are computed again, after every warp has stored its columns.
-  const unsigned bad = __ballot_sync(0xffffffffu, valid && odd != 0.f);
-  if (lane == 0 && bad) atomicOr(&odd_rows, bad);
-  __syncthreads();
-  const unsigned redo = odd_rows;
-  if (!redo) return;
-  for (int i = warp; i < 32; i += D / 16) {
-    if (!(redo >> i & 1u)) continue;
-    const int y = first.b * kBlock + blockIdx.y * 32 + i;
-    attention_row<T, D>(a, first.s, first.q0 + y / group, len - cnt + y / group, len, first.h * group + y % group,
-                        first.h);
+  };
+  store();
+  const bool counts = valid && inv == inv && inv != 0.f;
+  if (__any_sync(0xffffffffu, counts && (odd != 0.f || cleared != 0))) {
+    settle_columns<T>(a, first, group, x, warp * 16, counts, o);
+    store();
   }
 }
 

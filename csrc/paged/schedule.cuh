@@ -88,10 +88,37 @@ struct Item {
   int row0, rows;  // rows of the block among the sequence's G n
   int pos0;        // position of the block's first row
   int begin, end;  // positions that some row sees
+  int see0, hide0;  // positions [see0, hide0) are seen by every row, if there are any: see0 may lie behind hide0
   int tile0, tiles, t0, t1;
   bool over;       // some row sees positions behind the page table
+  int cleared;     // values were taken out of V (attention_kernel)
 
   __device__ __forceinline__ bool whole() const { return t1 - t0 == tiles; }
+  // Whether the row x of the sequence's G n sees anything: with a window its own position at least.
+  __device__ __forceinline__ bool sees(int x, int group, bool causal) const {
+    return causal ? len - n + x / group >= 0 : len > 0;
+  }
+  // Whether the tile from position c0 on has some that not every row sees.
+  __device__ __forceinline__ bool cut(int c0) const { return c0 < see0 || c0 + kTile > hide0; }
+
+  // All but the part: block b of KV head h of sequence s, whose n new rows of len tokens start at row q0.
+  __device__ __forceinline__ void set_block(const AttnArgs& p, int group, int s_, int h_, int b_, int n_, int len_,
+                                            int q0_) {
+    s = s_, h = h_, b = b_, n = n_, len = len_, q0 = q0_;
+    row0 = b * kBlock;
+    rows = min(kBlock, n * group - row0);
+    pos0 = len - n + row0 / group;
+    const int last = len - n + (row0 + rows - 1) / group;
+    begin = p.window > 0 ? max(0, pos0 - p.window + 1) : 0;
+    end = max(0, p.causal ? last + 1 : len);
+    over = end > p.capacity;
+    end = min(end, p.capacity);
+    see0 = p.window > 0 ? max(0, last - p.window + 1) : 0;
+    hide0 = p.causal ? min(end, max(0, pos0 + 1)) : end;
+    tile0 = begin / kTile;
+    tiles = end > begin ? (end + kTile - 1) / kTile - tile0 : 1;
+    cleared = 0;
+  }
 };
 
 // Walks a CTA's items. Every role of the kernel walks them by itself.
@@ -136,23 +163,7 @@ struct Walk {
       }
       if (s > part.s1 || (s == part.s1 && at >= part.off1)) return false;
       const int64_t weight = w.weight(b);
-      it.s = s;
-      it.h = h;
-      it.b = b;
-      it.n = w.n;
-      it.len = w.len;
-      it.q0 = w.q0;
-      it.row0 = b * kBlock;
-      it.rows = min(kBlock, w.n * group - it.row0);
-      const int i0 = it.row0 / group, i1 = (it.row0 + it.rows - 1) / group;
-      it.pos0 = w.len - w.n + i0;
-      const int last = w.len - w.n + i1;
-      it.begin = p.window > 0 ? max(0, it.pos0 - p.window + 1) : 0;
-      it.end = max(0, p.causal ? last + 1 : w.len);
-      it.over = it.end > p.capacity;
-      it.end = min(it.end, p.capacity);
-      it.tile0 = it.begin / kTile;
-      it.tiles = it.end > it.begin ? (it.end + kTile - 1) / kTile - it.tile0 : 1;
+      it.set_block(p, group, s, h, b, w.n, w.len, w.q0);
       const int64_t x0 = s == part.s0 ? max(part.off0 - at, static_cast<int64_t>(0)) : 0;
       const int64_t x1 = s == part.s1 ? min(part.off1 - at, weight) : weight;
       it.t0 = x0 == 0 ? 0 : static_cast<int>(quotient(x0 * it.tiles, weight));

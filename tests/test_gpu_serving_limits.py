@@ -113,3 +113,75 @@ def test_attention_infinite_value_under_a_vanishing_weight(new, total, decode, d
     # Recomputed rows round elsewhere: both are within u A + u |o| of the formula, A the mean of |v|, at most 4.
     u = torch.finfo(dtype).eps / 2
     assert (out.float() - clean.float()).abs().max() <= 2 * u * (4 + clean.float().abs().max())
+
+
+def _settled(out0, v, batch, hq, hkv, d, causal=True, window=0):
+    """Outputs over values that are not finite, from those over the same values with zeros in their places: a column
+    is inf, -inf or NaN as the sum of what the row sees in it that is not finite, whatever its (positive) weight."""
+    want = out0.view(-1, hkv, hq // hkv, d).clone()
+    starts = list(range(batch.sequences + 1)) if batch.q_start is None else batch.q_start.tolist()
+    table = batch.page_table.cpu()
+    for s, total in enumerate(batch.kv_len.tolist()):
+        n = starts[s + 1] - starts[s]
+        p = torch.arange(total)
+        vals = v[table[s, p // PAGE].long(), p % PAGE]
+        odd = torch.where(torch.isfinite(vals), torch.zeros_like(vals), vals).float()
+        for i in range(n):
+            pos = total - n + i
+            hi, lo = (pos + 1 if causal else total), (max(0, pos - window + 1) if window else 0)
+            add = odd[lo:hi].sum(0).to(want.dtype)[:, None]
+            want[starts[s] + i] = torch.where(torch.isfinite(add), want[starts[s] + i], add)
+    return want.view(out0.shape)
+
+
+@pytest.mark.parametrize("new,total,decode", BLOCKS + [([260], [700], False), ([70, 1, 33], [70, 400, 3000], False)])
+@pytest.mark.parametrize("dtype,d", [(BF, 128), (HF, 64)])
+@pytest.mark.parametrize("hkv", [1, 4, 8])
+def test_attention_values_that_are_not_finite(new, total, decode, dtype, d, hkv):
+    """Infinities and NaN among the values: seen by every row, by some, behind the lengths, in several columns."""
+    from b200ar.ops.paged import paged_attention
+
+    q, k, v, batch = _inputs(new, total, decode, dtype, d, 8, hkv)
+    g = torch.Generator().manual_seed(5)
+    for s, t in enumerate(total):
+        for value in (INF, -INF, NAN, INF):
+            for p in {0, t - 1, max(t - new[s] // 2 - 1, 0), *torch.randint(t, (3,), generator=g).tolist()}:
+                pg, slot = _slot(batch, s, p)
+                v[pg, slot, int(torch.randint(hkv, (1,), generator=g)), int(torch.randint(d, (1,), generator=g))] = value
+        end = torch.arange(t, -(-t // PAGE) * PAGE)
+        v[batch.page_table.cpu()[s, end // PAGE].long(), end % PAGE] = NAN
+    clean = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+    for kw in ({}, {"window": 1}, {"window": 50}, {"window": 300}, {"causal": False}):
+        want = _settled(paged_attention(q, k, clean, batch, **kw), v, batch, 8, hkv, d, **kw)
+        out = paged_attention(q, k, v, batch, **kw)
+        assert torch.equal(torch.isnan(out), torch.isnan(want))
+        assert torch.equal(out.nan_to_num(nan=7.0), want.nan_to_num(nan=7.0))
+
+
+@pytest.mark.parametrize("decode", [True, False])
+def test_attention_nan_before_a_long_context(decode):
+    """What a NaN costs does not grow with rows times positions: every wait ends in time, and the sequences beside
+    it are what they were."""
+    from b200ar.ops.paged import paged_attention
+
+    new, total = ([1, 1, 1], [90, 120000, 3000]) if decode else ([40, 600, 1, 9], [90, 120000, 3000, 9])
+    q, k, v, batch = _inputs(new, total, decode, BF, 128)
+    clean = paged_attention(q, k, v, batch).view(-1, 8, 128)
+    pg, slot = _slot(batch, 1, 0)
+    v[pg, slot, 0, 5] = NAN
+    out = paged_attention(q, k, v, batch).view(-1, 8, 128)
+    sees = slice(new[0], new[0] + new[1])
+    assert torch.isnan(out[sees, :, 5]).all()
+    out[sees, :, 5] = clean[sees, :, 5]
+    assert torch.equal(out, clean)
+
+
+@pytest.mark.parametrize("new,total,decode", BLOCKS)
+def test_attention_large_values_within_the_type(new, total, decode):
+    """Values of 2^114 under weights that sum up to 6000, below 2^13: in range as long as none counts more than 1."""
+    from b200ar.ops.paged import paged_attention
+
+    q, k, v, batch = _inputs(new, total, decode, BF, 128)
+    k.mul_(torch.linspace(0.01, 3, k.shape[0], device="cuda").to(BF)[:, None, None, None])  # the largest score comes late
+    small = paged_attention(q, k, v.sign(), batch)
+    assert torch.equal(paged_attention(q, k, v.sign() * 2.0 ** 114, batch), small * 2.0 ** 114)
