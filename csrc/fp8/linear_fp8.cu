@@ -95,6 +95,39 @@ __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
 }
 __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
+__device__ __forceinline__ uint64_t pack64(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+__device__ __forceinline__ void unpack64(uint64_t v, float& lo, float& hi) {
+  uint32_t a, b;
+  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
+  lo = __uint_as_float(a);
+  hi = __uint_as_float(b);
+}
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t both(float x) { return pack64(__float_as_uint(x), __float_as_uint(x)); }
+
+// A block's sum r (0, or from 2^-18 to 2^25) times two scales a and b, as (r first) b second: whatever the scales, a
+// product on the way is out of range only if the result is. (r a is a normal number for a between 2^-100 and 2^100;
+// outside, a power of two of a's is left for the end.)
+__device__ __forceinline__ void around(float a, float& first, float& second) {
+  const bool high = fabsf(a) > 0x1p100f, low = fabsf(a) < 0x1p-100f;
+  first = high ? 0x1p64f : low ? 0x1p-64f : a;
+  second = high ? a * 0x1p-64f : low ? a * 0x1p64f : 1.f;
+}
+
 struct Args {
   const float* sx;  // [kblocks, M], row stride lds
   const float* sw;  // [ceil(N / 128), kblocks]
@@ -178,9 +211,9 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
     if (!*s_err && !sm100::mbar_wait(b, parity)) *s_err = 1;
   };
 
-  float acc[MP];
+  uint64_t acc[MP / 2];  // pairs of rows of x
 #pragma unroll
-  for (int i = 0; i < MP; ++i) acc[i] = 0.f;
+  for (int i = 0; i < MP / 2; ++i) acc[i] = 0;
 
   if (warp == 0) {
     if (sm100::elect_one()) {
@@ -257,6 +290,9 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
       wait(&tfull[bf], (i / C::kBufs) & 1);
       sm100::tc_fence_after();
       constexpr int kStep = MP < 32 ? MP : 32;
+      float first, second;
+      around(sw, first, second);
+      const uint64_t first2 = both(first), second2 = both(second);
 #pragma unroll
       for (int c = 0; c < MP; c += kStep) {
         uint32_t r[kStep];
@@ -267,11 +303,10 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
         sm100::tmem_ld_wait();
 #pragma unroll
         for (int e = 0; e < kStep; e += 4) {
-          const float4 s = *reinterpret_cast<const float4*>(sc + c + e);
-          acc[c + e] = fmaf(__uint_as_float(r[e]) * s.x, sw, acc[c + e]);
-          acc[c + e + 1] = fmaf(__uint_as_float(r[e + 1]) * s.y, sw, acc[c + e + 1]);
-          acc[c + e + 2] = fmaf(__uint_as_float(r[e + 2]) * s.z, sw, acc[c + e + 2]);
-          acc[c + e + 3] = fmaf(__uint_as_float(r[e + 3]) * s.w, sw, acc[c + e + 3]);
+          const ulonglong2 s = *reinterpret_cast<const ulonglong2*>(sc + c + e);  // scales of four rows
+          uint64_t* sum = acc + (c + e) / 2;
+          sum[0] = fma2(mul2(mul2(pack64(r[e], r[e + 1]), first2), s.x), second2, sum[0]);
+          sum[1] = fma2(mul2(mul2(pack64(r[e + 2], r[e + 3]), first2), s.y), second2, sum[1]);
         }
       }
       sm100::tc_fence_before();
@@ -294,8 +329,12 @@ __global__ void __launch_bounds__(RowsCfg<MP>::kThreads)
   if (warp >= 2 && warp < 6) {
     const int id = (warp & 3) * 32 + lane;
 #pragma unroll
-    for (int i = 0; i < MP; ++i)
-      if (m0 + i < a.M) sums[i * 128 + id] = acc[i];
+    for (int i = 0; i < MP; i += 2) {
+      float x, y;
+      unpack64(acc[i / 2], x, y);
+      if (m0 + i < a.M) sums[i * 128 + id] = x;
+      if (m0 + i + 1 < a.M) sums[(i + 1) * 128 + id] = y;
+    }
   }
   if (splits > 1)
     sm100::cluster_sync();
@@ -355,24 +394,6 @@ struct Line {
 };
 
 __device__ __forceinline__ void sum_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
-__device__ __forceinline__ uint64_t pack64(uint32_t lo, uint32_t hi) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-  return r;
-}
-__device__ __forceinline__ void unpack64(uint64_t v, float& lo, float& hi) {
-  uint32_t a, b;
-  asm("mov.b64 {%0, %1}, %2;" : "=r"(a), "=r"(b) : "l"(v));
-  lo = __uint_as_float(a);
-  hi = __uint_as_float(b);
-}
-// Two fp32 sums in one instruction.
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-  return d;
-}
-
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 1)
     pair_kernel(const __grid_constant__ CUtensorMap tx, const __grid_constant__ CUtensorMap tw, const Args a,

@@ -185,3 +185,59 @@ def test_attention_large_values_within_the_type(new, total, decode):
     k.mul_(torch.linspace(0.01, 3, k.shape[0], device="cuda").to(BF)[:, None, None, None])  # the largest score comes late
     small = paged_attention(q, k, v.sign(), batch)
     assert torch.equal(paged_attention(q, k, v.sign() * 2.0 ** 114, batch), small * 2.0 ** 114)
+
+
+# ------------------------------------------------------------------ 8-bit linear
+# On 148 SMs a K block of 256 x 256 outputs is a unit, and from 888 units on a call of over 128 rows takes pairs of CTAs.
+FEW = [(3, 264, 512), (17, 264, 512), (40, 264, 512), (100, 264, 512), (200, 264, 512)]
+MANY = [(300, 4096, 8192)]
+
+
+def _linear_inputs(m, n, k, x_scale, w_scale):
+    from b200ar.ops.fp8 import quantize_fp8, quantize_fp8_weight
+
+    x = (randn((m, k), torch.float32, "cuda", 1) * x_scale).to(BF)
+    w = randn((n, k), torch.float32, "cuda", 2) * w_scale
+    return (x, *quantize_fp8(x), *quantize_fp8_weight(w))
+
+
+def _check_linear(out, x_q, x_s, w_q, w_s):
+    """check_linear's bound, whose smallest rounding step also covers sums of subnormal fp32 numbers: 64 blocks are
+    off by 64 2^-149, far below u 2^-126."""
+    from serving_util import check_linear
+
+    assert torch.isfinite(out).all()
+    check_linear(out, x_q, x_s, w_q, w_s)
+
+
+@pytest.mark.parametrize("m,n,k", FEW)
+def test_linear_fp8_large_activations_few_rows(m, n, k):
+    """Activations of 1e36 against weights of 0.02: sums of 1e36 are in the type, sums of codes times x's scales not."""
+    from b200ar.ops.fp8 import linear_fp8
+
+    size = torch.ones(m, 1, device="cuda")
+    size[::2] = 1e36
+    x, x_q, x_s, w_q, w_s = _linear_inputs(m, n, k, size, 0.02)
+    _check_linear(linear_fp8(x, w_q, w_s), x_q, x_s, w_q, w_s)
+    _check_linear(linear_fp8(x_q, w_q, w_s, x_scale=x_s), x_q, x_s, w_q, w_s)
+
+
+def _tiny_and_zero(m, n, k):
+    from b200ar.ops.fp8 import linear_fp8, quantize_fp8_weight
+
+    # Scales whose product is below fp32 (1e-45), sums of K products of 1e-40 that are not.
+    x, x_q, x_s, w_q, w_s = _linear_inputs(m, n, k, 1e-20, 1e-20)
+    x, x_q = x.abs(), x_q.float().abs().to(x_q.dtype)
+    w_q = w_q.float().abs().to(w_q.dtype)
+    _check_linear(linear_fp8(x, w_q, w_s), x_q, x_s, w_q, w_s)
+    # Scales whose product is above fp32, and products of zero.
+    x[:, ::2] = 0
+    w = randn((n, k), torch.float32, "cuda", 2, 1e16)
+    w[:, 1::2] = 0
+    w_q, w_s = quantize_fp8_weight(w)
+    assert (linear_fp8((x.float() * 1e36 * 1e20).to(BF), w_q, w_s) == 0).all()
+
+
+@pytest.mark.parametrize("m,n,k", FEW)
+def test_linear_fp8_scales_at_the_ends_of_fp32_few_rows(m, n, k):
+    _tiny_and_zero(m, n, k)
