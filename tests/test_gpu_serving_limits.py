@@ -241,3 +241,13 @@ def _tiny_and_zero(m, n, k):
 @pytest.mark.parametrize("m,n,k", FEW)
 def test_linear_fp8_scales_at_the_ends_of_fp32_few_rows(m, n, k):
     _tiny_and_zero(m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", MANY)
+def test_linear_fp8_large_activations_many_rows(m, n, k):
+    test_linear_fp8_large_activations_few_rows(m, n, k)
+
+
+@pytest.mark.parametrize("m,n,k", MANY)
+def test_linear_fp8_scales_at_the_ends_of_fp32_many_rows(m, n, k):
+    _tiny_and_zero(m, n, k)
