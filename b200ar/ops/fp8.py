@@ -2,7 +2,7 @@
 
 e4m3 values with an fp32 scale for each block of 128 along K: one scale for
 each row and block of the activations, one for each 128 x 128 block of a
-weight. A block's scale is ``amax / 448`` (1 for a block of zeros), a value's
+weight. A block's scale is ``amax / 448`` (1 where that is 0), a value's
 code ``x / scale`` rounded to the nearest e4m3 number, both quotients in fp32.
 
 * ``quantize_fp8_weight(w)``       once, when weights are loaded
@@ -121,6 +121,11 @@ def _like(dtype: torch.dtype) -> torch.Tensor:
 
 
 # ------------------------------------------------------------------ references
+def _scale(amax: torch.Tensor) -> torch.Tensor:
+    scale = amax / torch.full_like(amax, E4M3_MAX)
+    return torch.where(scale == 0, torch.ones_like(scale), scale)
+
+
 def ref_quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """fp32 reference of ``quantize_fp8`` for [rows, K]."""
     m, k = x.shape
@@ -128,7 +133,7 @@ def ref_quantize_fp8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     full[:, :k] = x.float()
     full = full.view(m, -1, BLOCK)
     amax = full.abs().amax(-1)
-    scale = torch.where(amax == 0, torch.ones_like(amax), amax / torch.full_like(amax, E4M3_MAX))
+    scale = _scale(amax)
     codes = (full / scale[..., None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
     return codes.view(m, -1)[:, :k].contiguous(), scale
 
@@ -141,7 +146,7 @@ def ref_quantize_fp8_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor
     full[:n, :k] = w.float()
     full = full.view(nb, BLOCK, kb, BLOCK)
     amax = full.abs().amax(dim=(1, 3))
-    scale = torch.where(amax == 0, torch.ones_like(amax), amax / torch.full_like(amax, E4M3_MAX))
+    scale = _scale(amax)
     codes = (full / scale[:, None, :, None]).clamp(-E4M3_MAX, E4M3_MAX).to(torch.float8_e4m3fn)
     return codes.view(nb * BLOCK, kb * BLOCK)[:n, :k].contiguous(), scale
 

@@ -85,7 +85,8 @@ struct Scale {
   float scale, low, high;
   bool divide;  // 1 / scale may not be a normal number
   __device__ __forceinline__ explicit Scale(unsigned amax_bits) {
-    scale = amax_bits == 0u ? 1.f : __fdiv_rn(__uint_as_float(amax_bits), kMax);
+    scale = __fdiv_rn(__uint_as_float(amax_bits), kMax);
+    if (scale == 0.f) scale = 1.f;  // a block of zeros, or of fp32 values up to 224 2^-149: all codes are 0
     const float inverse = __frcp_rn(scale);
     low = inverse * (1.f - 0x1p-21f);
     high = inverse * (1.f + 0x1p-21f);

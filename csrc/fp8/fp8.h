@@ -2,7 +2,7 @@
 //
 // e4m3 values with one fp32 scale for each block of 128 along K: activations
 // have a scale for each row and block, weights one for each 128 x 128 block.
-// A block's scale is amax / 448 (1 where every value is zero), a value's code
+// A block's scale is amax / 448 (1 where that is zero), a value's code
 // is x / scale rounded to the nearest e4m3 number.
 #pragma once
 

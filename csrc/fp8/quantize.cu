@@ -1,6 +1,6 @@
 // Quantization to e4m3 with one scale for each block of 128.
 //
-//   scale = amax / 448 (1 for a block of zeros),  q = e4m3(x / scale)
+//   scale = amax / 448 (1 where that is 0),  q = e4m3(x / scale)
 //
 // Both quotients are the correctly rounded fp32 ones, so the codes are those
 // of the formula and not an approximation of it. (The products with a number

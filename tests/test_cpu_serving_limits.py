@@ -36,3 +36,21 @@ def test_attention_scores_and_values_that_are_not_finite(dtype):
     out = paged_attention(q, far, odd, batch).view(3, 2, 64)
     assert (out[:, :, 5] == INF).all() and (out[2, :, 6] == -INF).all() and torch.isnan(out[:, :, 7]).all()
     assert torch.isfinite(out[:2, :, 6]).all() and torch.isfinite(out[:, :, :5]).all()
+
+
+@pytest.mark.parametrize("rows,k", [(3, 48), (5, 384)])
+def test_quantize_fp8_blocks_whose_scale_is_below_fp32(rows, k):
+    """amax / 448 rounds to 0 up to 224 2^-149, and to 2^-149 above: no code is NaN, those of zeros are zero."""
+    from b200ar.ops.fp8 import quantize_fp8, quantize_fp8_weight
+
+    step = 2.0 ** -149
+    for top, scale in ((1, 1.0), (224, 1.0), (225, step), (448, step)):
+        x = torch.zeros(rows, k)
+        x[0, 1], x[0, 2], x[rows - 1, k - 1] = top * step, -step, -top * step
+        codes, scales = quantize_fp8(x)
+        codes_w, scales_w = quantize_fp8_weight(x)
+        want = torch.where(x == 0, torch.zeros_like(x), (x.double() / scale).clamp(-448, 448).float())
+        want = want.to(torch.float8_e4m3fn).float()
+        assert torch.equal(codes.float(), want) and torch.equal(codes_w.float(), want)
+        assert scales[0, 0] == scale and scales[rows - 1, -1] == scale and (scales[1:-1] == 1).all()
+        assert scales_w[0, 0] == scale

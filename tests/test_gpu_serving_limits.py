@@ -251,3 +251,21 @@ def test_linear_fp8_large_activations_many_rows(m, n, k):
 @pytest.mark.parametrize("m,n,k", MANY)
 def test_linear_fp8_scales_at_the_ends_of_fp32_many_rows(m, n, k):
     _tiny_and_zero(m, n, k)
+
+
+@pytest.mark.parametrize("rows,k", [(3, 48), (5, 384)])
+def test_quantize_fp8_blocks_whose_scale_is_below_fp32(rows, k):
+    """amax / 448 rounds to 0 up to 224 2^-149, and to 2^-149 above: no code is NaN, those of zeros are zero."""
+    from b200ar.ops.fp8 import quantize_fp8, quantize_fp8_weight
+
+    step = 2.0 ** -149
+    for top, scale in ((1, 1.0), (224, 1.0), (225, step), (448, step)):
+        x = torch.zeros(rows, k, device="cuda")
+        x[0, 1], x[0, 2], x[rows - 1, k - 1] = top * step, -step, -top * step
+        codes, scales = quantize_fp8(x)
+        codes_w, scales_w = quantize_fp8_weight(x)
+        want = torch.where(x == 0, torch.zeros_like(x), (x.double() / scale).clamp(-448, 448).float())
+        want = want.to(torch.float8_e4m3fn).float()
+        assert torch.equal(codes.float(), want) and torch.equal(codes_w.float(), want)
+        assert scales[0, 0] == scale and scales[rows - 1, -1] == scale and (scales[1:-1] == 1).all()
+        assert scales_w[0, 0] == scale
