@@ -112,6 +112,29 @@ def _overlaps(a: torch.Tensor, b: torch.Tensor) -> bool:
     return a0 < b1 and b0 < a1
 
 
+def _share_memory(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether an element of ``a`` may be one of ``b``, of the same sizes and
+    type. Dimension by dimension from the largest stride down: where both have
+    the same, not below what the rest spans, only the two slices can meet whose
+    distance is less than it. Other strides count as meeting."""
+    dims = sorted(((sa, sb, n) for n, sa, sb in zip(a.shape, a.stride(), b.stride()) if n > 1), reverse=True)
+
+    def meet(dims, at):
+        span_a, span_b = (1 + sum((d[2] - 1) * d[i] for d in dims) for i in (0, 1))
+        if at >= span_a or -at >= span_b:
+            return False
+        if not dims:
+            return True
+        stride, other, n = dims[0]
+        if stride != other or stride < max(span_a, span_b) - (n - 1) * stride:
+            return True
+        steps, rest = divmod(at, stride)
+        return (abs(steps) < n and meet(dims[1:], rest)) or (abs(steps + 1) < n and meet(dims[1:], rest - stride))
+
+    at, odd = divmod(b.data_ptr() - a.data_ptr(), a.element_size())
+    return a.numel() > 0 and _overlaps(a, b) and (odd != 0 or meet(dims, at))
+
+
 def _shares_memory(t: torch.Tensor) -> bool:
     """Whether two indices of ``t`` may be one element."""
     span = 1
@@ -164,9 +187,10 @@ def qk_norm_rope_paged(qkv: torch.Tensor, batch: PagedBatch, rot: RotaryTable, k
     for t, name in ((q_out, "q_out"), (k_pages, "k_pages"), (v_pages, "v_pages")):
         if t.numel() and _shares_memory(t):
             raise ValueError(f"{name} is written and its rows must not share memory")
-    if k_pages.data_ptr() == v_pages.data_ptr() or any(
-            _overlaps(a, b) for a in (qkv, q_out) for b in (k_pages, v_pages)):
-        raise ValueError("the pools overlap each other, qkv or q_out")
+    if _share_memory(k_pages, v_pages):
+        raise ValueError("k_pages and v_pages share memory")
+    if any(_overlaps(a, b) for a in (qkv, q_out) for b in (k_pages, v_pages)):
+        raise ValueError("the pools overlap qkv or q_out")
     ref_qk_norm_rope_paged(qkv, batch, rot, k_pages, v_pages, hq, hkv, q_gamma, k_gamma, eps, q_out)
     return q_out
 

@@ -10,6 +10,8 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
+#include <functional>
 #include <optional>
 #include <utility>
 #include <vector>
@@ -77,6 +79,35 @@ bool overlaps(const at::Tensor& a, const at::Tensor& b) {
   };
   const auto x = span(a), y = span(b);
   return x.first < y.second && y.first < x.second;
+}
+
+// Whether an element of a may be one of b; both have the same sizes and type. Dimension by dimension from the largest
+// stride down: where both have the same, not below what the rest spans, only the two slices can meet whose distance is
+// less than it. Other strides count as meeting.
+bool share_memory(const at::Tensor& a, const at::Tensor& b) {
+  if (!overlaps(a, b)) return false;
+  struct Dim {
+    int64_t size, a, b;
+  };
+  std::vector<Dim> dims;
+  for (int64_t i = 0; i < a.dim(); ++i)
+    if (a.size(i) > 1) dims.push_back({a.size(i), a.stride(i), b.stride(i)});
+  std::sort(dims.begin(), dims.end(), [](const Dim& x, const Dim& y) { return x.a > y.a; });
+  const std::function<bool(size_t, int64_t)> meet = [&](size_t i, int64_t at) {  // b's dimensions from i on, `at` behind a's
+    int64_t span_a = 1, span_b = 1;
+    for (size_t k = i; k < dims.size(); ++k) {
+      span_a += (dims[k].size - 1) * dims[k].a;
+      span_b += (dims[k].size - 1) * dims[k].b;
+    }
+    if (at >= span_a || -at >= span_b) return false;
+    if (i == dims.size()) return true;
+    if (dims[i].a != dims[i].b || dims[i].a < std::max(span_a, span_b) - (dims[i].size - 1) * dims[i].a) return true;
+    const int64_t stride = dims[i].a, steps = at >= 0 ? at / stride : -((stride - 1 - at) / stride);
+    const int64_t rest = at - steps * stride, last = dims[i].size - 1;
+    return (std::abs(steps) <= last && meet(i + 1, rest)) || (std::abs(steps + 1) <= last && meet(i + 1, rest - stride));
+  };
+  const int64_t bytes = reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr());
+  return bytes % a.element_size() != 0 || meet(0, bytes / a.element_size());
 }
 
 Half half_of(const at::Tensor& t) {
@@ -171,7 +202,7 @@ void register_serving_ops(py::module& m) {
         a.k = pool_of(k_pages, qkv, k_pages, hkv, d, "k_pages", true);
         a.v = pool_of(v_pages, qkv, k_pages, hkv, d, "v_pages", true);
         check_heads(qkv, "qkv", false);
-        VALUE_CHECK(k_pages.data_ptr() != v_pages.data_ptr(), "k_pages and v_pages are the same memory");
+        VALUE_CHECK(!share_memory(k_pages, v_pages), "k_pages and v_pages share memory");
         VALUE_CHECK(!overlaps(qkv, k_pages) && !overlaps(qkv, v_pages), "qkv overlaps the pools");
         const int64_t rows = qkv.size(0);
         a.batch = batch_of(table, kv_len, q_start, qkv, rows);

@@ -54,3 +54,10 @@ def test_quantize_fp8_blocks_whose_scale_is_below_fp32(rows, k):
         assert torch.equal(codes.float(), want) and torch.equal(codes_w.float(), want)
         assert scales[0, 0] == scale and scales[rows - 1, -1] == scale and (scales[1:-1] == 1).all()
         assert scales_w[0, 0] == scale
+
+
+def test_rope_refuses_pools_that_share_memory():
+    """Shifted views of one buffer are refused, views that lie between each other taken."""
+    from serving_pools import rope_on_pools
+
+    rope_on_pools("cpu")
