@@ -23,6 +23,7 @@ import torch
 
 from .._native import _C
 from .gemm import error_word
+from .paged import _overlaps
 
 BLOCK = 128
 E4M3_MAX = 448.0
@@ -104,6 +105,8 @@ def linear_fp8(x: torch.Tensor, w_q: torch.Tensor, w_scale: torch.Tensor, out: O
         out = torch.empty(shape, dtype=dtype, device=x.device)
     elif tuple(out.shape) != shape or out.dtype != dtype or out.device != x.device:
         raise ValueError(f"out must be {dtype} {list(shape)} on {x.device}")
+    if any(t is not None and _overlaps(out, t) for t in (x, w_q, w_scale, x_scale)):
+        raise ValueError("out overlaps an input")
     x2 = x.reshape(-1, k)
     codes, scale = ref_quantize_fp8(x2) if x_scale is None else (x2, x_scale.reshape(-1, _blocks(k)))
     out.view(-1, n).copy_(ref_linear_fp8(codes, scale, w_q, w_scale).to(dtype))

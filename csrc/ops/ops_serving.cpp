@@ -391,7 +391,9 @@ void register_serving_ops(py::module& m) {
         }
         const at::Tensor out2 = out.dim() == 2 ? out : out.view({M, N});
         check_heads(out2, "out", true);
-        VALUE_CHECK(!overlaps(out, x) && !overlaps(out, w) && !overlaps(out, w_scale), "out overlaps an input");
+        VALUE_CHECK(!overlaps(out, x) && !overlaps(out, w) && !overlaps(out, w_scale) &&
+                        !(x_scale.has_value() && overlaps(out, *x_scale)),
+                    "out overlaps an input");
         b200ar::fp8::LinearArgs a{};
         a.w = static_cast<const uint8_t*>(w.data_ptr());
         a.sw = w_scale.data_ptr<float>();

@@ -59,3 +59,24 @@ def rope_on_pools(device):
         got = (q, k[:PAGES].clone(), v[:PAGES].clone())
         want = want or got
         assert all(torch.equal(a, b) for a, b in zip(got, want)), name
+
+
+def linear_over_inputs(device):
+    from b200ar.ops.fp8 import linear_fp8, quantize_fp8, quantize_fp8_weight
+
+    x = randn((32, 256), torch.bfloat16, device, 1)
+    w_q, w_s = quantize_fp8_weight(randn((16, 256), torch.bfloat16, device, 2))
+    x_q, x_s = quantize_fp8(x)
+    out = torch.zeros(32, 2 * 256, dtype=torch.bfloat16, device=device)
+    scale = out.view(torch.float32)[:, 8:10]  # bytes 32 to 40 of a row of 1024
+    scale.copy_(x_s)
+    want = linear_fp8(x, w_q, w_s)
+    assert torch.equal(linear_fp8(x_q, w_q, w_s, x_scale=scale), want)
+    codes = out.view(torch.float8_e4m3fn)[:, :256]
+    with pytest.raises(ValueError):
+        linear_fp8(x_q, w_q, w_s, out=out[:, 16:32], x_scale=scale)
+    with pytest.raises(ValueError):
+        linear_fp8(codes, w_q, w_s, out=out[:, 256:272], x_scale=x_s)
+    with pytest.raises(ValueError):
+        linear_fp8(x, w_q, w_s, out=x[:, :16])
+    assert torch.equal(scale, x_s)

@@ -276,3 +276,9 @@ def test_rope_refuses_pools_that_share_memory():
     from serving_pools import rope_on_pools
 
     rope_on_pools("cuda")
+
+
+def test_linear_fp8_refuses_an_output_over_an_input():
+    from serving_pools import linear_over_inputs
+
+    linear_over_inputs("cuda")
