@@ -7,9 +7,10 @@ prompts and single tokens in one call.
 * ``paged_attention``     attention of the new tokens over the pages
 
 The cache of a layer is two pools ``[pages, page_size, kv_heads, d]`` (bf16 or
-fp16, d 64 or 128). Any strides with contiguous heads work, so the pools may be
-views of one buffer ``[pages, 2, page_size, kv_heads, d]`` or of a pool that
-keeps heads before tokens. Position p of sequence s lives in slot
+fp16, d 64 or 128) with contiguous heads that start on 16-byte boundaries and,
+for ``paged_attention``, are a multiple of 64 values apart. They may be views of
+one buffer ``[pages, 2, page_size, kv_heads, d]`` or of a pool that keeps heads
+before tokens. Position p of sequence s lives in slot
 ``p % page_size`` of page ``page_table[s, p // page_size]``.
 
 Lengths, offsets and page tables stay on the device: nothing is read back, so
@@ -222,6 +223,8 @@ def paged_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tenso
         raise ValueError(f"the page size must be a multiple of 8, got {k_pages.shape[1]}")
     if hkv < 1 or hq < 1 or hq % hkv:
         raise ValueError("query heads must be a multiple of the KV heads")
+    if hkv > 1 and (k_pages.stride(2) % 64 or v_pages.stride(2) % 64):
+        raise ValueError("the pools' heads must be a multiple of 64 values apart")
     _check_batch(batch, rows, q.device)
     if window < 0 or (window and not causal):
         raise ValueError("window must be 0 (all) or a number of positions, with causal attention")

@@ -276,6 +276,8 @@ void register_serving_ops(py::module& m) {
         VALUE_CHECK(std::isfinite(a.scale), "scale must be finite");
         a.k = pool_of(k_pages, q, k_pages, hkv, d, "k_pages", false);
         a.v = pool_of(v_pages, q, k_pages, hkv, d, "v_pages", false);
+        for (const at::Tensor* t : {&k_pages, &v_pages})  // heads are counted in units of 64 values (pool_map())
+          VALUE_CHECK(hkv == 1 || t->stride(2) % 64 == 0, "the pools' heads must be a multiple of 64 values apart");
         check_heads(q, "q", false);
         a.batch = batch_of(table, kv_len, q_start, q, rows);
         const at::cuda::OptionalCUDAGuard guard(device_of(q));

@@ -80,3 +80,25 @@ def linear_over_inputs(device):
     with pytest.raises(ValueError):
         linear_fp8(x, w_q, w_s, out=x[:, :16])
     assert torch.equal(scale, x_s)
+
+
+def attention_on_padded_heads(device):
+    """Heads d + 64 values apart are read, d + 8 apart refused before anything runs; a single head has no distance."""
+    from b200ar.ops.paged import paged_attention
+
+    batch, pool = make_batch([2, 1], [30, 9], PAGE, device)
+    q = randn((3, 4, D), torch.bfloat16, device, 1)
+    k, v = (randn((pool, PAGE, HKV, D), torch.bfloat16, device, i) for i in (2, 3))
+    want = paged_attention(q, k, v, batch)
+
+    def padded(t, by):
+        wide = torch.zeros(*t.shape[:3], D + by, dtype=t.dtype, device=device)
+        wide[..., :D] = t
+        return wide[..., :D]
+
+    assert torch.equal(paged_attention(q, padded(k, 64), padded(v, 64), batch), want)
+    for a, b in ((padded(k, 8), v), (k, padded(v, 8))):
+        with pytest.raises(ValueError, match="64 values apart"):
+            paged_attention(q, a, b, batch)
+    one = paged_attention(q, k[:, :, :1], v[:, :, :1], batch)
+    assert torch.equal(paged_attention(q, padded(k, 8)[:, :, :1], padded(v, 8)[:, :, :1], batch), one)

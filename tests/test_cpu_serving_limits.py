@@ -67,3 +67,9 @@ def test_linear_fp8_refuses_an_output_over_an_input():
     from serving_pools import linear_over_inputs
 
     linear_over_inputs("cpu")
+
+
+def test_attention_refuses_heads_between_units_of_64_values():
+    from serving_pools import attention_on_padded_heads
+
+    attention_on_padded_heads("cpu")
