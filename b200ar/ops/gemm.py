@@ -27,9 +27,15 @@ def error_word(device) -> torch.Tensor:
     return word
 
 
-# What the codes of the error word above the bounded waits' say.
-_ERROR_TEXT = {3: "a token's position is outside the rotary table or before its sequence",
-               4: "a position that a row needs has no page in the pool"}
+# What the codes of the error word say.
+_EXPIRED = "reported error {code} (a bounded wait expired)"
+_ERROR_TEXT = {1: "tcgen05 GEMM on {device} " + _EXPIRED,
+               2: "paged_attention on {device} " + _EXPIRED + "; its outputs are not complete",
+               3: "paged KV cache on {device}: a token's position is outside the rotary table or before its sequence "
+                  "(error {code}); it was skipped",
+               4: "paged KV cache on {device}: a position that a row needs has no page in the pool (error {code}); "
+                  "it was skipped",
+               5: "linear_fp8 on {device} " + _EXPIRED + "; its outputs are not complete"}
 
 
 def check_errors(device=None) -> None:
@@ -41,9 +47,7 @@ def check_errors(device=None) -> None:
         v = int(t.item())
         if v:
             t.zero_()
-            if v in _ERROR_TEXT:
-                raise RuntimeError(f"paged KV cache on cuda:{idx}: {_ERROR_TEXT[v]} (error {v}); it was skipped")
-            raise RuntimeError(f"tcgen05 GEMM on cuda:{idx} reported error {v} (a bounded wait expired)")
+            raise RuntimeError(_ERROR_TEXT.get(v, "error {code} on {device}").format(code=v, device=f"cuda:{idx}"))
 
 
 _SKINNY: Dict[int, dict] = {}

@@ -51,7 +51,7 @@ namespace fp8 {
 
 namespace {
 
-constexpr int kErrTimeout = 1;
+constexpr int kErrTimeout = 5;  // in the error word that other operators share; a bounded wait expired
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi);

@@ -73,3 +73,19 @@ def test_attention_refuses_heads_between_units_of_64_values():
     from serving_pools import attention_on_padded_heads
 
     attention_on_padded_heads("cpu")
+
+
+def test_error_texts_name_the_operator():
+    from b200ar.ops import gemm
+
+    old = dict(gemm._ERR)
+    try:
+        for code, text in ((1, "GEMM"), (2, "paged_attention.*bounded wait"), (3, "rotary table"), (4, "no page"),
+                           (5, "linear_fp8.*bounded wait"), (9, "error 9 on cuda:0")):
+            gemm._ERR.clear()
+            gemm._ERR[0] = torch.tensor([code], dtype=torch.int32)
+            with pytest.raises(RuntimeError, match=text):
+                gemm.check_errors()
+    finally:
+        gemm._ERR.clear()
+        gemm._ERR.update(old)
