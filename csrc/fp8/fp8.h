@@ -44,6 +44,8 @@ struct LinearArgs {
   float* workspace;    // set by linear()
   unsigned* counters;
 };
+// Whether a call of these sizes on the current device takes the kernel for many rows.
+bool linear_takes_pairs(int64_t M, int64_t N, int64_t K);
 // Bytes of scratch of a call; not kept from call to call.
 int64_t linear_scratch(const LinearArgs& a);
 // out = sum over blocks b of sx[b, m] sw[n / 128, b] (x[m, b] . w[n, b])

@@ -835,6 +835,13 @@ Layout layout(const LinearArgs& l) {
 
 }  // namespace
 
+bool linear_takes_pairs(int64_t M, int64_t N, int64_t K) {
+  LinearArgs l{};
+  l.M = M, l.N = N, l.K = K;
+  check(l);
+  return many_rows(l);
+}
+
 int64_t linear_scratch(const LinearArgs& l) {
   check(l);
   return l.M == 0 ? 0 : layout(l).bytes;

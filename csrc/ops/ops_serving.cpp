@@ -359,6 +359,9 @@ void register_serving_ops(py::module& m) {
         return std::make_pair(q, scale);
       },
       "e4m3 values and a scale for each 128 x 128 block", py::arg("w"));
+  m.def("linear_fp8_takes_pairs", &b200ar::fp8::linear_takes_pairs,
+        "whether linear_fp8 runs these sizes on the kernel for many rows (tests)", py::arg("m"), py::arg("n"),
+        py::arg("k"));
   m.def(
       "linear_fp8",
       [](const at::Tensor& x, const at::Tensor& w, const at::Tensor& w_scale, const OptTensor& out_opt,
