@@ -120,6 +120,8 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
 }
 __device__ __forceinline__ uint64_t both(float x) { return pack64(__float_as_uint(x), __float_as_uint(x)); }
 
+__device__ __forceinline__ bool normal(float x) { return fabsf(x) >= 0x1p-126f && fabsf(x) < INFINITY; }
+
 // A block's sum r (0, or from 2^-18 to 2^25) times two scales a and b, as (r first) b second: whatever the scales, a
 // product on the way is out of range only if the result is. (r a is a normal number for a between 2^-100 and 2^100;
 // outside, a power of two of a's is left for the end.)
@@ -553,16 +555,16 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int sl = (i + e) % kScales;
           wait(&sempty[sl], (((i + e) / kScales) & 1u) ^ 1u);
           float* dst = scales + sl * kScaleFloats;
-          bool normal = true;
+          bool all = true;
 #pragma unroll
           for (int g = 0; g < 2; ++g)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
               const float f = x[e][h] * w[e][g];
               dst[g * 128 + id + 64 * h] = f;
-              normal = normal && fabsf(f) >= 0x1p-126f && fabsf(f) < INFINITY;
+              all = all && normal(f);
             }
-          const unsigned odd = __ballot_sync(0xffffffffu, !normal);
+          const unsigned odd = __ballot_sync(0xffffffffu, !all);
           if (lane == 0) reinterpret_cast<unsigned*>(dst)[256 + warp - 10] = odd;
           sm100::mbar_arrive(&sfull[sl]);
           if (i + e + kAhead < count) load(x[e], w[e]);
@@ -594,14 +596,18 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) sm100::mbar_arrive(&sempty[sl]);
         wait(&tfull[bf * 2 + g], (n >> 1) & 1u);
         sm100::tc_fence_after();
-        // Where a factor of the block is not a normal number, two of three (around()) are multiplied into the sums in
-        // tensor memory first. (Measured for 4093 x 7168 x 8192, this kernel alone: with one product for every block,
-        // right or not, 266 us; this way 270; tested here 275; with a second form of the loop below 314.)
+        // Where a factor of the block is not a normal number, two of three (around()) are multiplied into the row's sums
+        // in tensor memory first; other rows' stay as they are. (Measured for 4093 x 7168 x 8192, this kernel alone:
+        // with one product for every block, right or not, 266 us; this way 270; tested here 275; with a second form of
+        // the loop below 314.)
         if ((odd.x | odd.y) != 0u) {
-          float first;
-          around(__ldg(a.sw + static_cast<int64_t>(min(tn * 2 + g, (a.N + kBlock - 1) / kBlock - 1)) * a.kblocks + kb),
-                 first, sf);
-          scale_sums(td + bf * BN, first, __ldg(a.sx + kb * a.lds + min(m, a.M - 1)));
+          float first = 1.f, sx = 1.f;
+          if (!normal(sf)) {
+            sx = __ldg(a.sx + kb * a.lds + min(m, a.M - 1));
+            around(__ldg(a.sw + static_cast<int64_t>(min(tn * 2 + g, (a.N + kBlock - 1) / kBlock - 1)) * a.kblocks + kb),
+                   first, sf);
+          }
+          scale_sums(td + bf * BN, first, sx);
         }
         const uint64_t s = both(sf);
 #pragma unroll

@@ -111,6 +111,30 @@ def test_linear_fp8_many_rows_on_two_streams_at_once():
     assert all(torch.equal(g, want[i]) for i in range(2) for g in got[i])
 
 
+def test_linear_fp8_many_rows_extremes():
+    """Rows of NaN and infinities leave the others as they are; blocks whose scales span many orders."""
+    from b200ar.ops.fp8 import linear_fp8, quantize_fp8, quantize_fp8_weight
+
+    m, n, k = 700, 3592, 2832
+    x = randn((m, k), BF, "cuda", 1)
+    w_q, w_s = quantize_fp8_weight(randn((n, k), BF, "cuda", 2))
+    clean = linear_fp8(x, w_q, w_s)
+    odd = x.clone()
+    odd[1, 300], odd[300, 7], odd[699, 511] = float("nan"), float("inf"), -float("inf")
+    out = linear_fp8(odd, w_q, w_s)
+    keep = [i for i in range(m) if i not in (1, 300, 699)]
+    assert torch.equal(out[keep], clean[keep]) and torch.isnan(out[[1, 300, 699]]).all()
+    steps = (10.0 ** torch.linspace(-30, 3, -(-k // 128), device="cuda")).repeat_interleave(128)[:k]
+    x = (x * steps).to(BF)
+    x[0] = 0
+    x_q, x_s = quantize_fp8(x)
+    codes, scales = plain_quantize(x)
+    assert torch.equal(x_q.double().cpu(), codes) and torch.equal(x_s.double().cpu(), scales)
+    out = linear_fp8(x, w_q, w_s)
+    check_linear(out, x_q, x_s, w_q, w_s)
+    assert not out[0].any()
+
+
 @pytest.mark.parametrize("m,k", [(1, 16), (5, 400), (600, 272)])
 def test_quantize_fp8_of_fp32(m, k):
     from b200ar.ops.fp8 import quantize_fp8, quantize_fp8_weight
