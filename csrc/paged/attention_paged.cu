@@ -907,6 +907,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool some = cleared(), counts = valid && inv == inv && inv != 0.f;
           const unsigned not_finite = __ballot_sync(0xffffffffu, counts && odd != 0.f);
           const unsigned rows = __ballot_sync(0xffffffffu, counts && (odd != 0.f || some));
+          __syncwarp();  // the rows are stored
           if (rows) settle<T, D>(a, it, group, (wide ? t * 128 : 0) + w4 * 32, rows, not_finite != 0, some);
         }
       };
