@@ -14,8 +14,9 @@
 //   which add their sums through distributed shared memory: no workspace. The
 //   weights' first tiles are on their way before the kernel waits for the
 //   quantization of x. Bound by the stream of the weights behind two launches:
-//   1 x 7168 x 8192 takes 14.6 us with the quantization (59 MB, 9.0 us at the
-//   copy rate), 48 x 8192 x 3584 13.0 us (30 MB, 4.7 us).
+//   1 x 7168 x 8192 takes 15.5 us with the quantization (59 MB, 9.0 us at the
+//   copy rate), 48 x 8192 x 3584 12.7 us (30 MB, 4.7 us). With 65 to 128 rows one
+//   CTA fits an SM (254 registers a thread) and 7168 x 8192 takes 36 to 38 us.
 // pair_kernel (many rows). CTA pairs (cta_group::2) compute 256 x 256 tiles. A K
 //   block's sums go to one of two buffers in tensor memory, each in two halves
 //   of 128 columns with a warpgroup and barriers of its own: handing a buffer
@@ -27,8 +28,9 @@
 //   one line that is cut into equal parts for the pairs, so no pair idles in a
 //   last partial wave. A tile that a cut falls into is finished by the pair that
 //   arrives last, which adds the parts in the order of K. Bound by the way of
-//   every block's sums out of tensor memory: 4093 x 7168 x 8192 takes 310 us with
-//   the quantization, 1550 TFLOP/s.
+//   every block's sums out of tensor memory (tensor core 44 % of the active cycles,
+//   issue slots 41 %, DRAM 23 %): 4093 x 7168 x 8192 with the quantization takes 306
+//   us in a short run, 1570 TFLOP/s, and 360 us in a long one, at the power limit.
 //
 // Every wait is bounded: on expiry the error word is set and all roles run
 // down without waiting.
@@ -145,7 +147,7 @@ template <int MP>  // rows of x in a tile
 struct RowsCfg {
   static constexpr int kThreads = 224;
   static constexpr uint32_t kW = 128 * 128, kX = MP * 128, kStage = kW + kX;
-  // Two CTAs fit an SM, or one at 128 rows, whose sums need the space once the ring is done.
+  // Two CTAs fit an SM, or one at 128 rows: their sums take 254 registers a thread (and the ring's space at the end).
   static constexpr int kStages = (100 * 1024) / kStage;
   static constexpr int kBufs = MP == 128 ? 2 : 4;  // accumulators in tensor memory
   static constexpr uint32_t kCols = kBufs * MP;    // a power of two from 64 to 256
@@ -604,8 +606,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           float first = 1.f, sx = 1.f;
           if (!normal(sf)) {
             sx = __ldg(a.sx + kb * a.lds + min(m, a.M - 1));
-            around(__ldg(a.sw + static_cast<int64_t>(min(tn * 2 + g, (a.N + kBlock - 1) / kBlock - 1)) * a.kblocks + kb),
-                   first, sf);
+            const int64_t nb = min(tn * 2 + g, (a.N + kBlock - 1) / kBlock - 1);
+            around(__ldg(a.sw + nb * a.kblocks + kb), first, sf);
           }
           scale_sums(td + bf * BN, first, sx);
         }
@@ -763,9 +765,10 @@ int pairs_of(const LinearArgs& l) {
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count() / 2, pair_units(l) / kPartUnits)));
 }
 
-// Whether pair_kernel takes a call: above one tile of rows_kernel, if there is a part for every pair. Measured
-// (rows_kernel, pair_kernel): 128 x 7168 x 8192 43, 45 us; 256 x 7168 x 8192 67, 45 us (1792 K blocks of tiles);
-// 512 x 1280 x 8192 41, 39 us (640); 300 x 4096 x 2048 29, 35 us (512); 333 x 1288 x 1040 14, 27 us (108).
+// Whether pair_kernel takes a call: above one tile of rows_kernel, if there is a part for every pair (888 K blocks of
+// tiles on 148 SMs). Measured (rows_kernel, pair_kernel): 128 x 7168 x 8192 43, 45 us; 256 x 7168 x 8192 67, 45 us (1792
+// K blocks of tiles); 512 x 1280 x 8192 41, 39 us (640), which the rule leaves to the slower by 2 us; 300 x 4096 x 2048
+// 29, 35 us (512); 333 x 1288 x 1040 14, 27 us (108).
 bool many_rows(const LinearArgs& l) {
   return l.M > 128 && (pair_units(l) >= sm_count() / 2 * kPartUnits || l.M > 65535 * 128);
 }

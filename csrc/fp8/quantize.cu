@@ -11,9 +11,10 @@
 // either reaches the outputs of its row.
 //
 // Each value is read once and its code written once, 3 bytes: 4096 x 8192 values
-// take 33 us (100 MB, 15 us at the copy rate) and a weight of 7168 x 8192 45 us;
-// the two conversions of each value and the scales' divisions share the rest.
-// (With a test of every product for the middle between two codes: 51 and 76 us.)
+// take 28 us (100 MB, 15 us at the copy rate) and a weight of 7168 x 8192 41 us.
+// What bounds it is the number of instructions, two conversions of each value
+// among them: issue slots 84 % of the active cycles, DRAM 29 %. (With a test of
+// every product for the middle between two codes it took nearly twice as long.)
 #include "../common/check.h"
 #include "../common/pdl.h"
 #include "../common/trace.h"

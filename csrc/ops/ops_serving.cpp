@@ -93,7 +93,8 @@ bool share_memory(const at::Tensor& a, const at::Tensor& b) {
   for (int64_t i = 0; i < a.dim(); ++i)
     if (a.size(i) > 1) dims.push_back({a.size(i), a.stride(i), b.stride(i)});
   std::sort(dims.begin(), dims.end(), [](const Dim& x, const Dim& y) { return x.a > y.a; });
-  const std::function<bool(size_t, int64_t)> meet = [&](size_t i, int64_t at) {  // b's dimensions from i on, `at` behind a's
+  // Whether the dimensions from i on meet, b's `at` elements behind a's.
+  const std::function<bool(size_t, int64_t)> meet = [&](size_t i, int64_t at) {
     int64_t span_a = 1, span_b = 1;
     for (size_t k = i; k < dims.size(); ++k) {
       span_a += (dims[k].size - 1) * dims[k].a;
@@ -104,7 +105,8 @@ bool share_memory(const at::Tensor& a, const at::Tensor& b) {
     if (dims[i].a != dims[i].b || dims[i].a < std::max(span_a, span_b) - (dims[i].size - 1) * dims[i].a) return true;
     const int64_t stride = dims[i].a, steps = at >= 0 ? at / stride : -((stride - 1 - at) / stride);
     const int64_t rest = at - steps * stride, last = dims[i].size - 1;
-    return (std::abs(steps) <= last && meet(i + 1, rest)) || (std::abs(steps + 1) <= last && meet(i + 1, rest - stride));
+    return (std::abs(steps) <= last && meet(i + 1, rest)) ||
+           (std::abs(steps + 1) <= last && meet(i + 1, rest - stride));
   };
   const int64_t bytes = reinterpret_cast<intptr_t>(b.data_ptr()) - reinterpret_cast<intptr_t>(a.data_ptr());
   return bytes % a.element_size() != 0 || meet(0, bytes / a.element_size());

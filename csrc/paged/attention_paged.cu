@@ -41,11 +41,14 @@
 // the product before is done: P stays in the type's range, and numerator and
 // denominator have the same factor.
 //
-// What bounds it: with many rows the softmax, whose exponentials alone (8 clocks
-// for a warp's 32) take the time of both products, next to the conversions and
-// maxima in the same schedulers; with single tokens over long caches the stream of
-// K and V (64 tokens over 1 to 4095 with 8 KV heads of 128: 102 us for 0.5 GB),
-// and over short ones the way of a block through the pipeline, about 3 us.
+// What bounds it: with many rows the way of a tile through a group, S, maximum,
+// exponentials, P, product, which the other group does not cover. By count the
+// exponentials (8 clocks for a warp's 32) take the time of both products, and for
+// 4096 tokens over 8192 the exponential unit is in use for 55 % of the active
+// cycles, the tensor core for 54 % and the issue slots for 35 %: none is full.
+// With single tokens over long caches it is the stream of K and V (64 tokens over
+// 1 to 4095 with 8 KV heads of 128: 100 us for 0.5 GB), and over short ones the way
+// of a block through the pipeline, about 3 us.
 //
 // Pages are read by TMA boxes of the largest power of two of tokens (8 to
 // 128) that divides the page size. Runs that no row sees are not looked up:
@@ -164,7 +167,8 @@ __device__ __noinline__ void settle(const AttnArgs& a, const Item& it, int group
       };
       uint32_t* at = reinterpret_cast<uint32_t*>(out + i * 64);
       const float2 old = to_float2<T>(*reinterpret_cast<volatile uint32_t*>(at));
-      if (seen >> (6 * i) & 63u) *at = pack2<T>(value(seen >> (6 * i) & 7u, old.x), value(seen >> (6 * i + 3) & 7u, old.y));
+      const unsigned x3 = seen >> (6 * i) & 7u, y3 = seen >> (6 * i + 3) & 7u;
+      if (x3 | y3) *at = pack2<T>(value(x3, old.x), value(y3, old.y));
     }
   }
 }
@@ -706,8 +710,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int j = st.tile(k), c0 = first_pos + j * kTile;
         wait(&bar.sfull[t], no & 1u);
         sm100::tc_fence_after();
-        // Single tokens, whose rows all see the same: what they must not see in V becomes zeros here, since zero times NaN is NaN. (After S
-        // of the step: what the slot of V held before is consumed or still waited for by this load.)
+        // Single tokens, whose rows all see the same: the rest becomes zeros in V here, since zero times NaN is NaN.
+        // (After S of the step: what the slot of V held before is consumed or still waited for by this load.)
         if constexpr (kTokens)
           if (c0 + kTile > hide0 || c0 < see0) {
             const unsigned at = base + st.v_at(j);
@@ -823,7 +827,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       auto cleared = [&] { return *static_cast<volatile int*>(&it.cleared) != 0; };
       auto describe = [&] {
         if (!whole && threadIdx.x == 0)
-          desc[which] = PartDesc{it.s, it.h, it.b, static_cast<short>(it.rows), cleared(), it.t0, it.t1, it.tiles, it.q0};
+          desc[which] =
+              PartDesc{it.s, it.h, it.b, static_cast<short>(it.rows), cleared(), it.t0, it.t1, it.tiles, it.q0};
       };
       if (wide) describe();
       auto out_of = [&](int r2) {
@@ -1004,7 +1009,8 @@ __global__ void __launch_bounds__(kThreads, 1)
           const bool some = cleared();
           if (bad != 0 || some) {
             const float inv = misc.inv[lane];
-            const unsigned rows = __ballot_sync(0xffffffffu, valid && inv == inv && inv != 0.f && (some || bad >> lane & 1u));
+            const bool counts = valid && inv == inv && inv != 0.f;
+            const unsigned rows = __ballot_sync(0xffffffffu, counts && (some || bad >> lane & 1u));
             const unsigned mine8 = rows & (0x01010101u << warp);  // every eighth row
             if (mine8) settle<T, D>(a, it, group, 0, mine8, (bad & mine8) != 0, some);
             group_sync();

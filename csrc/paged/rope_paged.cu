@@ -14,8 +14,10 @@
 //
 // Every value is read once and written once, so memory bounds the large calls
 // and one chain of loads (length, offset, page, value) the small ones: five
-// prompts with 64 + 2 x 8 heads of 128 (279 MB) take 57 us, 4.9 TB/s, and one or
-// 64 tokens 2 us.
+// prompts with 64 + 2 x 8 heads of 128 (279 MB) take 58 us, 4.8 TB/s, and one or
+// 64 tokens 2 us. (Prompts: DRAM 49 % of its nominal rate, issue slots 59 %. A block
+// serves one row, so the chain is walked for each and its loads do not run beside
+// the stores of the row before.)
 #include <algorithm>
 
 #include "../common/check.h"

@@ -147,7 +147,8 @@ def test_attention_values_that_are_not_finite(new, total, decode, dtype, d, hkv)
         for value in (INF, -INF, NAN, INF):
             for p in {0, t - 1, max(t - new[s] // 2 - 1, 0), *torch.randint(t, (3,), generator=g).tolist()}:
                 pg, slot = _slot(batch, s, p)
-                v[pg, slot, int(torch.randint(hkv, (1,), generator=g)), int(torch.randint(d, (1,), generator=g))] = value
+                head, column = (int(torch.randint(top, (1,), generator=g)) for top in (hkv, d))
+                v[pg, slot, head, column] = value
         end = torch.arange(t, -(-t // PAGE) * PAGE)
         v[batch.page_table.cpu()[s, end // PAGE].long(), end % PAGE] = NAN
     clean = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
@@ -182,13 +183,14 @@ def test_attention_large_values_within_the_type(new, total, decode):
     from b200ar.ops.paged import paged_attention
 
     q, k, v, batch = _inputs(new, total, decode, BF, 128)
-    k.mul_(torch.linspace(0.01, 3, k.shape[0], device="cuda").to(BF)[:, None, None, None])  # the largest score comes late
+    # Pages of different sizes, so that the bound on a row's maximum moves.
+    k.mul_(torch.linspace(0.01, 3, k.shape[0], device="cuda").to(BF)[:, None, None, None])
     small = paged_attention(q, k, v.sign(), batch)
     assert torch.equal(paged_attention(q, k, v.sign() * 2.0 ** 114, batch), small * 2.0 ** 114)
 
 
 # ------------------------------------------------------------------ 8-bit linear
-# On 148 SMs a K block of 256 x 256 outputs is a unit, and from 888 units on a call of over 128 rows takes pairs of CTAs.
+# On 148 SMs a K block of 256 x 256 outputs is a unit, and from 888 units on a call of over 128 rows takes CTA pairs.
 FEW = [(3, 264, 512), (17, 264, 512), (40, 264, 512), (100, 264, 512), (200, 264, 512)]
 MANY = [(300, 4096, 8192)]
 
